@@ -215,6 +215,24 @@ SIGNATURES['gs_link_head_mse_fwd_bwd_static'] = (_i32, [_vp, _vp, _i64, _i32, _v
 SIGNATURES['gs_stage_batch'] = (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _f32, _vp, _vp])
 SIGNATURES['gs_adam_step'] = (_i32, [_vp, _vp, _vp, _vp, _i64, _f32, _vp, _f32, _f32, _f32, _f32, _vp])
 
+
+class Neighbors(_c.Structure):
+    """gs_neighbors of include/gsage_ops.h."""
+    _fields_ = [('indptr', _vp), ('n_parents', _i64), ('n_child', _i64), ('ids', _vp), ('n_edges', _i64),
+                ('id_offset', _i64), ('n_rows', _i64)]
+
+
+# The operators of include/gsage_ops.h, declaration by declaration.
+SIGNATURES_OPS = {
+    'gs_dropout': (_i32, [_vp, _i64, _i32, _c.c_double, _u64, _vp, _u64, _vp, _vp]),
+    'gs_neighbor_attention_workspace': (_sz, [_c.POINTER(Neighbors), _i32, _i32, _i32, _i32]),
+    'gs_neighbor_attention_fwd': (_i32, [_vp, _vp, _vp, _c.POINTER(Neighbors), _i32, _i32, _i32, _i32, _f32, _vp, _vp, _vp,
+                                         _sz, _vp]),
+    'gs_neighbor_attention_bwd_workspace': (_sz, [_c.POINTER(Neighbors), _i32, _i32, _i32, _i32, _i64]),
+    'gs_neighbor_attention_bwd': (_i32, [_vp, _vp, _vp, _c.POINTER(Neighbors), _i32, _i32, _i32, _i32, _f32, _vp, _vp, _vp,
+                                         _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
+}
+
 _lib = None
 
 
@@ -233,7 +251,7 @@ def load():
             "`python -c 'import __graft_entry__ as g; g.build()'`; there is no CPU fallback" % LIB_PATH)
     import torch  # noqa: F401  (loads the HIP runtime the library must share)
     lib = ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_GLOBAL)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in list(SIGNATURES.items()) + list(SIGNATURES_OPS.items()):
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -130,3 +130,42 @@ class L2Normalize(torch.autograd.Function):
     def backward(ctx, g):
         (x,) = ctx.saved_tensors
         return kernels.l2_normalize_bwd(x, g.contiguous())
+
+
+class Dropout(torch.autograd.Function):
+    """``kernels.dropout``; the backward pass draws the mask again.  A seed that lives in GPU memory is copied, so that
+    the gradient goes by the mask that was drawn even if the caller has changed the seed since."""
+
+    @staticmethod
+    def forward(ctx, x, rate, seed, offset):
+        if isinstance(seed, torch.Tensor):
+            seed = seed.clone()
+        ctx.mask = (rate, seed, offset)
+        return kernels.dropout(x, rate, seed, offset)
+
+    @staticmethod
+    def backward(ctx, g):
+        return kernels.dropout(g.contiguous(), *ctx.mask), None, None, None
+
+
+class NeighborAttention(torch.autograd.Function):
+    """``kernels.neighbor_attention``: (out, lse); gradients through ``out`` only.  With child_ids, the gradient of
+    the tables takes ``inverse`` (``kernels.neighbor_inverse``; built in the backward pass when it is None)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, child_ids, n_child, id_offset, scale, indptr, inverse):
+        out, lse = kernels.neighbor_attention(q, k, v, child_ids, n_child, id_offset, scale, indptr)
+        ctx.save_for_backward(q, k, v, child_ids, out, lse, indptr)
+        ctx.meta = (n_child, int(id_offset), scale, inverse)
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    def backward(ctx, g, _):
+        q, k, v, child_ids, out, lse, indptr = ctx.saved_tensors
+        n_child, id_offset, scale, inverse = ctx.meta
+        need = ctx.needs_input_grad
+        g_q, g_k, g_v = kernels.neighbor_attention_bwd(
+            q, k, v, child_ids, n_child, out, lse, g.contiguous(), id_offset, scale, indptr, inverse,
+            need_q=need[0], need_rows=need[1] or need[2])
+        return (g_q, g_k if need[1] else None, g_v if need[2] else None) + (None,) * 6

@@ -1,0 +1,132 @@
+// Attention over neighbors: how the edges are dealt to the lanes, shared by the forward and the backward kernels.
+//
+// A row of dim elements is covered by a "worker" of L lanes, 16 bytes each (L = the power of two >= dim / (elements in
+// 16 bytes)); a dot product is a few multiply-adds per lane and a sum over the worker's lanes, the running softmax
+// (maximum, sum, weighted row) lives in the worker's registers, and the row is read once, whatever the number of
+// heads that share it.  Tables whose rows do not start on 16 bytes are read element by element: lane l then holds
+// elements l, l + L, ...; nothing else depends on which element sits where.
+//
+// Edges are dealt by count, not by parent: worker w takes edges [w C, (w + 1) C), so a popular parent's list is spread
+// over the chip and short lists cost no idle lanes.  Parents with at most a fixed number of neighbors each are dealt
+// whole (C a multiple of their n_child) and leave no pieces.  A parent that lies in one worker is finished there; for one that
+// crosses a border every worker leaves a piece (maximum, sum, unnormalised row) in the workspace and a second launch
+// joins them in worker order.  The result depends on C, which depends on the sizes only.
+#pragma once
+
+#include "ops_common.h"
+
+namespace gs {
+
+constexpr int kAttnThreads = 256;
+constexpr int kAttnRows = 8;                        // rows a worker has in flight
+
+struct Neighbors {
+    const int64_t *indptr;
+    const int32_t *ids;
+    int64_t n_parents, id_offset, n_rows;
+    uint32_t n_child, n_edges;
+
+    // [begin, end) of parent p, inside [0, n_edges] whatever indptr holds
+    __device__ __forceinline__ void range(int64_t p, uint32_t &b, uint32_t &e) const {
+        if (!indptr) { b = (uint32_t)p * n_child; e = b + n_child; return; }
+        const int64_t x = indptr[p], y = indptr[p + 1];
+        b = (uint32_t)(x < 0 ? 0 : x > n_edges ? n_edges : x);
+        e = (uint32_t)(y < 0 ? 0 : y > n_edges ? n_edges : y);
+        if (e < b) e = b;
+    }
+    // the first parent whose range ends behind edge e, from p0 on; n_parents if there is none
+    __device__ __forceinline__ int64_t parent_of(uint32_t e, int64_t p0) const {
+        if (!indptr) return e / n_child;
+        int64_t lo = p0, hi = n_parents;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi) >> 1;
+            if (indptr[mid + 1] > (int64_t)e) hi = mid; else lo = mid + 1;
+        }
+        return lo;
+    }
+    // table row of edge e, or -1
+    __device__ __forceinline__ int64_t row_of(uint32_t e) const {
+        const int64_t r = ids ? (int64_t)ids[e] - id_offset : (int64_t)e;
+        return (uint64_t)r < (uint64_t)n_rows ? r : -1;
+    }
+};
+
+// 16 bytes of a row per lane, as they arrive.
+template <class T, int L, bool ALIGNED> struct RowPart {
+    static constexpr int E = Pack<T>::E;
+    T x[E];
+    __device__ __forceinline__ void load(const T *row, int lane, int dim) {
+        if (ALIGNED) {
+            if (lane * E < dim) *reinterpret_cast<uint4 *>(x) = reinterpret_cast<const uint4 *>(row)[lane];
+            else *reinterpret_cast<uint4 *>(x) = make_uint4(0, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = lane + i * L < dim ? row[lane + i * L] : (T)0.f;
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = (T)0.f;
+    }
+    __device__ __forceinline__ float at(int i) const { return (float)x[i]; }
+};
+
+template <class T, int L, bool ALIGNED>
+__device__ __forceinline__ void store_row(T *row, int lane, int dim, const float *v) {
+    constexpr int E = Pack<T>::E;
+    if (ALIGNED) {
+        if (lane * E < dim) {
+            alignas(16) T x[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = (T)v[i];
+            reinterpret_cast<uint4 *>(row)[lane] = *reinterpret_cast<const uint4 *>(x);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (lane + i * L < dim) row[lane + i * L] = (T)v[i];
+    }
+}
+
+// Element index of part i of a lane, for the fp32 pieces in the workspace.
+template <class T, int L, bool ALIGNED> __device__ __forceinline__ int element_of(int lane, int i) {
+    return ALIGNED ? lane * Pack<T>::E + i : lane + i * L;
+}
+
+// Lanes per row: enough for dim elements at 16 bytes a lane.
+inline int lanes_for(int dim, int size) {
+    const int per = 16 / size;
+    int l = 4;
+    while (l * per < dim) l *= 2;
+    return l;
+}
+
+// Edges per worker, and whether parents are dealt whole.
+struct Deal {
+    int64_t chunk, workers;
+    bool whole;
+};
+
+inline Deal deal_edges(const int64_t *indptr, int64_t n_parents, int64_t n_child, int64_t n_edges, int lanes) {
+    Deal d;
+    const int64_t per_wave = 64 / lanes;
+    // parents of one length are dealt whole where that gives the chip enough waves to hide the row loads' latency, or
+    // where a list is too short to be worth cutting
+    d.whole = !indptr && n_child > 0 && (n_child <= 4 * kAttnRows || n_parents >= 4096 * per_wave);
+    if (d.whole) {
+        const int64_t group = n_child < kAttnRows && n_parents >= 32768 * per_wave ? (kAttnRows + n_child - 1) / n_child : 1;
+        d.chunk = group * n_child;
+    } else {
+        // 8 edges (one round of loads) at least, then as many as leave 8192 waves, at most 128
+        int64_t c = n_edges / (8192 * per_wave);
+        c = (c + kAttnRows - 1) / kAttnRows * kAttnRows;
+        d.chunk = c < kAttnRows ? kAttnRows : c > 128 ? 128 : c;
+    }
+    d.workers = n_edges ? (n_edges + d.chunk - 1) / d.chunk : 0;
+    return d;
+}
+
+// Checks a gs_neighbors; 0 or the error.
+int check_neighbors(const char *what, const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype);
+
+}  // namespace gs

@@ -1,0 +1,275 @@
+// Attention of every parent over its neighbors, forward (the dealing of edges: attention.h).
+//
+// Bound by the row gathers: an edge costs one row of dim elements (two with separate values) and, per head, dim
+// multiply-adds for the score and as many for the sum, about a fifth of what the vector ALU does in the time the row
+// takes to arrive.  Scores are kept in units of log 2 (scale * log2 e goes into the query), so an exponential is one
+// instruction.
+#include "attention.h"
+
+namespace gs {
+
+int check_neighbors(const char *what, const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype) {
+    if (!nb) return fail(GS_EINVAL, "%s: null pointer argument", what);
+    if (!dtype_size(dtype)) return fail(GS_EINVAL, "%s: dtype %d", what, dtype);
+    if (nb->n_parents < 0 || nb->n_edges < 0 || nb->n_rows < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || dim < 1)
+        return fail(GS_EINVAL, "%s: parents=%lld edges=%lld rows=%lld heads=%d kv_heads=%d dim=%d", what,
+                    (long long)nb->n_parents, (long long)nb->n_edges, (long long)nb->n_rows, heads, kv_heads, dim);
+    if (dim > 256 || heads > 1024) return fail(GS_ELIMIT, "%s: dim=%d (at most 256), heads=%d (at most 1024)", what, dim, heads);
+    if (nb->n_edges >= (int64_t)1 << 31 || nb->n_parents >= (int64_t)1 << 31)
+        return fail(GS_ELIMIT, "%s: %lld edges, %lld parents (less than 2^31)", what, (long long)nb->n_edges, (long long)nb->n_parents);
+    if (!nb->indptr && (nb->n_child < 0 || nb->n_child >= (int64_t)1 << 31 || nb->n_parents * nb->n_child != nb->n_edges))
+        return fail(GS_EINVAL, "%s: %lld edges for %lld parents of %lld", what, (long long)nb->n_edges, (long long)nb->n_parents,
+                    (long long)nb->n_child);
+    return GS_OK;
+}
+
+}  // namespace gs
+
+namespace {
+
+using gs::Neighbors;
+using gs::RowPart;
+
+struct FwdArgs {
+    Neighbors nb;
+    const void *q, *k, *v;
+    void *out;
+    float *lse;
+    float2 *piece_ms;                               // [workers][2][heads]: maximum (log 2), sum
+    float *piece_acc;                               // [workers][2][heads][dim]
+    float scale2;                                   // scale * log2 e
+    int heads, kv_heads, dim, chunk, parts;         // parts: head groups per key head
+};
+
+template <class T, int L, int G, bool ALIGNED>
+__global__ __launch_bounds__(gs::kAttnThreads)
+void attn_fwd_kernel(FwdArgs a) {
+    constexpr int E = gs::Pack<T>::E, U = gs::kAttnRows;
+    const int lane = threadIdx.x & (L - 1);
+    const uint32_t w = blockIdx.x * (gs::kAttnThreads / L) + threadIdx.x / L;
+    const int share = a.heads / a.kv_heads;
+    const int j = blockIdx.y / a.parts, h0 = j * share + (blockIdx.y % a.parts) * G;
+    const int n_heads = min(G, (j + 1) * share - h0);
+    const uint32_t C = a.chunk, e0 = min((uint64_t)w * C, (uint64_t)a.nb.n_edges), e1 = min((uint64_t)e0 + C, (uint64_t)a.nb.n_edges);
+    const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = a.v ? static_cast<const T *>(a.v) + (int64_t)j * a.dim : nullptr;
+    const int64_t stride = (int64_t)a.kv_heads * a.dim;
+
+    if (e0 < e1 && a.piece_ms)                      // no piece yet in either place
+        for (int i = lane; i < 2 * n_heads; i += L)
+            a.piece_ms[((size_t)w * 2 + i / n_heads) * a.heads + h0 + i % n_heads] = make_float2(-INFINITY, 0.f);
+
+    uint32_t e = e0;
+    int64_t p = e < e1 ? a.nb.parent_of(e, 0) : a.nb.n_parents;
+    while (e < e1 && p < a.nb.n_parents) {
+        uint32_t sb, se;
+        a.nb.range(p, sb, se);
+        if (se <= e) { p = a.nb.parent_of(e, p + 1); continue; }
+        if (sb > e) { e = sb; continue; }
+        const uint32_t end = min(se, e1), begin = e;
+
+        float q[G][E], acc[G][E], m[G], s[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            RowPart<T, L, ALIGNED> r;
+            if (g < n_heads) r.load(static_cast<const T *>(a.q) + (p * a.heads + h0 + g) * a.dim, lane, a.dim); else r.zero();
+            m[g] = -INFINITY;
+            s[g] = 0.f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) { q[g][i] = r.at(i) * a.scale2; acc[g][i] = 0.f; }
+        }
+        for (; e < end; e += U) {
+            int64_t row[U];
+            RowPart<T, L, ALIGNED> kr[U], vr[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) row[u] = e + u < end ? a.nb.row_of(e + u) : -1;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (row[u] >= 0) kr[u].load(K + row[u] * stride, lane, a.dim); else kr[u].zero();
+                if (V) { if (row[u] >= 0) vr[u].load(V + row[u] * stride, lane, a.dim); else vr[u].zero(); }
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                float sc[U], top = m[g];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float d = 0.f;
+#pragma unroll
+                    for (int i = 0; i < E; ++i) d += q[g][i] * kr[u].at(i);
+                    d = gs::lanes_sum<L>(d);
+                    sc[u] = row[u] >= 0 ? d : -INFINITY;
+                    top = fmaxf(top, sc[u]);
+                }
+                const float ref = top == -INFINITY ? 0.f : top;        // nothing yet: exponentials of -inf, zeros
+                const float keep = gs::fast_exp2(m[g] - ref);
+                m[g] = top;
+                s[g] *= keep;
+#pragma unroll
+                for (int i = 0; i < E; ++i) acc[g][i] *= keep;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float pr = gs::fast_exp2(sc[u] - ref);
+                    s[g] += pr;
+#pragma unroll
+                    for (int i = 0; i < E; ++i) acc[g][i] += pr * (V ? vr[u].at(i) : kr[u].at(i));
+                }
+            }
+        }
+        e = end;
+        const bool complete = begin == sb && end == se;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            if (g >= n_heads) continue;
+            const int64_t o = p * a.heads + h0 + g;
+            if (complete) {
+                const float inv = s[g] > 0.f ? 1.f / s[g] : s[g] == 0.f ? 0.f : s[g];   // (a NaN stays one)
+#pragma unroll
+                for (int i = 0; i < E; ++i) acc[g][i] *= inv;
+                gs::store_row<T, L, ALIGNED>(static_cast<T *>(a.out) + o * a.dim, lane, a.dim, acc[g]);
+                if (lane == 0) a.lse[o] = (m[g] + gs::fast_log2(s[g])) * gs::kLn2;
+            } else {
+                const size_t at = ((size_t)w * 2 + (begin == e0 ? 0 : 1)) * a.heads + h0 + g;
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const int d = gs::element_of<T, L, ALIGNED>(lane, i);
+                    if (d < a.dim) a.piece_acc[at * a.dim + d] = acc[g][i];
+                }
+                if (lane == 0) a.piece_ms[at] = make_float2(m[g], s[g]);
+            }
+        }
+        if (e < e1) p = a.nb.parent_of(e, p + 1);
+    }
+}
+
+// Joins the pieces of the parents that cross a worker's border and writes those without edges.  A block looks at 64
+// parents, far apart (popular parents tend to be neighbors); its four waves take every fourth piece of one.
+template <class T>
+__global__ __launch_bounds__(256)
+void attn_join_kernel(FwdArgs a) {
+    __shared__ float part[4][256 + 2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.y;
+    const int64_t mine = (int64_t)lane * gridDim.x + blockIdx.x;
+    uint32_t b = 0, e = 0;
+    if (mine < a.nb.n_parents) a.nb.range(mine, b, e);
+    unsigned long long todo = __ballot(mine < a.nb.n_parents && (b == e || b / a.chunk != (e - 1) / a.chunk));
+    while (todo) {
+        const int src = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
+        const int64_t p = (int64_t)src * gridDim.x + blockIdx.x;
+        float m = -INFINITY, s = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+        if (se > sb) {
+            const uint32_t first = sb / a.chunk, last = (se - 1) / a.chunk;
+            for (uint32_t w = first + wave; w <= last; w += 4) {
+                const size_t at = ((size_t)w * 2 + (w == first && sb % a.chunk ? 1 : 0)) * a.heads + h;
+                const float2 ms = a.piece_ms[at];
+                const float top = fmaxf(m, ms.x), ref = top == -INFINITY ? 0.f : top;
+                const float ko = gs::fast_exp2(m - ref), kn = gs::fast_exp2(ms.x - ref);
+                if (ms.x == -INFINITY && ms.y == 0.f) continue;         // merged into another piece, or all masked
+                m = top;
+                s = s * ko + ms.y * kn;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (lane + 64 * i < a.dim) acc[i] = acc[i] * ko + a.piece_acc[at * a.dim + lane + 64 * i] * kn;
+            }
+        }
+        __syncthreads();                            // the last parent's parts are read
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = acc[i];
+        if (lane == 0) { part[wave][256] = m; part[wave][257] = s; }
+        __syncthreads();
+        const float top = fmaxf(fmaxf(part[0][256], part[1][256]), fmaxf(part[2][256], part[3][256]));
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, o = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float f = gs::fast_exp2(part[i][256] - ref);
+            sum += part[i][257] * f;
+            o += part[i][threadIdx.x] * f;
+        }
+        const int64_t at = p * a.heads + h;
+        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+        if (threadIdx.x < a.dim) static_cast<T *>(a.out)[at * a.dim + threadIdx.x] = (T)(o * inv);
+        if (threadIdx.x == 0) a.lse[at] = (top + gs::fast_log2(sum)) * gs::kLn2;
+    }
+}
+
+template <class T, int L, bool ALIGNED>
+void launch_fwd(const FwdArgs &a, int64_t workers, hipStream_t stream) {
+    const int share = a.heads / a.kv_heads;
+    FwdArgs b = a;
+    const int g = share >= 3 ? 4 : share;
+    b.parts = (share + g - 1) / g;
+    const dim3 grid((unsigned)((workers * L + gs::kAttnThreads - 1) / gs::kAttnThreads), (unsigned)(a.kv_heads * b.parts));
+    if (g == 1) attn_fwd_kernel<T, L, 1, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
+    else if (g == 2) attn_fwd_kernel<T, L, 2, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
+    else attn_fwd_kernel<T, L, 4, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
+}
+
+template <class T>
+int run_fwd(const FwdArgs &a, const gs::Deal &d, int lanes, bool aligned, hipStream_t stream) {
+    if (d.workers) {
+        if (aligned) {
+            if (lanes == 4) launch_fwd<T, 4, true>(a, d.workers, stream);
+            else if (lanes == 8) launch_fwd<T, 8, true>(a, d.workers, stream);
+            else if (lanes == 16) launch_fwd<T, 16, true>(a, d.workers, stream);
+            else if (lanes == 32) launch_fwd<T, 32, true>(a, d.workers, stream);
+            else launch_fwd<T, 64, true>(a, d.workers, stream);
+        } else {
+            if (lanes == 4) launch_fwd<T, 4, false>(a, d.workers, stream);
+            else if (lanes == 8) launch_fwd<T, 8, false>(a, d.workers, stream);
+            else if (lanes == 16) launch_fwd<T, 16, false>(a, d.workers, stream);
+            else if (lanes == 32) launch_fwd<T, 32, false>(a, d.workers, stream);
+            else launch_fwd<T, 64, false>(a, d.workers, stream);
+        }
+        if (int rc = gs::check_launch("gs_neighbor_attention_fwd")) return rc;
+    }
+    if (!d.whole) {
+        const dim3 grid((unsigned)((a.nb.n_parents + 63) / 64), (unsigned)a.heads);
+        attn_join_kernel<T><<<grid, 256, 0, stream>>>(a);
+        return gs::check_launch("gs_neighbor_attention_fwd (join)");
+    }
+    return GS_OK;
+}
+
+size_t pieces_bytes(const gs::Deal &d, int heads, int dim, size_t *off_acc) {
+    if (d.whole || !d.workers) { if (off_acc) *off_acc = 0; return 0; }
+    const size_t ms = gs::align256((size_t)d.workers * 2 * heads * sizeof(float2));
+    if (off_acc) *off_acc = ms;
+    return ms + (size_t)d.workers * 2 * heads * dim * sizeof(float);
+}
+
+}  // namespace
+
+extern "C" size_t gs_neighbor_attention_workspace(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype) {
+    if (gs::check_neighbors("gs_neighbor_attention_workspace", nb, heads, kv_heads, dim, dtype)) return 0;
+    const gs::Deal d = gs::deal_edges(nb->indptr, nb->n_parents, nb->n_child, nb->n_edges, gs::lanes_for(dim, gs::dtype_size(dtype)));
+    return pieces_bytes(d, heads, dim, nullptr);
+}
+
+extern "C" int gs_neighbor_attention_fwd(const void *q, const void *k, const void *v, const gs_neighbors *nb, int heads,
+                                         int kv_heads, int dim, int dtype, float scale, void *out, float *lse,
+                                         void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = gs::check_neighbors("gs_neighbor_attention_fwd", nb, heads, kv_heads, dim, dtype)) return rc;
+    if (nb->n_parents == 0) return GS_OK;
+    if (!q || !out || !lse || (nb->n_edges && nb->n_rows && !k)) return gs::fail(GS_EINVAL, "gs_neighbor_attention_fwd: null pointer argument");
+    const int size = gs::dtype_size(dtype), lanes = gs::lanes_for(dim, size);
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & (size - 1))
+        return gs::fail(GS_EINVAL, "gs_neighbor_attention_fwd: pointer not aligned to its element");
+    const gs::Deal d = gs::deal_edges(nb->indptr, nb->n_parents, nb->n_child, nb->n_edges, lanes);
+    size_t off_acc = 0;
+    const size_t need = pieces_bytes(d, heads, dim, &off_acc);
+    if (workspace_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 15))))
+        return gs::fail(GS_EINVAL, "gs_neighbor_attention_fwd: aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    FwdArgs a;
+    a.nb = Neighbors{nb->indptr, nb->ids, nb->n_parents, nb->id_offset, nb->n_rows, (uint32_t)(nb->indptr ? 0 : nb->n_child), (uint32_t)nb->n_edges};
+    a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse;
+    a.piece_ms = need ? static_cast<float2 *>(workspace) : nullptr;
+    a.piece_acc = need ? reinterpret_cast<float *>(static_cast<char *>(workspace) + off_acc) : nullptr;
+    a.scale2 = scale * gs::kLog2e;
+    a.heads = heads; a.kv_heads = kv_heads; a.dim = dim; a.chunk = (int)d.chunk; a.parts = 1;
+    const bool aligned = (dim * size) % 16 == 0 && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == GS_F32) return run_fwd<float>(a, d, lanes, aligned, s);
+    if (dtype == GS_BF16) return run_fwd<__bf16>(a, d, lanes, aligned, s);
+    return run_fwd<_Float16>(a, d, lanes, aligned, s);
+}

@@ -1379,3 +1379,184 @@ def stage_batch(seeds, seeds_dst, walk_ids, walk_ids_dst, targets, targets_dst, 
     check(lib.gs_stage_batch(ptr(seeds), ptr(seeds_dst), seeds.numel(), ptr(walk_ids), ptr(walk_ids_dst), walk_ids.numel(),
                              ptr(targets), ptr(targets_dst), targets.numel(), float(lr_t), ptr(lr_dst), stream_handle()),
           'gs_stage_batch')
+
+
+# ---- operators around learning and ranking (include/gsage_ops.h) ------------------------------------------------------
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _table(t, name, dtype=None, shape=None, device=None, ndim=None):
+    """A contiguous float32 / bfloat16 / float16 GPU tensor, of a given type, shape and device where these are set."""
+    if isinstance(t, torch.Tensor) and dtype is None and t.dtype not in _DTYPES:
+        raise TypeError("%s must be float32, bfloat16 or float16 (got %s)" % (name, t.dtype))
+    _dev(t, t.dtype if dtype is None and isinstance(t, torch.Tensor) else dtype, name, ndim)
+    if device is not None and t.device != device:
+        raise ValueError("%s lives on %s, not on %s" % (name, t.device, device))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError("%s must have shape %s (got %s)" % (name, tuple(shape), tuple(t.shape)))
+    return t
+
+
+def _stream_of(device):
+    """The current stream of a tensor's device, which need not be the current device."""
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _scratch(n_bytes, device):
+    return torch.empty(max(int(n_bytes), 1), dtype=torch.uint8, device=device)
+
+
+def dropout(x, rate, seed, offset=0, out=None):
+    """Elements of ``x`` (any shape) dropped at ``rate``, the others divided by the share that is kept; which ones is a
+    function of ``seed``, ``offset`` and the position alone (``gs_dropout``), so the gradient is the same call on the
+    gradient of the result.  ``seed``: a whole number, or an int64 GPU tensor of one element that the kernel reads (a
+    captured graph then draws other masks when the caller changes it).  ``offset`` counts blocks of eight elements that
+    earlier calls under the seed have used.  ``out`` may be ``x``."""
+    lib = load()
+    _table(x, 'x')
+    rate = float(rate)
+    if not 0.0 <= rate or not rate * 65536.0 < 65536.0:
+        raise ValueError("rate must lie in [0, 1) (got %r)" % (rate,))
+    seed_t = seed if isinstance(seed, torch.Tensor) else None
+    if seed_t is not None:
+        _table(seed_t, 'seed', torch.int64, device=x.device)
+        if seed_t.numel() != 1:
+            raise ValueError("seed must have one element")
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        _table(out, 'out', x.dtype, x.shape, x.device)
+    with torch.cuda.device(x.device):
+        check(lib.gs_dropout(ptr(x), x.numel(), _DTYPES[x.dtype], rate,
+                             0 if seed_t is not None else int(seed) & 0xFFFFFFFFFFFFFFFF, ptr(seed_t),
+                             int(offset) & 0xFFFFFFFFFFFFFFFF, ptr(out), _stream_of(x.device)), 'gs_dropout')
+    return out
+
+
+def _neighbors(q, k, v, child_ids, n_child, indptr, id_offset):
+    """Checks the arguments the attention calls share; (gs_neighbors, heads, kv_heads, dim)."""
+    _table(q, 'q', ndim=3)
+    _table(k, 'k', q.dtype, device=q.device, ndim=3)
+    if v is not None:
+        _table(v, 'v', q.dtype, k.shape, q.device)
+    n_parents, heads, dim = q.shape
+    n_rows, kv_heads = k.shape[0], k.shape[1]
+    if k.shape[2] != dim:
+        raise ValueError("queries of %d elements, keys of %d" % (dim, k.shape[2]))
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError("%d heads are no multiple of %d key heads" % (heads, kv_heads))
+    if child_ids is not None:
+        _table(child_ids, 'child_ids', torch.int32, device=q.device)
+    if (indptr is None) == (n_child is None):
+        raise ValueError("either n_child or indptr says which neighbors belong to a parent")
+    if indptr is not None:
+        _table(indptr, 'indptr', torch.int64, (n_parents + 1,), q.device)
+        n_child, n_edges = 0, n_rows if child_ids is None else child_ids.numel()
+    else:
+        n_child = int(n_child)
+        n_edges = n_parents * n_child
+        if n_child < 0:
+            raise ValueError("n_child must not be negative")
+        if child_ids is not None and child_ids.numel() != n_edges:
+            raise ValueError("child_ids has %d entries, %d needed" % (child_ids.numel(), n_edges))
+        if child_ids is None and n_edges > n_rows:
+            raise ValueError("dense groups need n_parents*n_child <= rows of k")
+    # (an empty tensor has no address, but the rows are read by id all the same)
+    ids = None if child_ids is None else ptr(child_ids) or 16
+    nb = _lib.Neighbors(ptr(indptr), n_parents, n_child, ids, n_edges, int(id_offset), n_rows)
+    return nb, heads, kv_heads, dim
+
+
+def neighbor_attention(q, k, v, child_ids, n_child, id_offset=0, scale=None, indptr=None, out=None, lse=None):
+    """Attention of every parent over its neighbors' rows, the aggregation beside ``gather_mean`` and ``gather_max``
+    (``gs_neighbor_attention_fwd``): (out like q, lse float32 [n_parents, heads]).
+
+    q [n_parents, heads, dim]; k, v [n_rows, kv_heads, dim], heads a multiple of kv_heads, v None: the keys are the
+    values; float32, bfloat16 or float16.  Parent p's neighbors are entries ``p*n_child ..`` of ``child_ids``, or, with
+    ``indptr`` (int64 [n_parents + 1]; n_child None), entries ``indptr[p] .. indptr[p+1]``; table row = id - id_offset, an
+    id outside the table is no neighbor.  child_ids None: dense, entry e is row e.  A parent without neighbors gets zeros
+    and an lse of -inf.  ``scale`` defaults to 1 / sqrt(dim)."""
+    lib = load()
+    nb, heads, kv_heads, dim = _neighbors(q, k, v, child_ids, n_child, indptr, id_offset)
+    dev, dt = q.device, _DTYPES[q.dtype]
+    out = torch.empty_like(q) if out is None else _table(out, 'out', q.dtype, q.shape, dev)
+    lse = (torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if lse is None
+           else _table(lse, 'lse', torch.float32, q.shape[:2], dev))
+    with torch.cuda.device(dev):
+        need = lib.gs_neighbor_attention_workspace(nb, heads, kv_heads, dim, dt)
+        ws = _scratch(need, dev) if need else None
+        check(lib.gs_neighbor_attention_fwd(ptr(q), ptr(k), ptr(v), nb, heads, kv_heads, dim, dt,
+                                            dim ** -0.5 if scale is None else float(scale), ptr(out), ptr(lse), ptr(ws), need,
+                                            _stream_of(dev)), 'gs_neighbor_attention_fwd')
+    return out, lse
+
+
+def neighbor_inverse(child_ids, n_rows, id_offset=0):
+    """Which entries of ``child_ids`` read a table row: (int64 [n_rows + 1], int32 [n_entries]) such that row r's are
+    ``edges[indptr[r]:indptr[r+1]]``, in increasing order; entries outside the table come last.  A graph that does not
+    change keeps this beside its adjacency; the gradients of a table read by id take it."""
+    lib = load()
+    _dev(child_ids, torch.int32, 'child_ids')
+    n_rows, n = int(n_rows), child_ids.numel()
+    if n_rows < 0 or max(n_rows + 1, n) >= 2 ** 31:
+        raise ValueError("row and entry counts must fit int32")
+    dev = child_ids.device
+    if torch.cuda.is_current_stream_capturing():
+        raise _lib.GsageError("neighbor_inverse cannot run inside a graph capture: build the lists before it")
+    with torch.cuda.device(dev):
+        row = child_ids.reshape(-1).to(torch.int64) - int(id_offset)
+        row = torch.where((row >= 0) & (row < n_rows), row, n_rows).to(torch.int32)
+        entry = torch.arange(n, dtype=torch.int32, device=dev)
+        n_nodes = max(n_rows + 1, n)
+        need = ctypes.c_size_t(0)
+        check(lib.gs_csr_build_workspace(n, n_nodes, 0, ctypes.byref(need)), 'gs_csr_build_workspace')
+        ws = _scratch(need.value, dev)
+        inv_indptr = torch.empty(n_nodes + 1, dtype=torch.int64, device=dev)
+        inv_edges = torch.empty(n, dtype=torch.int32, device=dev)
+        err = torch.zeros(1, dtype=torch.int32, device=dev)            # (every row and entry above is inside)
+        check(lib.gs_csr_build(ptr(row), ptr(entry), n, 0, n_nodes, ptr(inv_indptr), ptr(inv_edges), ptr(err), 0, ptr(ws),
+                               ws.numel(), _stream_of(dev)), 'gs_csr_build')
+    return inv_indptr[:n_rows + 1], inv_edges
+
+
+def neighbor_attention_bwd(q, k, v, child_ids, n_child, out, lse, g_out, id_offset=0, scale=None, indptr=None, inverse=None,
+                           need_q=True, need_rows=True, g_q=None, g_k=None, g_v=None):
+    """Gradients of ``neighbor_attention`` (``gs_neighbor_attention_bwd``): (g_q, g_k, g_v), g_v None where v is None (g_k
+    then holds both parts).  ``out`` and ``lse`` are what the forward call returned; the probabilities are computed again.
+    With ``child_ids`` the tables' gradients need ``inverse`` (``neighbor_inverse``; built here when it is None, not
+    inside a graph capture).  Destinations may be passed in: every row is written, except dense rows beyond the
+    neighborhoods, which stay as they are."""
+    lib = load()
+    nb, heads, kv_heads, dim = _neighbors(q, k, v, child_ids, n_child, indptr, id_offset)
+    dev, dt = q.device, _DTYPES[q.dtype]
+    _table(out, 'out', q.dtype, q.shape, dev)
+    _table(lse, 'lse', torch.float32, q.shape[:2], dev)
+    _table(g_out, 'g_out', q.dtype, q.shape, dev)
+    inv_indptr = inv_edges = None
+    n_inv = 0
+    if need_rows and child_ids is not None:
+        inv_indptr, inv_edges = neighbor_inverse(child_ids, k.shape[0], id_offset) if inverse is None else inverse
+        _table(inv_indptr, 'inverse[0]', torch.int64, (k.shape[0] + 1,), dev)
+        _table(inv_edges, 'inverse[1]', torch.int32, device=dev, ndim=1)
+        n_inv = inv_edges.numel()
+        if n_inv > child_ids.numel():
+            raise ValueError("inverse lists %d entries, child_ids has %d" % (n_inv, child_ids.numel()))
+
+    def dest(t, like, name):
+        if t is not None:
+            return _table(t, name, like.dtype, like.shape, dev)
+        # dense rows beyond the neighborhoods are not written
+        whole = child_ids is not None or (indptr is None and nb.n_edges == like.shape[0]) or name == 'g_q'
+        return torch.empty_like(like) if whole else torch.zeros_like(like)
+    g_q = dest(g_q, q, 'g_q') if need_q else None
+    g_k = dest(g_k, k, 'g_k') if need_rows else None
+    g_v = dest(g_v, v, 'g_v') if need_rows and v is not None else None
+    with torch.cuda.device(dev):
+        need = lib.gs_neighbor_attention_bwd_workspace(nb, heads, kv_heads, dim, dt, n_inv)
+        ws = _scratch(need, dev)
+        check(lib.gs_neighbor_attention_bwd(ptr(q), ptr(k), ptr(v), nb, heads, kv_heads, dim, dt,
+                                            dim ** -0.5 if scale is None else float(scale), ptr(out), ptr(lse), ptr(g_out),
+                                            ptr(inv_indptr), ptr(inv_edges), n_inv, ptr(g_q), ptr(g_k), ptr(g_v), ptr(ws),
+                                            ws.numel(), _stream_of(dev)), 'gs_neighbor_attention_bwd')
+    return g_q, g_k, g_v
