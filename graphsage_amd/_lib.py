@@ -231,6 +231,11 @@ SIGNATURES_OPS = {
     'gs_neighbor_attention_bwd_workspace': (_sz, [_c.POINTER(Neighbors), _i32, _i32, _i32, _i32, _i64]),
     'gs_neighbor_attention_bwd': (_i32, [_vp, _vp, _vp, _c.POINTER(Neighbors), _i32, _i32, _i32, _i32, _f32, _vp, _vp, _vp,
                                          _vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
+    'gs_catalog_workspace': (_sz, [_i64, _i64, _i32, _i32, _i32]),
+    'gs_catalog_fwd': (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _f32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _sz, _vp]),
+    'gs_catalog_bwd_workspace': (_sz, [_i64, _i64, _i32, _i32]),
+    'gs_catalog_bwd': (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                              _vp]),
 }
 
 _lib = None

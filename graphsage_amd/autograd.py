@@ -169,3 +169,24 @@ class NeighborAttention(torch.autograd.Function):
             q, k, v, child_ids, n_child, out, lse, g.contiguous(), id_offset, scale, indptr, inverse,
             need_q=need[0], need_rows=need[1] or need[2])
         return (g_q, g_k if need[1] else None, g_v if need[2] else None) + (None,) * 6
+
+
+class CatalogLogProbs(torch.autograd.Function):
+    """``kernels.catalog_log_probs``: (log_prob, entropy) of users over a catalog, with gradients to users, items and
+    bias."""
+
+    @staticmethod
+    def forward(ctx, user, item, targets, bias, scale):
+        r = kernels.catalog_log_probs(user, item, targets, bias, scale)
+        ctx.save_for_backward(user, item, targets, bias, r.lse, r.entropy)
+        ctx.scale = scale
+        return r.log_prob, r.entropy
+
+    @staticmethod
+    def backward(ctx, g_log_prob, g_entropy):
+        user, item, targets, bias, lse, entropy = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        g = [None if x is None else x.contiguous() for x in (g_log_prob, g_entropy)]
+        g_user, g_item, g_bias = kernels.catalog_log_probs_bwd(user, item, targets, bias, ctx.scale, lse, entropy, *g,
+                                                               need_user=need[0], need_item=need[1], need_bias=need[3])
+        return g_user, g_item, None, g_bias, None

@@ -1,0 +1,99 @@
+// Users against a catalog of items: operand layout and tile product, shared by the forward and backward kernels.
+//
+// The scores z = scale <user, item> + bias are a matrix product whose result is only ever reduced, so it stays in
+// registers.  All table types run on the bf16 matrix instruction (v_mfma_f32_32x32x16_bf16, fp32 accumulators): an element
+// is cut by truncation into pieces of eight significand bits whose sum it is exactly -- one piece for bf16, two for
+// fp16, three for fp32 -- and the piece products (exact in fp32) of weight 2^-16 and more are added, smallest first: what
+// is left out is below 2^-23 of |user| |item|, the size of one fp32 rounding.
+//
+// Operands are laid out once per call in the order in which lanes use them (one kilobyte per fragment, 16 bytes a
+// lane), rows padded to 32, elements to a multiple of 32, with zeros:
+//   rows layout   fragment (tile, kc, piece): lane l holds row 32 tile + (l & 31), elements 16 kc + 8 (l >> 5) + 0..7
+//   cols layout   fragment (tile, t, db, piece): lane l holds element 32 db + (l & 31) of rows
+//                 32 tile + 16 t + 8 (i >> 2) + 4 (l >> 5) + (i & 3), i = 0..7
+// The product of two row fragments puts the wave's own row (l & 31) in the lane and the streamed row 8 (r >> 2) +
+// 4 (l >> 5) + (r & 3) in register r: a lane keeps its own row's running maximum and sum without talking to other lanes, and
+// eight registers of it ARE the operand of the next product (gradient times streamed rows) whose other operand is a
+// cols fragment -- that is the order of rows inside one.
+//
+// An item whose bias is below kOffer is not on offer: its row is laid out as zeros (whatever it holds) and its score
+// becomes kMasked, far below kFloor where every running maximum starts, so that its exponential is an exact zero.
+#pragma once
+
+#include "ops_common.h"
+
+namespace gs {
+
+constexpr float kOffer = -1e10f;
+constexpr float kFloor = -1e12f;                    // in units of log 2, as all scores in the kernels
+constexpr float kMasked = -1e14f;
+constexpr int kCatThreads = 256;
+
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+
+template <class T> struct Pieces;
+template <> struct Pieces<__bf16>   { static constexpr int P = 1; };
+template <> struct Pieces<_Float16> { static constexpr int P = 2; };
+template <> struct Pieces<float>    { static constexpr int P = 3; };
+inline int pieces_of(int dtype) { return dtype == GS_F32 ? 3 : dtype == GS_F16 ? 2 : 1; }
+
+// Blocks of 32 elements a row is padded to: 1, 2, 4 or 8.
+inline int blocks_of(int dim) { return dim <= 32 ? 1 : dim <= 64 ? 2 : dim <= 128 ? 4 : 8; }
+inline int64_t tiles_of(int64_t rows) { return (rows + 31) / 32; }
+inline size_t layout_bytes(int64_t rows, int dim, int dtype) { return (size_t)tiles_of(rows) * 2 * blocks_of(dim) * pieces_of(dtype) * 1024; }
+
+// Row in a tile of register r of a lane.
+__device__ __forceinline__ int row_of_reg(int r, int lane) { return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
+
+// The next piece of x, as a bf16 in the upper half of the word; x becomes the rest.
+__device__ __forceinline__ uint32_t next_piece(float &x) {
+    const uint32_t hi = __float_as_uint(x) & 0xFFFF0000u;
+    x -= __uint_as_float(hi);
+    return hi;
+}
+
+template <int P> struct Fragment { bf16x8 p[P]; };
+
+// frag: the first fragment of a tile plus this lane's 16 bytes.
+template <int P>
+__device__ __forceinline__ Fragment<P> load_fragment(const uint4 *frag, int index) {
+    Fragment<P> f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const uint4 v = frag[(size_t)(index * P + i) * 64];
+        f.p[i] = *reinterpret_cast<const bf16x8 *>(&v);
+    }
+    return f;
+}
+
+// acc += a b over the pieces whose product counts.
+template <int PA, int PB, int MOST>
+__device__ __forceinline__ void multiply(f32x16 &acc, const bf16x8 *a, const bf16x8 *b) {
+#pragma unroll
+    for (int w = MOST; w >= 0; --w)
+#pragma unroll
+        for (int i = PA - 1; i >= 0; --i)
+            if (w - i >= 0 && w - i < PB) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[w - i], acc, 0, 0, 0);
+}
+
+__device__ __forceinline__ float half_max(float v) {           // the larger of lane l's and lane l ^ 32's
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+}
+
+struct Layout {                                     // one table to lay out
+    const void *x;
+    int64_t n_rows;
+    int dim, blocks;
+    const float *bias;                              // nullable
+    uint4 *rows, *cols;                             // nullable
+    float *bias2;                                   // nullable: bias in units of log 2, or kMasked
+    uint32_t *largest;                              // nullable: the largest |element|, as its bits (zeroed by the first table's launch)
+    uint32_t *clear;                                // nullable: a word to zero
+};
+
+int launch_layout(const Layout &l, int dtype, hipStream_t stream);
+int check_catalog(const char *what, int64_t n_users, int64_t n_items, int dim, int dtype, float scale);
+
+}  // namespace gs

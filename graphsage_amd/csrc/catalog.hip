@@ -1,0 +1,506 @@
+// Log probabilities, entropy and best items of users over a catalog (layout and tile product: catalog.h).
+//
+// A wave keeps the fragments of 32 or 64 users in registers and streams the tiles of its share of the items; per tile the
+// matrix cores give it 32 scores per user, sixteen in each of two lanes, and each lane runs the softmax over its own:
+// a running maximum m, sum s = sum 2^(z - m) and w = sum 2^(z - m) (z - m), z in units of log 2 (scale log2 e goes into one
+// multiply-add).  The shares' (m, s, w) are joined by a second launch: lse = m + log s, entropy = log s - w / s.
+// The score of the target is picked up as its tile passes, so that log_prob is exactly 0 for a catalog of one item.
+//
+// Best items: the first launch also writes the largest score of every tile.  The k best items lie in tiles whose largest
+// score is among the k largest (each of k better tiles would hold a better item), so only about k tiles of a user are
+// scored again, in 64 bits, from the tables themselves; tiles within the rounding error of the first product count as
+// candidates too.  The list is then a function of the tables alone, whatever the product's order of additions.
+#include "catalog.h"
+
+namespace gs {
+
+int check_catalog(const char *what, int64_t n_users, int64_t n_items, int dim, int dtype, float scale) {
+    if (!dtype_size(dtype)) return fail(GS_EINVAL, "%s: dtype %d", what, dtype);
+    if (n_users < 0 || n_items < 0 || dim < 1) return fail(GS_EINVAL, "%s: users=%lld items=%lld dim=%d", what, (long long)n_users, (long long)n_items, dim);
+    if (dim > 256) return fail(GS_ELIMIT, "%s: dim=%d (at most 256)", what, dim);
+    if (n_items >= ((int64_t)1 << 31) - 512 || n_users >= ((int64_t)1 << 31) - 512)
+        return fail(GS_ELIMIT, "%s: %lld users, %lld items (less than 2^31 - 512)", what, (long long)n_users, (long long)n_items);
+    if (!(scale > 0.f) || !(scale < INFINITY)) return fail(GS_EINVAL, "%s: scale %g", what, scale);
+    return GS_OK;
+}
+
+namespace {
+
+// One thread per 16-byte place of a layout; places of the rows layout come first.
+template <class T>
+__global__ __launch_bounds__(kCatThreads)
+void layout_kernel(Layout l, int64_t n_places) {
+    constexpr int P = Pieces<T>::P;
+    if (l.clear && blockIdx.x == 0 && threadIdx.x == 0) l.clear[0] = 0u;
+    const int64_t place = (int64_t)blockIdx.x * kCatThreads + threadIdx.x;
+    const int64_t n_tiles = (l.n_rows + 31) / 32;
+    const int64_t of_rows = l.rows ? n_tiles * l.blocks * 2 * 64 : 0;
+    const T *X = static_cast<const T *>(l.x);
+    const bool cols = place >= of_rows;
+    const int64_t at = cols ? place - of_rows : place;
+    const int lane = (int)(at & 63);
+    const int64_t frag = at >> 6, tile = frag / (l.blocks * 2);
+    const int sub = (int)(frag - tile * (l.blocks * 2));
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        int64_t row;
+        int d;
+        if (!cols) { row = tile * 32 + (lane & 31); d = sub * 16 + (lane >> 5) * 8 + i; }
+        else { row = tile * 32 + (sub / l.blocks) * 16 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3); d = (sub % l.blocks) * 32 + (lane & 31); }
+        const bool in = place < n_places && row < l.n_rows && d < l.dim && !(l.bias && l.bias[row] < kOffer);
+        v[i] = in ? (float)X[row * l.dim + d] : 0.f;
+    }
+    if (l.largest && !cols) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, v[i] == v[i] ? fabsf(v[i]) : INFINITY);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        if ((threadIdx.x & 63) == 0) atomicMax(l.largest, __float_as_uint(top));
+    }
+    if (place >= n_places) return;
+    uint4 *out = (cols ? l.cols : l.rows) + (size_t)frag * P * 64 + lane;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t a = next_piece(v[2 * i]), b = next_piece(v[2 * i + 1]);
+            w[i] = (a >> 16) | b;
+        }
+        out[(size_t)p * 64] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (l.bias2 && !cols && sub == 0 && lane < 32) {
+        const int64_t row = tile * 32 + lane;
+        float b = kMasked;
+        if (row < l.n_rows) b = !l.bias ? 0.f : l.bias[row] < kOffer ? kMasked : l.bias[row] * kLog2e;
+        l.bias2[row] = b;
+    }
+}
+
+}  // namespace
+
+int launch_layout(const Layout &l, int dtype, hipStream_t stream) {
+    const int64_t each = tiles_of(l.n_rows) * l.blocks * 2 * 64, places = each * ((l.rows ? 1 : 0) + (l.cols ? 1 : 0));
+    if (places == 0) return GS_OK;
+    const dim3 grid((unsigned)((places + kCatThreads - 1) / kCatThreads));
+    if (dtype == GS_F32) layout_kernel<float><<<grid, kCatThreads, 0, stream>>>(l, places);
+    else if (dtype == GS_BF16) layout_kernel<__bf16><<<grid, kCatThreads, 0, stream>>>(l, places);
+    else layout_kernel<_Float16><<<grid, kCatThreads, 0, stream>>>(l, places);
+    return check_launch("gs_catalog (layout)");
+}
+
+}  // namespace gs
+
+namespace {
+
+using namespace gs;
+
+constexpr int kMaxTop = 64;
+
+struct FwdArgs {
+    const uint4 *user, *item;                       // rows layouts
+    const float *bias2;
+    const int32_t *targets;
+    float4 *part;                                   // [users][shares]: m, s, w, target's score
+    float *tile_max;                                // [item tiles][user tiles * 32], with TOP
+    int64_t n_users, n_items;
+    int user_tiles, item_tiles, groups, shares, tiles_per_share;
+    float scale2;
+};
+
+template <int P, int DB, int OF, bool TOP>
+__global__ __launch_bounds__(kCatThreads)
+void catalog_fwd_kernel(FwdArgs a) {
+    constexpr int KC = 2 * DB;
+    const int lane = threadIdx.x & 63;
+    const int64_t task = (int64_t)blockIdx.x * (kCatThreads / 64) + (threadIdx.x >> 6);
+    if (task >= (int64_t)a.groups * a.shares) return;
+    const int group = (int)(task % a.groups), share = (int)(task / a.groups);
+    const int t0 = share * a.tiles_per_share, t1 = min(t0 + a.tiles_per_share, a.item_tiles);
+
+    Fragment<P> own[OF][KC];
+    float m[OF], s[OF], w[OF], hit[OF];
+    int target[OF];
+#pragma unroll
+    for (int f = 0; f < OF; ++f) {
+        const int tile = min(group * OF + f, a.user_tiles - 1);            // (a tile past the end repeats the last one)
+        const uint4 *src = a.user + (size_t)tile * KC * P * 64 + lane;
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) own[f][kc] = load_fragment<P>(src, kc);
+        const int64_t n = (int64_t)tile * 32 + (lane & 31);
+        target[f] = a.targets && n < a.n_users ? a.targets[n] : -1;
+        if (target[f] >= a.n_items) target[f] = -1;
+        m[f] = kFloor;
+        s[f] = w[f] = 0.f;
+        hit[f] = -INFINITY;
+    }
+    for (int t = t0; t < t1; ++t) {
+        const uint4 *src = a.item + (size_t)t * KC * P * 64 + lane;
+        f32x16 acc[OF];
+#pragma unroll
+        for (int f = 0; f < OF; ++f)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[f][r] = 0.f;
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+            const Fragment<P> it = load_fragment<P>(src, kc);
+#pragma unroll
+            for (int f = 0; f < OF; ++f) multiply<P, P, 2>(acc[f], it.p, own[f][kc].p);
+        }
+        float b[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<float4 *>(b + 4 * g) = *reinterpret_cast<const float4 *>(a.bias2 + (size_t)t * 32 + 8 * g + 4 * (lane >> 5));
+#pragma unroll
+        for (int f = 0; f < OF; ++f) {
+            float z[16], top = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                z[r] = __builtin_fmaf(acc[f][r], a.scale2, b[r]);
+                top = fmaxf(top, z[r]);
+            }
+            const int local = target[f] - t * 32;
+            if (__any(target[f] >= 0 && (unsigned)local < 32u))
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (target[f] >= 0 && local == row_of_reg(r, lane)) hit[f] = z[r];
+            if (TOP) {
+                const float both = half_max(top);
+                const int tile = group * OF + f;
+                if (lane < 32 && tile < a.user_tiles) a.tile_max[(size_t)t * a.user_tiles * 32 + tile * 32 + lane] = both;
+            }
+            if (__any(top > m[f])) {
+                const float m1 = fmaxf(m[f], top), step = m[f] - m1, keep = fast_exp2(step);
+                w[f] = keep * (w[f] + s[f] * step);
+                s[f] *= keep;
+                m[f] = m1;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float d = z[r] - m[f], p = fast_exp2(d);
+                s[f] += p;
+                w[f] = __builtin_fmaf(p, d, w[f]);
+            }
+        }
+    }
+#pragma unroll
+    for (int f = 0; f < OF; ++f) {
+        const int tile = group * OF + f;
+        // the two lanes of a user
+        const float m1 = half_max(m[f]), step = m[f] - m1, keep = fast_exp2(step);
+        const float s1 = s[f] * keep, w1 = keep * (w[f] + s[f] * step);
+        const float s2 = s1 + __shfl_xor(s1, 32, 64), w2 = w1 + __shfl_xor(w1, 32, 64);
+        const float hit1 = half_max(hit[f]);
+        const int64_t n = (int64_t)tile * 32 + lane;
+        if (lane < 32 && tile < a.user_tiles && n < a.n_users) a.part[(size_t)n * a.shares + share] = make_float4(m1, s2, w2, hit1);
+    }
+}
+
+// One wave per user joins the shares.
+__global__ __launch_bounds__(kCatThreads)
+void catalog_join_kernel(const float4 *part, int shares, int64_t n_users, int64_t n_items, const int32_t *targets,
+                         float *log_prob, float *entropy, float *lse) {
+    const int lane = threadIdx.x & 63;
+    const int64_t n = (int64_t)blockIdx.x * (kCatThreads / 64) + (threadIdx.x >> 6);
+    if (n >= n_users) return;
+    float m = kFloor, s = 0.f, w = 0.f, hit = -INFINITY;
+    for (int i = lane; i < shares; i += 64) {
+        const float4 q = part[(size_t)n * shares + i];
+        const float m1 = fmaxf(m, q.x), da = m - m1, db = q.x - m1, fa = fast_exp2(da), fb = fast_exp2(db);
+        w = fa * (w + s * da) + fb * (q.z + q.y * db);
+        s = s * fa + q.y * fb;
+        m = m1;
+        hit = fmaxf(hit, q.w);
+    }
+    float top = m;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float d = m - top, f = fast_exp2(d);
+    w = f * (w + s * d);
+    s *= f;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        s += __shfl_xor(s, o, 64);
+        w += __shfl_xor(w, o, 64);
+        hit = fmaxf(hit, __shfl_xor(hit, o, 64));
+    }
+    if (lane) return;
+    const float l2 = fast_log2(s);                  // s 0: nothing on offer
+    if (lse) lse[n] = s == 0.f ? -INFINITY : (top + l2) * kLn2;
+    if (entropy) entropy[n] = s == 0.f ? 0.f : (l2 - w / s) * kLn2;
+    if (log_prob) {
+        const bool there = targets && targets[n] >= 0 && targets[n] < n_items;
+        log_prob[n] = !there ? 0.f : s != s ? s : hit < kFloor ? -INFINITY : (hit - (top + l2)) * kLn2;
+    }
+}
+
+struct TopArgs {
+    const void *user, *item;
+    const float *bias, *tile_max, *lse;
+    const uint32_t *largest;
+    int64_t n_users, n_items;
+    int dim, item_tiles, stride, k;
+    float scale;
+    float *top_log_prob;
+    int32_t *top_ids;
+};
+
+// One block per user.  Thresholds and candidates: see the head of the file.
+template <class T>
+__global__ __launch_bounds__(256)
+void catalog_top_kernel(TopArgs a) {
+    constexpr int kBuf = 1024;
+    __shared__ double user[256];
+    __shared__ double val[kBuf];
+    __shared__ int32_t id[kBuf];
+    __shared__ double best_val[kMaxTop];
+    __shared__ int32_t best_id[kMaxTop];
+    __shared__ float group_max[256];
+    __shared__ int32_t cand[512];
+    __shared__ int n_val, n_cand;
+    __shared__ float low;
+    const int tid = threadIdx.x;
+    const int64_t n = blockIdx.x;
+    const float *tm = a.tile_max + n;
+    const T *U = static_cast<const T *>(a.user) + n * a.dim, *I = static_cast<const T *>(a.item);
+    for (int d = tid; d < a.dim; d += 256) user[d] = (double)(float)U[d];
+    float top = -INFINITY;
+    for (int t = tid; t < a.item_tiles; t += 256) top = fmaxf(top, tm[(size_t)t * a.stride]);
+    group_max[tid] = top;
+    if (tid == 0) { n_val = 0; n_cand = 0; low = -INFINITY; }
+    __syncthreads();
+    // the k-th largest of 256 groups' maxima: at least k tiles reach it
+    int rank = 0;
+    for (int i = 0; i < 256; ++i) rank += group_max[i] > top || (group_max[i] == top && i < tid);
+    if (rank == a.k - 1) low = top;
+    __syncthreads();
+    double norm = 0.0;
+    for (int d = 0; d < a.dim; ++d) norm += user[d] * user[d];
+    // |z - its product in the matrix cores| <= (terms) 2^-23 sum |user| |item|, sum |user| |item| <= |user| sqrt(dim) max |item|
+    const double most = sqrt(norm) * sqrt((double)a.dim) * (double)__uint_as_float(a.largest[0]) * (double)a.scale;
+    const double z_low = (double)low * (double)kLn2;
+    const double margin = (6.0 * 256 + 16) * 0x1p-23 * most + 0x1p-20 * (fabs(z_low) + most);
+    double thr = low > kFloor ? z_low - margin : -INFINITY;
+    if (thr != thr) thr = -INFINITY;
+
+    const auto better = [](double v, int32_t i, double w, int32_t j) { return v > w || (v == w && i < j); };
+    // keeps the k best of the buffer, in order
+    const auto compress = [&]() {
+        __syncthreads();
+        const int c = n_val;
+        for (int i = tid; i < c; i += 256) {
+            int r = 0;
+            for (int j = 0; j < c; ++j) r += better(val[j], id[j], val[i], id[i]);
+            if (r < a.k) { best_val[r] = val[i]; best_id[r] = id[i]; }
+        }
+        __syncthreads();
+        const int kept = min(c, a.k);
+        if (tid < kept) { val[tid] = best_val[tid]; id[tid] = best_id[tid]; }
+        if (tid == 0) n_val = kept;
+        __syncthreads();
+        if (kept == a.k && val[a.k - 1] > thr) thr = val[a.k - 1];
+    };
+    const float thr_tile = (float)(thr * (1.0 / (double)kLn2));
+    const float thr_down = thr == -INFINITY ? -INFINITY : thr_tile - fabsf(thr_tile) * 0x1p-20f;
+    for (int t0 = 0; t0 < a.item_tiles; t0 += 256) {
+        const int t = t0 + tid;
+        if (t < a.item_tiles && !(tm[(size_t)t * a.stride] < thr_down)) cand[atomicAdd(&n_cand, 1)] = t;
+        __syncthreads();
+        int left = n_cand;
+        const bool final_round = t0 + 256 >= a.item_tiles;
+        while (left >= 8 || (final_round && left > 0)) {
+            const int take = min(left, 8);
+            left -= take;
+            const int slot = tid >> 5;
+            if (slot < take) {
+                const int64_t j = (int64_t)cand[left + slot] * 32 + (tid & 31);
+                const float b = j < a.n_items && a.bias ? a.bias[j] : 0.f;
+                if (j < a.n_items && !(b < kOffer)) {
+                    double dot = 0.0;
+                    for (int d = 0; d < a.dim; ++d) dot += user[d] * (double)(float)I[j * a.dim + d];
+                    const double z = dot * (double)a.scale + (double)b;
+                    if (z >= thr && z > -INFINITY) {
+                        const int at = atomicAdd(&n_val, 1);
+                        val[at] = z;
+                        id[at] = (int32_t)j;
+                    }
+                }
+            }
+            __syncthreads();
+            const bool full = n_val > kBuf - 256;
+            __syncthreads();                        // everybody has looked before anybody adds
+            if (full) compress();
+        }
+        __syncthreads();
+        if (tid == 0) n_cand = left;
+        __syncthreads();
+    }
+    compress();
+    if (tid < a.k) {
+        const bool has = tid < n_val;
+        a.top_log_prob[n * a.k + tid] = has ? (float)(val[tid] - (double)a.lse[n]) : -INFINITY;
+        a.top_ids[n * a.k + tid] = has ? id[tid] : -1;
+    }
+}
+
+// How a call is cut: users in slices that bound the table of tile maxima, a slice in waves.
+struct Cut {
+    int64_t slice;                                  // users per slice
+    int of;
+};
+
+Cut cut_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
+    Cut c;
+    const int regs = pieces_of(dtype) * blocks_of(dim);                   // registers of a fragment row: 8 each
+    c.of = n_users > 32 && regs <= 8 ? 2 : 1;
+    c.slice = n_users;
+    if (top_k > 0) {
+        const int64_t most = ((int64_t)1 << 26) / (tiles_of(n_items) ? tiles_of(n_items) : 1) / 256 * 256;
+        if (c.slice > most) c.slice = most < 256 ? 256 : most;
+    }
+    return c;
+}
+
+constexpr int64_t kWaves = 4096;                    // waves a launch is cut into: four per SIMD
+
+void shares_of(int64_t users, int64_t n_items, int of, int *groups, int *shares, int *per_share) {
+    const int64_t ut = tiles_of(users), it = tiles_of(n_items);
+    *groups = (int)((ut + of - 1) / of);
+    int64_t sh = kWaves / *groups;
+    if (sh > it / 2) sh = it / 2;
+    if (sh < 1) sh = 1;
+    *per_share = it ? (int)((it + sh - 1) / sh) : 1;
+    *shares = (int)((it + *per_share - 1) / *per_share);
+}
+
+struct Space {
+    size_t user, item, bias2, part, lse, tile_max, words, total;
+};
+
+Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
+    Space s;
+    const Cut c = cut_of(n_users, n_items, dim, dtype, top_k);
+    int groups, shares, per;
+    shares_of(c.slice, n_items, c.of, &groups, &shares, &per);
+    size_t off = 0;
+    s.words = off; off += 256;
+    s.user = off; off += align256(layout_bytes(c.slice, dim, dtype));
+    s.item = off; off += align256(layout_bytes(n_items, dim, dtype));
+    s.bias2 = off; off += align256((size_t)tiles_of(n_items) * 32 * sizeof(float));
+    s.part = off;
+    // the last slice may be smaller and have more shares: the product of both is bounded by the waves
+    off += align256((size_t)(c.slice * (int64_t)shares + kWaves * 64) * sizeof(float4));
+    s.lse = off; off += align256((size_t)c.slice * sizeof(float));
+    s.tile_max = off;
+    if (top_k > 0) off += (size_t)tiles_of(n_items) * tiles_of(c.slice) * 32 * sizeof(float);
+    s.total = off;
+    return s;
+}
+
+template <int P, int DB, int OF>
+void launch_tile(const FwdArgs &a, hipStream_t stream) {
+    const dim3 grid((unsigned)(((int64_t)a.groups * a.shares + kCatThreads / 64 - 1) / (kCatThreads / 64)));
+    if (a.tile_max) catalog_fwd_kernel<P, DB, OF, true><<<grid, kCatThreads, 0, stream>>>(a);
+    else catalog_fwd_kernel<P, DB, OF, false><<<grid, kCatThreads, 0, stream>>>(a);
+}
+
+template <int P>
+void launch_fwd(const FwdArgs &a, int blocks, int of, hipStream_t stream) {
+    if (of == 2) {
+        if (blocks == 1) launch_tile<P, 1, 2>(a, stream);
+        else if (blocks == 2) launch_tile<P, 2, 2>(a, stream);
+        else if constexpr (P * 4 <= 8) {
+            if (blocks == 4) launch_tile<P, 4, 2>(a, stream);
+            else if constexpr (P == 1) launch_tile<P, 8, 2>(a, stream);
+        }
+        return;
+    }
+    if (blocks == 1) launch_tile<P, 1, 1>(a, stream);
+    else if (blocks == 2) launch_tile<P, 2, 1>(a, stream);
+    else if (blocks == 4) launch_tile<P, 4, 1>(a, stream);
+    else launch_tile<P, 8, 1>(a, stream);
+}
+
+}  // namespace
+
+extern "C" size_t gs_catalog_workspace(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
+    if (gs::check_catalog("gs_catalog_workspace", n_users, n_items, dim, dtype, 1.f)) return 0;
+    if (top_k < 0 || top_k > kMaxTop) { gs::fail(GS_ELIMIT, "gs_catalog_workspace: top_k=%d (at most %d)", top_k, kMaxTop); return 0; }
+    if (n_users == 0) return 0;
+    return space_of(n_users, n_items, dim, dtype, top_k).total;
+}
+
+extern "C" int gs_catalog_fwd(const void *user, int64_t n_users, const void *item, int64_t n_items, int dim, int dtype,
+                              const float *bias, float scale, const int32_t *targets, float *log_prob, float *entropy,
+                              float *lse, int top_k, float *top_log_prob, int32_t *top_ids, void *workspace,
+                              size_t workspace_bytes, void *stream) {
+    const char *what = "gs_catalog_fwd";
+    if (int rc = gs::check_catalog(what, n_users, n_items, dim, dtype, scale)) return rc;
+    if (top_k < 0) return gs::fail(GS_EINVAL, "%s: top_k=%d", what, top_k);
+    if (top_k > kMaxTop) return gs::fail(GS_ELIMIT, "%s: top_k=%d (at most %d)", what, top_k, kMaxTop);
+    if (n_users == 0) return GS_OK;
+    if (!user || (n_items && !item) || (top_k && (!top_log_prob || !top_ids)))
+        return gs::fail(GS_EINVAL, "%s: null pointer argument", what);
+    const int size = gs::dtype_size(dtype);
+    if (((uintptr_t)user | (uintptr_t)item) & (size - 1)) return gs::fail(GS_EINVAL, "%s: pointer not aligned to its element", what);
+    const Space sp = space_of(n_users, n_items, dim, dtype, top_k);
+    if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < sp.total)
+        return gs::fail(GS_EINVAL, "%s: 256-byte aligned workspace of %zu bytes needed, %zu given", what, sp.total, workspace_bytes);
+    const Cut cut = cut_of(n_users, n_items, dim, dtype, top_k);
+    char *ws = static_cast<char *>(workspace);
+    hipStream_t s = (hipStream_t)stream;
+    const int blocks = gs::blocks_of(dim), pieces = gs::pieces_of(dtype);
+    uint32_t *words = reinterpret_cast<uint32_t *>(ws + sp.words);
+    for (int64_t u0 = 0; u0 < n_users; u0 += cut.slice) {
+        const int64_t nu = n_users - u0 < cut.slice ? n_users - u0 : cut.slice;
+        gs::Layout l{};
+        l.x = static_cast<const char *>(user) + (size_t)u0 * dim * size;
+        l.n_rows = nu; l.dim = dim; l.blocks = blocks;
+        l.rows = reinterpret_cast<uint4 *>(ws + sp.user);
+        l.clear = u0 == 0 ? words : nullptr;
+        if (int rc = gs::launch_layout(l, dtype, s)) return rc;
+        if (u0 == 0) {
+            l = gs::Layout{};
+            l.x = item; l.n_rows = n_items; l.dim = dim; l.blocks = blocks; l.bias = bias;
+            l.rows = reinterpret_cast<uint4 *>(ws + sp.item);
+            l.bias2 = reinterpret_cast<float *>(ws + sp.bias2);
+            l.largest = top_k ? words : nullptr;
+            if (int rc = gs::launch_layout(l, dtype, s)) return rc;
+        }
+        FwdArgs a;
+        a.user = reinterpret_cast<const uint4 *>(ws + sp.user);
+        a.item = reinterpret_cast<const uint4 *>(ws + sp.item);
+        a.bias2 = reinterpret_cast<const float *>(ws + sp.bias2);
+        a.targets = targets ? targets + u0 : nullptr;
+        a.part = reinterpret_cast<float4 *>(ws + sp.part);
+        a.tile_max = top_k ? reinterpret_cast<float *>(ws + sp.tile_max) : nullptr;
+        a.n_users = nu; a.n_items = n_items;
+        a.user_tiles = (int)gs::tiles_of(nu); a.item_tiles = (int)gs::tiles_of(n_items);
+        shares_of(nu, n_items, cut.of, &a.groups, &a.shares, &a.tiles_per_share);
+        a.scale2 = scale * gs::kLog2e;
+        if (n_items == 0) a.shares = 0;
+        else {
+            if (pieces == 1) launch_fwd<1>(a, blocks, cut.of, s);
+            else if (pieces == 2) launch_fwd<2>(a, blocks, cut.of, s);
+            else launch_fwd<3>(a, blocks, cut.of, s);
+            if (int rc = gs::check_launch(what)) return rc;
+        }
+        float *lse_out = lse ? lse + u0 : reinterpret_cast<float *>(ws + sp.lse);
+        catalog_join_kernel<<<dim3((unsigned)((nu + 3) / 4)), gs::kCatThreads, 0, s>>>(
+            a.part, a.shares, nu, n_items, a.targets, log_prob ? log_prob + u0 : nullptr, entropy ? entropy + u0 : nullptr, lse_out);
+        if (int rc = gs::check_launch("gs_catalog_fwd (join)")) return rc;
+        if (!top_k) continue;
+        TopArgs t;
+        t.user = static_cast<const char *>(user) + (size_t)u0 * dim * size;
+        t.item = item; t.bias = bias; t.tile_max = a.tile_max; t.lse = lse_out; t.largest = words;
+        t.n_users = nu; t.n_items = n_items; t.dim = dim; t.item_tiles = a.item_tiles; t.stride = a.user_tiles * 32; t.k = top_k;
+        t.scale = scale; t.top_log_prob = top_log_prob + u0 * top_k; t.top_ids = top_ids + u0 * top_k;
+        if (dtype == GS_F32) catalog_top_kernel<float><<<dim3((unsigned)nu), 256, 0, s>>>(t);
+        else if (dtype == GS_BF16) catalog_top_kernel<__bf16><<<dim3((unsigned)nu), 256, 0, s>>>(t);
+        else catalog_top_kernel<_Float16><<<dim3((unsigned)nu), 256, 0, s>>>(t);
+        if (int rc = gs::check_launch("gs_catalog_fwd (best items)")) return rc;
+    }
+    return GS_OK;
+}

@@ -5,6 +5,7 @@ device, dtype, contiguity and shapes on the host (a kernel that is handed a
 shape it does not expect faults the GPU), then passes raw pointers and the
 current HIP stream to ``libgsage.so``.  Nothing in this file computes.
 """
+import collections
 import ctypes
 import os
 
@@ -1560,3 +1561,74 @@ def neighbor_attention_bwd(q, k, v, child_ids, n_child, out, lse, g_out, id_offs
                                             ptr(inv_indptr), ptr(inv_edges), n_inv, ptr(g_q), ptr(g_k), ptr(g_v), ptr(ws),
                                             ws.numel(), _stream_of(dev)), 'gs_neighbor_attention_bwd')
     return g_q, g_k, g_v
+
+
+CatalogLogProbs = collections.namedtuple('CatalogLogProbs', 'log_prob, entropy, lse, top_log_prob, top_ids')
+
+
+def _catalog(user, item, targets, bias, scale):
+    """Checks the arguments the catalog calls share; (n_users, n_items, dim)."""
+    _table(user, 'user', ndim=2)
+    _table(item, 'item', user.dtype, device=user.device, ndim=2)
+    if user.shape[1] != item.shape[1]:
+        raise ValueError("users of %d elements, items of %d" % (user.shape[1], item.shape[1]))
+    if targets is not None:
+        _table(targets, 'targets', torch.int32, (user.shape[0],), user.device)
+    if bias is not None:
+        _table(bias, 'bias', torch.float32, (item.shape[0],), user.device)
+    if not 0.0 < float(scale) < float('inf'):
+        raise ValueError("scale must be positive and finite (got %r)" % (scale,))
+    return user.shape[0], item.shape[0], user.shape[1]
+
+
+def catalog_log_probs(user, item, targets=None, bias=None, scale=1.0, top_k=0):
+    """Every user against every item, ``z = scale * user @ item.T + bias``, without the scores ever passing through memory
+    (``gs_catalog_fwd``): a ``CatalogLogProbs`` of log_prob [n_users] (of ``targets``, int32; outside the catalog: no
+    target, 0; None without targets), entropy [n_users], lse [n_users], and the ``top_k`` best items: top_log_prob,
+    top_ids [n_users, top_k] (the scores compared in 64 bits, the lower index first where two are equal; -inf / -1 beyond the items
+    on offer; None without top_k).
+
+    user [n_users, dim], item [n_items, dim]: float32, bfloat16 or float16.  ``bias`` float32 [n_items], for instance
+    minus the logarithm of how often an item is drawn; an item whose bias is below -1e10 (-inf, the type's lowest value)
+    is not on offer and its row is never looked at.  A user for whom nothing is on offer has an lse of -inf and an
+    entropy of 0; a target that is not on offer a log_prob of -inf."""
+    lib = load()
+    n, v, d = _catalog(user, item, targets, bias, scale)
+    top_k = int(top_k)
+    if top_k < 0:
+        raise ValueError("top_k must not be negative")
+    dev, dt = user.device, _DTYPES[user.dtype]
+    row = lambda *shape, t=torch.float32: torch.empty(shape, dtype=t, device=dev)
+    log_prob = None if targets is None else row(n)
+    entropy, lse = row(n), row(n)
+    top_log_prob, top_ids = (row(n, top_k), row(n, top_k, t=torch.int32)) if top_k else (None, None)
+    with torch.cuda.device(dev):
+        ws = _scratch(lib.gs_catalog_workspace(n, v, d, dt, top_k), dev)
+        check(lib.gs_catalog_fwd(ptr(user), n, ptr(item), v, d, dt, ptr(bias), float(scale), ptr(targets), ptr(log_prob),
+                                 ptr(entropy), ptr(lse), top_k, ptr(top_log_prob), ptr(top_ids), ptr(ws), ws.numel(),
+                                 _stream_of(dev)), 'gs_catalog_fwd')
+    return CatalogLogProbs(log_prob, entropy, lse, top_log_prob, top_ids)
+
+
+def catalog_log_probs_bwd(user, item, targets, bias, scale, lse, entropy, g_log_prob=None, g_entropy=None, need_user=True,
+                          need_item=True, need_bias=True):
+    """Gradients of ``catalog_log_probs`` for those of log_prob and entropy (float32 [n_users] or None), with what the
+    forward call returned: (g_user, g_item, g_bias), None where not wanted (g_bias also without bias).  An item that is
+    not on offer gets zeros."""
+    lib = load()
+    n, v, d = _catalog(user, item, targets, bias, scale)
+    dev, dt = user.device, _DTYPES[user.dtype]
+    for t, name in ((lse, 'lse'), (entropy, 'entropy'), (g_log_prob, 'g_log_prob'), (g_entropy, 'g_entropy')):
+        if t is not None:
+            _table(t, name, torch.float32, (n,), dev)
+    if lse is None or (g_entropy is not None and entropy is None):
+        raise ValueError("lse is needed, and entropy for the gradient of the entropy")
+    g_user = torch.empty_like(user) if need_user else None
+    g_item = torch.empty_like(item) if need_item else None
+    g_bias = torch.empty_like(bias) if need_bias and bias is not None else None
+    with torch.cuda.device(dev):
+        ws = _scratch(lib.gs_catalog_bwd_workspace(n, v, d, dt), dev)
+        check(lib.gs_catalog_bwd(ptr(user), n, ptr(item), v, d, dt, ptr(bias), float(scale), ptr(targets), ptr(lse),
+                                 ptr(entropy), ptr(g_log_prob), ptr(g_entropy), ptr(g_user), ptr(g_item), ptr(g_bias), ptr(ws),
+                                 ws.numel(), _stream_of(dev)), 'gs_catalog_bwd')
+    return g_user, g_item, g_bias

@@ -102,8 +102,8 @@ int gs_neighbor_attention_bwd(const void *q, const void *k, const void *v, const
  * and the top_k items by z, the scores compared in 64 bits, the lower index first where two
  * are equal.  The scores never pass through memory.
  *   user device [n_users][dim], item device [n_items][dim] of `dtype`
- *   bias     nullable device float[n_items]; -inf: the item is not on offer, and its
- *            row is never looked at.  A user for whom nothing is on offer: lse -inf, entropy 0
+ *   bias     nullable device float[n_items]; below -1e10 (-inf, the type's lowest value): the item is
+ *            not on offer, and its row is never looked at.  A user for whom nothing is on offer: lse -inf, entropy 0
  *   targets  nullable device int32[n_users]; outside [0, n_items): no target, log_prob 0;
  *            a target that is not on offer: log_prob -inf
  *   log_prob, entropy, lse  device float[n_users], each nullable
