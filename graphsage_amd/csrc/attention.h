@@ -10,7 +10,8 @@
 // over the chip and short lists cost no idle lanes.  Parents with at most a fixed number of neighbors each are dealt
 // whole (C a multiple of their n_child) and leave no pieces.  A parent that lies in one worker is finished there; for one that
 // crosses a border every worker leaves a piece (maximum, sum, unnormalised row) in the workspace and a second launch
-// joins them in worker order.  The result depends on C, which depends on the sizes only.
+// joins them in worker order; a wave that lies inside one parent joins its workers' pieces in registers first and leaves
+// one (a list of 20 000: 312 pieces instead of 1250).  The result depends on C, which depends on the sizes only.
 #pragma once
 
 #include "ops_common.h"
@@ -18,7 +19,7 @@
 namespace gs {
 
 constexpr int kAttnThreads = 256;
-constexpr int kAttnRows = 8;                        // rows a worker has in flight
+constexpr int kAttnRows = 8;                        // rows a worker has in flight, at most
 
 struct Neighbors {
     const int64_t *indptr;
@@ -45,11 +46,40 @@ struct Neighbors {
         return lo;
     }
     // table row of edge e, or -1
-    __device__ __forceinline__ int64_t row_of(uint32_t e) const {
+    __device__ __forceinline__ int32_t row_of(uint32_t e) const {
         const int64_t r = ids ? (int64_t)ids[e] - id_offset : (int64_t)e;
-        return (uint64_t)r < (uint64_t)n_rows ? r : -1;
+        return (uint64_t)r < (uint64_t)n_rows ? (int32_t)r : -1;
     }
 };
+
+// The pieces of a parent with edges [b, e) that crosses a worker's border, in order: the workers of a wave that is only
+// partly inside, one piece for each wave that lies inside (left by its first worker), the workers of the last wave.
+struct PieceList {
+    uint32_t first, n_head, n_full, full0, n_tail, tail0, cut;
+    __device__ __forceinline__ PieceList(uint32_t b, uint32_t e, uint32_t chunk, uint32_t per_wave) {
+        const uint32_t span = chunk * per_wave, a = (b + span - 1) / span, z = e / span;
+        first = b / chunk;
+        cut = b % chunk;                            // not 0: the first piece lies in its worker's second place
+        if (z > a && per_wave > 1) {
+            n_head = a * per_wave - first;
+            n_full = z - a;
+            full0 = a * per_wave;
+            tail0 = z * per_wave;
+            n_tail = e > z * span ? (e - 1) / chunk - tail0 + 1 : 0;
+        } else { n_head = (e - 1) / chunk - first + 1; n_full = n_tail = full0 = tail0 = 0; }
+        step = per_wave;
+    }
+    uint32_t step;
+    __device__ __forceinline__ uint32_t count() const { return n_head + n_full + n_tail; }
+    // place (worker * 2 + 0 or 1) of piece i
+    __device__ __forceinline__ size_t place(uint32_t i) const {
+        if (i < n_head) return (size_t)(first + i) * 2 + (i == 0 && cut ? 1 : 0);
+        if (i < n_head + n_full) return (size_t)(full0 + (i - n_head) * step) * 2;
+        return (size_t)(tail0 + (i - n_head - n_full)) * 2;
+    }
+};
+
+constexpr int kJoinWaves = 8;
 
 // 16 bytes of a row per lane, as they arrive.
 template <class T, int L, bool ALIGNED> struct RowPart {

@@ -15,8 +15,9 @@ int check_neighbors(const char *what, const gs_neighbors *nb, int heads, int kv_
         return fail(GS_EINVAL, "%s: parents=%lld edges=%lld rows=%lld heads=%d kv_heads=%d dim=%d", what,
                     (long long)nb->n_parents, (long long)nb->n_edges, (long long)nb->n_rows, heads, kv_heads, dim);
     if (dim > 256 || heads > 1024) return fail(GS_ELIMIT, "%s: dim=%d (at most 256), heads=%d (at most 1024)", what, dim, heads);
-    if (nb->n_edges >= (int64_t)1 << 31 || nb->n_parents >= (int64_t)1 << 31)
-        return fail(GS_ELIMIT, "%s: %lld edges, %lld parents (less than 2^31)", what, (long long)nb->n_edges, (long long)nb->n_parents);
+    if (nb->n_edges >= (int64_t)1 << 31 || nb->n_parents >= (int64_t)1 << 31 || nb->n_rows >= (int64_t)1 << 31)
+        return fail(GS_ELIMIT, "%s: %lld edges, %lld parents, %lld rows (less than 2^31)", what, (long long)nb->n_edges,
+                    (long long)nb->n_parents, (long long)nb->n_rows);
     if (!nb->indptr && (nb->n_child < 0 || nb->n_child >= (int64_t)1 << 31 || nb->n_parents * nb->n_child != nb->n_edges))
         return fail(GS_EINVAL, "%s: %lld edges for %lld parents of %lld", what, (long long)nb->n_edges, (long long)nb->n_parents,
                     (long long)nb->n_child);
@@ -44,7 +45,8 @@ struct FwdArgs {
 template <class T, int L, int G, bool ALIGNED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_fwd_kernel(FwdArgs a) {
-    constexpr int E = gs::Pack<T>::E, U = gs::kAttnRows;
+    constexpr int E = gs::Pack<T>::E, U = G * E >= 32 ? gs::kAttnRows / 2 : gs::kAttnRows;
+    constexpr uint32_t W = 64 / L;                  // workers per wave
     const int lane = threadIdx.x & (L - 1);
     const uint32_t w = blockIdx.x * (gs::kAttnThreads / L) + threadIdx.x / L;
     const int share = a.heads / a.kv_heads;
@@ -53,10 +55,6 @@ void attn_fwd_kernel(FwdArgs a) {
     const uint32_t C = a.chunk, e0 = min((uint64_t)w * C, (uint64_t)a.nb.n_edges), e1 = min((uint64_t)e0 + C, (uint64_t)a.nb.n_edges);
     const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = a.v ? static_cast<const T *>(a.v) + (int64_t)j * a.dim : nullptr;
     const int64_t stride = (int64_t)a.kv_heads * a.dim;
-
-    if (e0 < e1 && a.piece_ms)                      // no piece yet in either place
-        for (int i = lane; i < 2 * n_heads; i += L)
-            a.piece_ms[((size_t)w * 2 + i / n_heads) * a.heads + h0 + i % n_heads] = make_float2(-INFINITY, 0.f);
 
     uint32_t e = e0;
     int64_t p = e < e1 ? a.nb.parent_of(e, 0) : a.nb.n_parents;
@@ -78,14 +76,14 @@ void attn_fwd_kernel(FwdArgs a) {
             for (int i = 0; i < E; ++i) { q[g][i] = r.at(i) * a.scale2; acc[g][i] = 0.f; }
         }
         for (; e < end; e += U) {
-            int64_t row[U];
+            int32_t row[U];
             RowPart<T, L, ALIGNED> kr[U], vr[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) row[u] = e + u < end ? a.nb.row_of(e + u) : -1;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (row[u] >= 0) kr[u].load(K + row[u] * stride, lane, a.dim); else kr[u].zero();
-                if (V) { if (row[u] >= 0) vr[u].load(V + row[u] * stride, lane, a.dim); else vr[u].zero(); }
+                if (row[u] >= 0) kr[u].load(K + (int64_t)row[u] * stride, lane, a.dim); else kr[u].zero();
+                if (V) { if (row[u] >= 0) vr[u].load(V + (int64_t)row[u] * stride, lane, a.dim); else vr[u].zero(); }
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
@@ -116,9 +114,25 @@ void attn_fwd_kernel(FwdArgs a) {
         }
         e = end;
         const bool complete = begin == sb && end == se;
+        const uint32_t wave_b = w / W * W * C;
+        const bool merge = W > 1 && !complete && sb <= wave_b && se >= wave_b + W * C;      // the same in all lanes
+        if (merge) {
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int o = L; o < 64; o *= 2) {
+                    const float mo = __shfl_xor(m[g], o, 64), so = __shfl_xor(s[g], o, 64);
+                    const float top = fmaxf(m[g], mo), ref = top == -INFINITY ? 0.f : top;
+                    const float ka = gs::fast_exp2(m[g] - ref), kb = gs::fast_exp2(mo - ref);
+                    m[g] = top;
+                    s[g] = s[g] * ka + so * kb;
+#pragma unroll
+                    for (int i = 0; i < E; ++i) acc[g][i] = acc[g][i] * ka + __shfl_xor(acc[g][i], o, 64) * kb;
+                }
+        }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            if (g >= n_heads) continue;
+            if (g >= n_heads || (merge && w % W)) continue;
             const int64_t o = p * a.heads + h0 + g;
             if (complete) {
                 const float inv = s[g] > 0.f ? 1.f / s[g] : s[g] == 0.f ? 0.f : s[g];   // (a NaN stays one)
@@ -141,11 +155,12 @@ void attn_fwd_kernel(FwdArgs a) {
 }
 
 // Joins the pieces of the parents that cross a worker's border and writes those without edges.  A block looks at 64
-// parents, far apart (popular parents tend to be neighbors); its four waves take every fourth piece of one.
+// parents, far apart (popular parents tend to be neighbors); its eight waves take every eighth piece of one.
 template <class T>
-__global__ __launch_bounds__(256)
-void attn_join_kernel(FwdArgs a) {
-    __shared__ float part[4][256 + 2];
+__global__ __launch_bounds__(gs::kJoinWaves * 64)
+void attn_join_kernel(FwdArgs a, int per_wave) {
+    constexpr int N = gs::kJoinWaves;
+    __shared__ float part[N][256 + 2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.y;
     const int64_t mine = (int64_t)lane * gridDim.x + blockIdx.x;
     uint32_t b = 0, e = 0;
@@ -158,18 +173,21 @@ void attn_join_kernel(FwdArgs a) {
         const int64_t p = (int64_t)src * gridDim.x + blockIdx.x;
         float m = -INFINITY, s = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
         if (se > sb) {
-            const uint32_t first = sb / a.chunk, last = (se - 1) / a.chunk;
-            for (uint32_t w = first + wave; w <= last; w += 4) {
-                const size_t at = ((size_t)w * 2 + (w == first && sb % a.chunk ? 1 : 0)) * a.heads + h;
+            const gs::PieceList list(sb, se, a.chunk, per_wave);
+            const uint32_t n = list.count();
+#pragma unroll 4
+            for (uint32_t i = wave; i < n; i += N) {
+                const size_t at = list.place(i) * a.heads + h;
                 const float2 ms = a.piece_ms[at];
+                float x[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[c] = lane + 64 * c < a.dim ? a.piece_acc[at * a.dim + lane + 64 * c] : 0.f;
                 const float top = fmaxf(m, ms.x), ref = top == -INFINITY ? 0.f : top;
                 const float ko = gs::fast_exp2(m - ref), kn = gs::fast_exp2(ms.x - ref);
-                if (ms.x == -INFINITY && ms.y == 0.f) continue;         // merged into another piece, or all masked
                 m = top;
                 s = s * ko + ms.y * kn;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (lane + 64 * i < a.dim) acc[i] = acc[i] * ko + a.piece_acc[at * a.dim + lane + 64 * i] * kn;
+                for (int c = 0; c < 4; ++c) acc[c] = acc[c] * ko + x[c] * kn;
             }
         }
         __syncthreads();                            // the last parent's parts are read
@@ -177,18 +195,21 @@ void attn_join_kernel(FwdArgs a) {
         for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = acc[i];
         if (lane == 0) { part[wave][256] = m; part[wave][257] = s; }
         __syncthreads();
-        const float top = fmaxf(fmaxf(part[0][256], part[1][256]), fmaxf(part[2][256], part[3][256]));
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = fmaxf(top, part[i][256]);
         const float ref = top == -INFINITY ? 0.f : top;
+        const int d = threadIdx.x & 255;
         float sum = 0.f, o = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < N; ++i) {
             const float f = gs::fast_exp2(part[i][256] - ref);
             sum += part[i][257] * f;
-            o += part[i][threadIdx.x] * f;
+            o += part[i][d] * f;
         }
         const int64_t at = p * a.heads + h;
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-        if (threadIdx.x < a.dim) static_cast<T *>(a.out)[at * a.dim + threadIdx.x] = (T)(o * inv);
+        if (threadIdx.x < a.dim) static_cast<T *>(a.out)[at * a.dim + d] = (T)(o * inv);
         if (threadIdx.x == 0) a.lse[at] = (top + gs::fast_log2(sum)) * gs::kLn2;
     }
 }
@@ -225,7 +246,7 @@ int run_fwd(const FwdArgs &a, const gs::Deal &d, int lanes, bool aligned, hipStr
     }
     if (!d.whole) {
         const dim3 grid((unsigned)((a.nb.n_parents + 63) / 64), (unsigned)a.heads);
-        attn_join_kernel<T><<<grid, 256, 0, stream>>>(a);
+        attn_join_kernel<T><<<grid, gs::kJoinWaves * 64, 0, stream>>>(a, 64 / lanes);
         return gs::check_launch("gs_neighbor_attention_fwd (join)");
     }
     return GS_OK;

@@ -33,6 +33,7 @@ template <class T, int L, int G, bool ALIGNED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_bwd_parents_kernel(BwdArgs a) {
     constexpr int E = gs::Pack<T>::E, U = 4;
+    constexpr uint32_t W = 64 / L;
     const int lane = threadIdx.x & (L - 1);
     const uint32_t w = blockIdx.x * (gs::kAttnThreads / L) + threadIdx.x / L;
     const int share = a.heads / a.kv_heads;
@@ -78,14 +79,14 @@ void attn_bwd_parents_kernel(BwdArgs a) {
             if (g < n_heads && begin == sb && lane == 0) a.delta[at] = delta[g];
         }
         for (; e < end; e += U) {
-            int64_t row[U];
+            int32_t row[U];
             RowPart<T, L, ALIGNED> kr[U], vr[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) row[u] = e + u < end ? a.nb.row_of(e + u) : -1;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (row[u] >= 0) kr[u].load(K + row[u] * stride, lane, a.dim); else kr[u].zero();
-                if (V) { if (row[u] >= 0) vr[u].load(V + row[u] * stride, lane, a.dim); else vr[u].zero(); }
+                if (row[u] >= 0) kr[u].load(K + (int64_t)row[u] * stride, lane, a.dim); else kr[u].zero();
+                if (V) { if (row[u] >= 0) vr[u].load(V + (int64_t)row[u] * stride, lane, a.dim); else vr[u].zero(); }
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
@@ -108,10 +109,17 @@ void attn_bwd_parents_kernel(BwdArgs a) {
         }
         e = end;
         const bool complete = begin == sb && end == se;
+        const uint32_t wave_b = w / W * W * C;
+        const bool merge = W > 1 && !complete && sb <= wave_b && se >= wave_b + W * C;      // the same in all lanes
         if (a.g_q) {
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                if (g >= n_heads) continue;
+                if (merge)
+#pragma unroll
+                    for (int o = L; o < 64; o *= 2)
+#pragma unroll
+                        for (int i = 0; i < E; ++i) acc[g][i] += __shfl_xor(acc[g][i], o, 64);
+                if (g >= n_heads || (merge && w % W)) continue;
 #pragma unroll
                 for (int i = 0; i < E; ++i) acc[g][i] *= a.scale;
                 if (complete) {
@@ -137,6 +145,7 @@ __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_bwd_rows_kernel(BwdArgs a) {
     constexpr int E = gs::Pack<T>::E;
     constexpr int U = G == 1 ? 4 : G == 2 ? 2 : 1;
+    constexpr uint32_t W = 64 / L;
     const int lane = threadIdx.x & (L - 1);
     const uint32_t w = blockIdx.x * (gs::kAttnThreads / L) + threadIdx.x / L;
     const int share = a.heads / a.kv_heads, j = blockIdx.y;
@@ -171,15 +180,15 @@ void attn_bwd_rows_kernel(BwdArgs a) {
         }
         bool read = false;
         for (; e < end; e += U) {
-            int64_t p[U];
+            int32_t p[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 p[u] = -1;
                 if (e + u < end) {
                     const int64_t x = a.inv_indptr ? (int64_t)a.inv_edges[e + u] : (int64_t)(e + u);
                     if (x >= first && x < last && (uint64_t)x < a.nb.n_edges) {
-                        p[u] = a.nb.indptr ? (int64_t)a.edge_parent[x] : (int64_t)((uint32_t)x / a.nb.n_child);
-                        if ((uint64_t)p[u] >= (uint64_t)a.nb.n_parents) p[u] = -1;
+                        p[u] = a.nb.indptr ? a.edge_parent[x] : (int32_t)((uint32_t)x / a.nb.n_child);
+                        if ((uint64_t)(int64_t)p[u] >= (uint64_t)a.nb.n_parents) p[u] = -1;
                     }
                 }
                 read |= p[u] >= 0;
@@ -194,7 +203,7 @@ void attn_bwd_rows_kernel(BwdArgs a) {
                         lse2[u][g] = -INFINITY;
                         delta[u][g] = 0.f;
                         if (p[u] >= 0 && h0 + g < (j + 1) * share) {
-                            const int64_t at = p[u] * a.heads + h0 + g;
+                            const int64_t at = (int64_t)p[u] * a.heads + h0 + g;
                             qr[u][g].load(Q + at * a.dim, lane, a.dim);
                             gr[u][g].load(GO + at * a.dim, lane, a.dim);
                             lse2[u][g] = a.lse[at] * gs::kLog2e;
@@ -229,6 +238,14 @@ void attn_bwd_rows_kernel(BwdArgs a) {
                 if (a.g_v) gs::store_row<T, L, ALIGNED>(static_cast<T *>(a.g_v) + at, lane, a.dim, gv);
             }
         } else {
+            const uint32_t wave_b = w / W * W * C;
+            if (W > 1 && sb <= wave_b && se >= wave_b + W * C) {       // the same in all lanes
+#pragma unroll
+                for (int o = L; o < 64; o *= 2)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) { gk[i] += __shfl_xor(gk[i], o, 64); gv[i] += __shfl_xor(gv[i], o, 64); }
+                if (w % W) { e = e1; break; }       // (its range ends inside the list)
+            }
             const size_t at = (((size_t)w * 2 + (begin == e0 ? 0 : 1)) * a.kv_heads + j) * 2;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
@@ -243,9 +260,11 @@ void attn_bwd_rows_kernel(BwdArgs a) {
 // Adds the pieces of the segments that cross a worker's border, in worker order, and writes zeros for empty ones.
 // `sets` vectors of dim floats per (segment, y): the parents' walk has one (y a head), the rows' two (y a key head).
 template <class T>
-__global__ __launch_bounds__(256)
-void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int sets, int dim, int chunk, T *out0, T *out1) {
-    __shared__ float part[4][256];
+__global__ __launch_bounds__(gs::kJoinWaves * 64)
+void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int sets, int dim, int chunk, int per_wave, T *out0,
+                          T *out1) {
+    constexpr int N = gs::kJoinWaves;
+    __shared__ float part[N][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, y = blockIdx.y;
     const int64_t mine = (int64_t)lane * gridDim.x + blockIdx.x;
     uint32_t b = 0, e = 0;
@@ -261,21 +280,26 @@ void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int s
             if (!out) continue;
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
             if (se > sb) {
-                const uint32_t first = sb / chunk, last = (se - 1) / chunk;
-                for (uint32_t w = first + wave; w <= last; w += 4) {
-                    const size_t at = ((((size_t)w * 2 + (w == first && sb % chunk ? 1 : 0)) * per_slot + y) * sets + set) * dim;
+                const gs::PieceList list(sb, se, chunk, per_wave);
+                const uint32_t n = list.count();
+#pragma unroll 4
+                for (uint32_t i = wave; i < n; i += N) {
+                    const size_t at = ((list.place(i) * per_slot + y) * sets + set) * dim;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (lane + 64 * i < dim) acc[i] += piece[at + lane + 64 * i];
+                    for (int c = 0; c < 4; ++c)
+                        if (lane + 64 * c < dim) acc[c] += piece[at + lane + 64 * c];
                 }
             }
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = acc[i];
             __syncthreads();
-            if (threadIdx.x < dim)
-                out[(p * per_slot + y) * dim + threadIdx.x] =
-                    (T)(((part[0][threadIdx.x] + part[1][threadIdx.x]) + part[2][threadIdx.x]) + part[3][threadIdx.x]);
+            if (threadIdx.x < dim) {
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum += part[i][threadIdx.x];
+                out[(p * per_slot + y) * dim + threadIdx.x] = (T)sum;
+            }
         }
     }
 }
@@ -352,8 +376,8 @@ int run_bwd(BwdArgs a, const Plan &p, int lanes, bool aligned, hipStream_t strea
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents)")) return rc;
     }
     if (a.g_q && a.nb.n_parents && !p.parents.whole) {
-        attn_bwd_join_kernel<T><<<dim3((unsigned)((a.nb.n_parents + 63) / 64), (unsigned)a.heads), 256, 0, stream>>>(
-            a.nb, a.piece, a.heads, 1, a.dim, a.chunk, static_cast<T *>(a.g_q), (T *)nullptr);
+        attn_bwd_join_kernel<T><<<dim3((unsigned)((a.nb.n_parents + 63) / 64), (unsigned)a.heads), gs::kJoinWaves * 64, 0, stream>>>(
+            a.nb, a.piece, a.heads, 1, a.dim, a.chunk, 64 / lanes, static_cast<T *>(a.g_q), (T *)nullptr);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents' join)")) return rc;
     }
     if (!a.g_k && !a.g_v) return GS_OK;
@@ -367,8 +391,8 @@ int run_bwd(BwdArgs a, const Plan &p, int lanes, bool aligned, hipStream_t strea
         rows.indptr = a.inv_indptr;
         rows.n_parents = a.nb.n_rows;
         rows.n_edges = a.n_inv;
-        attn_bwd_join_kernel<T><<<dim3((unsigned)((a.nb.n_rows + 63) / 64), (unsigned)a.kv_heads), 256, 0, stream>>>(
-            rows, a.piece, a.kv_heads, 2, a.dim, a.chunk, static_cast<T *>(a.g_k), static_cast<T *>(a.g_v));
+        attn_bwd_join_kernel<T><<<dim3((unsigned)((a.nb.n_rows + 63) / 64), (unsigned)a.kv_heads), gs::kJoinWaves * 64, 0, stream>>>(
+            rows, a.piece, a.kv_heads, 2, a.dim, a.chunk, 64 / lanes, static_cast<T *>(a.g_k), static_cast<T *>(a.g_v));
         return gs::check_launch("gs_neighbor_attention_bwd (rows' join)");
     }
     return GS_OK;
@@ -399,7 +423,6 @@ extern "C" int gs_neighbor_attention_bwd(const void *q, const void *k, const voi
     if (rows && nb->ids && (!inv_indptr || n_inv < 0 || n_inv > nb->n_edges || (n_inv && !inv_edges)))
         return gs::fail(GS_EINVAL, "%s: rows read by id need the inverse lists (n_inv=%lld of %lld edges)", what,
                         (long long)n_inv, (long long)nb->n_edges);
-    if (rows && nb->n_rows >= (int64_t)1 << 31) return gs::fail(GS_ELIMIT, "%s: %lld rows (less than 2^31)", what, (long long)nb->n_rows);
     const uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)g_out | (uintptr_t)g_q |
                           (uintptr_t)g_k | (uintptr_t)g_v;
     if (all & (size - 1)) return gs::fail(GS_EINVAL, "%s: pointer not aligned to its element", what);

@@ -68,7 +68,7 @@ typedef struct gs_neighbors {
  *   v        NULL: the keys are the values
  *   lse      device float[n_parents][heads]
  *   workspace of gs_neighbor_attention_workspace(...) bytes (may be 0), 16-byte aligned
- * 1 <= dim <= 256, else GS_ELIMIT.
+ * 1 <= dim <= 256; parents, edges and rows below 2^31, else GS_ELIMIT.
  */
 size_t gs_neighbor_attention_workspace(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype);
 int gs_neighbor_attention_fwd(const void *q, const void *k, const void *v, const gs_neighbors *nb, int heads,
