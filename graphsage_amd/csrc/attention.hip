@@ -52,19 +52,14 @@ void attn_fwd_kernel(FwdArgs a) {
     const int share = a.heads / a.kv_heads;
     const int j = blockIdx.y / a.parts, h0 = j * share + (blockIdx.y % a.parts) * G;
     const int n_heads = min(G, (j + 1) * share - h0);
-    const uint32_t C = a.chunk, e0 = min((uint64_t)w * C, (uint64_t)a.nb.n_edges), e1 = min((uint64_t)e0 + C, (uint64_t)a.nb.n_edges);
+    const uint32_t C = a.chunk;
     const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = a.v ? static_cast<const T *>(a.v) + (int64_t)j * a.dim : nullptr;
     const int64_t stride = (int64_t)a.kv_heads * a.dim;
 
-    uint32_t e = e0;
-    int64_t p = e < e1 ? a.nb.parent_of(e, 0) : a.nb.n_parents;
-    while (e < e1 && p < a.nb.n_parents) {
-        uint32_t sb, se;
-        a.nb.range(p, sb, se);
-        if (se <= e) { p = a.nb.parent_of(e, p + 1); continue; }
-        if (sb > e) { e = sb; continue; }
-        const uint32_t end = min(se, e1), begin = e;
-
+    gs::Walk walk(a.nb, w, C, L);
+    while (walk.next()) {
+        const int64_t p = walk.p;
+        const uint32_t end = walk.end;
         float q[G][E], acc[G][E], m[G], s[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -75,7 +70,7 @@ void attn_fwd_kernel(FwdArgs a) {
 #pragma unroll
             for (int i = 0; i < E; ++i) { q[g][i] = r.at(i) * a.scale2; acc[g][i] = 0.f; }
         }
-        for (; e < end; e += U) {
+        for (uint32_t e = walk.begin; e < end; e += U) {
             int32_t row[U];
             RowPart<T, L, ALIGNED> kr[U], vr[U];
 #pragma unroll
@@ -112,10 +107,7 @@ void attn_fwd_kernel(FwdArgs a) {
                 }
             }
         }
-        e = end;
-        const bool complete = begin == sb && end == se;
-        const uint32_t wave_b = w / W * W * C;
-        const bool merge = W > 1 && !complete && sb <= wave_b && se >= wave_b + W * C;      // the same in all lanes
+        const bool complete = walk.complete(), merge = walk.inside(w, C, W);
         if (merge) {
 #pragma unroll
             for (int g = 0; g < G; ++g)
@@ -135,13 +127,13 @@ void attn_fwd_kernel(FwdArgs a) {
             if (g >= n_heads || (merge && w % W)) continue;
             const int64_t o = p * a.heads + h0 + g;
             if (complete) {
-                const float inv = s[g] > 0.f ? 1.f / s[g] : s[g] == 0.f ? 0.f : s[g];   // (a NaN stays one)
+                const float inv = s[g] > 0.f ? 1.f / s[g] : s[g] == 0.f ? 0.f : s[g];   // (nothing: zeros; a NaN stays one)
 #pragma unroll
                 for (int i = 0; i < E; ++i) acc[g][i] *= inv;
                 gs::store_row<T, L, ALIGNED>(static_cast<T *>(a.out) + o * a.dim, lane, a.dim, acc[g]);
                 if (lane == 0) a.lse[o] = (m[g] + gs::fast_log2(s[g])) * gs::kLn2;
             } else {
-                const size_t at = ((size_t)w * 2 + (begin == e0 ? 0 : 1)) * a.heads + h0 + g;
+                const size_t at = walk.place(w) * a.heads + h0 + g;
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
                     const int d = gs::element_of<T, L, ALIGNED>(lane, i);
@@ -150,12 +142,38 @@ void attn_fwd_kernel(FwdArgs a) {
                 if (lane == 0) a.piece_ms[at] = make_float2(m[g], s[g]);
             }
         }
-        if (e < e1) p = a.nb.parent_of(e, p + 1);
     }
 }
 
-// Joins the pieces of the parents that cross a worker's border and writes those without edges.  A block looks at 64
-// parents, far apart (popular parents tend to be neighbors); its eight waves take every eighth piece of one.
+// Joins the pieces of the lists that were cut and writes the parents without edges.  A block looks at 64 parents, far
+// apart (popular parents tend to be neighbors).  A wave joins a list of a few pieces by itself; of a long one the eight
+// waves take every eighth piece.
+constexpr uint32_t kFewPieces = 16;
+
+struct Joined {
+    float m, s, acc[4];
+};
+
+__device__ __forceinline__ void join_pieces(const FwdArgs &a, const gs::PieceList &list, uint32_t i0, uint32_t step, int h, int lane, Joined &j) {
+    const uint32_t n = list.count();
+#pragma unroll 4
+    for (uint32_t i = i0; i < n; i += step) {
+        const size_t at = list.place(i) * a.heads + h;
+        const float2 ms = a.piece_ms[at];
+        float x[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[c] = lane + 64 * c < a.dim ? a.piece_acc[at * a.dim + lane + 64 * c] : 0.f;
+        const float top = fmaxf(j.m, ms.x), ref = top == -INFINITY ? 0.f : top;
+        const float ko = gs::fast_exp2(j.m - ref), kn = gs::fast_exp2(ms.x - ref);
+        j.m = top;
+        j.s = j.s * ko + ms.y * kn;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) j.acc[c] = j.acc[c] * ko + x[c] * kn;
+    }
+}
+
+__device__ __forceinline__ float inverse_of(float s) { return s > 0.f ? 1.f / s : s == 0.f ? 0.f : s; }
+
 template <class T>
 __global__ __launch_bounds__(gs::kJoinWaves * 64)
 void attn_join_kernel(FwdArgs a, int per_wave) {
@@ -165,35 +183,31 @@ void attn_join_kernel(FwdArgs a, int per_wave) {
     const int64_t mine = (int64_t)lane * gridDim.x + blockIdx.x;
     uint32_t b = 0, e = 0;
     if (mine < a.nb.n_parents) a.nb.range(mine, b, e);
-    unsigned long long todo = __ballot(mine < a.nb.n_parents && (b == e || b / a.chunk != (e - 1) / a.chunk));
-    while (todo) {
-        const int src = __builtin_ctzll(todo);
-        todo &= todo - 1;
+    const bool mine_todo = mine < a.nb.n_parents && gs::needs_join(b, e, a.chunk);
+    const bool many = mine_todo && e > b && gs::PieceList(b, e, a.chunk, per_wave).count() > kFewPieces;
+    unsigned long long few = __ballot(mine_todo && !many), long_ones = __ballot(many);
+    for (int turn = 0; few; ++turn, few &= few - 1) {
+        if (turn % N != wave) continue;
+        const int src = __builtin_ctzll(few);
         const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
-        const int64_t p = (int64_t)src * gridDim.x + blockIdx.x;
-        float m = -INFINITY, s = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-        if (se > sb) {
-            const gs::PieceList list(sb, se, a.chunk, per_wave);
-            const uint32_t n = list.count();
-#pragma unroll 4
-            for (uint32_t i = wave; i < n; i += N) {
-                const size_t at = list.place(i) * a.heads + h;
-                const float2 ms = a.piece_ms[at];
-                float x[4];
+        Joined j{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
+        if (se > sb) join_pieces(a, gs::PieceList(sb, se, a.chunk, per_wave), 0, 1, h, lane, j);
+        const int64_t at = ((int64_t)src * gridDim.x + blockIdx.x) * a.heads + h;
+        const float inv = inverse_of(j.s);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) x[c] = lane + 64 * c < a.dim ? a.piece_acc[at * a.dim + lane + 64 * c] : 0.f;
-                const float top = fmaxf(m, ms.x), ref = top == -INFINITY ? 0.f : top;
-                const float ko = gs::fast_exp2(m - ref), kn = gs::fast_exp2(ms.x - ref);
-                m = top;
-                s = s * ko + ms.y * kn;
+        for (int c = 0; c < 4; ++c)
+            if (lane + 64 * c < a.dim) static_cast<T *>(a.out)[at * a.dim + lane + 64 * c] = (T)(j.acc[c] * inv);
+        if (lane == 0) a.lse[at] = (j.m + gs::fast_log2(j.s)) * gs::kLn2;
+    }
+    for (; long_ones; long_ones &= long_ones - 1) {
+        const int src = __builtin_ctzll(long_ones);
+        const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
+        Joined j{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
+        join_pieces(a, gs::PieceList(sb, se, a.chunk, per_wave), wave, N, h, lane, j);
+        __syncthreads();                            // the last list's parts are read
 #pragma unroll
-                for (int c = 0; c < 4; ++c) acc[c] = acc[c] * ko + x[c] * kn;
-            }
-        }
-        __syncthreads();                            // the last parent's parts are read
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = acc[i];
-        if (lane == 0) { part[wave][256] = m; part[wave][257] = s; }
+        for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = j.acc[i];
+        if (lane == 0) { part[wave][256] = j.m; part[wave][257] = j.s; }
         __syncthreads();
         float top = -INFINITY;
 #pragma unroll
@@ -207,9 +221,8 @@ void attn_join_kernel(FwdArgs a, int per_wave) {
             sum += part[i][257] * f;
             o += part[i][d] * f;
         }
-        const int64_t at = p * a.heads + h;
-        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-        if (threadIdx.x < a.dim) static_cast<T *>(a.out)[at * a.dim + d] = (T)(o * inv);
+        const int64_t at = ((int64_t)src * gridDim.x + blockIdx.x) * a.heads + h;
+        if (threadIdx.x < a.dim) static_cast<T *>(a.out)[at * a.dim + d] = (T)(o * inverse_of(sum));
         if (threadIdx.x == 0) a.lse[at] = (top + gs::fast_log2(sum)) * gs::kLn2;
     }
 }
@@ -244,7 +257,7 @@ int run_fwd(const FwdArgs &a, const gs::Deal &d, int lanes, bool aligned, hipStr
         }
         if (int rc = gs::check_launch("gs_neighbor_attention_fwd")) return rc;
     }
-    if (!d.whole) {
+    if (d.pieces) {
         const dim3 grid((unsigned)((a.nb.n_parents + 63) / 64), (unsigned)a.heads);
         attn_join_kernel<T><<<grid, gs::kJoinWaves * 64, 0, stream>>>(a, 64 / lanes);
         return gs::check_launch("gs_neighbor_attention_fwd (join)");
@@ -253,7 +266,7 @@ int run_fwd(const FwdArgs &a, const gs::Deal &d, int lanes, bool aligned, hipStr
 }
 
 size_t pieces_bytes(const gs::Deal &d, int heads, int dim, size_t *off_acc) {
-    if (d.whole || !d.workers) { if (off_acc) *off_acc = 0; return 0; }
+    if (!d.pieces || !d.workers) { if (off_acc) *off_acc = 0; return 0; }
     const size_t ms = gs::align256((size_t)d.workers * 2 * heads * sizeof(float2));
     if (off_acc) *off_acc = ms;
     return ms + (size_t)d.workers * 2 * heads * dim * sizeof(float);

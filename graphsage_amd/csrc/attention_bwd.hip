@@ -39,19 +39,15 @@ void attn_bwd_parents_kernel(BwdArgs a) {
     const int share = a.heads / a.kv_heads;
     const int j = blockIdx.y / a.parts, h0 = j * share + (blockIdx.y % a.parts) * G;
     const int n_heads = min(G, (j + 1) * share - h0);
-    const uint32_t C = a.chunk, e0 = min((uint64_t)w * C, (uint64_t)a.nb.n_edges), e1 = min((uint64_t)e0 + C, (uint64_t)a.nb.n_edges);
+    const uint32_t C = a.chunk;
     const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = a.v ? static_cast<const T *>(a.v) + (int64_t)j * a.dim : nullptr;
     const int64_t stride = (int64_t)a.kv_heads * a.dim;
     const float scale2 = a.scale * gs::kLog2e;
 
-    uint32_t e = e0;
-    int64_t p = e < e1 ? a.nb.parent_of(e, 0) : a.nb.n_parents;
-    while (e < e1 && p < a.nb.n_parents) {
-        uint32_t sb, se;
-        a.nb.range(p, sb, se);
-        if (se <= e) { p = a.nb.parent_of(e, p + 1); continue; }
-        if (sb > e) { e = sb; continue; }
-        const uint32_t end = min(se, e1), begin = e;
+    gs::Walk walk(a.nb, w, C, L);
+    while (walk.next()) {
+        const int64_t p = walk.p;
+        const uint32_t begin = walk.begin, end = walk.end;
         if (a.edge_parent && blockIdx.y == 0)
             for (uint32_t i = begin + lane; i < end; i += L) a.edge_parent[i] = (int32_t)p;
 
@@ -76,9 +72,9 @@ void attn_bwd_parents_kernel(BwdArgs a) {
                 acc[g][i] = 0.f;
             }
             delta[g] = gs::lanes_sum<L>(dot);
-            if (g < n_heads && begin == sb && lane == 0) a.delta[at] = delta[g];
+            if (g < n_heads && begin == walk.sb && lane == 0) a.delta[at] = delta[g];
         }
-        for (; e < end; e += U) {
+        for (uint32_t e = begin; e < end; e += U) {
             int32_t row[U];
             RowPart<T, L, ALIGNED> kr[U], vr[U];
 #pragma unroll
@@ -107,10 +103,7 @@ void attn_bwd_parents_kernel(BwdArgs a) {
                 }
             }
         }
-        e = end;
-        const bool complete = begin == sb && end == se;
-        const uint32_t wave_b = w / W * W * C;
-        const bool merge = W > 1 && !complete && sb <= wave_b && se >= wave_b + W * C;      // the same in all lanes
+        const bool complete = walk.complete(), merge = walk.inside(w, C, W);
         if (a.g_q) {
 #pragma unroll
             for (int g = 0; g < G; ++g) {
@@ -125,7 +118,7 @@ void attn_bwd_parents_kernel(BwdArgs a) {
                 if (complete) {
                     gs::store_row<T, L, ALIGNED>(static_cast<T *>(a.g_q) + (p * a.heads + h0 + g) * a.dim, lane, a.dim, acc[g]);
                 } else {
-                    const size_t at = ((size_t)w * 2 + (begin == e0 ? 0 : 1)) * a.heads + h0 + g;
+                    const size_t at = walk.place(w) * a.heads + h0 + g;
 #pragma unroll
                     for (int i = 0; i < E; ++i) {
                         const int d = gs::element_of<T, L, ALIGNED>(lane, i);
@@ -134,7 +127,6 @@ void attn_bwd_parents_kernel(BwdArgs a) {
                 }
             }
         }
-        if (e < e1) p = a.nb.parent_of(e, p + 1);
     }
 }
 
@@ -155,21 +147,17 @@ void attn_bwd_rows_kernel(BwdArgs a) {
     rows.n_parents = a.nb.n_rows;
     rows.n_child = 1;
     rows.n_edges = a.n_inv;
-    const uint32_t C = a.chunk, e0 = min((uint64_t)w * C, (uint64_t)a.n_inv), e1 = min((uint64_t)e0 + C, (uint64_t)a.n_inv);
+    const uint32_t C = a.chunk;
     const T *Q = static_cast<const T *>(a.q), *GO = static_cast<const T *>(a.g_out);
     const int64_t stride = (int64_t)a.kv_heads * a.dim;
     const float scale2 = a.scale * gs::kLog2e;
     int64_t first = 0, last = a.nb.n_edges;         // edges that belong to a parent
     if (!a.inv_indptr && a.nb.indptr) { first = a.nb.indptr[0]; last = a.nb.indptr[a.nb.n_parents]; }
 
-    uint32_t e = e0;
-    int64_t r = e < e1 ? rows.parent_of(e, 0) : rows.n_parents;
-    while (e < e1 && r < rows.n_parents) {
-        uint32_t sb, se;
-        rows.range(r, sb, se);
-        if (se <= e) { r = rows.parent_of(e, r + 1); continue; }
-        if (sb > e) { e = sb; continue; }
-        const uint32_t end = min(se, e1), begin = e;
+    gs::Walk walk(rows, w, C, L);
+    while (walk.next()) {
+        const int64_t r = walk.p;
+        const uint32_t end = walk.end;
         float key[E], val[E], gk[E], gv[E];
         {
             RowPart<T, L, ALIGNED> kr, vr;
@@ -179,7 +167,7 @@ void attn_bwd_rows_kernel(BwdArgs a) {
             for (int i = 0; i < E; ++i) { key[i] = kr.at(i) * scale2; val[i] = vr.at(i); gk[i] = 0.f; gv[i] = 0.f; }
         }
         bool read = false;
-        for (; e < end; e += U) {
+        for (uint32_t e = walk.begin; e < end; e += U) {
             int32_t p[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -226,8 +214,7 @@ void attn_bwd_rows_kernel(BwdArgs a) {
                     }
             }
         }
-        e = end;
-        const bool complete = begin == sb && end == se;
+        const bool complete = walk.complete();
         if (!a.v)
 #pragma unroll
             for (int i = 0; i < E; ++i) gk[i] += gv[i];
@@ -238,27 +225,27 @@ void attn_bwd_rows_kernel(BwdArgs a) {
                 if (a.g_v) gs::store_row<T, L, ALIGNED>(static_cast<T *>(a.g_v) + at, lane, a.dim, gv);
             }
         } else {
-            const uint32_t wave_b = w / W * W * C;
-            if (W > 1 && sb <= wave_b && se >= wave_b + W * C) {       // the same in all lanes
+            if (walk.inside(w, C, W)) {
 #pragma unroll
                 for (int o = L; o < 64; o *= 2)
 #pragma unroll
                     for (int i = 0; i < E; ++i) { gk[i] += __shfl_xor(gk[i], o, 64); gv[i] += __shfl_xor(gv[i], o, 64); }
-                if (w % W) { e = e1; break; }       // (its range ends inside the list)
+                if (w % W) continue;
             }
-            const size_t at = (((size_t)w * 2 + (begin == e0 ? 0 : 1)) * a.kv_heads + j) * 2;
+            const size_t at = (walk.place(w) * a.kv_heads + j) * 2;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 const int d = gs::element_of<T, L, ALIGNED>(lane, i);
                 if (d < a.dim) { a.piece[at * a.dim + d] = gk[i]; a.piece[(at + 1) * a.dim + d] = gv[i]; }
             }
         }
-        if (e < e1) r = rows.parent_of(e, r + 1);
     }
 }
 
-// Adds the pieces of the segments that cross a worker's border, in worker order, and writes zeros for empty ones.
-// `sets` vectors of dim floats per (segment, y): the parents' walk has one (y a head), the rows' two (y a key head).
+// Adds the pieces of the lists that were cut, in worker order, and writes zeros for empty ones.  `sets` vectors of dim
+// floats per (list, y): the parents' walk has one (y a head), the rows' two (y a key head).  Few pieces: one wave alone.
+constexpr uint32_t kFewPieces = 16;
+
 template <class T>
 __global__ __launch_bounds__(gs::kJoinWaves * 64)
 void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int sets, int dim, int chunk, int per_wave, T *out0,
@@ -269,27 +256,44 @@ void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int s
     const int64_t mine = (int64_t)lane * gridDim.x + blockIdx.x;
     uint32_t b = 0, e = 0;
     if (mine < seg.n_parents) seg.range(mine, b, e);
-    unsigned long long todo = __ballot(mine < seg.n_parents && (b == e || b / chunk != (e - 1) / chunk));
-    while (todo) {
-        const int src = __builtin_ctzll(todo);
-        todo &= todo - 1;
+    const bool mine_todo = mine < seg.n_parents && gs::needs_join(b, e, chunk);
+    const bool many = mine_todo && e > b && gs::PieceList(b, e, chunk, per_wave).count() > kFewPieces;
+    unsigned long long few = __ballot(mine_todo && !many), long_ones = __ballot(many);
+    const auto add = [&](uint32_t sb, uint32_t se, uint32_t i0, uint32_t step, int set, float (&acc)[4]) {
+        const gs::PieceList list(sb, se, chunk, per_wave);
+        const uint32_t n = list.count();
+#pragma unroll 4
+        for (uint32_t i = i0; i < n; i += step) {
+            const size_t at = ((list.place(i) * per_slot + y) * sets + set) * dim;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (lane + 64 * c < dim) acc[c] += piece[at + lane + 64 * c];
+        }
+    };
+    for (int turn = 0; few; ++turn, few &= few - 1) {
+        if (turn % N != wave) continue;
+        const int src = __builtin_ctzll(few);
         const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
         const int64_t p = (int64_t)src * gridDim.x + blockIdx.x;
         for (int set = 0; set < sets; ++set) {
             T *out = set ? out1 : out0;
             if (!out) continue;
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            if (se > sb) {
-                const gs::PieceList list(sb, se, chunk, per_wave);
-                const uint32_t n = list.count();
-#pragma unroll 4
-                for (uint32_t i = wave; i < n; i += N) {
-                    const size_t at = ((list.place(i) * per_slot + y) * sets + set) * dim;
+            if (se > sb) add(sb, se, 0, 1, set, acc);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (lane + 64 * c < dim) acc[c] += piece[at + lane + 64 * c];
-                }
-            }
+            for (int c = 0; c < 4; ++c)
+                if (lane + 64 * c < dim) out[(p * per_slot + y) * dim + lane + 64 * c] = (T)acc[c];
+        }
+    }
+    for (; long_ones; long_ones &= long_ones - 1) {
+        const int src = __builtin_ctzll(long_ones);
+        const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
+        const int64_t p = (int64_t)src * gridDim.x + blockIdx.x;
+        for (int set = 0; set < sets; ++set) {
+            T *out = set ? out1 : out0;
+            if (!out) continue;
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            add(sb, se, wave, N, set, acc);
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = acc[i];
@@ -359,8 +363,8 @@ Plan make_plan(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dty
     if (nb->indptr) off += gs::align256((size_t)nb->n_edges * sizeof(int32_t));
     p.off_piece = off;
     size_t piece = 0;
-    if (!p.parents.whole) piece = (size_t)p.parents.workers * 2 * heads * dim * sizeof(float);
-    if (!p.rows.whole) {
+    if (p.parents.pieces) piece = (size_t)p.parents.workers * 2 * heads * dim * sizeof(float);
+    if (p.rows.pieces) {
         const size_t r = (size_t)p.rows.workers * 4 * kv_heads * dim * sizeof(float);
         if (r > piece) piece = r;
     }
@@ -375,7 +379,7 @@ int run_bwd(BwdArgs a, const Plan &p, int lanes, bool aligned, hipStream_t strea
         GS_BY_LANES(launch_parents, a, p.parents.workers, stream);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents)")) return rc;
     }
-    if (a.g_q && a.nb.n_parents && !p.parents.whole) {
+    if (a.g_q && a.nb.n_parents && p.parents.pieces) {
         attn_bwd_join_kernel<T><<<dim3((unsigned)((a.nb.n_parents + 63) / 64), (unsigned)a.heads), gs::kJoinWaves * 64, 0, stream>>>(
             a.nb, a.piece, a.heads, 1, a.dim, a.chunk, 64 / lanes, static_cast<T *>(a.g_q), (T *)nullptr);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents' join)")) return rc;

@@ -57,7 +57,9 @@ void layout_kernel(Layout l, int64_t n_places) {
         for (int i = 0; i < 8; ++i) top = fmaxf(top, v[i] == v[i] ? fabsf(v[i]) : INFINITY);
 #pragma unroll
         for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        if ((threadIdx.x & 63) == 0) atomicMax(l.largest, __float_as_uint(top));
+        // (most waves find a larger one there already)
+        if ((threadIdx.x & 63) == 0 && __float_as_uint(top) > __hip_atomic_load(l.largest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+            atomicMax(l.largest, __float_as_uint(top));
     }
     if (place >= n_places) return;
     uint4 *out = (cols ? l.cols : l.rows) + (size_t)frag * P * 64 + lane;

@@ -1401,7 +1401,23 @@ def _table(t, name, dtype=None, shape=None, device=None, ndim=None):
 
 def _stream_of(device):
     """The current stream of a tensor's device, which need not be the current device."""
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _AlreadyThere:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *_):
+        return None
+
+
+_already_there = _AlreadyThere()
+
+
+def _on(device):
+    """The tensors' device made the current one, where it is not."""
+    return _already_there if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _scratch(n_bytes, device):
@@ -1428,7 +1444,7 @@ def dropout(x, rate, seed, offset=0, out=None):
         out = torch.empty_like(x)
     else:
         _table(out, 'out', x.dtype, x.shape, x.device)
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         check(lib.gs_dropout(ptr(x), x.numel(), _DTYPES[x.dtype], rate,
                              0 if seed_t is not None else int(seed) & 0xFFFFFFFFFFFFFFFF, ptr(seed_t),
                              int(offset) & 0xFFFFFFFFFFFFFFFF, ptr(out), _stream_of(x.device)), 'gs_dropout')
@@ -1484,7 +1500,7 @@ def neighbor_attention(q, k, v, child_ids, n_child, id_offset=0, scale=None, ind
     out = torch.empty_like(q) if out is None else _table(out, 'out', q.dtype, q.shape, dev)
     lse = (torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if lse is None
            else _table(lse, 'lse', torch.float32, q.shape[:2], dev))
-    with torch.cuda.device(dev):
+    with _on(dev):
         need = lib.gs_neighbor_attention_workspace(nb, heads, kv_heads, dim, dt)
         ws = _scratch(need, dev) if need else None
         check(lib.gs_neighbor_attention_fwd(ptr(q), ptr(k), ptr(v), nb, heads, kv_heads, dim, dt,
@@ -1505,7 +1521,7 @@ def neighbor_inverse(child_ids, n_rows, id_offset=0):
     dev = child_ids.device
     if torch.cuda.is_current_stream_capturing():
         raise _lib.GsageError("neighbor_inverse cannot run inside a graph capture: build the lists before it")
-    with torch.cuda.device(dev):
+    with _on(dev):
         row = child_ids.reshape(-1).to(torch.int64) - int(id_offset)
         row = torch.where((row >= 0) & (row < n_rows), row, n_rows).to(torch.int32)
         entry = torch.arange(n, dtype=torch.int32, device=dev)
@@ -1553,7 +1569,7 @@ def neighbor_attention_bwd(q, k, v, child_ids, n_child, out, lse, g_out, id_offs
     g_q = dest(g_q, q, 'g_q') if need_q else None
     g_k = dest(g_k, k, 'g_k') if need_rows else None
     g_v = dest(g_v, v, 'g_v') if need_rows and v is not None else None
-    with torch.cuda.device(dev):
+    with _on(dev):
         need = lib.gs_neighbor_attention_bwd_workspace(nb, heads, kv_heads, dim, dt, n_inv)
         ws = _scratch(need, dev)
         check(lib.gs_neighbor_attention_bwd(ptr(q), ptr(k), ptr(v), nb, heads, kv_heads, dim, dt,
@@ -1602,7 +1618,7 @@ def catalog_log_probs(user, item, targets=None, bias=None, scale=1.0, top_k=0):
     log_prob = None if targets is None else row(n)
     entropy, lse = row(n), row(n)
     top_log_prob, top_ids = (row(n, top_k), row(n, top_k, t=torch.int32)) if top_k else (None, None)
-    with torch.cuda.device(dev):
+    with _on(dev):
         ws = _scratch(lib.gs_catalog_workspace(n, v, d, dt, top_k), dev)
         check(lib.gs_catalog_fwd(ptr(user), n, ptr(item), v, d, dt, ptr(bias), float(scale), ptr(targets), ptr(log_prob),
                                  ptr(entropy), ptr(lse), top_k, ptr(top_log_prob), ptr(top_ids), ptr(ws), ws.numel(),
@@ -1626,7 +1642,7 @@ def catalog_log_probs_bwd(user, item, targets, bias, scale, lse, entropy, g_log_
     g_user = torch.empty_like(user) if need_user else None
     g_item = torch.empty_like(item) if need_item else None
     g_bias = torch.empty_like(bias) if need_bias and bias is not None else None
-    with torch.cuda.device(dev):
+    with _on(dev):
         ws = _scratch(lib.gs_catalog_bwd_workspace(n, v, d, dt), dev)
         check(lib.gs_catalog_bwd(ptr(user), n, ptr(item), v, d, dt, ptr(bias), float(scale), ptr(targets), ptr(lse),
                                  ptr(entropy), ptr(g_log_prob), ptr(g_entropy), ptr(g_user), ptr(g_item), ptr(g_bias), ptr(ws),
