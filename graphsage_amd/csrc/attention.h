@@ -1,17 +1,21 @@
-// Attention over neighbors: how the edges are dealt to the lanes, shared by the forward and the backward kernels.
+// Attention over neighbors: how the edges are dealt to the waves, shared by the forward and the backward kernels.
 //
-// A row of dim elements is covered by a "worker" of L lanes, 16 bytes each (L = the power of two >= dim / (elements in
-// 16 bytes)); a dot product is a few multiply-adds per lane and a sum over the worker's lanes, the running softmax
-// (maximum, sum, weighted row) lives in the worker's registers, and the row is read once, whatever the number of
-// heads that share it.  Tables whose rows do not start on 16 bytes are read element by element: lane l then holds
-// elements l, l + L, ...; nothing else depends on which element sits where.
+// A row of dim elements is covered by L lanes, 16 bytes each (L = the power of two >= dim / (elements in 16 bytes)), so
+// a wave holds 64 / L rows at a time and keeps kAttnRows such groups in flight.  A dot product is a few multiply-adds per
+// lane and a sum over L lanes; a row is read once, whatever the number of heads that share it.  Tables whose rows do not
+// start on 16 bytes are read element by element: lane l then holds elements l, l + L, ...; nothing else depends on which
+// element sits where.
 //
-// Edges are dealt by count, not by parent: worker w takes the parents whose edges begin in [w C, (w + 1) C), so short
-// lists cost no idle lanes, and of a list longer than 4 C the part that lies in there: a popular parent's list is spread
-// over the chip.  Every worker leaves a piece (maximum, sum, unnormalised row) of such a list in the workspace and a second
-// launch joins them in worker order; a wave that lies inside one list joins its workers' pieces in registers first and
-// leaves one.  Where no list is that long there is no second launch.  The result depends on C, which depends on the
-// sizes only.
+// A wave works on one list (the neighbors of one parent) at a time: control flow and list bounds are scalar, lists of any
+// length leave no lane waiting for another lane's list (measured against a list per L lanes: the ragged whole graph, 2M
+// edges, 768 -> 303 us), and the running softmax of each of the 64 / L row groups is joined at the end of the list by
+// half-wave and quarter-wave swaps that leave every lane the results it stores.  Entries come 64 at a time, one a lane,
+// one load ahead: the next list's ids are on their way while this list's rows are used.
+//
+// Lists are dealt by edges: wave w takes the lists that begin in edges [w C, (w + 1) C) and, of a list longer than 4 C, the
+// part that lies in there, so that a popular parent's list is spread over the chip.  Every wave leaves a piece (maximum,
+// sum, unnormalised row) of such a list in the workspace and a second launch joins them in wave order.  Where no list is
+// that long there is no second launch.  The result depends on C, which depends on the sizes only.
 #pragma once
 
 #include "ops_common.h"
@@ -19,7 +23,7 @@
 namespace gs {
 
 constexpr int kAttnThreads = 256;
-constexpr int kAttnRows = 8;                        // rows a worker has in flight, at most
+constexpr int kAttnRows = 4;                        // rows in flight per L lanes
 
 struct Neighbors {
     const int64_t *indptr;
@@ -71,78 +75,138 @@ struct Neighbors {
     }
 };
 
-// A worker's way through its edges, list by list.
-struct Walk {
-    const Neighbors &nb;
-    uint32_t e, e0, e1, most;
-    int64_t p_next;
-    // the piece at hand: parent p with edges [sb, se), of which [begin, end) are this worker's
-    int64_t p;
-    uint32_t sb, se, begin, end;
+// A wave's way through its edges, list by list, in units of at most 64 entries.  All of it is the same in every lane.
+struct Unit {
+    int64_t p;                                      // the list
+    uint32_t e, n;                                  // entries e .. e + n - 1
+    bool first, last;                               // of this wave's part of the list
+    bool complete;                                  // the part is the list
+    uint32_t place;                                 // wave * 2 + 0 or 1: where a piece goes
+};
 
-    __device__ __forceinline__ Walk(const Neighbors &n, uint32_t w, uint32_t chunk, int lanes) : nb(n), most(4 * chunk) {
+struct Walk {
+    Neighbors nb;
+    uint32_t e, e0, e1, most, w, left;              // left: entries of the list at hand that no unit has yet
+    int64_t p_next;
+    Unit u;
+
+    __device__ __forceinline__ Walk(const Neighbors &n, uint32_t wave, uint32_t chunk) : nb(n), most(4 * chunk), w(wave), left(0) {
         e0 = (uint32_t)min((uint64_t)w * chunk, (uint64_t)nb.n_edges);
         e1 = (uint32_t)min((uint64_t)e0 + chunk, (uint64_t)nb.n_edges);
         e = e0;
-        const uint32_t first = w & ~(uint32_t)(64 / lanes - 1);
-        const uint32_t ef = (uint32_t)min((uint64_t)first * chunk, (uint64_t)nb.n_edges);
-        p_next = nb.n_parents;
-        if (ef < nb.n_edges) p_next = nb.seek_wave(ef);                // (the same for all lanes)
-        if (e < e1 && p_next < nb.n_parents) p_next = nb.seek(e, p_next);
+        p_next = e < e1 ? nb.seek_wave(e) : nb.n_parents;
     }
     __device__ __forceinline__ bool next() {
+        if (left) {
+            u.e += u.n;
+            u.n = min(left, 64u);
+            left -= u.n;
+            u.first = false;
+            u.last = left == 0;
+            return true;
+        }
         while (e < e1 && p_next < nb.n_parents) {
+            uint32_t sb, se;
             nb.range(p_next, sb, se);
             if (se <= e) { p_next = nb.seek(e, p_next + 1); continue; }
             const bool cut = se - sb > most;
-            if (!cut && sb < e0) { e = se; ++p_next; continue; }       // begins before this worker's edges: another's
+            if (!cut && sb < e0) { e = se; ++p_next; continue; }       // begins before this wave's edges: another's
             if (sb > e) { e = sb; if (e >= e1) return false; }
-            begin = e;
-            end = cut ? min(se, e1) : se;
+            const uint32_t end = cut ? min(se, e1) : se;
+            u.p = p_next++;
+            u.e = e;
+            u.n = min(end - e, 64u);
+            left = end - e - u.n;
+            u.first = true;
+            u.last = left == 0;
+            u.complete = !cut;
+            u.place = w * 2 + (e == e0 ? 0 : 1);
             e = end;
-            p = p_next++;
             return true;
         }
         return false;
     }
-    __device__ __forceinline__ bool complete() const { return begin == sb && end == se; }
-    // whether the whole wave lies inside this list; the same in all its lanes
-    __device__ __forceinline__ bool inside(uint32_t w, uint32_t chunk, uint32_t per_wave) const {
-        const uint32_t b = w / per_wave * per_wave * chunk;
-        return per_wave > 1 && se - sb > most && sb <= b && se >= b + per_wave * chunk;
-    }
-    // place (worker * 2 + 0 or 1) of this piece
-    __device__ __forceinline__ size_t place(uint32_t w) const { return (size_t)w * 2 + (begin == e0 ? 0 : 1); }
 };
 
-// The pieces of a parent with edges [b, e), more than 4 C, in order: the workers of a wave that is only
-// partly inside, one piece for each wave that lies inside (left by its first worker), the workers of the last wave.
-struct PieceList {
-    uint32_t first, n_head, n_full, full0, n_tail, tail0, cut;
-    __device__ __forceinline__ PieceList(uint32_t b, uint32_t e, uint32_t chunk, uint32_t per_wave) {
-        const uint32_t span = chunk * per_wave, a = (b + span - 1) / span, z = e / span;
-        first = b / chunk;
-        cut = b % chunk;                            // not 0: the first piece lies in its worker's second place
-        if (z > a && per_wave > 1) {
-            n_head = a * per_wave - first;
-            n_full = z - a;
-            full0 = a * per_wave;
-            tail0 = z * per_wave;
-            n_tail = e > z * span ? (e - 1) / chunk - tail0 + 1 : 0;
-        } else { n_head = (e - 1) / chunk - first + 1; n_full = n_tail = full0 = tail0 = 0; }
-        step = per_wave;
+// Pieces of a list [b, e) that was cut: the first lies in its wave's second place unless the list begins there.
+__device__ __forceinline__ size_t piece_place(uint32_t b, uint32_t chunk, uint32_t i) {
+    return (size_t)(b / chunk + i) * 2 + (i == 0 && b % chunk ? 1 : 0);
+}
+
+// Joins across the 64 / L row groups of a wave.  other<O>: the value of lane ^ O (or, for 8, of the lane half a row of 16
+// away, which is the same lane).
+template <int O> __device__ __forceinline__ float other(float v) {
+    if (O == 4) return __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), (4 << 10) | 0x1F));
+    if (O == 8) return dpp<0x128>(v);               // row_ror 8
+    return __shfl_xor(v, O, 64);
+}
+template <int L> __device__ __forceinline__ float groups_max(float v) {
+    if (L <= 32) {
+        auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+        v = fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
     }
-    uint32_t step;
-    __device__ __forceinline__ uint32_t count() const { return n_head + n_full + n_tail; }
-    // place (worker * 2 + 0 or 1) of piece i
-    __device__ __forceinline__ size_t place(uint32_t i) const {
-        if (i < n_head) return (size_t)(first + i) * 2 + (i == 0 && cut ? 1 : 0);
-        if (i < n_head + n_full) return (size_t)(full0 + (i - n_head) * step) * 2;
-        return (size_t)(tail0 + (i - n_head - n_full)) * 2;
+    if (L <= 16) {
+        auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+        v = fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+    }
+    if (L <= 8) v = fmaxf(v, other<8>(v));
+    if (L <= 4) v = fmaxf(v, other<4>(v));
+    return v;
+}
+template <int L> __device__ __forceinline__ float groups_sum(float v) {
+    if (L <= 32) {
+        auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+        v = __int_as_float(r[0]) + __int_as_float(r[1]);
+    }
+    if (L <= 16) {
+        auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+        v = __int_as_float(r[0]) + __int_as_float(r[1]);
+    }
+    if (L <= 8) v += other<8>(v);
+    if (L <= 4) v += other<4>(v);
+    return v;
+}
+
+// Sums N values per lane over the row groups, halving what a lane keeps at every step: x[0 .. kept) are then the sums of
+// values start .. start + kept - 1 of its element lane.  Lanes with dup set hold copies of another's.
+template <int N, int L> struct Scatter {
+    static constexpr int kGroups = 64 / L, kKept = N > kGroups ? N / kGroups : 1;
+    int start;
+    bool dup;
+    template <int C, int O> __device__ __forceinline__ void step(float *x, int lane64) {
+        if constexpr (O >= L) {
+            const bool up = lane64 & O;
+            if constexpr (C > 1) {
+                constexpr int H = C / 2;
+#pragma unroll
+                for (int i = 0; i < H; ++i) {
+                    if constexpr (O == 32) {
+                        auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x[i]), __float_as_int(x[i + H]), false, false);
+                        x[i] = __int_as_float(r[0]) + __int_as_float(r[1]);
+                    } else if constexpr (O == 16) {
+                        auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(x[i]), __float_as_int(x[i + H]), false, false);
+                        x[i] = __int_as_float(r[0]) + __int_as_float(r[1]);
+                    } else {
+                        const float a = x[i] + other<O>(x[i]), b = x[i + H] + other<O>(x[i + H]);
+                        x[i] = up ? b : a;
+                    }
+                }
+                if (up) start += H;
+            } else {
+                x[0] += other<O>(x[0]);
+                if (up) dup = true;
+            }
+            step<(C > 1 ? C / 2 : 1), O / 2>(x, lane64);
+        }
+    }
+    __device__ __forceinline__ void run(float *x, int lane64) {
+        start = 0;
+        dup = false;
+        step<N, 32>(x, lane64);
     }
 };
 
-constexpr int kJoinWaves = 8;
+constexpr int kJoinWaves = 16;
 
 // 16 bytes of a row per lane, as they arrive.
 template <class T, int L, bool ALIGNED> struct RowPart {
@@ -164,20 +228,19 @@ template <class T, int L, bool ALIGNED> struct RowPart {
     __device__ __forceinline__ float at(int i) const { return (float)x[i]; }
 };
 
-template <class T, int L, bool ALIGNED>
-__device__ __forceinline__ void store_row(T *row, int lane, int dim, const float *v) {
+// Stores values start .. start + N - 1 of a lane's part of a row.
+template <class T, int L, bool ALIGNED, int N>
+__device__ __forceinline__ void store_part(T *row, int lane, int dim, int start, const float *v) {
     constexpr int E = Pack<T>::E;
     if (ALIGNED) {
-        if (lane * E < dim) {
-            alignas(16) T x[E];
+        struct alignas(N * sizeof(T)) Part { T x[N]; } part;
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = (T)v[i];
-            reinterpret_cast<uint4 *>(row)[lane] = *reinterpret_cast<const uint4 *>(x);
-        }
+        for (int i = 0; i < N; ++i) part.x[i] = (T)v[i];
+        if (lane * E < dim) *reinterpret_cast<Part *>(row + lane * E + start) = part;
     } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (lane + i * L < dim) row[lane + i * L] = (T)v[i];
+        for (int i = 0; i < N; ++i)
+            if (lane + (start + i) * L < dim) row[lane + (start + i) * L] = (T)v[i];
     }
 }
 
@@ -194,32 +257,32 @@ inline int lanes_for(int dim, int size) {
     return l;
 }
 
-// Edges per worker, and whether any list may be cut.
+// Edges per wave, and whether any list may be cut.
 struct Deal {
-    int64_t chunk, workers;
+    int64_t chunk, waves;
     bool pieces;
 };
 
-inline Deal deal_edges(const int64_t *indptr, int64_t n_parents, int64_t n_child, int64_t n_edges, int lanes) {
+inline Deal deal_edges(const int64_t *indptr, int64_t n_child, int64_t n_edges, int lanes) {
     Deal d;
-    const int64_t per_wave = 64 / lanes;
-    if (!indptr && n_child > 0 && (n_child <= 4 * kAttnRows || n_parents >= 4096 * per_wave)) {
-        // lists of one length, short or many: whole lists, several where they are shorter than a round of loads
-        const int64_t group = n_child < kAttnRows && n_parents >= 32768 * per_wave ? (kAttnRows + n_child - 1) / n_child : 1;
-        d.chunk = group * n_child;
-    } else {
-        // one round of loads at least, then as many edges as leave 8192 waves (eight per SIMD), at most 128
-        int64_t c = n_edges / (8192 * per_wave);
-        c = (c + kAttnRows - 1) / kAttnRows * kAttnRows;
-        d.chunk = c < kAttnRows ? kAttnRows : c > 128 ? 128 : c;
-    }
-    d.pieces = indptr || n_child > 4 * d.chunk || n_child == 0;
-    d.workers = n_edges ? (n_edges + d.chunk - 1) / d.chunk : 0;
+    // two rounds of row loads at least, then as many edges as leave 8192 waves (eight per SIMD), at most 512
+    const int64_t round = 2 * kAttnRows * (64 / lanes);
+    int64_t c = (n_edges / 8192 + round - 1) / round * round;
+    c = c < round ? round : c > 512 ? 512 : c;
+    // lists of one length that are shorter than that: whole lists
+    if (!indptr && n_child > 0 && n_child <= c) c = c / n_child * n_child;
+    d.chunk = c;
+    d.pieces = indptr || n_child > 4 * c || n_child == 0;
+    d.waves = n_edges ? (n_edges + c - 1) / c : 0;
     return d;
 }
 
 // Whether the second launch has something to do for a list: it is empty, or was cut.
 __device__ __forceinline__ bool needs_join(uint32_t b, uint32_t e, uint32_t chunk) { return b == e || e - b > 4 * chunk; }
+
+__device__ __forceinline__ uint32_t this_wave() {
+    return __builtin_amdgcn_readfirstlane(blockIdx.x * (kAttnThreads / 64) + (threadIdx.x >> 6));
+}
 
 // Checks a gs_neighbors; 0 or the error.
 int check_neighbors(const char *what, const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype);

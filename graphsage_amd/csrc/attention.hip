@@ -36,8 +36,8 @@ struct FwdArgs {
     const void *q, *k, *v;
     void *out;
     float *lse;
-    float2 *piece_ms;                               // [workers][2][heads]: maximum (log 2), sum
-    float *piece_acc;                               // [workers][2][heads][dim]
+    float2 *piece_ms;                               // [waves][2][heads]: maximum (log 2), sum
+    float *piece_acc;                               // [waves][2][heads][dim]
     float scale2;                                   // scale * log2 e
     int heads, kv_heads, dim, chunk, parts;         // parts: head groups per key head
 };
@@ -45,36 +45,50 @@ struct FwdArgs {
 template <class T, int L, int G, bool ALIGNED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_fwd_kernel(FwdArgs a) {
-    constexpr int E = gs::Pack<T>::E, U = G * E >= 32 ? gs::kAttnRows / 2 : gs::kAttnRows;
-    constexpr uint32_t W = 64 / L;                  // workers per wave
-    const int lane = threadIdx.x & (L - 1);
-    const uint32_t w = blockIdx.x * (gs::kAttnThreads / L) + threadIdx.x / L;
+    constexpr int E = gs::Pack<T>::E, U = gs::kAttnRows, W = 64 / L;
+    const int lane64 = threadIdx.x & 63, lane = lane64 & (L - 1), group = lane64 / L;
     const int share = a.heads / a.kv_heads;
     const int j = blockIdx.y / a.parts, h0 = j * share + (blockIdx.y % a.parts) * G;
     const int n_heads = min(G, (j + 1) * share - h0);
-    const uint32_t C = a.chunk;
+    const T *Q = static_cast<const T *>(a.q);
     const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = a.v ? static_cast<const T *>(a.v) + (int64_t)j * a.dim : nullptr;
     const int64_t stride = (int64_t)a.kv_heads * a.dim;
 
-    gs::Walk walk(a.nb, w, C, L);
-    while (walk.next()) {
-        const int64_t p = walk.p;
-        const uint32_t end = walk.end;
-        float q[G][E], acc[G][E], m[G], s[G];
+    gs::Walk walk(a.nb, gs::this_wave(), a.chunk);
+    bool have = walk.next();
+    if (!have) return;
+    gs::Unit cur = walk.u;
+    int32_t rows = lane64 < cur.n ? a.nb.row_of(cur.e + lane64) : -1;
+    RowPart<T, L, ALIGNED> q_next[G];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            RowPart<T, L, ALIGNED> r;
-            if (g < n_heads) r.load(static_cast<const T *>(a.q) + (p * a.heads + h0 + g) * a.dim, lane, a.dim); else r.zero();
-            m[g] = -INFINITY;
-            s[g] = 0.f;
+    for (int g = 0; g < G; ++g)
+        if (g < n_heads) q_next[g].load(Q + (cur.p * a.heads + h0 + g) * a.dim, lane, a.dim); else q_next[g].zero();
+    float q[G][E], acc[G * E], m[G], s[G];
+    while (have) {
+        if (cur.first) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) { q[g][i] = r.at(i) * a.scale2; acc[g][i] = 0.f; }
+            for (int g = 0; g < G; ++g) {
+                m[g] = -INFINITY;
+                s[g] = 0.f;
+#pragma unroll
+                for (int i = 0; i < E; ++i) { q[g][i] = q_next[g].at(i) * a.scale2; acc[g * E + i] = 0.f; }
+            }
         }
-        for (uint32_t e = walk.begin; e < end; e += U) {
+        // the next unit's entries and queries are on their way while this one's rows are used
+        have = walk.next();
+        int32_t rows_next = -1;
+        if (have) {
+            if (lane64 < walk.u.n) rows_next = a.nb.row_of(walk.u.e + lane64);
+            if (walk.u.first)
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+                    if (g < n_heads) q_next[g].load(Q + (walk.u.p * a.heads + h0 + g) * a.dim, lane, a.dim);
+        }
+        for (uint32_t b = 0; b < cur.n; b += W * U) {
             int32_t row[U];
             RowPart<T, L, ALIGNED> kr[U], vr[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) row[u] = e + u < end ? a.nb.row_of(e + u) : -1;
+            for (int u = 0; u < U; ++u) row[u] = __shfl(rows, b + u * W + group, 64);     // (-1 behind the last entry)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (row[u] >= 0) kr[u].load(K + (int64_t)row[u] * stride, lane, a.dim); else kr[u].zero();
@@ -97,78 +111,96 @@ void attn_fwd_kernel(FwdArgs a) {
                 m[g] = top;
                 s[g] *= keep;
 #pragma unroll
-                for (int i = 0; i < E; ++i) acc[g][i] *= keep;
+                for (int i = 0; i < E; ++i) acc[g * E + i] *= keep;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const float pr = gs::fast_exp2(sc[u] - ref);
                     s[g] += pr;
 #pragma unroll
-                    for (int i = 0; i < E; ++i) acc[g][i] += pr * (V ? vr[u].at(i) : kr[u].at(i));
+                    for (int i = 0; i < E; ++i) acc[g * E + i] += pr * (V ? vr[u].at(i) : kr[u].at(i));
                 }
             }
         }
-        const bool complete = walk.complete(), merge = walk.inside(w, C, W);
-        if (merge) {
+        if (cur.last) {
 #pragma unroll
-            for (int g = 0; g < G; ++g)
+            for (int g = 0; g < G; ++g) {
+                const float top = gs::groups_max<L>(m[g]), ref = top == -INFINITY ? 0.f : top;
+                const float keep = gs::fast_exp2(m[g] - ref);
+                m[g] = top;
+                s[g] = gs::groups_sum<L>(s[g] * keep);
+                const float f = !cur.complete ? keep : s[g] > 0.f ? keep / s[g] : s[g] == 0.f ? 0.f : s[g];    // (a NaN stays one)
 #pragma unroll
-                for (int o = L; o < 64; o *= 2) {
-                    const float mo = __shfl_xor(m[g], o, 64), so = __shfl_xor(s[g], o, 64);
-                    const float top = fmaxf(m[g], mo), ref = top == -INFINITY ? 0.f : top;
-                    const float ka = gs::fast_exp2(m[g] - ref), kb = gs::fast_exp2(mo - ref);
-                    m[g] = top;
-                    s[g] = s[g] * ka + so * kb;
+                for (int i = 0; i < E; ++i) acc[g * E + i] *= f;
+            }
+            gs::Scatter<G * E, L> mine;
+            mine.run(acc, lane64);
+            constexpr int N = gs::Scatter<G * E, L>::kKept, S = N < E ? N : E;
 #pragma unroll
-                    for (int i = 0; i < E; ++i) acc[g][i] = acc[g][i] * ka + __shfl_xor(acc[g][i], o, 64) * kb;
+            for (int x = 0; x < N; x += S) {
+                const int g = (mine.start + x) / E, start = (mine.start + x) % E;
+                if (g >= n_heads || mine.dup) continue;
+                const int64_t o = cur.p * a.heads + h0 + g;
+                if (cur.complete) gs::store_part<T, L, ALIGNED, S>(static_cast<T *>(a.out) + o * a.dim, lane, a.dim, start, acc + x);
+                else {
+                    const size_t at = (size_t)cur.place * a.heads + h0 + g;
+#pragma unroll
+                    for (int i = 0; i < S; ++i) {
+                        const int d = gs::element_of<T, L, ALIGNED>(lane, start + i);
+                        if (d < a.dim) a.piece_acc[at * a.dim + d] = acc[x + i];
+                    }
                 }
-        }
+            }
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            if (g >= n_heads || (merge && w % W)) continue;
-            const int64_t o = p * a.heads + h0 + g;
-            if (complete) {
-                const float inv = s[g] > 0.f ? 1.f / s[g] : s[g] == 0.f ? 0.f : s[g];   // (nothing: zeros; a NaN stays one)
-#pragma unroll
-                for (int i = 0; i < E; ++i) acc[g][i] *= inv;
-                gs::store_row<T, L, ALIGNED>(static_cast<T *>(a.out) + o * a.dim, lane, a.dim, acc[g]);
-                if (lane == 0) a.lse[o] = (m[g] + gs::fast_log2(s[g])) * gs::kLn2;
-            } else {
-                const size_t at = walk.place(w) * a.heads + h0 + g;
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const int d = gs::element_of<T, L, ALIGNED>(lane, i);
-                    if (d < a.dim) a.piece_acc[at * a.dim + d] = acc[g][i];
-                }
-                if (lane == 0) a.piece_ms[at] = make_float2(m[g], s[g]);
+            for (int g = 0; g < G; ++g) {
+                if (lane64 != 0 || g >= n_heads) continue;
+                if (cur.complete) a.lse[cur.p * a.heads + h0 + g] = (m[g] + gs::fast_log2(s[g])) * gs::kLn2;
+                else a.piece_ms[(size_t)cur.place * a.heads + h0 + g] = make_float2(m[g], s[g]);
             }
         }
+        cur = walk.u;
+        rows = rows_next;
     }
 }
 
 // Joins the pieces of the lists that were cut and writes the parents without edges.  A block looks at 64 parents, far
-// apart (popular parents tend to be neighbors).  A wave joins a list of a few pieces by itself; of a long one the eight
-// waves take every eighth piece.
+// apart (popular parents tend to be neighbors).  A wave joins a list of a few pieces by itself; of a long one every
+// wave takes every sixteenth piece.
 constexpr uint32_t kFewPieces = 16;
 
 struct Joined {
     float m, s, acc[4];
 };
 
-__device__ __forceinline__ void join_pieces(const FwdArgs &a, const gs::PieceList &list, uint32_t i0, uint32_t step, int h, int lane, Joined &j) {
-    const uint32_t n = list.count();
-#pragma unroll 4
-    for (uint32_t i = i0; i < n; i += step) {
-        const size_t at = list.place(i) * a.heads + h;
-        const float2 ms = a.piece_ms[at];
-        float x[4];
+// Pieces i0, i0 + step, ... of list [b, e), four loads in flight.
+__device__ __forceinline__ void join_pieces(const FwdArgs &a, uint32_t b, uint32_t e, uint32_t i0, uint32_t step, int h, int lane, Joined &j) {
+    const uint32_t n = (e - 1) / a.chunk - b / a.chunk + 1;
+    for (uint32_t i = i0; i < n; i += 4 * step) {
+        float2 ms[4];
+        float x[4][4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) x[c] = lane + 64 * c < a.dim ? a.piece_acc[at * a.dim + lane + 64 * c] : 0.f;
-        const float top = fmaxf(j.m, ms.x), ref = top == -INFINITY ? 0.f : top;
-        const float ko = gs::fast_exp2(j.m - ref), kn = gs::fast_exp2(ms.x - ref);
+        for (int k = 0; k < 4; ++k) {
+            const bool in = i + k * step < n;
+            const size_t at = gs::piece_place(b, a.chunk, in ? i + k * step : i) * a.heads + h;
+            ms[k] = a.piece_ms[at];
+            if (!in) ms[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[k][c] = in && lane + 64 * c < a.dim ? a.piece_acc[at * a.dim + lane + 64 * c] : 0.f;
+        }
+        float top = j.m;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = fmaxf(top, ms[k].x);
+        const float ref = top == -INFINITY ? 0.f : top, ko = gs::fast_exp2(j.m - ref);
         j.m = top;
-        j.s = j.s * ko + ms.y * kn;
+        j.s *= ko;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) j.acc[c] = j.acc[c] * ko + x[c] * kn;
+        for (int c = 0; c < 4; ++c) j.acc[c] *= ko;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float kn = gs::fast_exp2(ms[k].x - ref);
+            j.s += ms[k].y * kn;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) j.acc[c] += x[k][c] * kn;
+        }
     }
 }
 
@@ -176,7 +208,7 @@ __device__ __forceinline__ float inverse_of(float s) { return s > 0.f ? 1.f / s 
 
 template <class T>
 __global__ __launch_bounds__(gs::kJoinWaves * 64)
-void attn_join_kernel(FwdArgs a, int per_wave) {
+void attn_join_kernel(FwdArgs a) {
     constexpr int N = gs::kJoinWaves;
     __shared__ float part[N][256 + 2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.y;
@@ -184,14 +216,14 @@ void attn_join_kernel(FwdArgs a, int per_wave) {
     uint32_t b = 0, e = 0;
     if (mine < a.nb.n_parents) a.nb.range(mine, b, e);
     const bool mine_todo = mine < a.nb.n_parents && gs::needs_join(b, e, a.chunk);
-    const bool many = mine_todo && e > b && gs::PieceList(b, e, a.chunk, per_wave).count() > kFewPieces;
+    const bool many = mine_todo && e > b && (e - 1) / a.chunk - b / a.chunk >= kFewPieces;
     unsigned long long few = __ballot(mine_todo && !many), long_ones = __ballot(many);
     for (int turn = 0; few; ++turn, few &= few - 1) {
         if (turn % N != wave) continue;
         const int src = __builtin_ctzll(few);
         const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
         Joined j{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
-        if (se > sb) join_pieces(a, gs::PieceList(sb, se, a.chunk, per_wave), 0, 1, h, lane, j);
+        if (se > sb) join_pieces(a, sb, se, 0, 1, h, lane, j);
         const int64_t at = ((int64_t)src * gridDim.x + blockIdx.x) * a.heads + h;
         const float inv = inverse_of(j.s);
 #pragma unroll
@@ -203,7 +235,7 @@ void attn_join_kernel(FwdArgs a, int per_wave) {
         const int src = __builtin_ctzll(long_ones);
         const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
         Joined j{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
-        join_pieces(a, gs::PieceList(sb, se, a.chunk, per_wave), wave, N, h, lane, j);
+        join_pieces(a, sb, se, wave, N, h, lane, j);
         __syncthreads();                            // the last list's parts are read
 #pragma unroll
         for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = j.acc[i];
@@ -228,12 +260,12 @@ void attn_join_kernel(FwdArgs a, int per_wave) {
 }
 
 template <class T, int L, bool ALIGNED>
-void launch_fwd(const FwdArgs &a, int64_t workers, hipStream_t stream) {
+void launch_fwd(const FwdArgs &a, int64_t waves, hipStream_t stream) {
     const int share = a.heads / a.kv_heads;
     FwdArgs b = a;
     const int g = share >= 3 ? 4 : share;
     b.parts = (share + g - 1) / g;
-    const dim3 grid((unsigned)((workers * L + gs::kAttnThreads - 1) / gs::kAttnThreads), (unsigned)(a.kv_heads * b.parts));
+    const dim3 grid((unsigned)((waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)(a.kv_heads * b.parts));
     if (g == 1) attn_fwd_kernel<T, L, 1, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
     else if (g == 2) attn_fwd_kernel<T, L, 2, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
     else attn_fwd_kernel<T, L, 4, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
@@ -241,42 +273,42 @@ void launch_fwd(const FwdArgs &a, int64_t workers, hipStream_t stream) {
 
 template <class T>
 int run_fwd(const FwdArgs &a, const gs::Deal &d, int lanes, bool aligned, hipStream_t stream) {
-    if (d.workers) {
+    if (d.waves) {
         if (aligned) {
-            if (lanes == 4) launch_fwd<T, 4, true>(a, d.workers, stream);
-            else if (lanes == 8) launch_fwd<T, 8, true>(a, d.workers, stream);
-            else if (lanes == 16) launch_fwd<T, 16, true>(a, d.workers, stream);
-            else if (lanes == 32) launch_fwd<T, 32, true>(a, d.workers, stream);
-            else launch_fwd<T, 64, true>(a, d.workers, stream);
+            if (lanes == 4) launch_fwd<T, 4, true>(a, d.waves, stream);
+            else if (lanes == 8) launch_fwd<T, 8, true>(a, d.waves, stream);
+            else if (lanes == 16) launch_fwd<T, 16, true>(a, d.waves, stream);
+            else if (lanes == 32) launch_fwd<T, 32, true>(a, d.waves, stream);
+            else launch_fwd<T, 64, true>(a, d.waves, stream);
         } else {
-            if (lanes == 4) launch_fwd<T, 4, false>(a, d.workers, stream);
-            else if (lanes == 8) launch_fwd<T, 8, false>(a, d.workers, stream);
-            else if (lanes == 16) launch_fwd<T, 16, false>(a, d.workers, stream);
-            else if (lanes == 32) launch_fwd<T, 32, false>(a, d.workers, stream);
-            else launch_fwd<T, 64, false>(a, d.workers, stream);
+            if (lanes == 4) launch_fwd<T, 4, false>(a, d.waves, stream);
+            else if (lanes == 8) launch_fwd<T, 8, false>(a, d.waves, stream);
+            else if (lanes == 16) launch_fwd<T, 16, false>(a, d.waves, stream);
+            else if (lanes == 32) launch_fwd<T, 32, false>(a, d.waves, stream);
+            else launch_fwd<T, 64, false>(a, d.waves, stream);
         }
         if (int rc = gs::check_launch("gs_neighbor_attention_fwd")) return rc;
     }
     if (d.pieces) {
         const dim3 grid((unsigned)((a.nb.n_parents + 63) / 64), (unsigned)a.heads);
-        attn_join_kernel<T><<<grid, gs::kJoinWaves * 64, 0, stream>>>(a, 64 / lanes);
+        attn_join_kernel<T><<<grid, gs::kJoinWaves * 64, 0, stream>>>(a);
         return gs::check_launch("gs_neighbor_attention_fwd (join)");
     }
     return GS_OK;
 }
 
 size_t pieces_bytes(const gs::Deal &d, int heads, int dim, size_t *off_acc) {
-    if (!d.pieces || !d.workers) { if (off_acc) *off_acc = 0; return 0; }
-    const size_t ms = gs::align256((size_t)d.workers * 2 * heads * sizeof(float2));
+    if (!d.pieces || !d.waves) { if (off_acc) *off_acc = 0; return 0; }
+    const size_t ms = gs::align256((size_t)d.waves * 2 * heads * sizeof(float2));
     if (off_acc) *off_acc = ms;
-    return ms + (size_t)d.workers * 2 * heads * dim * sizeof(float);
+    return ms + (size_t)d.waves * 2 * heads * dim * sizeof(float);
 }
 
 }  // namespace
 
 extern "C" size_t gs_neighbor_attention_workspace(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype) {
     if (gs::check_neighbors("gs_neighbor_attention_workspace", nb, heads, kv_heads, dim, dtype)) return 0;
-    const gs::Deal d = gs::deal_edges(nb->indptr, nb->n_parents, nb->n_child, nb->n_edges, gs::lanes_for(dim, gs::dtype_size(dtype)));
+    const gs::Deal d = gs::deal_edges(nb->indptr, nb->n_child, nb->n_edges, gs::lanes_for(dim, gs::dtype_size(dtype)));
     return pieces_bytes(d, heads, dim, nullptr);
 }
 
@@ -289,7 +321,7 @@ extern "C" int gs_neighbor_attention_fwd(const void *q, const void *k, const voi
     const int size = gs::dtype_size(dtype), lanes = gs::lanes_for(dim, size);
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & (size - 1))
         return gs::fail(GS_EINVAL, "gs_neighbor_attention_fwd: pointer not aligned to its element");
-    const gs::Deal d = gs::deal_edges(nb->indptr, nb->n_parents, nb->n_child, nb->n_edges, lanes);
+    const gs::Deal d = gs::deal_edges(nb->indptr, nb->n_child, nb->n_edges, lanes);
     size_t off_acc = 0;
     const size_t need = pieces_bytes(d, heads, dim, &off_acc);
     if (workspace_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 15))))

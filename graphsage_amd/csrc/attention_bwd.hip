@@ -23,7 +23,7 @@ struct BwdArgs {
     int32_t *edge_parent;                           // [n_edges], ragged neighborhoods only
     const int64_t *inv_indptr;
     const int32_t *inv_edges;
-    float *piece;                                   // parents: [workers][2][heads][dim]; rows: [workers][2][kv_heads][2][dim]
+    float *piece;                                   // parents: [waves][2][heads][dim]; rows: [waves][2][kv_heads][2][dim]
     float scale;
     int heads, kv_heads, dim, chunk, parts;
     uint32_t n_inv;
@@ -32,53 +32,55 @@ struct BwdArgs {
 template <class T, int L, int G, bool ALIGNED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_bwd_parents_kernel(BwdArgs a) {
-    constexpr int E = gs::Pack<T>::E, U = 4;
-    constexpr uint32_t W = 64 / L;
-    const int lane = threadIdx.x & (L - 1);
-    const uint32_t w = blockIdx.x * (gs::kAttnThreads / L) + threadIdx.x / L;
+    constexpr int E = gs::Pack<T>::E, U = gs::kAttnRows, W = 64 / L;
+    const int lane64 = threadIdx.x & 63, lane = lane64 & (L - 1), group = lane64 / L;
     const int share = a.heads / a.kv_heads;
     const int j = blockIdx.y / a.parts, h0 = j * share + (blockIdx.y % a.parts) * G;
     const int n_heads = min(G, (j + 1) * share - h0);
-    const uint32_t C = a.chunk;
     const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = a.v ? static_cast<const T *>(a.v) + (int64_t)j * a.dim : nullptr;
     const int64_t stride = (int64_t)a.kv_heads * a.dim;
     const float scale2 = a.scale * gs::kLog2e;
 
-    gs::Walk walk(a.nb, w, C, L);
-    while (walk.next()) {
-        const int64_t p = walk.p;
-        const uint32_t begin = walk.begin, end = walk.end;
-        if (a.edge_parent && blockIdx.y == 0)
-            for (uint32_t i = begin + lane; i < end; i += L) a.edge_parent[i] = (int32_t)p;
-
-        float q[G][E], go[G][E], acc[G][E], delta[G], lse2[G];
+    gs::Walk walk(a.nb, gs::this_wave(), a.chunk);
+    bool have = walk.next();
+    if (!have) return;
+    gs::Unit cur = walk.u;
+    int32_t rows = lane64 < cur.n ? a.nb.row_of(cur.e + lane64) : -1;
+    float q[G][E], go[G][E], acc[G * E], delta[G], lse2[G];
+    while (have) {
+        if (a.edge_parent && blockIdx.y == 0 && lane64 < cur.n) a.edge_parent[cur.e + lane64] = (int32_t)cur.p;
+        if (cur.first) {
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            RowPart<T, L, ALIGNED> r, o, d;
-            const int64_t at = p * a.heads + h0 + g;
-            lse2[g] = -INFINITY;
-            if (g < n_heads) {
-                r.load(static_cast<const T *>(a.q) + at * a.dim, lane, a.dim);
-                o.load(static_cast<const T *>(a.out) + at * a.dim, lane, a.dim);
-                d.load(static_cast<const T *>(a.g_out) + at * a.dim, lane, a.dim);
-                lse2[g] = a.lse[at] * gs::kLog2e;
-            } else { r.zero(); o.zero(); d.zero(); }
-            float dot = 0.f;
+            for (int g = 0; g < G; ++g) {
+                RowPart<T, L, ALIGNED> r, o, d;
+                const int64_t at = cur.p * a.heads + h0 + g;
+                lse2[g] = -INFINITY;
+                if (g < n_heads) {
+                    r.load(static_cast<const T *>(a.q) + at * a.dim, lane, a.dim);
+                    o.load(static_cast<const T *>(a.out) + at * a.dim, lane, a.dim);
+                    d.load(static_cast<const T *>(a.g_out) + at * a.dim, lane, a.dim);
+                    lse2[g] = a.lse[at] * gs::kLog2e;
+                } else { r.zero(); o.zero(); d.zero(); }
+                float dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                q[g][i] = r.at(i) * scale2;
-                go[g][i] = d.at(i);
-                dot += d.at(i) * o.at(i);
-                acc[g][i] = 0.f;
+                for (int i = 0; i < E; ++i) {
+                    q[g][i] = r.at(i) * scale2;
+                    go[g][i] = d.at(i);
+                    dot += d.at(i) * o.at(i);
+                    acc[g * E + i] = 0.f;
+                }
+                delta[g] = gs::lanes_sum<L>(dot);
+                // (written by every wave that has a part of the list: the same bits)
+                if (g < n_heads && lane64 == 0) a.delta[at] = delta[g];
             }
-            delta[g] = gs::lanes_sum<L>(dot);
-            if (g < n_heads && begin == walk.sb && lane == 0) a.delta[at] = delta[g];
         }
-        for (uint32_t e = begin; e < end; e += U) {
+        have = walk.next();
+        const int32_t rows_next = have && lane64 < walk.u.n ? a.nb.row_of(walk.u.e + lane64) : -1;
+        for (uint32_t b = 0; b < cur.n; b += W * U) {
             int32_t row[U];
             RowPart<T, L, ALIGNED> kr[U], vr[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) row[u] = e + u < end ? a.nb.row_of(e + u) : -1;
+            for (int u = 0; u < U; ++u) row[u] = __shfl(rows, b + u * W + group, 64);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (row[u] >= 0) kr[u].load(K + (int64_t)row[u] * stride, lane, a.dim); else kr[u].zero();
@@ -99,34 +101,34 @@ void attn_bwd_parents_kernel(BwdArgs a) {
                     const bool live = row[u] >= 0 && lse2[g] != -INFINITY;
                     const float ds = live ? gs::fast_exp2(s - lse2[g]) * (dp - delta[g]) : 0.f;
 #pragma unroll
-                    for (int i = 0; i < E; ++i) acc[g][i] += ds * kr[u].at(i);
+                    for (int i = 0; i < E; ++i) acc[g * E + i] += ds * kr[u].at(i);
                 }
             }
         }
-        const bool complete = walk.complete(), merge = walk.inside(w, C, W);
-        if (a.g_q) {
+        if (cur.last && a.g_q) {
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                if (merge)
+            for (int i = 0; i < G * E; ++i) acc[i] *= a.scale;
+            gs::Scatter<G * E, L> mine;
+            mine.run(acc, lane64);
+            constexpr int N = gs::Scatter<G * E, L>::kKept, S = N < E ? N : E;
 #pragma unroll
-                    for (int o = L; o < 64; o *= 2)
+            for (int x = 0; x < N; x += S) {
+                const int g = (mine.start + x) / E, start = (mine.start + x) % E;
+                if (g >= n_heads || mine.dup) continue;
+                if (cur.complete)
+                    gs::store_part<T, L, ALIGNED, S>(static_cast<T *>(a.g_q) + (cur.p * a.heads + h0 + g) * a.dim, lane, a.dim, start, acc + x);
+                else {
+                    const size_t at = (size_t)cur.place * a.heads + h0 + g;
 #pragma unroll
-                        for (int i = 0; i < E; ++i) acc[g][i] += __shfl_xor(acc[g][i], o, 64);
-                if (g >= n_heads || (merge && w % W)) continue;
-#pragma unroll
-                for (int i = 0; i < E; ++i) acc[g][i] *= a.scale;
-                if (complete) {
-                    gs::store_row<T, L, ALIGNED>(static_cast<T *>(a.g_q) + (p * a.heads + h0 + g) * a.dim, lane, a.dim, acc[g]);
-                } else {
-                    const size_t at = walk.place(w) * a.heads + h0 + g;
-#pragma unroll
-                    for (int i = 0; i < E; ++i) {
-                        const int d = gs::element_of<T, L, ALIGNED>(lane, i);
-                        if (d < a.dim) a.piece[at * a.dim + d] = acc[g][i];
+                    for (int i = 0; i < S; ++i) {
+                        const int d = gs::element_of<T, L, ALIGNED>(lane, start + i);
+                        if (d < a.dim) a.piece[at * a.dim + d] = acc[x + i];
                     }
                 }
             }
         }
+        cur = walk.u;
+        rows = rows_next;
     }
 }
 
@@ -135,52 +137,52 @@ void attn_bwd_parents_kernel(BwdArgs a) {
 template <class T, int L, int G, bool ALIGNED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_bwd_rows_kernel(BwdArgs a) {
-    constexpr int E = gs::Pack<T>::E;
+    constexpr int E = gs::Pack<T>::E, W = 64 / L;
     constexpr int U = G == 1 ? 4 : G == 2 ? 2 : 1;
-    constexpr uint32_t W = 64 / L;
-    const int lane = threadIdx.x & (L - 1);
-    const uint32_t w = blockIdx.x * (gs::kAttnThreads / L) + threadIdx.x / L;
+    const int lane64 = threadIdx.x & 63, lane = lane64 & (L - 1), group = lane64 / L;
     const int share = a.heads / a.kv_heads, j = blockIdx.y;
-    Neighbors rows;                                 // the lists of the rows, walked as the parents' are
-    rows.indptr = a.inv_indptr;
-    rows.ids = nullptr;
-    rows.n_parents = a.nb.n_rows;
-    rows.n_child = 1;
-    rows.n_edges = a.n_inv;
-    const uint32_t C = a.chunk;
+    Neighbors lists;                                // the lists of the rows, walked as the parents' are
+    lists.indptr = a.inv_indptr;
+    lists.ids = nullptr;
+    lists.n_parents = lists.n_rows = a.nb.n_rows;
+    lists.id_offset = 0;
+    lists.n_child = 1;
+    lists.n_edges = a.n_inv;
     const T *Q = static_cast<const T *>(a.q), *GO = static_cast<const T *>(a.g_out);
     const int64_t stride = (int64_t)a.kv_heads * a.dim;
     const float scale2 = a.scale * gs::kLog2e;
     int64_t first = 0, last = a.nb.n_edges;         // edges that belong to a parent
     if (!a.inv_indptr && a.nb.indptr) { first = a.nb.indptr[0]; last = a.nb.indptr[a.nb.n_parents]; }
+    const auto parent_of = [&](uint32_t entry) -> int32_t {
+        const int64_t x = a.inv_indptr ? (int64_t)a.inv_edges[entry] : (int64_t)entry;
+        if (x < first || x >= last || (uint64_t)x >= a.nb.n_edges) return -1;
+        const int32_t p = a.nb.indptr ? a.edge_parent[x] : (int32_t)((uint32_t)x / a.nb.n_child);
+        return (uint64_t)(int64_t)p < (uint64_t)a.nb.n_parents ? p : -1;
+    };
 
-    gs::Walk walk(rows, w, C, L);
-    while (walk.next()) {
-        const int64_t r = walk.p;
-        const uint32_t end = walk.end;
-        float key[E], val[E], gk[E], gv[E];
-        {
+    gs::Walk walk(lists, gs::this_wave(), a.chunk);
+    bool have = walk.next();
+    if (!have) return;
+    gs::Unit cur = walk.u;
+    int32_t parents = lane64 < cur.n ? parent_of(cur.e + lane64) : -1;
+    float key[E], val[E], sum[2 * E];               // sum: g_k, g_v
+    bool read = false;
+    while (have) {
+        if (cur.first) {
             RowPart<T, L, ALIGNED> kr, vr;
-            kr.load(static_cast<const T *>(a.k) + r * stride + (int64_t)j * a.dim, lane, a.dim);
-            if (a.v) vr.load(static_cast<const T *>(a.v) + r * stride + (int64_t)j * a.dim, lane, a.dim); else vr = kr;
+            kr.load(static_cast<const T *>(a.k) + cur.p * stride + (int64_t)j * a.dim, lane, a.dim);
+            if (a.v) vr.load(static_cast<const T *>(a.v) + cur.p * stride + (int64_t)j * a.dim, lane, a.dim); else vr = kr;
 #pragma unroll
-            for (int i = 0; i < E; ++i) { key[i] = kr.at(i) * scale2; val[i] = vr.at(i); gk[i] = 0.f; gv[i] = 0.f; }
+            for (int i = 0; i < E; ++i) { key[i] = kr.at(i) * scale2; val[i] = vr.at(i); sum[i] = sum[E + i] = 0.f; }
+            read = false;
         }
-        bool read = false;
-        for (uint32_t e = walk.begin; e < end; e += U) {
+        have = walk.next();
+        const int32_t parents_next = have && lane64 < walk.u.n ? parent_of(walk.u.e + lane64) : -1;
+        read |= __any(parents >= 0);
+        for (uint32_t b = 0; b < cur.n; b += W * U) {
             int32_t p[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                p[u] = -1;
-                if (e + u < end) {
-                    const int64_t x = a.inv_indptr ? (int64_t)a.inv_edges[e + u] : (int64_t)(e + u);
-                    if (x >= first && x < last && (uint64_t)x < a.nb.n_edges) {
-                        p[u] = a.nb.indptr ? a.edge_parent[x] : (int32_t)((uint32_t)x / a.nb.n_child);
-                        if ((uint64_t)(int64_t)p[u] >= (uint64_t)a.nb.n_parents) p[u] = -1;
-                    }
-                }
-                read |= p[u] >= 0;
-            }
+            for (int u = 0; u < U; ++u) p[u] = __shfl(parents, b + u * W + group, 64);
             for (int h0 = j * share; h0 < (j + 1) * share; h0 += G) {
                 RowPart<T, L, ALIGNED> qr[U][G], gr[U][G];
                 float lse2[U][G], delta[U][G];
@@ -210,35 +212,35 @@ void attn_bwd_rows_kernel(BwdArgs a) {
                         const float pr = lse2[u][g] != -INFINITY ? gs::fast_exp2(s - lse2[u][g]) : 0.f;
                         const float ds = pr * (dp - delta[u][g]) * a.scale;
 #pragma unroll
-                        for (int i = 0; i < E; ++i) { gk[i] += ds * qr[u][g].at(i); gv[i] += pr * gr[u][g].at(i); }
+                        for (int i = 0; i < E; ++i) { sum[i] += ds * qr[u][g].at(i); sum[E + i] += pr * gr[u][g].at(i); }
                     }
             }
         }
-        const bool complete = walk.complete();
-        if (!a.v)
+        if (cur.last && (a.inv_indptr || read)) {
+            if (!a.v)
 #pragma unroll
-            for (int i = 0; i < E; ++i) gk[i] += gv[i];
-        if (complete) {
-            if (a.inv_indptr || read) {
-                const int64_t at = r * stride + (int64_t)j * a.dim;
-                if (a.g_k) gs::store_row<T, L, ALIGNED>(static_cast<T *>(a.g_k) + at, lane, a.dim, gk);
-                if (a.g_v) gs::store_row<T, L, ALIGNED>(static_cast<T *>(a.g_v) + at, lane, a.dim, gv);
-            }
-        } else {
-            if (walk.inside(w, C, W)) {
+                for (int i = 0; i < E; ++i) sum[i] += sum[E + i];
+            gs::Scatter<2 * E, L> mine;
+            mine.run(sum, lane64);
+            constexpr int N = gs::Scatter<2 * E, L>::kKept, S = N < E ? N : E;
 #pragma unroll
-                for (int o = L; o < 64; o *= 2)
+            for (int x = 0; x < N; x += S) {
+                const int set = (mine.start + x) / E, start = (mine.start + x) % E;
+                T *out = static_cast<T *>(set ? a.g_v : a.g_k);
+                if (!out || mine.dup) continue;
+                if (cur.complete) gs::store_part<T, L, ALIGNED, S>(out + cur.p * stride + (int64_t)j * a.dim, lane, a.dim, start, sum + x);
+                else {
+                    const size_t at = ((size_t)cur.place * a.kv_heads + j) * 2 + set;
 #pragma unroll
-                    for (int i = 0; i < E; ++i) { gk[i] += __shfl_xor(gk[i], o, 64); gv[i] += __shfl_xor(gv[i], o, 64); }
-                if (w % W) continue;
-            }
-            const size_t at = (walk.place(w) * a.kv_heads + j) * 2;
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const int d = gs::element_of<T, L, ALIGNED>(lane, i);
-                if (d < a.dim) { a.piece[at * a.dim + d] = gk[i]; a.piece[(at + 1) * a.dim + d] = gv[i]; }
+                    for (int i = 0; i < S; ++i) {
+                        const int d = gs::element_of<T, L, ALIGNED>(lane, start + i);
+                        if (d < a.dim) a.piece[at * a.dim + d] = sum[x + i];
+                    }
+                }
             }
         }
+        cur = walk.u;
+        parents = parents_next;
     }
 }
 
@@ -248,8 +250,7 @@ constexpr uint32_t kFewPieces = 16;
 
 template <class T>
 __global__ __launch_bounds__(gs::kJoinWaves * 64)
-void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int sets, int dim, int chunk, int per_wave, T *out0,
-                          T *out1) {
+void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int sets, int dim, uint32_t chunk, T *out0, T *out1) {
     constexpr int N = gs::kJoinWaves;
     __shared__ float part[N][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, y = blockIdx.y;
@@ -257,17 +258,23 @@ void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int s
     uint32_t b = 0, e = 0;
     if (mine < seg.n_parents) seg.range(mine, b, e);
     const bool mine_todo = mine < seg.n_parents && gs::needs_join(b, e, chunk);
-    const bool many = mine_todo && e > b && gs::PieceList(b, e, chunk, per_wave).count() > kFewPieces;
+    const bool many = mine_todo && e > b && (e - 1) / chunk - b / chunk >= kFewPieces;
     unsigned long long few = __ballot(mine_todo && !many), long_ones = __ballot(many);
     const auto add = [&](uint32_t sb, uint32_t se, uint32_t i0, uint32_t step, int set, float (&acc)[4]) {
-        const gs::PieceList list(sb, se, chunk, per_wave);
-        const uint32_t n = list.count();
-#pragma unroll 4
-        for (uint32_t i = i0; i < n; i += step) {
-            const size_t at = ((list.place(i) * per_slot + y) * sets + set) * dim;
+        const uint32_t n = (se - 1) / chunk - sb / chunk + 1;
+        for (uint32_t i = i0; i < n; i += 4 * step) {
+            float x[4][4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (lane + 64 * c < dim) acc[c] += piece[at + lane + 64 * c];
+            for (int k = 0; k < 4; ++k) {
+                const bool in = i + k * step < n;
+                const size_t at = ((gs::piece_place(sb, chunk, in ? i + k * step : i) * per_slot + y) * sets + set) * dim;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[k][c] = in && lane + 64 * c < dim ? piece[at + lane + 64 * c] : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[c] += x[k][c];
         }
     };
     for (int turn = 0; few; ++turn, few &= few - 1) {
@@ -309,20 +316,20 @@ void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int s
 }
 
 template <class T, int L, bool ALIGNED>
-void launch_parents(const BwdArgs &a, int64_t workers, hipStream_t stream) {
+void launch_parents(const BwdArgs &a, int64_t waves, hipStream_t stream) {
     const int share = a.heads / a.kv_heads, g = share >= 3 ? 4 : share;
     BwdArgs b = a;
     b.parts = (share + g - 1) / g;
-    const dim3 grid((unsigned)((workers * L + gs::kAttnThreads - 1) / gs::kAttnThreads), (unsigned)(a.kv_heads * b.parts));
+    const dim3 grid((unsigned)((waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)(a.kv_heads * b.parts));
     if (g == 1) attn_bwd_parents_kernel<T, L, 1, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
     else if (g == 2) attn_bwd_parents_kernel<T, L, 2, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
     else attn_bwd_parents_kernel<T, L, 4, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
 }
 
 template <class T, int L, bool ALIGNED>
-void launch_rows(const BwdArgs &a, int64_t workers, hipStream_t stream) {
+void launch_rows(const BwdArgs &a, int64_t waves, hipStream_t stream) {
     const int share = a.heads / a.kv_heads;
-    const dim3 grid((unsigned)((workers * L + gs::kAttnThreads - 1) / gs::kAttnThreads), (unsigned)a.kv_heads);
+    const dim3 grid((unsigned)((waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)a.kv_heads);
     if (share == 1) attn_bwd_rows_kernel<T, L, 1, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
     else if (share == 2) attn_bwd_rows_kernel<T, L, 2, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
     else attn_bwd_rows_kernel<T, L, 4, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
@@ -354,18 +361,18 @@ struct Plan {
 Plan make_plan(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype, int64_t n_inv) {
     Plan p;
     const int lanes = gs::lanes_for(dim, gs::dtype_size(dtype));
-    p.parents = gs::deal_edges(nb->indptr, nb->n_parents, nb->n_child, nb->n_edges, lanes);
+    p.parents = gs::deal_edges(nb->indptr, nb->n_child, nb->n_edges, lanes);
     static const int64_t ragged = 0;                // any address: the rows' lists are ragged
-    p.rows = nb->ids ? gs::deal_edges(&ragged, nb->n_rows, 0, n_inv, lanes)
-                     : gs::deal_edges(nullptr, nb->n_rows, 1, nb->n_rows, lanes);
+    p.rows = nb->ids ? gs::deal_edges(&ragged, 0, n_inv, lanes)
+                     : gs::deal_edges(nullptr, 1, nb->n_rows, lanes);
     size_t off = gs::align256((size_t)nb->n_parents * heads * sizeof(float));        // delta
     p.off_parent = off;
     if (nb->indptr) off += gs::align256((size_t)nb->n_edges * sizeof(int32_t));
     p.off_piece = off;
     size_t piece = 0;
-    if (p.parents.pieces) piece = (size_t)p.parents.workers * 2 * heads * dim * sizeof(float);
+    if (p.parents.pieces) piece = (size_t)p.parents.waves * 2 * heads * dim * sizeof(float);
     if (p.rows.pieces) {
-        const size_t r = (size_t)p.rows.workers * 4 * kv_heads * dim * sizeof(float);
+        const size_t r = (size_t)p.rows.waves * 4 * kv_heads * dim * sizeof(float);
         if (r > piece) piece = r;
     }
     p.total = off + piece;
@@ -375,19 +382,19 @@ Plan make_plan(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dty
 template <class T>
 int run_bwd(BwdArgs a, const Plan &p, int lanes, bool aligned, hipStream_t stream) {
     a.chunk = (int)p.parents.chunk;
-    if (p.parents.workers) {
-        GS_BY_LANES(launch_parents, a, p.parents.workers, stream);
+    if (p.parents.waves) {
+        GS_BY_LANES(launch_parents, a, p.parents.waves, stream);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents)")) return rc;
     }
     if (a.g_q && a.nb.n_parents && p.parents.pieces) {
         attn_bwd_join_kernel<T><<<dim3((unsigned)((a.nb.n_parents + 63) / 64), (unsigned)a.heads), gs::kJoinWaves * 64, 0, stream>>>(
-            a.nb, a.piece, a.heads, 1, a.dim, a.chunk, 64 / lanes, static_cast<T *>(a.g_q), (T *)nullptr);
+            a.nb, a.piece, a.heads, 1, a.dim, a.chunk, static_cast<T *>(a.g_q), (T *)nullptr);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents' join)")) return rc;
     }
     if (!a.g_k && !a.g_v) return GS_OK;
     a.chunk = (int)p.rows.chunk;
-    if (p.rows.workers) {
-        GS_BY_LANES(launch_rows, a, p.rows.workers, stream);
+    if (p.rows.waves) {
+        GS_BY_LANES(launch_rows, a, p.rows.waves, stream);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (rows)")) return rc;
     }
     if (a.inv_indptr && a.nb.n_rows) {
@@ -396,7 +403,7 @@ int run_bwd(BwdArgs a, const Plan &p, int lanes, bool aligned, hipStream_t strea
         rows.n_parents = a.nb.n_rows;
         rows.n_edges = a.n_inv;
         attn_bwd_join_kernel<T><<<dim3((unsigned)((a.nb.n_rows + 63) / 64), (unsigned)a.kv_heads), gs::kJoinWaves * 64, 0, stream>>>(
-            rows, a.piece, a.kv_heads, 2, a.dim, a.chunk, 64 / lanes, static_cast<T *>(a.g_k), static_cast<T *>(a.g_v));
+            rows, a.piece, a.kv_heads, 2, a.dim, a.chunk, static_cast<T *>(a.g_k), static_cast<T *>(a.g_v));
         return gs::check_launch("gs_neighbor_attention_bwd (rows' join)");
     }
     return GS_OK;
