@@ -2,9 +2,10 @@
 //
 // A row of dim elements is covered by L lanes, 16 bytes each (L = the power of two >= dim / (elements in 16 bytes)), so
 // a wave holds 64 / L rows at a time and keeps kAttnRows such groups in flight.  A dot product is a few multiply-adds per
-// lane and a sum over L lanes; a row is read once, whatever the number of heads that share it.  Tables whose rows do not
-// start on 16 bytes are read element by element: lane l then holds elements l, l + L, ...; nothing else depends on which
-// element sits where.
+// lane (16-bit types: two products per instruction, straight from the packed row) and a sum over L lanes; a row is read
+// once, whatever the number of heads that share it.  Loads ask for the alignment of an element only, which the hardware
+// serves at 16 bytes a lane; where dim is not a multiple of those, the last lane takes the last 16 bytes of the row and
+// the elements it shares with its neighbor count there alone.
 //
 // A wave works on one list (the neighbors of one parent) at a time: control flow and list bounds are scalar, lists of any
 // length leave no lane waiting for another lane's list (measured against a list per L lanes: the ragged whole graph, 2M
@@ -23,18 +24,23 @@
 namespace gs {
 
 constexpr int kAttnThreads = 256;
-constexpr int kAttnRows = 4;                        // rows in flight per L lanes
+constexpr int kAttnRows = 4;                        // rows in flight per L lanes (L = 2: two, 64 in a wave)
+
+// Offsets are read with scalar loads: they do not change while a kernel runs.
+using ConstOffsets = const __attribute__((address_space(4))) int64_t *;
 
 struct Neighbors {
     const int64_t *indptr;
+    __device__ __forceinline__ int64_t offset(int64_t i) const { return ((ConstOffsets)(uintptr_t)indptr)[i]; }
     const int32_t *ids;
     int64_t n_parents, id_offset, n_rows;
     uint32_t n_child, n_edges;
 
     // [begin, end) of parent p, inside [0, n_edges] whatever indptr holds
-    __device__ __forceinline__ void range(int64_t p, uint32_t &b, uint32_t &e) const {
+    // (scalar: p is the same in all lanes)
+    __device__ __forceinline__ void range(int64_t p, uint32_t &b, uint32_t &e, bool scalar = false) const {
         if (!indptr) { b = (uint32_t)p * n_child; e = b + n_child; return; }
-        const int64_t x = indptr[p], y = indptr[p + 1];
+        const int64_t x = scalar ? offset(p) : indptr[p], y = scalar ? offset(p + 1) : indptr[p + 1];
         b = (uint32_t)(x < 0 ? 0 : x > n_edges ? n_edges : x);
         e = (uint32_t)(y < 0 ? 0 : y > n_edges ? n_edges : y);
         if (e < b) e = b;
@@ -44,11 +50,11 @@ struct Neighbors {
     __device__ __forceinline__ int64_t seek(uint32_t e, int64_t p) const {
         if (!indptr) return e / n_child;
         int64_t step = 1, lo = p, hi = p;
-        while (hi < n_parents && indptr[hi + 1] <= (int64_t)e) { lo = hi + 1; hi += step; step *= 2; }
+        while (hi < n_parents && offset(hi + 1) <= (int64_t)e) { lo = hi + 1; hi += step; step *= 2; }
         if (hi > n_parents) hi = n_parents;
         while (lo < hi) {
             const int64_t mid = (lo + hi) >> 1;
-            if (indptr[mid + 1] > (int64_t)e) hi = mid; else lo = mid + 1;
+            if (offset(mid + 1) > (int64_t)e) hi = mid; else lo = mid + 1;
         }
         return lo;
     }
@@ -68,9 +74,11 @@ struct Neighbors {
         }
         return lo;
     }
-    // table row of edge e, or -1
-    __device__ __forceinline__ int32_t row_of(uint32_t e) const {
-        const int64_t r = ids ? (int64_t)ids[e] - id_offset : (int64_t)e;
+    // Entry e of the lists as it stands in memory, and the table row it means, or -1: two steps, so that a load can be
+    // on its way for a while.
+    __device__ __forceinline__ int32_t entry(uint32_t e) const { return ids ? ids[min(e, n_edges - 1)] : (int32_t)e; }
+    __device__ __forceinline__ int32_t row_of(int32_t entry) const {
+        const int64_t r = ids ? (int64_t)entry - id_offset : (int64_t)entry;
         return (uint64_t)r < (uint64_t)n_rows ? (int32_t)r : -1;
     }
 };
@@ -107,7 +115,7 @@ struct Walk {
         }
         while (e < e1 && p_next < nb.n_parents) {
             uint32_t sb, se;
-            nb.range(p_next, sb, se);
+            nb.range(p_next, sb, se, true);
             if (se <= e) { p_next = nb.seek(e, p_next + 1); continue; }
             const bool cut = se - sb > most;
             if (!cut && sb < e0) { e = se; ++p_next; continue; }       // begins before this wave's edges: another's
@@ -137,6 +145,7 @@ __device__ __forceinline__ size_t piece_place(uint32_t b, uint32_t chunk, uint32
 // away, which is the same lane).
 template <int O> __device__ __forceinline__ float other(float v) {
     if (O == 4) return __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), (4 << 10) | 0x1F));
+    if (O == 2) return dpp<0x4E>(v);                // quad_perm 2 3 0 1
     if (O == 8) return dpp<0x128>(v);               // row_ror 8
     return __shfl_xor(v, O, 64);
 }
@@ -151,6 +160,7 @@ template <int L> __device__ __forceinline__ float groups_max(float v) {
     }
     if (L <= 8) v = fmaxf(v, other<8>(v));
     if (L <= 4) v = fmaxf(v, other<4>(v));
+    if (L <= 2) v = fmaxf(v, other<2>(v));
     return v;
 }
 template <int L> __device__ __forceinline__ float groups_sum(float v) {
@@ -164,6 +174,7 @@ template <int L> __device__ __forceinline__ float groups_sum(float v) {
     }
     if (L <= 8) v += other<8>(v);
     if (L <= 4) v += other<4>(v);
+    if (L <= 2) v += other<2>(v);
     return v;
 }
 
@@ -208,50 +219,88 @@ template <int N, int L> struct Scatter {
 
 constexpr int kJoinWaves = 16;
 
-// 16 bytes of a row per lane, as they arrive.
-template <class T, int L, bool ALIGNED> struct RowPart {
+// Where a lane's 16 bytes of a row begin, and how many of its elements belong to the lane before it (E or more: all).
+// L = 2 stands for rows shorter than 16 bytes, read element by element.
+template <class T, int L> struct Place {
+    static constexpr int E = Pack<T>::E;
+    int off, skip, dim;
+    __device__ __forceinline__ Place(int lane, int d) {
+        off = L == 2 ? 0 : min(lane * E, d - E);
+        skip = lane * E - off;
+        dim = d;
+    }
+};
+
+// 16 bytes of a row, as they arrive.
+template <class T> struct RowPart {
     static constexpr int E = Pack<T>::E;
     T x[E];
-    __device__ __forceinline__ void load(const T *row, int lane, int dim) {
-        if (ALIGNED) {
-            if (lane * E < dim) *reinterpret_cast<uint4 *>(x) = reinterpret_cast<const uint4 *>(row)[lane];
-            else *reinterpret_cast<uint4 *>(x) = make_uint4(0, 0, 0, 0);
-        } else {
-#pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = lane + i * L < dim ? row[lane + i * L] : (T)0.f;
-        }
-    }
     __device__ __forceinline__ void zero() {
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        __builtin_memcpy(x, &z, 16);
+    }
+    __device__ __forceinline__ void zero_if(bool c) {
+        uint4 v;
+        __builtin_memcpy(&v, x, 16);
+        v.x = c ? 0 : v.x; v.y = c ? 0 : v.y; v.z = c ? 0 : v.z; v.w = c ? 0 : v.w;
+        __builtin_memcpy(x, &v, 16);
+    }
+    template <int L> __device__ __forceinline__ void load(const T *row, const Place<T, L> &at) {
+        if (L != 2) __builtin_memcpy(x, row + at.off, 16);
+        else
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = (T)0.f;
+            for (int i = 0; i < E; ++i) x[i] = i < at.dim ? row[i] : (T)0.f;
+    }
+    // zeros in place of the elements that count in another lane: for one side of every dot product
+    template <int L> __device__ __forceinline__ void own(const Place<T, L> &at) {
+        if (L == 2 || at.dim % E)
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = i < at.skip ? (T)0.f : x[i];
+        else zero_if(at.skip > 0);
     }
     __device__ __forceinline__ float at(int i) const { return (float)x[i]; }
 };
 
-// Stores values start .. start + N - 1 of a lane's part of a row.
-template <class T, int L, bool ALIGNED, int N>
-__device__ __forceinline__ void store_part(T *row, int lane, int dim, int start, const float *v) {
-    constexpr int E = Pack<T>::E;
-    if (ALIGNED) {
-        struct alignas(N * sizeof(T)) Part { T x[N]; } part;
+__device__ __forceinline__ float dot(const RowPart<float> &a, const RowPart<float> &b) {
+    float d = a.x[0] * b.x[0];
 #pragma unroll
-        for (int i = 0; i < N; ++i) part.x[i] = (T)v[i];
-        if (lane * E < dim) *reinterpret_cast<Part *>(row + lane * E + start) = part;
+    for (int i = 1; i < 4; ++i) d = __builtin_fmaf(a.x[i], b.x[i], d);
+    return d;
+}
+__device__ __forceinline__ float dot(const RowPart<__bf16> &a, const RowPart<__bf16> &b) {
+    using V = __attribute__((ext_vector_type(2))) __bf16;
+    float d = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) d = __builtin_amdgcn_fdot2_f32_bf16(V{a.x[i], a.x[i + 1]}, V{b.x[i], b.x[i + 1]}, d, false);
+    return d;
+}
+__device__ __forceinline__ float dot(const RowPart<_Float16> &a, const RowPart<_Float16> &b) {
+    using V = __attribute__((ext_vector_type(2))) _Float16;
+    float d = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) d = __builtin_amdgcn_fdot2(V{a.x[i], a.x[i + 1]}, V{b.x[i], b.x[i + 1]}, d, false);
+    return d;
+}
+
+// Stores values start .. start + N - 1 of a lane's part of a row, those that count in this lane.
+template <int N, class T, int L, class O>
+__device__ __forceinline__ void store_part(O *row, const Place<T, L> &at, int start, const float *v) {
+    if (L != 2 && at.skip <= 0) {
+        O x[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = (O)v[i];
+        __builtin_memcpy(row + at.off + start, x, N * sizeof(O));
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (lane + (start + i) * L < dim) row[lane + (start + i) * L] = (T)v[i];
+            if (start + i >= at.skip && at.off + start + i < at.dim) row[at.off + start + i] = (O)v[i];
     }
-}
-
-// Element index of part i of a lane, for the fp32 pieces in the workspace.
-template <class T, int L, bool ALIGNED> __device__ __forceinline__ int element_of(int lane, int i) {
-    return ALIGNED ? lane * Pack<T>::E + i : lane + i * L;
 }
 
 // Lanes per row: enough for dim elements at 16 bytes a lane.
 inline int lanes_for(int dim, int size) {
     const int per = 16 / size;
+    if (dim < per) return 2;
     int l = 4;
     while (l * per < dim) l *= 2;
     return l;
@@ -277,12 +326,42 @@ inline Deal deal_edges(const int64_t *indptr, int64_t n_child, int64_t n_edges, 
     return d;
 }
 
+// A table without rows leaves every parent without neighbors.
+inline Deal deal_edges(const gs_neighbors *nb, int lanes) {
+    return nb->n_rows ? deal_edges(nb->indptr, nb->n_child, nb->n_edges, lanes) : deal_edges(nullptr, 0, 0, lanes);
+}
+inline Neighbors device_neighbors(const gs_neighbors *nb) {
+    if (!nb->n_rows) return Neighbors{nullptr, nb->ids, nb->n_parents, 0, 0, 0, 0};
+    return Neighbors{nb->indptr, nb->ids, nb->n_parents, nb->id_offset, nb->n_rows, (uint32_t)(nb->indptr ? 0 : nb->n_child),
+                     (uint32_t)nb->n_edges};
+}
+
 // Whether the second launch has something to do for a list: it is empty, or was cut.
 __device__ __forceinline__ bool needs_join(uint32_t b, uint32_t e, uint32_t chunk) { return b == e || e - b > 4 * chunk; }
 
 __device__ __forceinline__ uint32_t this_wave() {
     return __builtin_amdgcn_readfirstlane(blockIdx.x * (kAttnThreads / 64) + (threadIdx.x >> 6));
 }
+
+// f<T, lanes, flag>(...)
+#define GS_BY_LANES(f, flag, ...)                                          \
+    do {                                                                   \
+        if (flag) {                                                        \
+            if (lanes == 2) f<T, 2, true>(__VA_ARGS__);                    \
+            else if (lanes == 4) f<T, 4, true>(__VA_ARGS__);               \
+            else if (lanes == 8) f<T, 8, true>(__VA_ARGS__);               \
+            else if (lanes == 16) f<T, 16, true>(__VA_ARGS__);             \
+            else if (lanes == 32) f<T, 32, true>(__VA_ARGS__);             \
+            else f<T, 64, true>(__VA_ARGS__);                              \
+        } else {                                                           \
+            if (lanes == 2) f<T, 2, false>(__VA_ARGS__);                   \
+            else if (lanes == 4) f<T, 4, false>(__VA_ARGS__);              \
+            else if (lanes == 8) f<T, 8, false>(__VA_ARGS__);              \
+            else if (lanes == 16) f<T, 16, false>(__VA_ARGS__);            \
+            else if (lanes == 32) f<T, 32, false>(__VA_ARGS__);            \
+            else f<T, 64, false>(__VA_ARGS__);                             \
+        }                                                                  \
+    } while (0)
 
 // Checks a gs_neighbors; 0 or the error.
 int check_neighbors(const char *what, const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype);

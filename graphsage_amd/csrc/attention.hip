@@ -42,68 +42,75 @@ struct FwdArgs {
     int heads, kv_heads, dim, chunk, parts;         // parts: head groups per key head
 };
 
-template <class T, int L, int G, bool ALIGNED>
+template <class T, int L, int G, bool SHARED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_fwd_kernel(FwdArgs a) {
-    constexpr int E = gs::Pack<T>::E, U = gs::kAttnRows, W = 64 / L;
+    constexpr int E = gs::Pack<T>::E, W = 64 / L, U = L == 2 ? 2 : gs::kAttnRows;
     const int lane64 = threadIdx.x & 63, lane = lane64 & (L - 1), group = lane64 / L;
     const int share = a.heads / a.kv_heads;
     const int j = blockIdx.y / a.parts, h0 = j * share + (blockIdx.y % a.parts) * G;
     const int n_heads = min(G, (j + 1) * share - h0);
     const T *Q = static_cast<const T *>(a.q);
-    const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = a.v ? static_cast<const T *>(a.v) + (int64_t)j * a.dim : nullptr;
+    const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = SHARED ? nullptr : static_cast<const T *>(a.v) + (int64_t)j * a.dim;
     const int64_t stride = (int64_t)a.kv_heads * a.dim;
+    const gs::Place<T, L> at(lane, a.dim);
 
     gs::Walk walk(a.nb, gs::this_wave(), a.chunk);
     bool have = walk.next();
     if (!have) return;
     gs::Unit cur = walk.u;
-    int32_t rows = lane64 < cur.n ? a.nb.row_of(cur.e + lane64) : -1;
-    RowPart<T, L, ALIGNED> q_next[G];
+    int32_t entry = a.nb.entry(cur.e + lane64);
+    RowPart<T> q[G], q_next[G];
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-        if (g < n_heads) q_next[g].load(Q + (cur.p * a.heads + h0 + g) * a.dim, lane, a.dim); else q_next[g].zero();
-    float q[G][E], acc[G * E], m[G], s[G];
+    for (int g = 0; g < G; ++g)                     // (heads past the last one repeat it)
+        q_next[g].load(Q + (cur.p * a.heads + h0 + min(g, n_heads - 1)) * a.dim, at);
+    float acc[G * E], m[G], s[G];
     while (have) {
         if (cur.first) {
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 m[g] = -INFINITY;
                 s[g] = 0.f;
+                q[g] = q_next[g];
+                q[g].own(at);
 #pragma unroll
-                for (int i = 0; i < E; ++i) { q[g][i] = q_next[g].at(i) * a.scale2; acc[g * E + i] = 0.f; }
+                for (int i = 0; i < E; ++i) acc[g * E + i] = 0.f;
             }
         }
+        const int32_t rows = lane64 < cur.n ? a.nb.row_of(entry) : -1;
+        const bool gaps = __any(rows < 0 && lane64 < cur.n) || cur.n % (W * U);
         // the next unit's entries and queries are on their way while this one's rows are used
         have = walk.next();
-        int32_t rows_next = -1;
         if (have) {
-            if (lane64 < walk.u.n) rows_next = a.nb.row_of(walk.u.e + lane64);
+            entry = a.nb.entry(walk.u.e + lane64);
             if (walk.u.first)
 #pragma unroll
-                for (int g = 0; g < G; ++g)
-                    if (g < n_heads) q_next[g].load(Q + (walk.u.p * a.heads + h0 + g) * a.dim, lane, a.dim);
+                for (int g = 0; g < G; ++g) q_next[g].load(Q + (walk.u.p * a.heads + h0 + min(g, n_heads - 1)) * a.dim, at);
         }
         for (uint32_t b = 0; b < cur.n; b += W * U) {
             int32_t row[U];
-            RowPart<T, L, ALIGNED> kr[U], vr[U];
+            RowPart<T> kr[U], vr[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) row[u] = __shfl(rows, b + u * W + group, 64);     // (-1 behind the last entry)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (row[u] >= 0) kr[u].load(K + (int64_t)row[u] * stride, lane, a.dim); else kr[u].zero();
-                if (V) { if (row[u] >= 0) vr[u].load(V + (int64_t)row[u] * stride, lane, a.dim); else vr[u].zero(); }
+                const int64_t to = (int64_t)max(row[u], 0) * stride;   // (what is no neighbor reads row 0 and forgets it)
+                kr[u].load(K + to, at);
+                if (!SHARED) vr[u].load(V + to, at);
             }
+            if (gaps)
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    kr[u].zero_if(row[u] < 0);
+                    if (!SHARED) vr[u].zero_if(row[u] < 0);
+                }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 float sc[U], top = m[g];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    float d = 0.f;
-#pragma unroll
-                    for (int i = 0; i < E; ++i) d += q[g][i] * kr[u].at(i);
-                    d = gs::lanes_sum<L>(d);
-                    sc[u] = row[u] >= 0 ? d : -INFINITY;
+                    const float d = gs::lanes_sum<L>(gs::dot(q[g], kr[u]));
+                    sc[u] = row[u] >= 0 ? d * a.scale2 : -INFINITY;
                     top = fmaxf(top, sc[u]);
                 }
                 const float ref = top == -INFINITY ? 0.f : top;        // nothing yet: exponentials of -inf, zeros
@@ -117,7 +124,7 @@ void attn_fwd_kernel(FwdArgs a) {
                     const float pr = gs::fast_exp2(sc[u] - ref);
                     s[g] += pr;
 #pragma unroll
-                    for (int i = 0; i < E; ++i) acc[g * E + i] += pr * (V ? vr[u].at(i) : kr[u].at(i));
+                    for (int i = 0; i < E; ++i) acc[g * E + i] += pr * (SHARED ? kr[u].at(i) : vr[u].at(i));
                 }
             }
         }
@@ -128,7 +135,7 @@ void attn_fwd_kernel(FwdArgs a) {
                 const float keep = gs::fast_exp2(m[g] - ref);
                 m[g] = top;
                 s[g] = gs::groups_sum<L>(s[g] * keep);
-                const float f = !cur.complete ? keep : s[g] > 0.f ? keep / s[g] : s[g] == 0.f ? 0.f : s[g];    // (a NaN stays one)
+                const float f = !cur.complete ? keep : s[g] > 0.f ? keep * __builtin_amdgcn_rcpf(s[g]) : s[g] == 0.f ? 0.f : s[g];    // (a NaN stays one)
 #pragma unroll
                 for (int i = 0; i < E; ++i) acc[g * E + i] *= f;
             }
@@ -140,15 +147,8 @@ void attn_fwd_kernel(FwdArgs a) {
                 const int g = (mine.start + x) / E, start = (mine.start + x) % E;
                 if (g >= n_heads || mine.dup) continue;
                 const int64_t o = cur.p * a.heads + h0 + g;
-                if (cur.complete) gs::store_part<T, L, ALIGNED, S>(static_cast<T *>(a.out) + o * a.dim, lane, a.dim, start, acc + x);
-                else {
-                    const size_t at = (size_t)cur.place * a.heads + h0 + g;
-#pragma unroll
-                    for (int i = 0; i < S; ++i) {
-                        const int d = gs::element_of<T, L, ALIGNED>(lane, start + i);
-                        if (d < a.dim) a.piece_acc[at * a.dim + d] = acc[x + i];
-                    }
-                }
+                if (cur.complete) gs::store_part<S>(static_cast<T *>(a.out) + o * a.dim, at, start, acc + x);
+                else gs::store_part<S>(a.piece_acc + ((size_t)cur.place * a.heads + h0 + g) * a.dim, at, start, acc + x);
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
@@ -158,7 +158,6 @@ void attn_fwd_kernel(FwdArgs a) {
             }
         }
         cur = walk.u;
-        rows = rows_next;
     }
 }
 
@@ -259,34 +258,22 @@ void attn_join_kernel(FwdArgs a) {
     }
 }
 
-template <class T, int L, bool ALIGNED>
+template <class T, int L, bool SHARED>
 void launch_fwd(const FwdArgs &a, int64_t waves, hipStream_t stream) {
     const int share = a.heads / a.kv_heads;
     FwdArgs b = a;
     const int g = share >= 3 ? 4 : share;
     b.parts = (share + g - 1) / g;
     const dim3 grid((unsigned)((waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)(a.kv_heads * b.parts));
-    if (g == 1) attn_fwd_kernel<T, L, 1, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
-    else if (g == 2) attn_fwd_kernel<T, L, 2, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
-    else attn_fwd_kernel<T, L, 4, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
+    if (g == 1) attn_fwd_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
+    else if (g == 2) attn_fwd_kernel<T, L, 2, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
+    else attn_fwd_kernel<T, L, 4, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
 }
 
 template <class T>
-int run_fwd(const FwdArgs &a, const gs::Deal &d, int lanes, bool aligned, hipStream_t stream) {
+int run_fwd(const FwdArgs &a, const gs::Deal &d, int lanes, hipStream_t stream) {
     if (d.waves) {
-        if (aligned) {
-            if (lanes == 4) launch_fwd<T, 4, true>(a, d.waves, stream);
-            else if (lanes == 8) launch_fwd<T, 8, true>(a, d.waves, stream);
-            else if (lanes == 16) launch_fwd<T, 16, true>(a, d.waves, stream);
-            else if (lanes == 32) launch_fwd<T, 32, true>(a, d.waves, stream);
-            else launch_fwd<T, 64, true>(a, d.waves, stream);
-        } else {
-            if (lanes == 4) launch_fwd<T, 4, false>(a, d.waves, stream);
-            else if (lanes == 8) launch_fwd<T, 8, false>(a, d.waves, stream);
-            else if (lanes == 16) launch_fwd<T, 16, false>(a, d.waves, stream);
-            else if (lanes == 32) launch_fwd<T, 32, false>(a, d.waves, stream);
-            else launch_fwd<T, 64, false>(a, d.waves, stream);
-        }
+        GS_BY_LANES(launch_fwd, a.v == nullptr, a, d.waves, stream);
         if (int rc = gs::check_launch("gs_neighbor_attention_fwd")) return rc;
     }
     if (d.pieces) {
@@ -308,7 +295,7 @@ size_t pieces_bytes(const gs::Deal &d, int heads, int dim, size_t *off_acc) {
 
 extern "C" size_t gs_neighbor_attention_workspace(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype) {
     if (gs::check_neighbors("gs_neighbor_attention_workspace", nb, heads, kv_heads, dim, dtype)) return 0;
-    const gs::Deal d = gs::deal_edges(nb->indptr, nb->n_child, nb->n_edges, gs::lanes_for(dim, gs::dtype_size(dtype)));
+    const gs::Deal d = gs::deal_edges(nb, gs::lanes_for(dim, gs::dtype_size(dtype)));
     return pieces_bytes(d, heads, dim, nullptr);
 }
 
@@ -321,21 +308,20 @@ extern "C" int gs_neighbor_attention_fwd(const void *q, const void *k, const voi
     const int size = gs::dtype_size(dtype), lanes = gs::lanes_for(dim, size);
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & (size - 1))
         return gs::fail(GS_EINVAL, "gs_neighbor_attention_fwd: pointer not aligned to its element");
-    const gs::Deal d = gs::deal_edges(nb->indptr, nb->n_child, nb->n_edges, lanes);
+    const gs::Deal d = gs::deal_edges(nb, lanes);
     size_t off_acc = 0;
     const size_t need = pieces_bytes(d, heads, dim, &off_acc);
     if (workspace_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 15))))
         return gs::fail(GS_EINVAL, "gs_neighbor_attention_fwd: aligned workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     FwdArgs a;
-    a.nb = Neighbors{nb->indptr, nb->ids, nb->n_parents, nb->id_offset, nb->n_rows, (uint32_t)(nb->indptr ? 0 : nb->n_child), (uint32_t)nb->n_edges};
+    a.nb = gs::device_neighbors(nb);
     a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse;
     a.piece_ms = need ? static_cast<float2 *>(workspace) : nullptr;
     a.piece_acc = need ? reinterpret_cast<float *>(static_cast<char *>(workspace) + off_acc) : nullptr;
     a.scale2 = scale * gs::kLog2e;
     a.heads = heads; a.kv_heads = kv_heads; a.dim = dim; a.chunk = (int)d.chunk; a.parts = 1;
-    const bool aligned = (dim * size) % 16 == 0 && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == GS_F32) return run_fwd<float>(a, d, lanes, aligned, s);
-    if (dtype == GS_BF16) return run_fwd<__bf16>(a, d, lanes, aligned, s);
-    return run_fwd<_Float16>(a, d, lanes, aligned, s);
+    if (dtype == GS_F32) return run_fwd<float>(a, d, lanes, s);
+    if (dtype == GS_BF16) return run_fwd<__bf16>(a, d, lanes, s);
+    return run_fwd<_Float16>(a, d, lanes, s);
 }

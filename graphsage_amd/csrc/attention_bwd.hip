@@ -4,9 +4,10 @@
 //     ds_e = P_e (<g_out, v_e> - delta) scale      g_q = sum over a parent's edges of ds_e k_e
 //     g_k[row] = sum over the edges that read it of ds_e q,    g_v[row] = the same sum of P_e g_out
 // Two walks.  The parents' walk is the forward's, with sums in place of the running softmax; it also leaves delta and, for
-// ragged neighborhoods, the parent of every edge.  The rows' walk is the same with the roles exchanged: the row's keys
-// and values stay in registers and the queries and g_out of the edges that read it arrive, so a row's gradient is summed
-// in registers in the order of its list, and no atomics are needed.
+// ragged neighborhoods read by id, the parent of every edge.  Dense rows have one reader each: their gradients are written
+// as they pass.  For rows read by id the rows' walk is the same with the roles exchanged: the row's keys and values
+// stay in registers and the queries and g_out of the edges that read it arrive, so a row's gradient is summed in registers
+// in the order of its list, and no atomics are needed.
 #include "attention.h"
 
 namespace {
@@ -23,91 +24,123 @@ struct BwdArgs {
     int32_t *edge_parent;                           // [n_edges], ragged neighborhoods only
     const int64_t *inv_indptr;
     const int32_t *inv_edges;
+    float *dense_part;                              // [parts][n_rows][kv_heads][2][dim], dense rows of more heads than one wave takes
     float *piece;                                   // parents: [waves][2][heads][dim]; rows: [waves][2][kv_heads][2][dim]
     float scale;
     int heads, kv_heads, dim, chunk, parts;
     uint32_t n_inv;
 };
 
-template <class T, int L, int G, bool ALIGNED>
+template <class T, int L, int G, bool SHARED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_bwd_parents_kernel(BwdArgs a) {
-    constexpr int E = gs::Pack<T>::E, U = gs::kAttnRows, W = 64 / L;
+    constexpr int E = gs::Pack<T>::E, W = 64 / L, U = L == 2 ? 2 : gs::kAttnRows;
     const int lane64 = threadIdx.x & 63, lane = lane64 & (L - 1), group = lane64 / L;
     const int share = a.heads / a.kv_heads;
     const int j = blockIdx.y / a.parts, h0 = j * share + (blockIdx.y % a.parts) * G;
     const int n_heads = min(G, (j + 1) * share - h0);
-    const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = a.v ? static_cast<const T *>(a.v) + (int64_t)j * a.dim : nullptr;
+    const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = SHARED ? nullptr : static_cast<const T *>(a.v) + (int64_t)j * a.dim;
     const int64_t stride = (int64_t)a.kv_heads * a.dim;
+    const gs::Place<T, L> at(lane, a.dim);
+    const bool dense = !a.nb.ids && (a.g_k || a.g_v);
     const float scale2 = a.scale * gs::kLog2e;
 
     gs::Walk walk(a.nb, gs::this_wave(), a.chunk);
     bool have = walk.next();
     if (!have) return;
     gs::Unit cur = walk.u;
-    int32_t rows = lane64 < cur.n ? a.nb.row_of(cur.e + lane64) : -1;
-    float q[G][E], go[G][E], acc[G * E], delta[G], lse2[G];
+    int32_t entry = a.nb.entry(cur.e + lane64);
+    RowPart<T> q[G], go[G], q_next[G], go_next[G], out_next[G];
+    float acc[G * E], delta[G], lse2[G], lse_next[G];
+    const auto fetch = [&](int64_t p) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {               // (heads past the last one repeat it)
+            const int64_t of = p * a.heads + h0 + min(g, n_heads - 1);
+            q_next[g].load(static_cast<const T *>(a.q) + of * a.dim, at);
+            go_next[g].load(static_cast<const T *>(a.g_out) + of * a.dim, at);
+            out_next[g].load(static_cast<const T *>(a.out) + of * a.dim, at);
+            lse_next[g] = a.lse[of];
+        }
+    };
+    fetch(cur.p);
     while (have) {
         if (a.edge_parent && blockIdx.y == 0 && lane64 < cur.n) a.edge_parent[cur.e + lane64] = (int32_t)cur.p;
         if (cur.first) {
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                RowPart<T, L, ALIGNED> r, o, d;
-                const int64_t at = cur.p * a.heads + h0 + g;
-                lse2[g] = -INFINITY;
-                if (g < n_heads) {
-                    r.load(static_cast<const T *>(a.q) + at * a.dim, lane, a.dim);
-                    o.load(static_cast<const T *>(a.out) + at * a.dim, lane, a.dim);
-                    d.load(static_cast<const T *>(a.g_out) + at * a.dim, lane, a.dim);
-                    lse2[g] = a.lse[at] * gs::kLog2e;
-                } else { r.zero(); o.zero(); d.zero(); }
-                float dot = 0.f;
+                q[g] = q_next[g];
+                go[g] = go_next[g];
+                q[g].own(at);
+                go[g].own(at);
+                if (g >= n_heads) { q[g].zero(); go[g].zero(); }       // their part of dense rows' gradients: nothing
+                lse2[g] = lse_next[g] * gs::kLog2e;
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    q[g][i] = r.at(i) * scale2;
-                    go[g][i] = d.at(i);
-                    dot += d.at(i) * o.at(i);
-                    acc[g * E + i] = 0.f;
-                }
-                delta[g] = gs::lanes_sum<L>(dot);
+                for (int i = 0; i < E; ++i) acc[g * E + i] = 0.f;
+                delta[g] = gs::lanes_sum<L>(gs::dot(go[g], out_next[g]));
                 // (written by every wave that has a part of the list: the same bits)
-                if (g < n_heads && lane64 == 0) a.delta[at] = delta[g];
+                if (g < n_heads && lane64 == 0) a.delta[cur.p * a.heads + h0 + g] = delta[g];
             }
         }
+        const int32_t rows = lane64 < cur.n ? a.nb.row_of(entry) : -1;
+        const bool gaps = __any(rows < 0 && lane64 < cur.n) || cur.n % (W * U);
         have = walk.next();
-        const int32_t rows_next = have && lane64 < walk.u.n ? a.nb.row_of(walk.u.e + lane64) : -1;
+        if (have) {
+            entry = a.nb.entry(walk.u.e + lane64);
+            if (walk.u.first) fetch(walk.u.p);
+        }
         for (uint32_t b = 0; b < cur.n; b += W * U) {
             int32_t row[U];
-            RowPart<T, L, ALIGNED> kr[U], vr[U];
+            RowPart<T> kr[U], vr[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) row[u] = __shfl(rows, b + u * W + group, 64);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (row[u] >= 0) kr[u].load(K + (int64_t)row[u] * stride, lane, a.dim); else kr[u].zero();
-                if (V) { if (row[u] >= 0) vr[u].load(V + (int64_t)row[u] * stride, lane, a.dim); else vr[u].zero(); }
+                const int64_t to = (int64_t)max(row[u], 0) * stride;   // (what is no neighbor reads row 0 and forgets it)
+                kr[u].load(K + to, at);
+                if (!SHARED) vr[u].load(V + to, at);
             }
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
+            if (gaps)
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    float s = 0.f, dp = 0.f;
+                    kr[u].zero_if(row[u] < 0);
+                    if (!SHARED) vr[u].zero_if(row[u] < 0);
+                }
 #pragma unroll
-                    for (int i = 0; i < E; ++i) {
-                        s += q[g][i] * kr[u].at(i);
-                        dp += go[g][i] * (V ? vr[u].at(i) : kr[u].at(i));
-                    }
-                    s = gs::lanes_sum<L>(s);
-                    dp = gs::lanes_sum<L>(dp);
+            for (int u = 0; u < U; ++u) {
+                float gk[E], gv[E];
+#pragma unroll
+                for (int i = 0; i < E; ++i) gk[i] = gv[i] = 0.f;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const float s = gs::lanes_sum<L>(gs::dot(q[g], kr[u])) * scale2;
+                    const float dp = gs::lanes_sum<L>(gs::dot(go[g], SHARED ? kr[u] : vr[u]));
                     const bool live = row[u] >= 0 && lse2[g] != -INFINITY;
-                    const float ds = live ? gs::fast_exp2(s - lse2[g]) * (dp - delta[g]) : 0.f;
+                    const float pr = live ? gs::fast_exp2(s - lse2[g]) : 0.f;
+                    const float ds = pr * (dp - delta[g]) * a.scale;
 #pragma unroll
                     for (int i = 0; i < E; ++i) acc[g * E + i] += ds * kr[u].at(i);
+                    if (dense)
+#pragma unroll
+                        for (int i = 0; i < E; ++i) { gk[i] += ds * q[g].at(i); gv[i] += pr * go[g].at(i); }
+                }
+                // dense rows: nobody else reads this one
+                if (dense && row[u] >= 0) {
+                    if (SHARED)
+#pragma unroll
+                        for (int i = 0; i < E; ++i) gk[i] += gv[i];
+                    const int64_t to = (int64_t)row[u] * stride + (int64_t)j * a.dim;
+                    if (a.parts > 1) {
+                        float *part = a.dense_part + ((int64_t)(blockIdx.y % a.parts) * a.nb.n_rows * stride + to) * 2;
+                        gs::store_part<E>(part, at, 0, gk);
+                        if (!SHARED) gs::store_part<E>(part + a.dim, at, 0, gv);
+                    } else {
+                        if (a.g_k) gs::store_part<E>(static_cast<T *>(a.g_k) + to, at, 0, gk);
+                        if (!SHARED && a.g_v) gs::store_part<E>(static_cast<T *>(a.g_v) + to, at, 0, gv);
+                    }
                 }
             }
         }
         if (cur.last && a.g_q) {
-#pragma unroll
-            for (int i = 0; i < G * E; ++i) acc[i] *= a.scale;
             gs::Scatter<G * E, L> mine;
             mine.run(acc, lane64);
             constexpr int N = gs::Scatter<G * E, L>::kKept, S = N < E ? N : E;
@@ -115,30 +148,20 @@ void attn_bwd_parents_kernel(BwdArgs a) {
             for (int x = 0; x < N; x += S) {
                 const int g = (mine.start + x) / E, start = (mine.start + x) % E;
                 if (g >= n_heads || mine.dup) continue;
-                if (cur.complete)
-                    gs::store_part<T, L, ALIGNED, S>(static_cast<T *>(a.g_q) + (cur.p * a.heads + h0 + g) * a.dim, lane, a.dim, start, acc + x);
-                else {
-                    const size_t at = (size_t)cur.place * a.heads + h0 + g;
-#pragma unroll
-                    for (int i = 0; i < S; ++i) {
-                        const int d = gs::element_of<T, L, ALIGNED>(lane, start + i);
-                        if (d < a.dim) a.piece[at * a.dim + d] = acc[x + i];
-                    }
-                }
+                if (cur.complete) gs::store_part<S>(static_cast<T *>(a.g_q) + (cur.p * a.heads + h0 + g) * a.dim, at, start, acc + x);
+                else gs::store_part<S>(a.piece + ((size_t)cur.place * a.heads + h0 + g) * a.dim, at, start, acc + x);
             }
         }
         cur = walk.u;
-        rows = rows_next;
     }
 }
 
-// The rows' walk: list entry x of row r is edge inv_edges[x] (or x itself where rows are not read by id: then row x
-// has the one entry x).
-template <class T, int L, int G, bool ALIGNED>
+// The rows' walk, for rows that are read by id: list entry x of row r is edge inv_edges[x].
+template <class T, int L, int G, bool SHARED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_bwd_rows_kernel(BwdArgs a) {
     constexpr int E = gs::Pack<T>::E, W = 64 / L;
-    constexpr int U = G == 1 ? 4 : G == 2 ? 2 : 1;
+    constexpr int U = G == 1 && L != 2 ? 4 : G <= 2 ? 2 : 1;
     const int lane64 = threadIdx.x & 63, lane = lane64 & (L - 1), group = lane64 / L;
     const int share = a.heads / a.kv_heads, j = blockIdx.y;
     Neighbors lists;                                // the lists of the rows, walked as the parents' are
@@ -151,64 +174,74 @@ void attn_bwd_rows_kernel(BwdArgs a) {
     const T *Q = static_cast<const T *>(a.q), *GO = static_cast<const T *>(a.g_out);
     const int64_t stride = (int64_t)a.kv_heads * a.dim;
     const float scale2 = a.scale * gs::kLog2e;
-    int64_t first = 0, last = a.nb.n_edges;         // edges that belong to a parent
-    if (!a.inv_indptr && a.nb.indptr) { first = a.nb.indptr[0]; last = a.nb.indptr[a.nb.n_parents]; }
-    const auto parent_of = [&](uint32_t entry) -> int32_t {
-        const int64_t x = a.inv_indptr ? (int64_t)a.inv_edges[entry] : (int64_t)entry;
-        if (x < first || x >= last || (uint64_t)x >= a.nb.n_edges) return -1;
-        const int32_t p = a.nb.indptr ? a.edge_parent[x] : (int32_t)((uint32_t)x / a.nb.n_child);
-        return (uint64_t)(int64_t)p < (uint64_t)a.nb.n_parents ? p : -1;
+    const gs::Place<T, L> at(lane, a.dim);
+    // an entry's edge, the edge's parent: three steps, each a load (or none) that can be on its way for a while
+    const auto edge_at = [&](uint32_t e) { return (uint32_t)a.inv_edges[min(e, a.n_inv - 1)]; };
+    const auto parent_at = [&](uint32_t x) { return a.nb.indptr ? a.edge_parent[min(x, a.nb.n_edges - 1)] : (int32_t)(x / a.nb.n_child); };
+    const auto checked = [&](uint32_t x, int32_t p) {
+        return x < a.nb.n_edges && (uint64_t)(int64_t)p < (uint64_t)a.nb.n_parents ? p : -1;
     };
 
     gs::Walk walk(lists, gs::this_wave(), a.chunk);
     bool have = walk.next();
     if (!have) return;
     gs::Unit cur = walk.u;
-    int32_t parents = lane64 < cur.n ? parent_of(cur.e + lane64) : -1;
-    float key[E], val[E], sum[2 * E];               // sum: g_k, g_v
-    bool read = false;
+    uint32_t edge = edge_at(cur.e + lane64);
+    int32_t parent = parent_at(edge);
+    RowPart<T> key, val, key_next, val_next;
+    const auto fetch = [&](int64_t r) {
+        key_next.load(static_cast<const T *>(a.k) + r * stride + (int64_t)j * a.dim, at);
+        if (!SHARED) val_next.load(static_cast<const T *>(a.v) + r * stride + (int64_t)j * a.dim, at);
+    };
+    fetch(cur.p);
+    float sum[2 * E];                               // g_k, g_v
     while (have) {
         if (cur.first) {
-            RowPart<T, L, ALIGNED> kr, vr;
-            kr.load(static_cast<const T *>(a.k) + cur.p * stride + (int64_t)j * a.dim, lane, a.dim);
-            if (a.v) vr.load(static_cast<const T *>(a.v) + cur.p * stride + (int64_t)j * a.dim, lane, a.dim); else vr = kr;
+            key = key_next;
+            key.own(at);
+            if (!SHARED) { val = val_next; val.own(at); }
 #pragma unroll
-            for (int i = 0; i < E; ++i) { key[i] = kr.at(i) * scale2; val[i] = vr.at(i); sum[i] = sum[E + i] = 0.f; }
-            read = false;
+            for (int i = 0; i < 2 * E; ++i) sum[i] = 0.f;
         }
+        const int32_t parents = lane64 < cur.n ? checked(edge, parent) : -1;
         have = walk.next();
-        const int32_t parents_next = have && lane64 < walk.u.n ? parent_of(walk.u.e + lane64) : -1;
-        read |= __any(parents >= 0);
+        if (have) {
+            edge = edge_at(walk.u.e + lane64);
+            if (walk.u.first) fetch(walk.u.p);
+        }
         for (uint32_t b = 0; b < cur.n; b += W * U) {
             int32_t p[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) p[u] = __shfl(parents, b + u * W + group, 64);
             for (int h0 = j * share; h0 < (j + 1) * share; h0 += G) {
-                RowPart<T, L, ALIGNED> qr[U][G], gr[U][G];
+                RowPart<T> qr[U][G], gr[U][G];
                 float lse2[U][G], delta[U][G];
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        lse2[u][g] = -INFINITY;
-                        delta[u][g] = 0.f;
-                        if (p[u] >= 0 && h0 + g < (j + 1) * share) {
-                            const int64_t at = (int64_t)p[u] * a.heads + h0 + g;
-                            qr[u][g].load(Q + at * a.dim, lane, a.dim);
-                            gr[u][g].load(GO + at * a.dim, lane, a.dim);
-                            lse2[u][g] = a.lse[at] * gs::kLog2e;
-                            delta[u][g] = a.delta[at];
-                        } else { qr[u][g].zero(); gr[u][g].zero(); }
+                    for (int g = 0; g < G; ++g) {   // (what is no neighbor, and heads past the last one, read another and forget it)
+                        const int64_t of = (int64_t)max(p[u], 0) * a.heads + min(h0 + g, (j + 1) * share - 1);
+                        qr[u][g].load(Q + of * a.dim, at);
+                        gr[u][g].load(GO + of * a.dim, at);
+                        lse2[u][g] = a.lse[of] * gs::kLog2e;
+                        delta[u][g] = a.delta[of];
                     }
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
-                        float s = 0.f, dp = 0.f;
+                        const bool none = p[u] < 0 || h0 + g >= (j + 1) * share || lse2[u][g] == -INFINITY;
+                        qr[u][g].zero_if(none);
+                        gr[u][g].zero_if(none);
+                        lse2[u][g] = none ? -INFINITY : lse2[u][g];
+                        delta[u][g] = none ? 0.f : delta[u][g];
+                    }
 #pragma unroll
-                        for (int i = 0; i < E; ++i) { s += key[i] * qr[u][g].at(i); dp += val[i] * gr[u][g].at(i); }
-                        s = gs::lanes_sum<L>(s);
-                        dp = gs::lanes_sum<L>(dp);
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float s = gs::lanes_sum<L>(gs::dot(key, qr[u][g])) * scale2;
+                        const float dp = gs::lanes_sum<L>(gs::dot(SHARED ? key : val, gr[u][g]));
                         const float pr = lse2[u][g] != -INFINITY ? gs::fast_exp2(s - lse2[u][g]) : 0.f;
                         const float ds = pr * (dp - delta[u][g]) * a.scale;
 #pragma unroll
@@ -216,8 +249,9 @@ void attn_bwd_rows_kernel(BwdArgs a) {
                     }
             }
         }
-        if (cur.last && (a.inv_indptr || read)) {
-            if (!a.v)
+        if (have) parent = parent_at(edge);
+        if (cur.last) {
+            if (SHARED)
 #pragma unroll
                 for (int i = 0; i < E; ++i) sum[i] += sum[E + i];
             gs::Scatter<2 * E, L> mine;
@@ -228,19 +262,11 @@ void attn_bwd_rows_kernel(BwdArgs a) {
                 const int set = (mine.start + x) / E, start = (mine.start + x) % E;
                 T *out = static_cast<T *>(set ? a.g_v : a.g_k);
                 if (!out || mine.dup) continue;
-                if (cur.complete) gs::store_part<T, L, ALIGNED, S>(out + cur.p * stride + (int64_t)j * a.dim, lane, a.dim, start, sum + x);
-                else {
-                    const size_t at = ((size_t)cur.place * a.kv_heads + j) * 2 + set;
-#pragma unroll
-                    for (int i = 0; i < S; ++i) {
-                        const int d = gs::element_of<T, L, ALIGNED>(lane, start + i);
-                        if (d < a.dim) a.piece[at * a.dim + d] = sum[x + i];
-                    }
-                }
+                if (cur.complete) gs::store_part<S>(out + cur.p * stride + (int64_t)j * a.dim, at, start, sum + x);
+                else gs::store_part<S>(a.piece + (((size_t)cur.place * a.kv_heads + j) * 2 + set) * a.dim, at, start, sum + x);
             }
         }
         cur = walk.u;
-        parents = parents_next;
     }
 }
 
@@ -315,75 +341,77 @@ void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int s
     }
 }
 
-template <class T, int L, bool ALIGNED>
+// Adds the head groups' parts of dense rows' gradients.
+template <class T>
+__global__ __launch_bounds__(256)
+void attn_bwd_dense_kernel(BwdArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = a.nb.n_rows * a.kv_heads * a.dim;
+    if (i >= n) return;
+    const int64_t row = i / ((int64_t)a.kv_heads * a.dim), vec = i / a.dim;
+    const int64_t first = a.nb.indptr ? a.nb.indptr[0] : 0, last = a.nb.indptr ? a.nb.indptr[a.nb.n_parents] : (int64_t)a.nb.n_edges;
+    if (row < first || row >= last) return;         // belongs to no parent: left as it is
+    float k = 0.f, v = 0.f;
+    for (int p = 0; p < a.parts; ++p) {
+        const float *part = a.dense_part + ((int64_t)p * n + vec * a.dim) * 2 + i % a.dim;
+        k += part[0];
+        if (a.v) v += part[a.dim];
+    }
+    if (a.g_k) static_cast<T *>(a.g_k)[i] = (T)k;
+    if (a.g_v) static_cast<T *>(a.g_v)[i] = (T)v;
+}
+
+int heads_per_wave(int share) { return share >= 3 ? 4 : share; }
+
+template <class T, int L, bool SHARED>
 void launch_parents(const BwdArgs &a, int64_t waves, hipStream_t stream) {
-    const int share = a.heads / a.kv_heads, g = share >= 3 ? 4 : share;
-    BwdArgs b = a;
-    b.parts = (share + g - 1) / g;
-    const dim3 grid((unsigned)((waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)(a.kv_heads * b.parts));
-    if (g == 1) attn_bwd_parents_kernel<T, L, 1, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
-    else if (g == 2) attn_bwd_parents_kernel<T, L, 2, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
-    else attn_bwd_parents_kernel<T, L, 4, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
+    const int g = heads_per_wave(a.heads / a.kv_heads);
+    const dim3 grid((unsigned)((waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)(a.kv_heads * a.parts));
+    if (g == 1) attn_bwd_parents_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+    else if (g == 2) attn_bwd_parents_kernel<T, L, 2, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+    else attn_bwd_parents_kernel<T, L, 4, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
 }
 
-template <class T, int L, bool ALIGNED>
+template <class T, int L, bool SHARED>
 void launch_rows(const BwdArgs &a, int64_t waves, hipStream_t stream) {
-    const int share = a.heads / a.kv_heads;
+    const int g = heads_per_wave(a.heads / a.kv_heads);
     const dim3 grid((unsigned)((waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)a.kv_heads);
-    if (share == 1) attn_bwd_rows_kernel<T, L, 1, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
-    else if (share == 2) attn_bwd_rows_kernel<T, L, 2, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
-    else attn_bwd_rows_kernel<T, L, 4, ALIGNED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+    if (g == 1) attn_bwd_rows_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+    else if (g == 2) attn_bwd_rows_kernel<T, L, 2, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+    else attn_bwd_rows_kernel<T, L, 4, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
 }
-
-#define GS_BY_LANES(f, ...)                                                \
-    do {                                                                   \
-        if (aligned) {                                                     \
-            if (lanes == 4) f<T, 4, true>(__VA_ARGS__);                    \
-            else if (lanes == 8) f<T, 8, true>(__VA_ARGS__);               \
-            else if (lanes == 16) f<T, 16, true>(__VA_ARGS__);             \
-            else if (lanes == 32) f<T, 32, true>(__VA_ARGS__);             \
-            else f<T, 64, true>(__VA_ARGS__);                              \
-        } else {                                                           \
-            if (lanes == 4) f<T, 4, false>(__VA_ARGS__);                   \
-            else if (lanes == 8) f<T, 8, false>(__VA_ARGS__);              \
-            else if (lanes == 16) f<T, 16, false>(__VA_ARGS__);            \
-            else if (lanes == 32) f<T, 32, false>(__VA_ARGS__);            \
-            else f<T, 64, false>(__VA_ARGS__);                             \
-        }                                                                  \
-    } while (0)
 
 struct Plan {
     gs::Deal parents, rows;
-    size_t off_parent, off_piece, total;
+    int parts;
+    size_t off_parent, off_dense, off_piece, total;
 };
 
 // The pieces of both walks share a region: the second walk starts when the first one's pieces are joined.
 Plan make_plan(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype, int64_t n_inv) {
     Plan p;
-    const int lanes = gs::lanes_for(dim, gs::dtype_size(dtype));
-    p.parents = gs::deal_edges(nb->indptr, nb->n_child, nb->n_edges, lanes);
+    const int lanes = gs::lanes_for(dim, gs::dtype_size(dtype)), share = heads / kv_heads;
+    p.parts = (share + heads_per_wave(share) - 1) / heads_per_wave(share);
+    p.parents = gs::deal_edges(nb, lanes);
     static const int64_t ragged = 0;                // any address: the rows' lists are ragged
-    p.rows = nb->ids ? gs::deal_edges(&ragged, 0, n_inv, lanes)
-                     : gs::deal_edges(nullptr, 1, nb->n_rows, lanes);
+    p.rows = gs::deal_edges(&ragged, 0, nb->ids && nb->n_rows && nb->n_parents ? n_inv : 0, lanes);
     size_t off = gs::align256((size_t)nb->n_parents * heads * sizeof(float));        // delta
     p.off_parent = off;
-    if (nb->indptr) off += gs::align256((size_t)nb->n_edges * sizeof(int32_t));
+    if (nb->indptr && nb->ids) off += gs::align256((size_t)nb->n_edges * sizeof(int32_t));
+    p.off_dense = off;
+    if (!nb->ids && p.parts > 1) off += gs::align256((size_t)p.parts * nb->n_rows * kv_heads * 2 * dim * sizeof(float));
     p.off_piece = off;
     size_t piece = 0;
     if (p.parents.pieces) piece = (size_t)p.parents.waves * 2 * heads * dim * sizeof(float);
-    if (p.rows.pieces) {
-        const size_t r = (size_t)p.rows.waves * 4 * kv_heads * dim * sizeof(float);
-        if (r > piece) piece = r;
-    }
-    p.total = off + piece;
+    const size_t r = (size_t)p.rows.waves * 4 * kv_heads * dim * sizeof(float);
+    p.total = off + (r > piece ? r : piece);
     return p;
 }
 
 template <class T>
-int run_bwd(BwdArgs a, const Plan &p, int lanes, bool aligned, hipStream_t stream) {
+int run_bwd(BwdArgs a, const Plan &p, int lanes, hipStream_t stream) {
     a.chunk = (int)p.parents.chunk;
     if (p.parents.waves) {
-        GS_BY_LANES(launch_parents, a, p.parents.waves, stream);
+        GS_BY_LANES(launch_parents, a.v == nullptr, a, p.parents.waves, stream);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents)")) return rc;
     }
     if (a.g_q && a.nb.n_parents && p.parents.pieces) {
@@ -392,21 +420,25 @@ int run_bwd(BwdArgs a, const Plan &p, int lanes, bool aligned, hipStream_t strea
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents' join)")) return rc;
     }
     if (!a.g_k && !a.g_v) return GS_OK;
+    if (!a.nb.ids) {
+        if (a.parts == 1 || !a.nb.n_rows || !p.parents.waves) return GS_OK;
+        attn_bwd_dense_kernel<T><<<dim3((unsigned)((a.nb.n_rows * a.kv_heads * a.dim + 255) / 256)), 256, 0, stream>>>(a);
+        return gs::check_launch("gs_neighbor_attention_bwd (dense rows)");
+    }
     a.chunk = (int)p.rows.chunk;
     if (p.rows.waves) {
-        GS_BY_LANES(launch_rows, a, p.rows.waves, stream);
+        GS_BY_LANES(launch_rows, a.v == nullptr, a, p.rows.waves, stream);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (rows)")) return rc;
     }
-    if (a.inv_indptr && a.nb.n_rows) {
-        Neighbors rows = a.nb;
-        rows.indptr = a.inv_indptr;
-        rows.n_parents = a.nb.n_rows;
-        rows.n_edges = a.n_inv;
-        attn_bwd_join_kernel<T><<<dim3((unsigned)((a.nb.n_rows + 63) / 64), (unsigned)a.kv_heads), gs::kJoinWaves * 64, 0, stream>>>(
-            rows, a.piece, a.kv_heads, 2, a.dim, a.chunk, static_cast<T *>(a.g_k), static_cast<T *>(a.g_v));
-        return gs::check_launch("gs_neighbor_attention_bwd (rows' join)");
-    }
-    return GS_OK;
+    if (!a.nb.n_rows) return GS_OK;
+    Neighbors rows = a.nb;
+    rows.indptr = a.nb.n_parents ? a.inv_indptr : nullptr;             // (without parents every row's list is empty)
+    rows.n_child = 0;
+    rows.n_parents = a.nb.n_rows;
+    rows.n_edges = a.n_inv;
+    attn_bwd_join_kernel<T><<<dim3((unsigned)((a.nb.n_rows + 63) / 64), (unsigned)a.kv_heads), gs::kJoinWaves * 64, 0, stream>>>(
+        rows, a.piece, a.kv_heads, 2, a.dim, a.chunk, static_cast<T *>(a.g_k), static_cast<T *>(a.g_v));
+    return gs::check_launch("gs_neighbor_attention_bwd (rows' join)");
 }
 
 }  // namespace
@@ -442,21 +474,21 @@ extern "C" int gs_neighbor_attention_bwd(const void *q, const void *k, const voi
         return gs::fail(GS_EINVAL, "%s: aligned workspace of %zu bytes needed, %zu given", what, p.total, workspace_bytes);
     if (nb->n_parents == 0 && (!rows || nb->n_rows == 0 || !nb->ids)) return GS_OK;
     BwdArgs a;
-    a.nb = Neighbors{nb->indptr, nb->ids, nb->n_parents, nb->id_offset, nb->n_rows, (uint32_t)(nb->indptr ? 0 : nb->n_child), (uint32_t)nb->n_edges};
+    a.nb = gs::device_neighbors(nb);
     a.q = q; a.k = k; a.v = v; a.out = out; a.g_out = g_out; a.lse = lse;
     a.g_q = g_q; a.g_k = g_k; a.g_v = g_v;
     char *ws = static_cast<char *>(workspace);
     a.delta = reinterpret_cast<float *>(ws);
-    a.edge_parent = nb->indptr ? reinterpret_cast<int32_t *>(ws + p.off_parent) : nullptr;
+    a.edge_parent = nb->indptr && nb->ids ? reinterpret_cast<int32_t *>(ws + p.off_parent) : nullptr;
+    a.dense_part = reinterpret_cast<float *>(ws + p.off_dense);
     a.piece = reinterpret_cast<float *>(ws + p.off_piece);
     a.inv_indptr = nb->ids ? inv_indptr : nullptr;
     a.inv_edges = nb->ids ? inv_edges : nullptr;
-    a.n_inv = (uint32_t)(nb->ids ? n_inv : nb->n_rows);
+    a.n_inv = (uint32_t)(nb->ids ? n_inv : 0);
     a.scale = scale;
-    a.heads = heads; a.kv_heads = kv_heads; a.dim = dim; a.chunk = 0; a.parts = 1;
-    const bool aligned = (dim * size) % 16 == 0 && (all & 15) == 0;
+    a.heads = heads; a.kv_heads = kv_heads; a.dim = dim; a.chunk = 0; a.parts = p.parts;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == GS_F32) return run_bwd<float>(a, p, lanes, aligned, s);
-    if (dtype == GS_BF16) return run_bwd<__bf16>(a, p, lanes, aligned, s);
-    return run_bwd<_Float16>(a, p, lanes, aligned, s);
+    if (dtype == GS_F32) return run_bwd<float>(a, p, lanes, s);
+    if (dtype == GS_BF16) return run_bwd<__bf16>(a, p, lanes, s);
+    return run_bwd<_Float16>(a, p, lanes, s);
 }

@@ -180,6 +180,11 @@ def test_parents_whose_neighbors_are_all_masked(cuda):
     _check(_case(11, torch.float32, 4, 1, 1, 8, 0, child=5))                            # a table without rows
     _check(_case(12, torch.float32, 0, 1, 1, 8, 9, child=5))                            # no parents
     _check(_case(12, torch.float32, 3, 1, 1, 8, 9, lengths=[0, 0, 0]))
+    none = _case(12, torch.float32, 0, 1, 1, 8, 9, lengths=[])                          # entries that belong to nobody
+    none['child_ids'] = torch.arange(7, dtype=torch.int32, device='cuda')
+    g_k = kernels.neighbor_attention_bwd(none['q'], none['k'], none['v'], none['child_ids'], None, none['q'],
+                                         torch.zeros((0, 1), device='cuda'), none['go'], indptr=none['indptr'])[1]
+    assert not g_k.any()
 
 
 def test_rows_that_are_no_neighbors_may_hold_anything(cuda):
