@@ -42,6 +42,70 @@ struct FwdArgs {
     int heads, kv_heads, dim, chunk, parts;         // parts: head groups per key head
 };
 
+// What the lanes of a row group keep of a list: the queries of G heads, their running maxima (units of log 2), sums and
+// weighted rows.
+template <class T, int L, int G, bool SHARED> struct FwdState {
+    static constexpr int E = gs::Pack<T>::E;
+    RowPart<T> q[G];
+    float acc[G * E], m[G], s[G];
+
+    __device__ __forceinline__ void begin(const RowPart<T> *queries, const gs::Place<T, L> &at) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            m[g] = -INFINITY;
+            s[g] = 0.f;
+            q[g] = queries[g];
+            q[g].own(at);
+#pragma unroll
+            for (int i = 0; i < E; ++i) acc[g * E + i] = 0.f;
+        }
+    }
+    // U rows at once; a negative one is none
+    template <int U>
+    __device__ __forceinline__ void rows(const int32_t (&row)[U], bool gaps, const T *K, const T *V, int64_t stride, float scale2,
+                                         const gs::Place<T, L> &at) {
+        RowPart<T> kr[U], vr[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t to = (int64_t)max(row[u], 0) * stride;       // (what is no neighbor reads row 0 and forgets it)
+            kr[u].load(K + to, at);
+            if (!SHARED) vr[u].load(V + to, at);
+        }
+        if (gaps)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                kr[u].zero_if(row[u] < 0);
+                if (!SHARED) vr[u].zero_if(row[u] < 0);
+            }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float sc[U], top = m[g];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float d = gs::lanes_sum<L>(gs::dot(q[g], kr[u])) * scale2;
+                sc[u] = row[u] >= 0 ? d : -INFINITY;
+                top = fmaxf(top, sc[u]);
+            }
+            const float ref = top == -INFINITY ? 0.f : top;            // nothing yet: exponentials of -inf, zeros
+            const float keep = gs::fast_exp2(m[g] - ref);
+            m[g] = top;
+            s[g] *= keep;
+#pragma unroll
+            for (int i = 0; i < E; ++i) acc[g * E + i] *= keep;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float pr = gs::fast_exp2(sc[u] - ref);
+                s[g] += pr;
+#pragma unroll
+                for (int i = 0; i < E; ++i) acc[g * E + i] += pr * (SHARED ? kr[u].at(i) : vr[u].at(i));
+            }
+        }
+    }
+};
+
+// 1 / s; nothing to divide by: zeros; a NaN stays one
+__device__ __forceinline__ float inverse_of(float s) { return s > 0.f ? __builtin_amdgcn_rcpf(s) : s == 0.f ? 0.f : s; }
+
 template <class T, int L, int G, bool SHARED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_fwd_kernel(FwdArgs a) {
@@ -60,23 +124,13 @@ void attn_fwd_kernel(FwdArgs a) {
     if (!have) return;
     gs::Unit cur = walk.u;
     int32_t entry = a.nb.entry(cur.e + lane64);
-    RowPart<T> q[G], q_next[G];
+    RowPart<T> q_next[G];
 #pragma unroll
     for (int g = 0; g < G; ++g)                     // (heads past the last one repeat it)
         q_next[g].load(Q + (cur.p * a.heads + h0 + min(g, n_heads - 1)) * a.dim, at);
-    float acc[G * E], m[G], s[G];
+    FwdState<T, L, G, SHARED> st;
     while (have) {
-        if (cur.first) {
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                m[g] = -INFINITY;
-                s[g] = 0.f;
-                q[g] = q_next[g];
-                q[g].own(at);
-#pragma unroll
-                for (int i = 0; i < E; ++i) acc[g * E + i] = 0.f;
-            }
-        }
+        if (cur.first) st.begin(q_next, at);
         const int32_t rows = lane64 < cur.n ? a.nb.row_of(entry) : -1;
         const bool gaps = __any(rows < 0 && lane64 < cur.n) || cur.n % (W * U);
         // the next unit's entries and queries are on their way while this one's rows are used
@@ -89,75 +143,102 @@ void attn_fwd_kernel(FwdArgs a) {
         }
         for (uint32_t b = 0; b < cur.n; b += W * U) {
             int32_t row[U];
-            RowPart<T> kr[U], vr[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) row[u] = __shfl(rows, b + u * W + group, 64);     // (-1 behind the last entry)
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t to = (int64_t)max(row[u], 0) * stride;   // (what is no neighbor reads row 0 and forgets it)
-                kr[u].load(K + to, at);
-                if (!SHARED) vr[u].load(V + to, at);
-            }
-            if (gaps)
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    kr[u].zero_if(row[u] < 0);
-                    if (!SHARED) vr[u].zero_if(row[u] < 0);
-                }
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                float sc[U], top = m[g];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const float d = gs::lanes_sum<L>(gs::dot(q[g], kr[u]));
-                    sc[u] = row[u] >= 0 ? d * a.scale2 : -INFINITY;
-                    top = fmaxf(top, sc[u]);
-                }
-                const float ref = top == -INFINITY ? 0.f : top;        // nothing yet: exponentials of -inf, zeros
-                const float keep = gs::fast_exp2(m[g] - ref);
-                m[g] = top;
-                s[g] *= keep;
-#pragma unroll
-                for (int i = 0; i < E; ++i) acc[g * E + i] *= keep;
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const float pr = gs::fast_exp2(sc[u] - ref);
-                    s[g] += pr;
-#pragma unroll
-                    for (int i = 0; i < E; ++i) acc[g * E + i] += pr * (SHARED ? kr[u].at(i) : vr[u].at(i));
-                }
-            }
+            st.template rows<U>(row, gaps, K, V, stride, a.scale2, at);
         }
         if (cur.last) {
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const float top = gs::groups_max<L>(m[g]), ref = top == -INFINITY ? 0.f : top;
-                const float keep = gs::fast_exp2(m[g] - ref);
-                m[g] = top;
-                s[g] = gs::groups_sum<L>(s[g] * keep);
-                const float f = !cur.complete ? keep : s[g] > 0.f ? keep * __builtin_amdgcn_rcpf(s[g]) : s[g] == 0.f ? 0.f : s[g];    // (a NaN stays one)
+                const float top = gs::groups_max<L>(st.m[g]), ref = top == -INFINITY ? 0.f : top;
+                const float keep = gs::fast_exp2(st.m[g] - ref);
+                st.m[g] = top;
+                st.s[g] = gs::groups_sum<L>(st.s[g] * keep);
+                const float f = cur.complete ? keep * inverse_of(st.s[g]) : keep;
 #pragma unroll
-                for (int i = 0; i < E; ++i) acc[g * E + i] *= f;
+                for (int i = 0; i < E; ++i) st.acc[g * E + i] *= f;
             }
             gs::Scatter<G * E, L> mine;
-            mine.run(acc, lane64);
+            mine.run(st.acc, lane64);
             constexpr int N = gs::Scatter<G * E, L>::kKept, S = N < E ? N : E;
 #pragma unroll
             for (int x = 0; x < N; x += S) {
                 const int g = (mine.start + x) / E, start = (mine.start + x) % E;
                 if (g >= n_heads || mine.dup) continue;
                 const int64_t o = cur.p * a.heads + h0 + g;
-                if (cur.complete) gs::store_part<S>(static_cast<T *>(a.out) + o * a.dim, at, start, acc + x);
-                else gs::store_part<S>(a.piece_acc + ((size_t)cur.place * a.heads + h0 + g) * a.dim, at, start, acc + x);
+                if (cur.complete) gs::store_part<S>(static_cast<T *>(a.out) + o * a.dim, at, start, st.acc + x);
+                else gs::store_part<S>(a.piece_acc + ((size_t)cur.place * a.heads + h0 + g) * a.dim, at, start, st.acc + x);
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 if (lane64 != 0 || g >= n_heads) continue;
-                if (cur.complete) a.lse[cur.p * a.heads + h0 + g] = (m[g] + gs::fast_log2(s[g])) * gs::kLn2;
-                else a.piece_ms[(size_t)cur.place * a.heads + h0 + g] = make_float2(m[g], s[g]);
+                if (cur.complete) a.lse[cur.p * a.heads + h0 + g] = (st.m[g] + gs::fast_log2(st.s[g])) * gs::kLn2;
+                else a.piece_ms[(size_t)cur.place * a.heads + h0 + g] = make_float2(st.m[g], st.s[g]);
             }
         }
         cur = walk.u;
+    }
+}
+
+// Short lists of one length: L lanes take a list each.  Entries come L at a time, one a lane, one load ahead.
+template <class T, int L, int G, bool SHARED>
+__global__ __launch_bounds__(gs::kAttnThreads)
+void attn_fwd_short_kernel(FwdArgs a) {
+    constexpr int E = gs::Pack<T>::E, W = 64 / L, U = L == 2 ? 2 : gs::kAttnRows;
+    const int lane64 = threadIdx.x & 63, lane = lane64 & (L - 1), group0 = lane64 & ~(L - 1);
+    const int share = a.heads / a.kv_heads;
+    const int j = blockIdx.y / a.parts, h0 = j * share + (blockIdx.y % a.parts) * G;
+    const int n_heads = min(G, (j + 1) * share - h0);
+    const T *Q = static_cast<const T *>(a.q);
+    const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = SHARED ? nullptr : static_cast<const T *>(a.v) + (int64_t)j * a.dim;
+    const int64_t stride = (int64_t)a.kv_heads * a.dim;
+    const gs::Place<T, L> at(lane, a.dim);
+    const uint32_t n = a.nb.n_child, n_lists = (uint32_t)a.nb.n_parents, waves = gridDim.x * (gs::kAttnThreads / 64);
+
+    uint32_t base = gs::this_wave() * W;            // of the wave; lists past the last one repeat it
+    if (base >= n_lists) return;
+    uint32_t p = min(base + lane64 / L, n_lists - 1);
+    int32_t entry = a.nb.entry(p * n + lane);
+    RowPart<T> q_next[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) q_next[g].load(Q + ((int64_t)p * a.heads + h0 + min(g, n_heads - 1)) * a.dim, at);
+    FwdState<T, L, G, SHARED> st;
+    for (;;) {
+        st.begin(q_next, at);
+        const uint32_t cur = p;
+        const bool mine = base + lane64 / L < n_lists;
+        base += waves * W;
+        const bool more = base < n_lists;
+        for (uint32_t c = 0; c < n; c += L) {
+            const int32_t rows = c + lane < n ? a.nb.row_of(entry) : -1;
+            const uint32_t here = min(n - c, (uint32_t)L);
+            const bool gaps = __any(rows < 0 && (uint32_t)lane < here) || here % U;
+            if (c + L < n) entry = a.nb.entry(p * n + c + L + lane);
+            else if (more) {
+                p = min(base + lane64 / L, n_lists - 1);
+                entry = a.nb.entry(p * n + lane);
+#pragma unroll
+                for (int g = 0; g < G; ++g) q_next[g].load(Q + ((int64_t)p * a.heads + h0 + min(g, n_heads - 1)) * a.dim, at);
+            }
+            for (uint32_t b = 0; b < here; b += U) {
+                int32_t row[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) row[u] = __shfl(rows, group0 + b + u, 64);
+                st.template rows<U>(row, gaps, K, V, stride, a.scale2, at);
+            }
+        }
+        if (mine)
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                if (g >= n_heads) continue;
+                const float f = inverse_of(st.s[g]);
+#pragma unroll
+                for (int i = 0; i < E; ++i) st.acc[g * E + i] *= f;
+                const int64_t o = (int64_t)cur * a.heads + h0 + g;
+                gs::store_part<E>(static_cast<T *>(a.out) + o * a.dim, at, 0, st.acc + g * E);
+                if (lane == 0) a.lse[o] = (st.m[g] + gs::fast_log2(st.s[g])) * gs::kLn2;
+            }
+        if (!more) return;
     }
 }
 
@@ -202,8 +283,6 @@ __device__ __forceinline__ void join_pieces(const FwdArgs &a, uint32_t b, uint32
         }
     }
 }
-
-__device__ __forceinline__ float inverse_of(float s) { return s > 0.f ? 1.f / s : s == 0.f ? 0.f : s; }
 
 template <class T>
 __global__ __launch_bounds__(gs::kJoinWaves * 64)
@@ -259,13 +338,17 @@ void attn_join_kernel(FwdArgs a) {
 }
 
 template <class T, int L, bool SHARED>
-void launch_fwd(const FwdArgs &a, int64_t waves, hipStream_t stream) {
+void launch_fwd(const FwdArgs &a, const gs::Deal &d, hipStream_t stream) {
     const int share = a.heads / a.kv_heads;
     FwdArgs b = a;
     const int g = share >= 3 ? 4 : share;
     b.parts = (share + g - 1) / g;
-    const dim3 grid((unsigned)((waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)(a.kv_heads * b.parts));
-    if (g == 1) attn_fwd_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
+    const dim3 grid((unsigned)((d.waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)(a.kv_heads * b.parts));
+    if (d.is_short) {
+        if (g == 1) attn_fwd_short_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
+        else if (g == 2) attn_fwd_short_kernel<T, L, 2, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
+        else attn_fwd_short_kernel<T, L, 4, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
+    } else if (g == 1) attn_fwd_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
     else if (g == 2) attn_fwd_kernel<T, L, 2, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
     else attn_fwd_kernel<T, L, 4, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(b);
 }
@@ -273,7 +356,7 @@ void launch_fwd(const FwdArgs &a, int64_t waves, hipStream_t stream) {
 template <class T>
 int run_fwd(const FwdArgs &a, const gs::Deal &d, int lanes, hipStream_t stream) {
     if (d.waves) {
-        GS_BY_LANES(launch_fwd, a.v == nullptr, a, d.waves, stream);
+        GS_BY_LANES(launch_fwd, a.v == nullptr, a, d, stream);
         if (int rc = gs::check_launch("gs_neighbor_attention_fwd")) return rc;
     }
     if (d.pieces) {

@@ -31,6 +31,91 @@ struct BwdArgs {
     uint32_t n_inv;
 };
 
+// What the lanes of a row group keep of a parent: queries and g_out of G heads, delta, lse and the sums of g_q.
+template <class T, int L, int G, bool SHARED> struct ParentState {
+    static constexpr int E = gs::Pack<T>::E;
+    RowPart<T> q[G], go[G], q_next[G], go_next[G], out_next[G];
+    float acc[G * E], delta[G], lse2[G], lse_next[G];
+
+    __device__ __forceinline__ void fetch(const BwdArgs &a, int64_t p, int h0, int n_heads, const gs::Place<T, L> &at) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {               // (heads past the last one repeat it)
+            const int64_t of = p * a.heads + h0 + min(g, n_heads - 1);
+            q_next[g].load(static_cast<const T *>(a.q) + of * a.dim, at);
+            go_next[g].load(static_cast<const T *>(a.g_out) + of * a.dim, at);
+            out_next[g].load(static_cast<const T *>(a.out) + of * a.dim, at);
+            lse_next[g] = a.lse[of];
+        }
+    }
+    // `writes`: the lane that leaves delta (every wave that has a part of the list leaves the same bits)
+    __device__ __forceinline__ void begin(const BwdArgs &a, int64_t p, int h0, int n_heads, const gs::Place<T, L> &at, bool writes) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            q[g] = q_next[g];
+            go[g] = go_next[g];
+            q[g].own(at);
+            go[g].own(at);
+            if (g >= n_heads) { q[g].zero(); go[g].zero(); }           // their part of dense rows' gradients: nothing
+            lse2[g] = lse_next[g] * gs::kLog2e;
+#pragma unroll
+            for (int i = 0; i < E; ++i) acc[g * E + i] = 0.f;
+            delta[g] = gs::lanes_sum<L>(gs::dot(go[g], out_next[g]));
+            if (g < n_heads && writes) a.delta[p * a.heads + h0 + g] = delta[g];
+        }
+    }
+    // U rows at once; a negative one is none.  Dense rows: nobody else reads them, their gradients are written (`live`).
+    template <int U>
+    __device__ __forceinline__ void rows(const BwdArgs &a, const int32_t (&row)[U], bool gaps, bool dense, bool live, int j, const T *K,
+                                         const T *V, int64_t stride, const gs::Place<T, L> &at) {
+        const float scale2 = a.scale * gs::kLog2e;
+        RowPart<T> kr[U], vr[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t to = (int64_t)max(row[u], 0) * stride;       // (what is no neighbor reads row 0 and forgets it)
+            kr[u].load(K + to, at);
+            if (!SHARED) vr[u].load(V + to, at);
+        }
+        if (gaps)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                kr[u].zero_if(row[u] < 0);
+                if (!SHARED) vr[u].zero_if(row[u] < 0);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float gk[E], gv[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) gk[i] = gv[i] = 0.f;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const float s = gs::lanes_sum<L>(gs::dot(q[g], kr[u])) * scale2;
+                const float dp = gs::lanes_sum<L>(gs::dot(go[g], SHARED ? kr[u] : vr[u]));
+                const float pr = row[u] >= 0 && lse2[g] != -INFINITY ? gs::fast_exp2(s - lse2[g]) : 0.f;
+                const float ds = pr * (dp - delta[g]) * a.scale;
+#pragma unroll
+                for (int i = 0; i < E; ++i) acc[g * E + i] += ds * kr[u].at(i);
+                if (dense)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) { gk[i] += ds * q[g].at(i); gv[i] += pr * go[g].at(i); }
+            }
+            if (dense && live && row[u] >= 0) {
+                if (SHARED)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) gk[i] += gv[i];
+                const int64_t to = (int64_t)row[u] * stride + (int64_t)j * a.dim;
+                if (a.parts > 1) {
+                    float *part = a.dense_part + ((int64_t)(blockIdx.y % a.parts) * a.nb.n_rows * stride + to) * 2;
+                    gs::store_part<E>(part, at, 0, gk);
+                    if (!SHARED) gs::store_part<E>(part + a.dim, at, 0, gv);
+                } else {
+                    if (a.g_k) gs::store_part<E>(static_cast<T *>(a.g_k) + to, at, 0, gk);
+                    if (!SHARED && a.g_v) gs::store_part<E>(static_cast<T *>(a.g_v) + to, at, 0, gv);
+                }
+            }
+        }
+    }
+};
+
 template <class T, int L, int G, bool SHARED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_bwd_parents_kernel(BwdArgs a) {
@@ -43,116 +128,95 @@ void attn_bwd_parents_kernel(BwdArgs a) {
     const int64_t stride = (int64_t)a.kv_heads * a.dim;
     const gs::Place<T, L> at(lane, a.dim);
     const bool dense = !a.nb.ids && (a.g_k || a.g_v);
-    const float scale2 = a.scale * gs::kLog2e;
 
     gs::Walk walk(a.nb, gs::this_wave(), a.chunk);
     bool have = walk.next();
     if (!have) return;
     gs::Unit cur = walk.u;
     int32_t entry = a.nb.entry(cur.e + lane64);
-    RowPart<T> q[G], go[G], q_next[G], go_next[G], out_next[G];
-    float acc[G * E], delta[G], lse2[G], lse_next[G];
-    const auto fetch = [&](int64_t p) {
-#pragma unroll
-        for (int g = 0; g < G; ++g) {               // (heads past the last one repeat it)
-            const int64_t of = p * a.heads + h0 + min(g, n_heads - 1);
-            q_next[g].load(static_cast<const T *>(a.q) + of * a.dim, at);
-            go_next[g].load(static_cast<const T *>(a.g_out) + of * a.dim, at);
-            out_next[g].load(static_cast<const T *>(a.out) + of * a.dim, at);
-            lse_next[g] = a.lse[of];
-        }
-    };
-    fetch(cur.p);
+    ParentState<T, L, G, SHARED> st;
+    st.fetch(a, cur.p, h0, n_heads, at);
     while (have) {
         if (a.edge_parent && blockIdx.y == 0 && lane64 < cur.n) a.edge_parent[cur.e + lane64] = (int32_t)cur.p;
-        if (cur.first) {
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                q[g] = q_next[g];
-                go[g] = go_next[g];
-                q[g].own(at);
-                go[g].own(at);
-                if (g >= n_heads) { q[g].zero(); go[g].zero(); }       // their part of dense rows' gradients: nothing
-                lse2[g] = lse_next[g] * gs::kLog2e;
-#pragma unroll
-                for (int i = 0; i < E; ++i) acc[g * E + i] = 0.f;
-                delta[g] = gs::lanes_sum<L>(gs::dot(go[g], out_next[g]));
-                // (written by every wave that has a part of the list: the same bits)
-                if (g < n_heads && lane64 == 0) a.delta[cur.p * a.heads + h0 + g] = delta[g];
-            }
-        }
+        if (cur.first) st.begin(a, cur.p, h0, n_heads, at, lane64 == 0);
         const int32_t rows = lane64 < cur.n ? a.nb.row_of(entry) : -1;
         const bool gaps = __any(rows < 0 && lane64 < cur.n) || cur.n % (W * U);
         have = walk.next();
         if (have) {
             entry = a.nb.entry(walk.u.e + lane64);
-            if (walk.u.first) fetch(walk.u.p);
+            if (walk.u.first) st.fetch(a, walk.u.p, h0, n_heads, at);
         }
         for (uint32_t b = 0; b < cur.n; b += W * U) {
             int32_t row[U];
-            RowPart<T> kr[U], vr[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) row[u] = __shfl(rows, b + u * W + group, 64);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t to = (int64_t)max(row[u], 0) * stride;   // (what is no neighbor reads row 0 and forgets it)
-                kr[u].load(K + to, at);
-                if (!SHARED) vr[u].load(V + to, at);
-            }
-            if (gaps)
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    kr[u].zero_if(row[u] < 0);
-                    if (!SHARED) vr[u].zero_if(row[u] < 0);
-                }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float gk[E], gv[E];
-#pragma unroll
-                for (int i = 0; i < E; ++i) gk[i] = gv[i] = 0.f;
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const float s = gs::lanes_sum<L>(gs::dot(q[g], kr[u])) * scale2;
-                    const float dp = gs::lanes_sum<L>(gs::dot(go[g], SHARED ? kr[u] : vr[u]));
-                    const bool live = row[u] >= 0 && lse2[g] != -INFINITY;
-                    const float pr = live ? gs::fast_exp2(s - lse2[g]) : 0.f;
-                    const float ds = pr * (dp - delta[g]) * a.scale;
-#pragma unroll
-                    for (int i = 0; i < E; ++i) acc[g * E + i] += ds * kr[u].at(i);
-                    if (dense)
-#pragma unroll
-                        for (int i = 0; i < E; ++i) { gk[i] += ds * q[g].at(i); gv[i] += pr * go[g].at(i); }
-                }
-                // dense rows: nobody else reads this one
-                if (dense && row[u] >= 0) {
-                    if (SHARED)
-#pragma unroll
-                        for (int i = 0; i < E; ++i) gk[i] += gv[i];
-                    const int64_t to = (int64_t)row[u] * stride + (int64_t)j * a.dim;
-                    if (a.parts > 1) {
-                        float *part = a.dense_part + ((int64_t)(blockIdx.y % a.parts) * a.nb.n_rows * stride + to) * 2;
-                        gs::store_part<E>(part, at, 0, gk);
-                        if (!SHARED) gs::store_part<E>(part + a.dim, at, 0, gv);
-                    } else {
-                        if (a.g_k) gs::store_part<E>(static_cast<T *>(a.g_k) + to, at, 0, gk);
-                        if (!SHARED && a.g_v) gs::store_part<E>(static_cast<T *>(a.g_v) + to, at, 0, gv);
-                    }
-                }
-            }
+            st.template rows<U>(a, row, gaps, dense, true, j, K, V, stride, at);
         }
         if (cur.last && a.g_q) {
             gs::Scatter<G * E, L> mine;
-            mine.run(acc, lane64);
+            mine.run(st.acc, lane64);
             constexpr int N = gs::Scatter<G * E, L>::kKept, S = N < E ? N : E;
 #pragma unroll
             for (int x = 0; x < N; x += S) {
                 const int g = (mine.start + x) / E, start = (mine.start + x) % E;
                 if (g >= n_heads || mine.dup) continue;
-                if (cur.complete) gs::store_part<S>(static_cast<T *>(a.g_q) + (cur.p * a.heads + h0 + g) * a.dim, at, start, acc + x);
-                else gs::store_part<S>(a.piece + ((size_t)cur.place * a.heads + h0 + g) * a.dim, at, start, acc + x);
+                if (cur.complete) gs::store_part<S>(static_cast<T *>(a.g_q) + (cur.p * a.heads + h0 + g) * a.dim, at, start, st.acc + x);
+                else gs::store_part<S>(a.piece + ((size_t)cur.place * a.heads + h0 + g) * a.dim, at, start, st.acc + x);
             }
         }
         cur = walk.u;
+    }
+}
+
+// Short lists of one length: L lanes take a parent each.
+template <class T, int L, int G, bool SHARED>
+__global__ __launch_bounds__(gs::kAttnThreads)
+void attn_bwd_short_kernel(BwdArgs a) {
+    constexpr int E = gs::Pack<T>::E, W = 64 / L, U = L == 2 ? 2 : gs::kAttnRows;
+    const int lane64 = threadIdx.x & 63, lane = lane64 & (L - 1), group0 = lane64 & ~(L - 1);
+    const int share = a.heads / a.kv_heads;
+    const int j = blockIdx.y / a.parts, h0 = j * share + (blockIdx.y % a.parts) * G;
+    const int n_heads = min(G, (j + 1) * share - h0);
+    const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = SHARED ? nullptr : static_cast<const T *>(a.v) + (int64_t)j * a.dim;
+    const int64_t stride = (int64_t)a.kv_heads * a.dim;
+    const gs::Place<T, L> at(lane, a.dim);
+    const bool dense = !a.nb.ids && (a.g_k || a.g_v);
+    const uint32_t n = a.nb.n_child, n_lists = (uint32_t)a.nb.n_parents, waves = gridDim.x * (gs::kAttnThreads / 64);
+
+    uint32_t base = gs::this_wave() * W;            // of the wave; lists past the last one repeat it
+    if (base >= n_lists) return;
+    uint32_t p = min(base + lane64 / L, n_lists - 1);
+    int32_t entry = a.nb.entry(p * n + lane);
+    ParentState<T, L, G, SHARED> st;
+    st.fetch(a, p, h0, n_heads, at);
+    for (;;) {
+        const uint32_t cur = p;
+        const bool mine = base + lane64 / L < n_lists;
+        st.begin(a, cur, h0, n_heads, at, lane == 0 && mine);
+        base += waves * W;
+        const bool more = base < n_lists;
+        for (uint32_t c = 0; c < n; c += L) {
+            const int32_t rows = c + lane < n ? a.nb.row_of(entry) : -1;
+            const uint32_t here = min(n - c, (uint32_t)L);
+            const bool gaps = __any(rows < 0 && (uint32_t)lane < here) || here % U;
+            if (c + L < n) entry = a.nb.entry(p * n + c + L + lane);
+            else if (more) {
+                p = min(base + lane64 / L, n_lists - 1);
+                entry = a.nb.entry(p * n + lane);
+                st.fetch(a, p, h0, n_heads, at);
+            }
+            for (uint32_t b = 0; b < here; b += U) {
+                int32_t row[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) row[u] = __shfl(rows, group0 + b + u, 64);
+                st.template rows<U>(a, row, gaps, dense, mine, j, K, V, stride, at);
+            }
+        }
+        if (mine && a.g_q)
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+                if (g < n_heads) gs::store_part<E>(static_cast<T *>(a.g_q) + ((int64_t)cur * a.heads + h0 + g) * a.dim, at, 0, st.acc + g * E);
+        if (!more) return;
     }
 }
 
@@ -363,10 +427,14 @@ void attn_bwd_dense_kernel(BwdArgs a) {
 int heads_per_wave(int share) { return share >= 3 ? 4 : share; }
 
 template <class T, int L, bool SHARED>
-void launch_parents(const BwdArgs &a, int64_t waves, hipStream_t stream) {
+void launch_parents(const BwdArgs &a, const gs::Deal &d, hipStream_t stream) {
     const int g = heads_per_wave(a.heads / a.kv_heads);
-    const dim3 grid((unsigned)((waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)(a.kv_heads * a.parts));
-    if (g == 1) attn_bwd_parents_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+    const dim3 grid((unsigned)((d.waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)(a.kv_heads * a.parts));
+    if (d.is_short) {
+        if (g == 1) attn_bwd_short_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+        else if (g == 2) attn_bwd_short_kernel<T, L, 2, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+        else attn_bwd_short_kernel<T, L, 4, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+    } else if (g == 1) attn_bwd_parents_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
     else if (g == 2) attn_bwd_parents_kernel<T, L, 2, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
     else attn_bwd_parents_kernel<T, L, 4, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
 }
@@ -411,7 +479,7 @@ template <class T>
 int run_bwd(BwdArgs a, const Plan &p, int lanes, hipStream_t stream) {
     a.chunk = (int)p.parents.chunk;
     if (p.parents.waves) {
-        GS_BY_LANES(launch_parents, a.v == nullptr, a, p.parents.waves, stream);
+        GS_BY_LANES(launch_parents, a.v == nullptr, a, p.parents, stream);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents)")) return rc;
     }
     if (a.g_q && a.nb.n_parents && p.parents.pieces) {
