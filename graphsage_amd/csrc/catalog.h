@@ -55,6 +55,10 @@ __device__ __forceinline__ uint32_t next_piece(float &x) {
 
 template <int P> struct Fragment { bf16x8 p[P]; };
 
+// Whether a tile's fragments fit the registers beside everything else: they are then requested while the scores before
+// them are worked on.  Otherwise each is requested where it is used and other waves cover the wait.
+template <int P, int KC> constexpr bool kAhead = P * KC <= 16;
+
 // frag: the first fragment of a tile plus this lane's 16 bytes.
 template <int P>
 __device__ __forceinline__ Fragment<P> load_fragment(const uint4 *frag, int index) {
@@ -82,18 +86,30 @@ __device__ __forceinline__ float half_max(float v) {           // the larger of 
     return fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
 }
 
+// What the backward kernels need of a user, padded to whole tiles (catalog_bwd.hip).
+struct Stats {
+    float *lse2, *a, *b2, *g;
+    int32_t *target;
+};
+struct StatsFrom {
+    int64_t n_items;
+    const int32_t *targets;
+    const float *lse, *entropy, *g_log_prob, *g_entropy;
+};
+
 struct Layout {                                     // one table to lay out
     const void *x;
     int64_t n_rows;
-    int dim, blocks;
     const float *bias;                              // nullable
     uint4 *rows, *cols;                             // nullable
     float *bias2;                                   // nullable: bias in units of log 2, or kMasked
-    uint32_t *largest;                              // nullable: the largest |element|, as its bits (zeroed by the first table's launch)
-    uint32_t *clear;                                // nullable: a word to zero
+    float *tile_abs;                                // nullable: the largest |element| of every tile
+    Stats st;                                       // st.lse2 nullable
+    StatsFrom from;
 };
 
-int launch_layout(const Layout &l, int dtype, hipStream_t stream);
+// Lays out two tables in one launch.
+int launch_layouts(const Layout &first, const Layout &second, int dim, int dtype, hipStream_t stream);
 int check_catalog(const char *what, int64_t n_users, int64_t n_items, int dim, int dtype, float scale);
 
 }  // namespace gs

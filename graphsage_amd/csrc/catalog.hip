@@ -26,71 +26,138 @@ int check_catalog(const char *what, int64_t n_users, int64_t n_items, int dim, i
 
 namespace {
 
-// One thread per 16-byte place of a layout; places of the rows layout come first.
+// One block per tile of 32 rows, which lie one behind the other in memory: they are read whole, in 16-byte pieces where
+// the table starts on one, into LDS as fp32, and leave in fragment order.
+constexpr int kLdsPad = 4;
+
 template <class T>
 __global__ __launch_bounds__(kCatThreads)
-void layout_kernel(Layout l, int64_t n_places) {
-    constexpr int P = Pieces<T>::P;
-    if (l.clear && blockIdx.x == 0 && threadIdx.x == 0) l.clear[0] = 0u;
-    const int64_t place = (int64_t)blockIdx.x * kCatThreads + threadIdx.x;
-    const int64_t n_tiles = (l.n_rows + 31) / 32;
-    const int64_t of_rows = l.rows ? n_tiles * l.blocks * 2 * 64 : 0;
-    const T *X = static_cast<const T *>(l.x);
-    const bool cols = place >= of_rows;
-    const int64_t at = cols ? place - of_rows : place;
-    const int lane = (int)(at & 63);
-    const int64_t frag = at >> 6, tile = frag / (l.blocks * 2);
-    const int sub = (int)(frag - tile * (l.blocks * 2));
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        int64_t row;
-        int d;
-        if (!cols) { row = tile * 32 + (lane & 31); d = sub * 16 + (lane >> 5) * 8 + i; }
-        else { row = tile * 32 + (sub / l.blocks) * 16 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3); d = (sub % l.blocks) * 32 + (lane & 31); }
-        const bool in = place < n_places && row < l.n_rows && d < l.dim && !(l.bias && l.bias[row] < kOffer);
-        v[i] = in ? (float)X[row * l.dim + d] : 0.f;
+void layout_kernel(Layout first, Layout second, int first_tiles, int dim, int blocks, uint32_t magic, int vector) {
+    constexpr int P = Pieces<T>::P, E = 16 / sizeof(T);
+    extern __shared__ float buf[];                  // [32][blocks * 32 + kLdsPad]
+    __shared__ int on[32];
+    __shared__ float tops[kCatThreads / 64];
+    const bool is_first = (int)blockIdx.x < first_tiles;
+    const Layout &l = is_first ? first : second;
+    const int64_t tile = is_first ? blockIdx.x : blockIdx.x - first_tiles, row0 = tile * 32;
+    const int rows = (int)min((int64_t)32, l.n_rows - row0), width = blocks * 32, ld = width + kLdsPad, tid = threadIdx.x;
+    if (tid < 32) {
+        const bool offered = tid < rows && !(l.bias && l.bias[row0 + tid] < kOffer);
+        on[tid] = offered;
+        if (l.bias2) l.bias2[row0 + tid] = !offered ? kMasked : l.bias ? l.bias[row0 + tid] * kLog2e : 0.f;
+        if (l.st.lse2) {
+            // lse2 = 1e14 silences a user: padding, or one for whom nothing is on offer
+            const int64_t n = row0 + tid;
+            float lse2 = 1e14f, ca = 0.f, cb = 0.f, g = 0.f;
+            int32_t t = -1;
+            if (tid < rows && l.from.lse[n] != -INFINITY) {
+                lse2 = l.from.lse[n] * kLog2e;
+                if (l.from.targets && l.from.g_log_prob && l.from.targets[n] >= 0 && l.from.targets[n] < l.from.n_items) {
+                    t = l.from.targets[n];
+                    g = l.from.g_log_prob[n];
+                }
+                const float ge = l.from.g_entropy ? l.from.g_entropy[n] : 0.f;
+                ca = -(g + (l.from.g_entropy ? ge * l.from.entropy[n] : 0.f));
+                cb = -ge * kLn2;
+            }
+            l.st.lse2[n] = lse2; l.st.a[n] = ca; l.st.b2[n] = cb; l.st.g[n] = g; l.st.target[n] = t;
+        }
     }
-    if (l.largest && !cols) {
-        float top = 0.f;
+    __syncthreads();
+    const T *X = static_cast<const T *>(l.x) + row0 * dim;
+    const int n = rows * dim;
+    const auto put = [&](int i, float v) {
+        const int r = dim == 1 ? i : (int)__umulhi((uint32_t)i, magic), d = i - r * dim;
+        buf[r * ld + d] = on[r] ? v : 0.f;
+    };
+    int i = tid * E;
+    if (vector)
+        for (; i + E <= n; i += kCatThreads * E) {
+            T v[E];
+            *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(X + i);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, v[i] == v[i] ? fabsf(v[i]) : INFINITY);
+            for (int k = 0; k < E; ++k) put(i + k, (float)v[k]);
+        }
+    for (; i < n; i += kCatThreads * E)
+        for (int k = 0; k < E && i + k < n; ++k) put(i + k, (float)X[i + k]);
+    // zeros behind the rows' ends and behind the last row
+    for (int r = tid >> 5; r < 32; r += kCatThreads / 32)
+        for (int d = (r < rows ? dim : 0) + (tid & 31); d < width; d += 32) buf[r * ld + d] = 0.f;
+    __syncthreads();
+
+    const int kcs = blocks * 2, lane = tid & 63;
+    float top = 0.f;
+    for (int f = tid >> 6; f < kcs; f += kCatThreads / 64) {
+        if (l.rows) {
+            float v[8];
+            const float *src = buf + (lane & 31) * ld + f * 16 + (lane >> 5) * 8;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[k] = src[k];
+                top = fmaxf(top, v[k] == v[k] ? fabsf(v[k]) : INFINITY);
+            }
+            uint4 *out = l.rows + ((size_t)tile * kcs + f) * P * 64 + lane;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t lo = next_piece(v[2 * k]), hi = next_piece(v[2 * k + 1]);
+                    w[k] = (lo >> 16) | hi;
+                }
+                out[(size_t)p * 64] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        if (l.cols) {
+            float v[8];
+            const int t = f / blocks, db = f % blocks;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = buf[(t * 16 + 8 * (k >> 2) + 4 * (lane >> 5) + (k & 3)) * ld + db * 32 + (lane & 31)];
+            uint4 *out = l.cols + ((size_t)tile * kcs + f) * P * 64 + lane;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t lo = next_piece(v[2 * k]), hi = next_piece(v[2 * k + 1]);
+                    w[k] = (lo >> 16) | hi;
+                }
+                out[(size_t)p * 64] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+    if (l.tile_abs) {
 #pragma unroll
         for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        // (most waves find a larger one there already)
-        if ((threadIdx.x & 63) == 0 && __float_as_uint(top) > __hip_atomic_load(l.largest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-            atomicMax(l.largest, __float_as_uint(top));
-    }
-    if (place >= n_places) return;
-    uint4 *out = (cols ? l.cols : l.rows) + (size_t)frag * P * 64 + lane;
+        if (lane == 0) tops[tid >> 6] = top;
+        __syncthreads();
+        if (tid == 0) {
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t a = next_piece(v[2 * i]), b = next_piece(v[2 * i + 1]);
-            w[i] = (a >> 16) | b;
+            for (int k = 1; k < kCatThreads / 64; ++k) top = fmaxf(top, tops[k]);
+            l.tile_abs[tile] = top;
         }
-        out[(size_t)p * 64] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    if (l.bias2 && !cols && sub == 0 && lane < 32) {
-        const int64_t row = tile * 32 + lane;
-        float b = kMasked;
-        if (row < l.n_rows) b = !l.bias ? 0.f : l.bias[row] < kOffer ? kMasked : l.bias[row] * kLog2e;
-        l.bias2[row] = b;
-    }
+}
+
+template <class T>
+int launch_layouts_of(const Layout &first, const Layout &second, int dim, hipStream_t stream) {
+    const int64_t t0 = tiles_of(first.n_rows), t1 = tiles_of(second.n_rows);
+    if (t0 + t1 == 0) return GS_OK;
+    const int blocks = blocks_of(dim);
+    const size_t lds = (size_t)32 * (blocks * 32 + kLdsPad) * sizeof(float);
+    // i / dim for i < 2^13: exact with the rounded-up reciprocal
+    const uint32_t magic = dim == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + dim - 1) / dim);
+    const int vector = (((uintptr_t)first.x | (uintptr_t)second.x) & 15) == 0;
+    layout_kernel<T><<<dim3((unsigned)(t0 + t1)), kCatThreads, lds, stream>>>(first, second, (int)t0, dim, blocks, magic, vector);
+    return check_launch("gs_catalog (layout)");
 }
 
 }  // namespace
 
-int launch_layout(const Layout &l, int dtype, hipStream_t stream) {
-    const int64_t each = tiles_of(l.n_rows) * l.blocks * 2 * 64, places = each * ((l.rows ? 1 : 0) + (l.cols ? 1 : 0));
-    if (places == 0) return GS_OK;
-    const dim3 grid((unsigned)((places + kCatThreads - 1) / kCatThreads));
-    if (dtype == GS_F32) layout_kernel<float><<<grid, kCatThreads, 0, stream>>>(l, places);
-    else if (dtype == GS_BF16) layout_kernel<__bf16><<<grid, kCatThreads, 0, stream>>>(l, places);
-    else layout_kernel<_Float16><<<grid, kCatThreads, 0, stream>>>(l, places);
-    return check_launch("gs_catalog (layout)");
+int launch_layouts(const Layout &first, const Layout &second, int dim, int dtype, hipStream_t stream) {
+    if (dtype == GS_F32) return launch_layouts_of<float>(first, second, dim, stream);
+    if (dtype == GS_BF16) return launch_layouts_of<__bf16>(first, second, dim, stream);
+    return launch_layouts_of<_Float16>(first, second, dim, stream);
 }
 
 }  // namespace gs
@@ -106,7 +173,8 @@ struct FwdArgs {
     const float *bias2;
     const int32_t *targets;
     float4 *part;                                   // [users][shares]: m, s, w, target's score
-    float *tile_max;                                // [item tiles][user tiles * 32], with TOP
+    float *tile_max;                                // [users][tile_stride], with TOP
+    int64_t tile_stride;
     int64_t n_users, n_items;
     int user_tiles, item_tiles, groups, shares, tiles_per_share;
     float scale2;
@@ -138,8 +206,14 @@ void catalog_fwd_kernel(FwdArgs a) {
         s[f] = w[f] = 0.f;
         hit[f] = -INFINITY;
     }
+    constexpr bool AHEAD = kAhead<P, KC>;
+    const uint4 *src = a.item + (size_t)t0 * KC * P * 64 + lane;
+    Fragment<P> it[AHEAD ? KC : 1];
+    if (AHEAD)
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(src, kc);
+    float tops[OF][4];
     for (int t = t0; t < t1; ++t) {
-        const uint4 *src = a.item + (size_t)t * KC * P * 64 + lane;
         f32x16 acc[OF];
 #pragma unroll
         for (int f = 0; f < OF; ++f)
@@ -147,10 +221,14 @@ void catalog_fwd_kernel(FwdArgs a) {
             for (int r = 0; r < 16; ++r) acc[f][r] = 0.f;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
-            const Fragment<P> it = load_fragment<P>(src, kc);
+            if (!AHEAD) it[0] = load_fragment<P>(src, kc);
 #pragma unroll
-            for (int f = 0; f < OF; ++f) multiply<P, P, 2>(acc[f], it.p, own[f][kc].p);
+            for (int f = 0; f < OF; ++f) multiply<P, P, 2>(acc[f], it[AHEAD ? kc : 0].p, own[f][kc].p);
         }
+        src += (size_t)KC * P * 64;
+        if (AHEAD && t + 1 < t1)
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(src, kc);
         float b[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g)
@@ -169,9 +247,11 @@ void catalog_fwd_kernel(FwdArgs a) {
                 for (int r = 0; r < 16; ++r)
                     if (target[f] >= 0 && local == row_of_reg(r, lane)) hit[f] = z[r];
             if (TOP) {
-                const float both = half_max(top);
-                const int tile = group * OF + f;
-                if (lane < 32 && tile < a.user_tiles) a.tile_max[(size_t)t * a.user_tiles * 32 + tile * 32 + lane] = both;
+                // four tiles' largest scores leave together
+                tops[f][t & 3] = half_max(top);
+                const int64_t n = ((int64_t)group * OF + f) * 32 + lane;
+                if (((t & 3) == 3 || t + 1 == t1) && lane < 32 && n < a.n_users)
+                    *reinterpret_cast<float4 *>(a.tile_max + n * a.tile_stride + (t & ~3)) = make_float4(tops[f][0], tops[f][1], tops[f][2], tops[f][3]);
             }
             if (__any(top > m[f])) {
                 const float m1 = fmaxf(m[f], top), step = m[f] - m1, keep = fast_exp2(step);
@@ -240,48 +320,65 @@ void catalog_join_kernel(const float4 *part, int shares, int64_t n_users, int64_
 
 struct TopArgs {
     const void *user, *item;
-    const float *bias, *tile_max, *lse;
-    const uint32_t *largest;
-    int64_t n_users, n_items;
-    int dim, item_tiles, stride, k;
+    const float *bias, *tile_max, *tile_abs, *lse;
+    int64_t n_users, n_items, tile_stride;
+    int dim, item_tiles, k, vector;
     float scale;
     float *top_log_prob;
     int32_t *top_ids;
 };
 
-// One block per user.  Thresholds and candidates: see the head of the file.
+// One block per user.  Thresholds and candidates: see the head of the file.  Four lanes score an item.
 template <class T>
 __global__ __launch_bounds__(256)
 void catalog_top_kernel(TopArgs a) {
-    constexpr int kBuf = 1024;
+    constexpr int kBuf = 1024, kChunk = 4096, E = 16 / sizeof(T);
     __shared__ double user[256];
     __shared__ double val[kBuf];
     __shared__ int32_t id[kBuf];
     __shared__ double best_val[kMaxTop];
     __shared__ int32_t best_id[kMaxTop];
-    __shared__ float group_max[256];
-    __shared__ int32_t cand[512];
+    __shared__ __align__(16) float group_max[256];
+    __shared__ float group_abs[256];
+    __shared__ uint16_t cand[kChunk];
     __shared__ int n_val, n_cand;
     __shared__ float low;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, quad = tid >> 2, part = tid & 3;
     const int64_t n = blockIdx.x;
-    const float *tm = a.tile_max + n;
+    const float *tm = a.tile_max + n * a.tile_stride;
     const T *U = static_cast<const T *>(a.user) + n * a.dim, *I = static_cast<const T *>(a.item);
     for (int d = tid; d < a.dim; d += 256) user[d] = (double)(float)U[d];
-    float top = -INFINITY;
-    for (int t = tid; t < a.item_tiles; t += 256) top = fmaxf(top, tm[(size_t)t * a.stride]);
+    float top = -INFINITY, most_abs = 0.f;
+#pragma unroll 4
+    for (int t = tid; t < a.item_tiles; t += 256) {
+        top = fmaxf(top, tm[t]);
+        most_abs = fmaxf(most_abs, a.tile_abs[t]);
+    }
     group_max[tid] = top;
+    group_abs[tid] = most_abs;
     if (tid == 0) { n_val = 0; n_cand = 0; low = -INFINITY; }
     __syncthreads();
     // the k-th largest of 256 groups' maxima: at least k tiles reach it
     int rank = 0;
-    for (int i = 0; i < 256; ++i) rank += group_max[i] > top || (group_max[i] == top && i < tid);
+#pragma unroll 8
+    for (int i = 0; i < 256; i += 4) {
+        const float4 o = *reinterpret_cast<const float4 *>(group_max + i);
+        rank += (o.x > top || (o.x == top && i < tid)) + (o.y > top || (o.y == top && i + 1 < tid)) +
+                (o.z > top || (o.z == top && i + 2 < tid)) + (o.w > top || (o.w == top && i + 3 < tid));
+    }
     if (rank == a.k - 1) low = top;
-    __syncthreads();
+    // |user|, and the largest |element| of an item, by every wave for itself
     double norm = 0.0;
-    for (int d = 0; d < a.dim; ++d) norm += user[d] * user[d];
+    for (int d = tid & 63; d < a.dim; d += 64) norm += user[d] * user[d];
+    most_abs = fmaxf(fmaxf(group_abs[tid & 63], group_abs[(tid & 63) + 64]), fmaxf(group_abs[(tid & 63) + 128], group_abs[(tid & 63) + 192]));
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        norm += __shfl_xor(norm, o, 64);
+        most_abs = fmaxf(most_abs, __shfl_xor(most_abs, o, 64));
+    }
+    __syncthreads();
     // |z - its product in the matrix cores| <= (terms) 2^-23 sum |user| |item|, sum |user| |item| <= |user| sqrt(dim) max |item|
-    const double most = sqrt(norm) * sqrt((double)a.dim) * (double)__uint_as_float(a.largest[0]) * (double)a.scale;
+    const double most = sqrt(norm) * sqrt((double)a.dim) * (double)most_abs * (double)a.scale;
     const double z_low = (double)low * (double)kLn2;
     const double margin = (6.0 * 256 + 16) * 0x1p-23 * most + 0x1p-20 * (fabs(z_low) + most);
     double thr = low > kFloor ? z_low - margin : -INFINITY;
@@ -293,9 +390,12 @@ void catalog_top_kernel(TopArgs a) {
         __syncthreads();
         const int c = n_val;
         for (int i = tid; i < c; i += 256) {
+            const double v = val[i];
+            const int32_t at = id[i];
             int r = 0;
-            for (int j = 0; j < c; ++j) r += better(val[j], id[j], val[i], id[i]);
-            if (r < a.k) { best_val[r] = val[i]; best_id[r] = id[i]; }
+#pragma unroll 4
+            for (int j = 0; j < c; ++j) r += better(val[j], id[j], v, at);
+            if (r < a.k) { best_val[r] = v; best_id[r] = at; }
         }
         __syncthreads();
         const int kept = min(c, a.k);
@@ -306,37 +406,47 @@ void catalog_top_kernel(TopArgs a) {
     };
     const float thr_tile = (float)(thr * (1.0 / (double)kLn2));
     const float thr_down = thr == -INFINITY ? -INFINITY : thr_tile - fabsf(thr_tile) * 0x1p-20f;
-    for (int t0 = 0; t0 < a.item_tiles; t0 += 256) {
-        const int t = t0 + tid;
-        if (t < a.item_tiles && !(tm[(size_t)t * a.stride] < thr_down)) cand[atomicAdd(&n_cand, 1)] = t;
+    for (int t0 = 0; t0 < a.item_tiles; t0 += kChunk) {
+        const int t1 = min(t0 + kChunk, a.item_tiles);
+#pragma unroll 4
+        for (int t = t0 + tid; t < t1; t += 256)
+            if (!(tm[t] < thr_down)) cand[atomicAdd(&n_cand, 1)] = (uint16_t)(t - t0);
         __syncthreads();
-        int left = n_cand;
-        const bool final_round = t0 + 256 >= a.item_tiles;
-        while (left >= 8 || (final_round && left > 0)) {
-            const int take = min(left, 8);
-            left -= take;
-            const int slot = tid >> 5;
-            if (slot < take) {
-                const int64_t j = (int64_t)cand[left + slot] * 32 + (tid & 31);
+        const int count = n_cand;
+        // two tiles a pass; the buffer takes sixteen between two looks at it
+        for (int c0 = 0; c0 < count; c0 += 16) {
+            for (int c = c0 + (quad >> 5); c < min(c0 + 16, count); c += 2) {
+                const int64_t j = ((int64_t)t0 + cand[c]) * 32 + (quad & 31);
                 const float b = j < a.n_items && a.bias ? a.bias[j] : 0.f;
-                if (j < a.n_items && !(b < kOffer)) {
-                    double dot = 0.0;
-                    for (int d = 0; d < a.dim; ++d) dot += user[d] * (double)(float)I[j * a.dim + d];
-                    const double z = dot * (double)a.scale + (double)b;
-                    if (z >= thr && z > -INFINITY) {
-                        const int at = atomicAdd(&n_val, 1);
-                        val[at] = z;
-                        id[at] = (int32_t)j;
+                const bool in = j < a.n_items && !(b < kOffer);
+                const T *row = I + (in ? j : 0) * a.dim;
+                double dot = 0.0;
+                int d = part * E;
+                if (a.vector)
+                    for (; d + E <= a.dim; d += 4 * E) {
+                        T v[E];
+                        __builtin_memcpy(v, row + d, 16);
+#pragma unroll
+                        for (int k = 0; k < E; ++k) dot += user[d + k] * (double)(float)v[k];
                     }
+                for (; d < a.dim; d += 4 * E)
+                    for (int k = 0; k < E && d + k < a.dim; ++k) dot += user[d + k] * (double)(float)row[d + k];
+                dot += __shfl_xor(dot, 1, 64);
+                dot += __shfl_xor(dot, 2, 64);
+                const double z = dot * (double)a.scale + (double)b;
+                if (part == 0 && in && z >= thr && z > -INFINITY) {
+                    const int at = atomicAdd(&n_val, 1);
+                    val[at] = z;
+                    id[at] = (int32_t)j;
                 }
             }
             __syncthreads();
-            const bool full = n_val > kBuf - 256;
+            const bool full = n_val > kBuf - 512;
             __syncthreads();                        // everybody has looked before anybody adds
             if (full) compress();
         }
         __syncthreads();
-        if (tid == 0) n_cand = left;
+        if (tid == 0) n_cand = 0;
         __syncthreads();
     }
     compress();
@@ -373,12 +483,14 @@ void shares_of(int64_t users, int64_t n_items, int of, int *groups, int *shares,
     int64_t sh = kWaves / *groups;
     if (sh > it / 2) sh = it / 2;
     if (sh < 1) sh = 1;
-    *per_share = it ? (int)((it + sh - 1) / sh) : 1;
+    *per_share = it ? (int)((it + sh - 1) / sh + 3) / 4 * 4 : 4;       // (tile maxima leave by fours)
     *shares = (int)((it + *per_share - 1) / *per_share);
 }
 
+int64_t tile_stride_of(int64_t n_items) { return (tiles_of(n_items) + 3) / 4 * 4; }
+
 struct Space {
-    size_t user, item, bias2, part, lse, tile_max, words, total;
+    size_t user, item, bias2, part, lse, tile_abs, tile_max, total;
 };
 
 Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
@@ -387,7 +499,6 @@ Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) 
     int groups, shares, per;
     shares_of(c.slice, n_items, c.of, &groups, &shares, &per);
     size_t off = 0;
-    s.words = off; off += 256;
     s.user = off; off += align256(layout_bytes(c.slice, dim, dtype));
     s.item = off; off += align256(layout_bytes(n_items, dim, dtype));
     s.bias2 = off; off += align256((size_t)tiles_of(n_items) * 32 * sizeof(float));
@@ -395,8 +506,10 @@ Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) 
     // the last slice may be smaller and have more shares: the product of both is bounded by the waves
     off += align256((size_t)(c.slice * (int64_t)shares + kWaves * 64) * sizeof(float4));
     s.lse = off; off += align256((size_t)c.slice * sizeof(float));
+    s.tile_abs = off;
+    if (top_k > 0) off += align256((size_t)tiles_of(n_items) * sizeof(float));
     s.tile_max = off;
-    if (top_k > 0) off += (size_t)tiles_of(n_items) * tiles_of(c.slice) * 32 * sizeof(float);
+    if (top_k > 0) off += (size_t)c.slice * tile_stride_of(n_items) * sizeof(float);
     s.total = off;
     return s;
 }
@@ -454,23 +567,21 @@ extern "C" int gs_catalog_fwd(const void *user, int64_t n_users, const void *ite
     char *ws = static_cast<char *>(workspace);
     hipStream_t s = (hipStream_t)stream;
     const int blocks = gs::blocks_of(dim), pieces = gs::pieces_of(dtype);
-    uint32_t *words = reinterpret_cast<uint32_t *>(ws + sp.words);
+    float *tile_abs = top_k ? reinterpret_cast<float *>(ws + sp.tile_abs) : nullptr;
+    const int vector = ((uintptr_t)item & 15) == 0 && (dim * size) % 16 == 0;
     for (int64_t u0 = 0; u0 < n_users; u0 += cut.slice) {
         const int64_t nu = n_users - u0 < cut.slice ? n_users - u0 : cut.slice;
-        gs::Layout l{};
-        l.x = static_cast<const char *>(user) + (size_t)u0 * dim * size;
-        l.n_rows = nu; l.dim = dim; l.blocks = blocks;
-        l.rows = reinterpret_cast<uint4 *>(ws + sp.user);
-        l.clear = u0 == 0 ? words : nullptr;
-        if (int rc = gs::launch_layout(l, dtype, s)) return rc;
+        gs::Layout lu{}, li{};
+        lu.x = static_cast<const char *>(user) + (size_t)u0 * dim * size;
+        lu.n_rows = nu;
+        lu.rows = reinterpret_cast<uint4 *>(ws + sp.user);
         if (u0 == 0) {
-            l = gs::Layout{};
-            l.x = item; l.n_rows = n_items; l.dim = dim; l.blocks = blocks; l.bias = bias;
-            l.rows = reinterpret_cast<uint4 *>(ws + sp.item);
-            l.bias2 = reinterpret_cast<float *>(ws + sp.bias2);
-            l.largest = top_k ? words : nullptr;
-            if (int rc = gs::launch_layout(l, dtype, s)) return rc;
+            li.x = item; li.n_rows = n_items; li.bias = bias;
+            li.rows = reinterpret_cast<uint4 *>(ws + sp.item);
+            li.bias2 = reinterpret_cast<float *>(ws + sp.bias2);
+            li.tile_abs = tile_abs;
         }
+        if (int rc = gs::launch_layouts(lu, li, dim, dtype, s)) return rc;
         FwdArgs a;
         a.user = reinterpret_cast<const uint4 *>(ws + sp.user);
         a.item = reinterpret_cast<const uint4 *>(ws + sp.item);
@@ -478,6 +589,7 @@ extern "C" int gs_catalog_fwd(const void *user, int64_t n_users, const void *ite
         a.targets = targets ? targets + u0 : nullptr;
         a.part = reinterpret_cast<float4 *>(ws + sp.part);
         a.tile_max = top_k ? reinterpret_cast<float *>(ws + sp.tile_max) : nullptr;
+        a.tile_stride = tile_stride_of(n_items);
         a.n_users = nu; a.n_items = n_items;
         a.user_tiles = (int)gs::tiles_of(nu); a.item_tiles = (int)gs::tiles_of(n_items);
         shares_of(nu, n_items, cut.of, &a.groups, &a.shares, &a.tiles_per_share);
@@ -496,8 +608,9 @@ extern "C" int gs_catalog_fwd(const void *user, int64_t n_users, const void *ite
         if (!top_k) continue;
         TopArgs t;
         t.user = static_cast<const char *>(user) + (size_t)u0 * dim * size;
-        t.item = item; t.bias = bias; t.tile_max = a.tile_max; t.lse = lse_out; t.largest = words;
-        t.n_users = nu; t.n_items = n_items; t.dim = dim; t.item_tiles = a.item_tiles; t.stride = a.user_tiles * 32; t.k = top_k;
+        t.item = item; t.bias = bias; t.tile_max = a.tile_max; t.tile_abs = tile_abs; t.lse = lse_out;
+        t.n_users = nu; t.n_items = n_items; t.tile_stride = a.tile_stride; t.dim = dim; t.item_tiles = a.item_tiles; t.k = top_k;
+        t.vector = vector;
         t.scale = scale; t.top_log_prob = top_log_prob + u0 * top_k; t.top_ids = top_ids + u0 * top_k;
         if (dtype == GS_F32) catalog_top_kernel<float><<<dim3((unsigned)nu), 256, 0, s>>>(t);
         else if (dtype == GS_BF16) catalog_top_kernel<__bf16><<<dim3((unsigned)nu), 256, 0, s>>>(t);

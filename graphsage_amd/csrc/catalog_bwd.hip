@@ -14,53 +14,36 @@ namespace {
 
 using namespace gs;
 
-struct Stats {                                      // per user, padded to whole tiles
-    float *lse2, *a, *b2, *g;
-    int32_t *target;
+struct Side {                                       // one of the two gradients
+    const uint4 *own, *stream_rows, *stream_cols;
+    float *part;                                    // [shares][own tiles * 32][blocks * 32]
+    void *out;                                      // written at once where there is one share
+    int64_t own_rows;
+    int own_tiles, stream_tiles, shares, tiles_per_share;
 };
-
-// lse2 = 1e14 silences a user: padding, or one for whom nothing is on offer.
-__global__ __launch_bounds__(kCatThreads)
-void catalog_stats_kernel(Stats s, int64_t n_users, int64_t n_padded, int64_t n_items, const int32_t *targets, const float *lse,
-                          const float *entropy, const float *g_log_prob, const float *g_entropy) {
-    const int64_t n = (int64_t)blockIdx.x * kCatThreads + threadIdx.x;
-    if (n >= n_padded) return;
-    float l = 1e14f, a = 0.f, b = 0.f, g = 0.f;
-    int32_t t = -1;
-    if (n < n_users && lse[n] != -INFINITY) {
-        l = lse[n] * kLog2e;
-        if (targets && g_log_prob && targets[n] >= 0 && targets[n] < n_items) { t = targets[n]; g = g_log_prob[n]; }
-        const float ge = g_entropy ? g_entropy[n] : 0.f;
-        a = -(g + (g_entropy ? ge * entropy[n] : 0.f));
-        b = -ge * kLn2;
-    }
-    s.lse2[n] = l; s.a[n] = a; s.b2[n] = b; s.g[n] = g; s.target[n] = t;
-}
 
 struct BwdArgs {
-    const uint4 *own, *stream_rows, *stream_cols;
+    Side users, items;
     const float *bias2;
     Stats st;
-    float *part;                                    // [shares][own tiles * 32][blocks * 32]
-    float *part_bias;                               // [shares][own tiles * 32], items only, nullable
-    int own_tiles, stream_tiles, shares, tiles_per_share;
-    float scale2;
+    float *part_bias, *g_bias;                      // [shares][own tiles * 32]; nullable
+    int user_blocks, dim;
+    float scale, scale2;
 };
 
-template <int P, int DB, bool USERS>
-__global__ __launch_bounds__(kCatThreads)
-void catalog_bwd_kernel(BwdArgs a) {
-    constexpr int KC = 2 * DB, NZ = P == 3 ? 3 : 2, MOST = P == 3 ? 2 : 1;
+template <class T, int DB, bool USERS>
+__device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, int64_t task) {
+    constexpr int P = Pieces<T>::P, KC = 2 * DB, NZ = P == 3 ? 3 : 2, MOST = P == 3 ? 2 : 1;
+    constexpr bool AHEAD = kAhead<P, KC>;
     const int lane = threadIdx.x & 63, half = lane >> 5;
-    const int64_t task = (int64_t)blockIdx.x * (kCatThreads / 64) + (threadIdx.x >> 6);
-    if (task >= (int64_t)a.own_tiles * a.shares) return;
-    const int tile = (int)(task % a.own_tiles), share = (int)(task / a.own_tiles);
-    const int t0 = share * a.tiles_per_share, t1 = min(t0 + a.tiles_per_share, a.stream_tiles);
+    if (task >= (int64_t)side.own_tiles * side.shares) return;
+    const int tile = (int)(task % side.own_tiles), share = (int)(task / side.own_tiles);
+    const int t0 = share * side.tiles_per_share, t1 = min(t0 + side.tiles_per_share, side.stream_tiles);
     const int mine = tile * 32 + (lane & 31);
 
     Fragment<P> own[KC];
     {
-        const uint4 *src = a.own + (size_t)tile * KC * P * 64 + lane;
+        const uint4 *src = side.own + (size_t)tile * KC * P * 64 + lane;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) own[kc] = load_fragment<P>(src, kc);
     }
@@ -74,56 +57,69 @@ void catalog_bwd_kernel(BwdArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) out[d][r] = 0.f;
 
+    const uint4 *rows = side.stream_rows + (size_t)t0 * KC * P * 64 + lane, *cols = side.stream_cols + (size_t)t0 * KC * P * 64 + lane;
+    Fragment<P> it[AHEAD ? KC : 1], ct[AHEAD ? KC : 1];
+    if (AHEAD)
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(rows, kc);
     for (int t = t0; t < t1; ++t) {
-        const uint4 *rows = a.stream_rows + (size_t)t * KC * P * 64 + lane, *cols = a.stream_cols + (size_t)t * KC * P * 64 + lane;
+        // what the scores are turned into dz with: of the streamed rows
+        float x[16], y[16], w[16];
+        int tg = -1;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int at = t * 32 + 8 * g + 4 * half;
+            if (USERS) *reinterpret_cast<float4 *>(x + 4 * g) = *reinterpret_cast<const float4 *>(a.bias2 + at);
+            else {
+                *reinterpret_cast<float4 *>(x + 4 * g) = *reinterpret_cast<const float4 *>(a.st.lse2 + at);
+                *reinterpret_cast<float4 *>(y + 4 * g) = *reinterpret_cast<const float4 *>(a.st.a + at);
+                *reinterpret_cast<float4 *>(w + 4 * g) = *reinterpret_cast<const float4 *>(a.st.b2 + at);
+            }
+        }
+        if (!USERS) tg = a.st.target[t * 32 + (lane & 31)];
         f32x16 acc;
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] = 0.f;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
-            const Fragment<P> f = load_fragment<P>(rows, kc);
-            multiply<P, P, 2>(acc, f.p, own[kc].p);
+            if (!AHEAD) it[0] = load_fragment<P>(rows, kc);
+            multiply<P, P, 2>(acc, it[AHEAD ? kc : 0].p, own[kc].p);
+        }
+        rows += (size_t)KC * P * 64;
+        if (AHEAD) {
+            // this tile's second operand and the next tile's first are on their way while dz is formed
+#pragma unroll
+            for (int kc = 0; kc < KC; ++kc) ct[kc] = load_fragment<P>(cols, kc);
+            if (t + 1 < t1)
+#pragma unroll
+                for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(rows, kc);
         }
         float dz[16];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int at = t * 32 + 8 * g + 4 * half;
-            float x[4], y[4], w[4];
-            if (USERS) *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(a.bias2 + at);
-            else {
-                *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(a.st.lse2 + at);
-                *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(a.st.a + at);
-                *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(a.st.b2 + at);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 4 * g + i;
-                const float lp = USERS ? __builtin_fmaf(acc[r], a.scale2, x[i]) - lse2 : __builtin_fmaf(acc[r], a.scale2, bias) - x[i];
-                dz[r] = fast_exp2(lp) * (USERS ? __builtin_fmaf(cb, lp, ca) : __builtin_fmaf(w[i], lp, y[i]));
-            }
+        for (int r = 0; r < 16; ++r) {
+            const float lp = USERS ? __builtin_fmaf(acc[r], a.scale2, x[r]) - lse2 : __builtin_fmaf(acc[r], a.scale2, bias) - x[r];
+            dz[r] = fast_exp2(lp) * (USERS ? __builtin_fmaf(cb, lp, ca) : __builtin_fmaf(w[r], lp, y[r]));
         }
         // the targets: rarely in this tile
         if (USERS) {
             const int local = target - t * 32;
-            if (__any(target >= 0 && (unsigned)local < 32u)) {
-                const bool on = target >= 0 && (unsigned)local < 32u && a.bias2[target >= 0 && (unsigned)local < 32u ? target : 0] > kFloor;
+            const bool here = target >= 0 && (unsigned)local < 32u;
+            if (__any(here)) {
+                const bool on = here && a.bias2[here ? target : 0] > kFloor;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dz[r] += on && local == row_of_reg(r, lane) ? cg : 0.f;
             }
-        } else {
-            const int tg = a.st.target[t * 32 + (lane & 31)];
-            if (__any(tg >= 0 && (tg >> 5) == tile)) {
-                const float g = a.st.g[t * 32 + (lane & 31)];
+        } else if (__any(tg >= 0 && (tg >> 5) == tile)) {
+            const float g = a.st.g[t * 32 + (lane & 31)];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int src = row_of_reg(r, lane);
-                    const int tr = __shfl(tg, src, 64);
-                    const float gr = __shfl(g, src, 64);
-                    dz[r] += tr == mine && bias > kFloor ? gr : 0.f;
-                }
+            for (int r = 0; r < 16; ++r) {
+                const int src = row_of_reg(r, lane);
+                const int tr = __shfl(tg, src, 64);
+                const float gr = __shfl(g, src, 64);
+                dz[r] += tr == mine && bias > kFloor ? gr : 0.f;
             }
         }
-        if (!USERS && a.part_bias)
+        if (!USERS && a.g_bias)
 #pragma unroll
             for (int r = 0; r < 16; ++r) sum += dz[r];
 #pragma unroll
@@ -141,37 +137,85 @@ void catalog_bwd_kernel(BwdArgs a) {
             }
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                const Fragment<P> f = load_fragment<P>(cols, h * DB + d);
-                multiply<NZ, P, MOST>(out[d], z, f.p);
+                if (!AHEAD) ct[0] = load_fragment<P>(cols, h * DB + d);
+                multiply<NZ, P, MOST>(out[d], z, ct[AHEAD ? h * DB + d : 0].p);
             }
         }
+        cols += (size_t)KC * P * 64;
     }
-    float *dst = a.part + ((size_t)share * a.own_tiles + tile) * 32 * (DB * 32) + (lane & 31);
+    if (side.out && side.shares == 1) {
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dst[(size_t)row_of_reg(r, lane) * (DB * 32) + d * 32] = out[d][r];
-    if (!USERS && a.part_bias) {
+            for (int r = 0; r < 16; ++r) {
+                const int64_t row = (int64_t)tile * 32 + row_of_reg(r, lane);
+                const int col = d * 32 + (lane & 31);
+                if (row < side.own_rows && col < a.dim) static_cast<T *>(side.out)[row * a.dim + col] = (T)(out[d][r] * a.scale);
+            }
+    } else if (side.out) {
+        float *dst = side.part + ((size_t)share * side.own_tiles + tile) * 32 * (DB * 32) + (lane & 31);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dst[(size_t)row_of_reg(r, lane) * (DB * 32) + d * 32] = out[d][r];
+    }
+    if (!USERS && a.g_bias) {
         sum += __shfl_xor(sum, 32, 64);
-        if (lane < 32) a.part_bias[(size_t)share * a.own_tiles * 32 + mine] = sum;
+        if (lane < 32 && side.shares > 1) a.part_bias[(size_t)share * side.own_tiles * 32 + mine] = sum;
+        else if (lane < 32 && mine < side.own_rows) a.g_bias[mine] = sum;
     }
 }
 
-// Adds the shares in order.
+// Both gradients in one launch: the first blocks own users, the others items.
+template <class T, int DB>
+__global__ __launch_bounds__(kCatThreads)
+void catalog_bwd_kernel(BwdArgs a) {
+    const int wave = threadIdx.x >> 6;
+    if ((int)blockIdx.x < a.user_blocks) backward<T, DB, true>(a, a.users, (int64_t)blockIdx.x * (kCatThreads / 64) + wave);
+    else backward<T, DB, false>(a, a.items, (int64_t)(blockIdx.x - a.user_blocks) * (kCatThreads / 64) + wave);
+}
+
+// Adds the shares in order: users' elements, then items', then the bias.
+struct JoinArgs {
+    const float *user_part, *item_part, *bias_part;
+    int user_shares, item_shares, dim, width;
+    int64_t user_n, item_n, bias_n, user_padded, item_padded;          // *_n: elements to write, 0 for none
+    float scale;
+    void *g_user, *g_item;
+    float *g_bias;
+};
+
 template <class T>
 __global__ __launch_bounds__(kCatThreads)
-void catalog_bwd_join_kernel(const float *part, int shares, int64_t rows, int64_t padded, int dim, int width, float scale, T *out) {
-    const int64_t i = (int64_t)blockIdx.x * kCatThreads + threadIdx.x;
-    if (i >= rows * dim) return;
-    const int64_t row = i / dim;
-    const int d = (int)(i - row * dim);
+void catalog_bwd_join_kernel(JoinArgs a) {
+    int64_t i = (int64_t)blockIdx.x * kCatThreads + threadIdx.x;
+    const float *part;
+    int64_t each;
+    int shares;
+    const bool user = i < a.user_n, item = !user && i < a.user_n + a.item_n;
+    if (user || item) {
+        if (item) i -= a.user_n;
+        const int64_t row = i / a.dim;
+        part = (user ? a.user_part : a.item_part) + row * a.width + (i - row * a.dim);
+        each = (user ? a.user_padded : a.item_padded) * a.width;
+        shares = user ? a.user_shares : a.item_shares;
+    } else {
+        i -= a.user_n + a.item_n;
+        if (i >= a.bias_n) return;
+        part = a.bias_part + i;
+        each = a.item_padded;
+        shares = a.item_shares;
+    }
     float s = 0.f;
-    for (int k = 0; k < shares; ++k) s += part[((size_t)k * padded + row) * width + d];
-    out[i] = (T)(s * scale);
+#pragma unroll 8
+    for (int k = 0; k < shares; ++k) s += part[(size_t)k * each];
+    if (user) static_cast<T *>(a.g_user)[i] = (T)(s * a.scale);
+    else if (item) static_cast<T *>(a.g_item)[i] = (T)(s * a.scale);
+    else a.g_bias[i] = s;
 }
 
 struct Space {
-    size_t user_rows, user_cols, item_rows, item_cols, bias2, stats, part, part_bias, total;
+    size_t user_rows, user_cols, item_rows, item_cols, bias2, stats, user_part, item_part, part_bias, total;
     int user_shares, user_per, item_shares, item_per;
 };
 
@@ -198,39 +242,30 @@ Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype) {
     s.item_cols = off; off += align256(layout_bytes(n_items, dim, dtype));
     s.bias2 = off; off += align256((size_t)it * 32 * sizeof(float));
     s.stats = off; off += 5 * align256((size_t)ut * 32 * sizeof(float));
-    const size_t pu = ut * s.user_shares * row, pi = it * s.item_shares * row;
-    s.part = off; off += align256(pu > pi ? pu : pi);
-    s.part_bias = off; off += align256((size_t)it * s.item_shares * 32 * sizeof(float));
+    s.user_part = off; off += s.user_shares > 1 ? align256(ut * s.user_shares * row) : 0;
+    s.item_part = off; off += s.item_shares > 1 ? align256(it * s.item_shares * row) : 0;
+    s.part_bias = off; off += s.item_shares > 1 ? align256((size_t)it * s.item_shares * 32 * sizeof(float)) : 0;
     s.total = off;
     return s;
 }
 
-template <int P, bool USERS>
-void launch_bwd(const BwdArgs &a, int blocks, hipStream_t stream) {
-    const dim3 grid((unsigned)(((int64_t)a.own_tiles * a.shares + kCatThreads / 64 - 1) / (kCatThreads / 64)));
-    if (blocks == 1) catalog_bwd_kernel<P, 1, USERS><<<grid, kCatThreads, 0, stream>>>(a);
-    else if (blocks == 2) catalog_bwd_kernel<P, 2, USERS><<<grid, kCatThreads, 0, stream>>>(a);
-    else if (blocks == 4) catalog_bwd_kernel<P, 4, USERS><<<grid, kCatThreads, 0, stream>>>(a);
-    else catalog_bwd_kernel<P, 8, USERS><<<grid, kCatThreads, 0, stream>>>(a);
-}
-
-template <bool USERS>
-int run_side(const BwdArgs &a, int pieces, int blocks, hipStream_t stream) {
-    if (a.shares > 0) {
-        if (pieces == 1) launch_bwd<1, USERS>(a, blocks, stream);
-        else if (pieces == 2) launch_bwd<2, USERS>(a, blocks, stream);
-        else launch_bwd<3, USERS>(a, blocks, stream);
+template <class T>
+int run_bwd(const BwdArgs &a, const JoinArgs &j, int blocks, hipStream_t stream) {
+    constexpr int W = kCatThreads / 64;
+    const unsigned n = (unsigned)(a.user_blocks + ((int64_t)a.items.own_tiles * a.items.shares + W - 1) / W);
+    if (n) {
+        if (blocks == 1) catalog_bwd_kernel<T, 1><<<dim3(n), kCatThreads, 0, stream>>>(a);
+        else if (blocks == 2) catalog_bwd_kernel<T, 2><<<dim3(n), kCatThreads, 0, stream>>>(a);
+        else if (blocks == 4) catalog_bwd_kernel<T, 4><<<dim3(n), kCatThreads, 0, stream>>>(a);
+        else catalog_bwd_kernel<T, 8><<<dim3(n), kCatThreads, 0, stream>>>(a);
+        if (int rc = gs::check_launch("gs_catalog_bwd")) return rc;
     }
-    return gs::check_launch("gs_catalog_bwd");
-}
-
-int run_join(const BwdArgs &a, int dtype, int64_t rows, int dim, int width, float scale, const float *part, void *out, hipStream_t stream) {
-    const dim3 grid((unsigned)((rows * dim + kCatThreads - 1) / kCatThreads));
-    const int64_t padded = (int64_t)a.own_tiles * 32;
-    if (dtype == GS_F32) catalog_bwd_join_kernel<float><<<grid, kCatThreads, 0, stream>>>(part, a.shares, rows, padded, dim, width, scale, static_cast<float *>(out));
-    else if (dtype == GS_BF16) catalog_bwd_join_kernel<__bf16><<<grid, kCatThreads, 0, stream>>>(part, a.shares, rows, padded, dim, width, scale, static_cast<__bf16 *>(out));
-    else catalog_bwd_join_kernel<_Float16><<<grid, kCatThreads, 0, stream>>>(part, a.shares, rows, padded, dim, width, scale, static_cast<_Float16 *>(out));
-    return gs::check_launch("gs_catalog_bwd (join)");
+    const int64_t elements = j.user_n + j.item_n + j.bias_n;
+    if (elements) {
+        catalog_bwd_join_kernel<T><<<dim3((unsigned)((elements + kCatThreads - 1) / kCatThreads)), kCatThreads, 0, stream>>>(j);
+        return gs::check_launch("gs_catalog_bwd (join)");
+    }
+    return GS_OK;
 }
 
 }  // namespace
@@ -259,57 +294,53 @@ extern "C" int gs_catalog_bwd(const void *user, int64_t n_users, const void *ite
         return gs::fail(GS_EINVAL, "%s: 256-byte aligned workspace of %zu bytes needed, %zu given", what, sp.total, workspace_bytes);
     char *ws = static_cast<char *>(workspace);
     hipStream_t s = (hipStream_t)stream;
-    const int blocks = gs::blocks_of(dim), pieces = gs::pieces_of(dtype);
+    const int blocks = gs::blocks_of(dim);
     const bool items = g_item || g_bias;
     const int ut = (int)gs::tiles_of(n_users), it = (int)gs::tiles_of(n_items);
     const size_t each = gs::align256((size_t)ut * 32 * sizeof(float));
-    Stats st;
-    st.lse2 = reinterpret_cast<float *>(ws + sp.stats);
-    st.a = reinterpret_cast<float *>(ws + sp.stats + each);
-    st.b2 = reinterpret_cast<float *>(ws + sp.stats + 2 * each);
-    st.g = reinterpret_cast<float *>(ws + sp.stats + 3 * each);
-    st.target = reinterpret_cast<int32_t *>(ws + sp.stats + 4 * each);
-    if (ut) {
-        catalog_stats_kernel<<<dim3((unsigned)((ut * 32 + gs::kCatThreads - 1) / gs::kCatThreads)), gs::kCatThreads, 0, s>>>(
-            st, n_users, (int64_t)ut * 32, n_items, targets, lse, entropy, g_log_prob, g_entropy);
-        if (int rc = gs::check_launch("gs_catalog_bwd (statistics)")) return rc;
-    }
-    gs::Layout l{};
-    l.x = user; l.n_rows = n_users; l.dim = dim; l.blocks = blocks;
-    l.rows = reinterpret_cast<uint4 *>(ws + sp.user_rows);
-    l.cols = items ? reinterpret_cast<uint4 *>(ws + sp.user_cols) : nullptr;
-    if (int rc = gs::launch_layout(l, dtype, s)) return rc;
-    l.x = item; l.n_rows = n_items; l.bias = bias;
-    l.rows = reinterpret_cast<uint4 *>(ws + sp.item_rows);
-    l.cols = g_user ? reinterpret_cast<uint4 *>(ws + sp.item_cols) : nullptr;
-    l.bias2 = reinterpret_cast<float *>(ws + sp.bias2);
-    if (int rc = gs::launch_layout(l, dtype, s)) return rc;
+    gs::Layout lu{}, li{};
+    lu.x = user; lu.n_rows = n_users;
+    lu.rows = reinterpret_cast<uint4 *>(ws + sp.user_rows);
+    lu.cols = items ? reinterpret_cast<uint4 *>(ws + sp.user_cols) : nullptr;
+    lu.st.lse2 = reinterpret_cast<float *>(ws + sp.stats);
+    lu.st.a = reinterpret_cast<float *>(ws + sp.stats + each);
+    lu.st.b2 = reinterpret_cast<float *>(ws + sp.stats + 2 * each);
+    lu.st.g = reinterpret_cast<float *>(ws + sp.stats + 3 * each);
+    lu.st.target = reinterpret_cast<int32_t *>(ws + sp.stats + 4 * each);
+    lu.from = gs::StatsFrom{n_items, targets, lse, entropy, g_log_prob, g_entropy};
+    li.x = item; li.n_rows = n_items; li.bias = bias;
+    li.rows = reinterpret_cast<uint4 *>(ws + sp.item_rows);
+    li.cols = g_user ? reinterpret_cast<uint4 *>(ws + sp.item_cols) : nullptr;
+    li.bias2 = reinterpret_cast<float *>(ws + sp.bias2);
+    if (int rc = gs::launch_layouts(lu, li, dim, dtype, s)) return rc;
 
-    BwdArgs a;
-    a.bias2 = l.bias2;
-    a.st = st;
-    a.part = reinterpret_cast<float *>(ws + sp.part);
-    a.part_bias = nullptr;
+    // a side without anything to stream has no shares: the join writes its zeros
+    BwdArgs a{};
+    a.bias2 = li.bias2;
+    a.st = lu.st;
+    a.dim = dim;
+    a.scale = scale;
     a.scale2 = scale * gs::kLog2e;
+    a.g_bias = g_bias;
+    a.part_bias = reinterpret_cast<float *>(ws + sp.part_bias);
+    JoinArgs j{};
+    j.dim = dim; j.width = blocks * 32; j.scale = scale;
+    j.g_user = g_user; j.g_item = g_item; j.g_bias = g_bias;
+    j.user_padded = (int64_t)ut * 32; j.item_padded = (int64_t)it * 32;
     if (g_user) {
-        a.own = reinterpret_cast<const uint4 *>(ws + sp.user_rows);
-        a.stream_rows = reinterpret_cast<const uint4 *>(ws + sp.item_rows);
-        a.stream_cols = reinterpret_cast<const uint4 *>(ws + sp.item_cols);
-        a.own_tiles = ut; a.stream_tiles = it; a.shares = n_items ? sp.user_shares : 0; a.tiles_per_share = sp.user_per;
-        if (int rc = run_side<true>(a, pieces, blocks, s)) return rc;
-        if (int rc = run_join(a, dtype, n_users, dim, blocks * 32, scale, a.part, g_user, s)) return rc;
+        a.users = Side{lu.rows, li.rows, li.cols, reinterpret_cast<float *>(ws + sp.user_part), g_user, n_users, ut, it,
+                       n_items ? sp.user_shares : 0, sp.user_per};
+        a.user_blocks = (int)(((int64_t)ut * a.users.shares + gs::kCatThreads / 64 - 1) / (gs::kCatThreads / 64));
+        j.user_part = a.users.part; j.user_shares = a.users.shares;
+        if (a.users.shares != 1) j.user_n = n_users * dim;
     }
     if (items) {
-        a.own = reinterpret_cast<const uint4 *>(ws + sp.item_rows);
-        a.stream_rows = reinterpret_cast<const uint4 *>(ws + sp.user_rows);
-        a.stream_cols = reinterpret_cast<const uint4 *>(ws + sp.user_cols);
-        a.own_tiles = it; a.stream_tiles = ut; a.shares = n_users ? sp.item_shares : 0; a.tiles_per_share = sp.item_per;
-        a.part_bias = g_bias ? reinterpret_cast<float *>(ws + sp.part_bias) : nullptr;
-        if (int rc = run_side<false>(a, pieces, blocks, s)) return rc;
-        if (g_item)
-            if (int rc = run_join(a, dtype, n_items, dim, blocks * 32, scale, a.part, g_item, s)) return rc;
-        if (g_bias)
-            if (int rc = run_join(a, GS_F32, n_items, 1, 1, 1.f, a.part_bias, g_bias, s)) return rc;
+        a.items = Side{li.rows, lu.rows, lu.cols, reinterpret_cast<float *>(ws + sp.item_part), g_item, n_items, it, ut,
+                       n_users ? sp.item_shares : 0, sp.item_per};
+        j.item_part = a.items.part; j.bias_part = a.part_bias; j.item_shares = a.items.shares;
+        if (a.items.shares != 1) { j.item_n = g_item ? n_items * dim : 0; j.bias_n = g_bias ? n_items : 0; }
     }
-    return GS_OK;
+    if (dtype == GS_F32) return run_bwd<float>(a, j, blocks, s);
+    if (dtype == GS_BF16) return run_bwd<__bf16>(a, j, blocks, s);
+    return run_bwd<_Float16>(a, j, blocks, s);
 }
