@@ -53,19 +53,49 @@ __device__ __forceinline__ uint32_t next_piece(float &x) {
     return hi;
 }
 
+// Eight floats cut into NZ pieces: all but the last by truncation, the last rounded to nearest (one that takes what is
+// left whole is not changed by it).
+__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) {
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+template <int NZ> __device__ __forceinline__ void cut_pieces(float *v, bf16x8 *z) {
+#pragma unroll
+    for (int p = 0; p < NZ; ++p) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float &lo = v[2 * i], &hi = v[2 * i + 1];
+            if (p + 1 < NZ) {
+                w[i] = upper_halves(lo, hi);
+                next_piece(lo);
+                next_piece(hi);
+            } else {
+                using pair = __attribute__((ext_vector_type(2))) __bf16;
+                const pair x = {(__bf16)lo, (__bf16)hi};
+                w[i] = __builtin_bit_cast(uint32_t, x);
+            }
+        }
+        z[p] = __builtin_bit_cast(bf16x8, *reinterpret_cast<uint4 *>(w));
+    }
+}
+
 template <int P> struct Fragment { bf16x8 p[P]; };
+
+// Waves per SIMD a kernel is compiled for: two where its operands leave room in 256 registers (the matrix results then
+// stay in the registers the vector ALU reads), else one.
+constexpr int waves_for(int registers) { return registers <= 160 ? 2 : 1; }
 
 // Whether a tile's fragments fit the registers beside everything else: they are then requested while the scores before
 // them are worked on.  Otherwise each is requested where it is used and other waves cover the wait.
 template <int P, int KC> constexpr bool kAhead = P * KC <= 16;
 
-// frag: the first fragment of a tile plus this lane's 16 bytes.
+// frag: the first fragment of a tile, the same in all lanes.
 template <int P>
-__device__ __forceinline__ Fragment<P> load_fragment(const uint4 *frag, int index) {
+__device__ __forceinline__ Fragment<P> load_fragment(const uint4 *frag, int index, int lane) {
     Fragment<P> f;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const uint4 v = frag[(size_t)(index * P + i) * 64];
+        const uint4 v = frag[(index * P + i) * 64 + lane];
         f.p[i] = *reinterpret_cast<const bf16x8 *>(&v);
     }
     return f;

@@ -181,13 +181,13 @@ struct FwdArgs {
 };
 
 template <int P, int DB, int OF, bool TOP>
-__global__ __launch_bounds__(kCatThreads)
+__global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * P * OF + (kAhead<P, 2 * DB> ? 8 * DB * P : 4 * P) + 16 * OF))
 void catalog_fwd_kernel(FwdArgs a) {
     constexpr int KC = 2 * DB;
     const int lane = threadIdx.x & 63;
-    const int64_t task = (int64_t)blockIdx.x * (kCatThreads / 64) + (threadIdx.x >> 6);
-    if (task >= (int64_t)a.groups * a.shares) return;
-    const int group = (int)(task % a.groups), share = (int)(task / a.groups);
+    const uint32_t task = __builtin_amdgcn_readfirstlane(blockIdx.x * (kCatThreads / 64) + (threadIdx.x >> 6));
+    if (task >= (uint32_t)a.groups * (uint32_t)a.shares) return;
+    const int group = (int)(task % (uint32_t)a.groups), share = (int)(task / (uint32_t)a.groups);
     const int t0 = share * a.tiles_per_share, t1 = min(t0 + a.tiles_per_share, a.item_tiles);
 
     Fragment<P> own[OF][KC];
@@ -196,9 +196,9 @@ void catalog_fwd_kernel(FwdArgs a) {
 #pragma unroll
     for (int f = 0; f < OF; ++f) {
         const int tile = min(group * OF + f, a.user_tiles - 1);            // (a tile past the end repeats the last one)
-        const uint4 *src = a.user + (size_t)tile * KC * P * 64 + lane;
+        const uint4 *src = a.user + (size_t)tile * KC * P * 64;
 #pragma unroll
-        for (int kc = 0; kc < KC; ++kc) own[f][kc] = load_fragment<P>(src, kc);
+        for (int kc = 0; kc < KC; ++kc) own[f][kc] = load_fragment<P>(src, kc, lane);
         const int64_t n = (int64_t)tile * 32 + (lane & 31);
         target[f] = a.targets && n < a.n_users ? a.targets[n] : -1;
         if (target[f] >= a.n_items) target[f] = -1;
@@ -207,11 +207,11 @@ void catalog_fwd_kernel(FwdArgs a) {
         hit[f] = -INFINITY;
     }
     constexpr bool AHEAD = kAhead<P, KC>;
-    const uint4 *src = a.item + (size_t)t0 * KC * P * 64 + lane;
+    const uint4 *src = a.item + (size_t)t0 * KC * P * 64;
     Fragment<P> it[AHEAD ? KC : 1];
     if (AHEAD)
 #pragma unroll
-        for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(src, kc);
+        for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(src, kc, lane);
     float tops[OF][4];
     for (int t = t0; t < t1; ++t) {
         f32x16 acc[OF];
@@ -221,14 +221,14 @@ void catalog_fwd_kernel(FwdArgs a) {
             for (int r = 0; r < 16; ++r) acc[f][r] = 0.f;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
-            if (!AHEAD) it[0] = load_fragment<P>(src, kc);
+            if (!AHEAD) it[0] = load_fragment<P>(src, kc, lane);
 #pragma unroll
             for (int f = 0; f < OF; ++f) multiply<P, P, 2>(acc[f], it[AHEAD ? kc : 0].p, own[f][kc].p);
         }
         src += (size_t)KC * P * 64;
         if (AHEAD && t + 1 < t1)
 #pragma unroll
-            for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(src, kc);
+            for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(src, kc, lane);
         float b[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g)

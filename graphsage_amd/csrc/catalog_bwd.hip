@@ -32,20 +32,20 @@ struct BwdArgs {
 };
 
 template <class T, int DB, bool USERS>
-__device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, int64_t task) {
+__device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uint32_t task) {
     constexpr int P = Pieces<T>::P, KC = 2 * DB, NZ = P == 3 ? 3 : 2, MOST = P == 3 ? 2 : 1;
     constexpr bool AHEAD = kAhead<P, KC>;
     const int lane = threadIdx.x & 63, half = lane >> 5;
-    if (task >= (int64_t)side.own_tiles * side.shares) return;
-    const int tile = (int)(task % side.own_tiles), share = (int)(task / side.own_tiles);
+    if (task >= (uint32_t)side.own_tiles * (uint32_t)side.shares) return;
+    const int tile = (int)(task % (uint32_t)side.own_tiles), share = (int)(task / (uint32_t)side.own_tiles);
     const int t0 = share * side.tiles_per_share, t1 = min(t0 + side.tiles_per_share, side.stream_tiles);
     const int mine = tile * 32 + (lane & 31);
 
     Fragment<P> own[KC];
     {
-        const uint4 *src = side.own + (size_t)tile * KC * P * 64 + lane;
+        const uint4 *src = side.own + (size_t)tile * KC * P * 64;
 #pragma unroll
-        for (int kc = 0; kc < KC; ++kc) own[kc] = load_fragment<P>(src, kc);
+        for (int kc = 0; kc < KC; ++kc) own[kc] = load_fragment<P>(src, kc, lane);
     }
     float lse2 = 0.f, ca = 0.f, cb = 0.f, cg = 0.f, bias = 0.f, sum = 0.f;
     int target = -1;
@@ -57,11 +57,11 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, int
 #pragma unroll
         for (int r = 0; r < 16; ++r) out[d][r] = 0.f;
 
-    const uint4 *rows = side.stream_rows + (size_t)t0 * KC * P * 64 + lane, *cols = side.stream_cols + (size_t)t0 * KC * P * 64 + lane;
+    const uint4 *rows = side.stream_rows + (size_t)t0 * KC * P * 64, *cols = side.stream_cols + (size_t)t0 * KC * P * 64;
     Fragment<P> it[AHEAD ? KC : 1], ct[AHEAD ? KC : 1];
     if (AHEAD)
 #pragma unroll
-        for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(rows, kc);
+        for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(rows, kc, lane);
     for (int t = t0; t < t1; ++t) {
         // what the scores are turned into dz with: of the streamed rows
         float x[16], y[16], w[16];
@@ -82,17 +82,17 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, int
         for (int r = 0; r < 16; ++r) acc[r] = 0.f;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
-            if (!AHEAD) it[0] = load_fragment<P>(rows, kc);
+            if (!AHEAD) it[0] = load_fragment<P>(rows, kc, lane);
             multiply<P, P, 2>(acc, it[AHEAD ? kc : 0].p, own[kc].p);
         }
         rows += (size_t)KC * P * 64;
         if (AHEAD) {
             // this tile's second operand and the next tile's first are on their way while dz is formed
 #pragma unroll
-            for (int kc = 0; kc < KC; ++kc) ct[kc] = load_fragment<P>(cols, kc);
+            for (int kc = 0; kc < KC; ++kc) ct[kc] = load_fragment<P>(cols, kc, lane);
             if (t + 1 < t1)
 #pragma unroll
-                for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(rows, kc);
+                for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(rows, kc, lane);
         }
         float dz[16];
 #pragma unroll
@@ -125,19 +125,10 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, int
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             bf16x8 z[NZ];
-#pragma unroll
-            for (int p = 0; p < NZ; ++p) {
-                uint32_t word[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t lo = next_piece(dz[8 * h + 2 * i]), hi = next_piece(dz[8 * h + 2 * i + 1]);
-                    word[i] = (lo >> 16) | hi;
-                }
-                z[p] = *reinterpret_cast<const bf16x8 *>(word);
-            }
+            cut_pieces<NZ>(dz + 8 * h, z);
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                if (!AHEAD) ct[0] = load_fragment<P>(cols, h * DB + d);
+                if (!AHEAD) ct[0] = load_fragment<P>(cols, h * DB + d, lane);
                 multiply<NZ, P, MOST>(out[d], z, ct[AHEAD ? h * DB + d : 0].p);
             }
         }
@@ -168,11 +159,11 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, int
 
 // Both gradients in one launch: the first blocks own users, the others items.
 template <class T, int DB>
-__global__ __launch_bounds__(kCatThreads)
+__global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * Pieces<T>::P * (kAhead<Pieces<T>::P, 2 * DB> ? 3 : 1) + 16 * DB + 16))
 void catalog_bwd_kernel(BwdArgs a) {
-    const int wave = threadIdx.x >> 6;
-    if ((int)blockIdx.x < a.user_blocks) backward<T, DB, true>(a, a.users, (int64_t)blockIdx.x * (kCatThreads / 64) + wave);
-    else backward<T, DB, false>(a, a.items, (int64_t)(blockIdx.x - a.user_blocks) * (kCatThreads / 64) + wave);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if ((int)blockIdx.x < a.user_blocks) backward<T, DB, true>(a, a.users, blockIdx.x * (kCatThreads / 64) + wave);
+    else backward<T, DB, false>(a, a.items, (blockIdx.x - a.user_blocks) * (kCatThreads / 64) + wave);
 }
 
 // Adds the shares in order: users' elements, then items', then the bias.
