@@ -85,9 +85,25 @@ template <int P> struct Fragment { bf16x8 p[P]; };
 // stay in the registers the vector ALU reads), else one.
 constexpr int waves_for(int registers) { return registers <= 160 ? 2 : 1; }
 
-// Whether a tile's fragments fit the registers beside everything else: they are then requested while the scores before
-// them are worked on.  Otherwise each is requested where it is used and other waves cover the wait.
-template <int P, int KC> constexpr bool kAhead = P * KC <= 16;
+// The four waves of a block own neighboring rows and stream the same tiles, which therefore pass through LDS: loads that
+// write LDS directly fill one half of it while the waves work on the other (a wave reading its fragments itself was
+// measured at 626 us for 4096 users and 100 000 items of 64 bf16, forward and backward, bound by 7 TB/s out of L2).
+// `fragments`: kilobytes of a tile; tiles per half so that a barrier is worth it.
+constexpr int tiles_per_stage(int fragments) { return fragments <= 4 ? 4 : fragments <= 12 ? 2 : 1; }
+constexpr bool fits_lds(int fragments) { return 2 * fragments * tiles_per_stage(fragments) <= 152; }
+
+// One fragment into LDS at byte offset dst; both the same in all lanes.  Done when vmcnt says so.
+__device__ __forceinline__ void fragment_to_lds(const uint4 *src, int lane, uint32_t dst) {
+    const unsigned long long from = reinterpret_cast<unsigned long long>(src + lane);
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(from), "s"(dst) : "memory");
+}
+// This wave's loads into LDS have arrived, and then everybody's.
+__device__ __forceinline__ void stage_ready() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
 
 // frag: the first fragment of a tile, the same in all lanes.
 template <int P>
@@ -116,10 +132,11 @@ __device__ __forceinline__ float half_max(float v) {           // the larger of 
     return fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
 }
 
-// What the backward kernels need of a user, padded to whole tiles (catalog_bwd.hip).
-struct Stats {
-    float *lse2, *a, *b2, *g;
-    int32_t *target;
+// What the backward kernels need of 32 users, as one more fragment of their tile (catalog_bwd.hip).
+struct alignas(16) Stats {
+    float lse2[32], a[32], b2[32], g[32];
+    int32_t target[32];
+    float unused[96];                               // (a fragment is a kilobyte)
 };
 struct StatsFrom {
     int64_t n_items;
@@ -134,7 +151,7 @@ struct Layout {                                     // one table to lay out
     uint4 *rows, *cols;                             // nullable
     float *bias2;                                   // nullable: bias in units of log 2, or kMasked
     float *tile_abs;                                // nullable: the largest |element| of every tile
-    Stats st;                                       // st.lse2 nullable
+    Stats *stats;                                   // nullable
     StatsFrom from;
 };
 

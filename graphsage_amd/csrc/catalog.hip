@@ -45,7 +45,7 @@ void layout_kernel(Layout first, Layout second, int first_tiles, int dim, int bl
         const bool offered = tid < rows && !(l.bias && l.bias[row0 + tid] < kOffer);
         on[tid] = offered;
         if (l.bias2) l.bias2[row0 + tid] = !offered ? kMasked : l.bias ? l.bias[row0 + tid] * kLog2e : 0.f;
-        if (l.st.lse2) {
+        if (l.stats) {
             // lse2 = 1e14 silences a user: padding, or one for whom nothing is on offer
             const int64_t n = row0 + tid;
             float lse2 = 1e14f, ca = 0.f, cb = 0.f, g = 0.f;
@@ -60,7 +60,8 @@ void layout_kernel(Layout first, Layout second, int first_tiles, int dim, int bl
                 ca = -(g + (l.from.g_entropy ? ge * l.from.entropy[n] : 0.f));
                 cb = -ge * kLn2;
             }
-            l.st.lse2[n] = lse2; l.st.a[n] = ca; l.st.b2[n] = cb; l.st.g[n] = g; l.st.target[n] = t;
+            Stats &st = l.stats[tile];
+            st.lse2[tid] = lse2; st.a[tid] = ca; st.b2[tid] = cb; st.g[tid] = g; st.target[tid] = t;
         }
     }
     __syncthreads();
@@ -176,19 +177,29 @@ struct FwdArgs {
     float *tile_max;                                // [users][tile_stride], with TOP
     int64_t tile_stride;
     int64_t n_users, n_items;
-    int user_tiles, item_tiles, groups, shares, tiles_per_share;
+    int user_tiles, item_tiles, group_blocks, shares, tiles_per_share;
     float scale2;
 };
 
 template <int P, int DB, int OF, bool TOP>
-__global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * P * OF + (kAhead<P, 2 * DB> ? 8 * DB * P : 4 * P) + 16 * OF))
+__global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * P * OF + 16 * OF + 24))
 void catalog_fwd_kernel(FwdArgs a) {
-    constexpr int KC = 2 * DB;
-    const int lane = threadIdx.x & 63;
-    const uint32_t task = __builtin_amdgcn_readfirstlane(blockIdx.x * (kCatThreads / 64) + (threadIdx.x >> 6));
-    if (task >= (uint32_t)a.groups * (uint32_t)a.shares) return;
-    const int group = (int)(task % (uint32_t)a.groups), share = (int)(task / (uint32_t)a.groups);
+    constexpr int KC = 2 * DB, F = KC * P, ST = tiles_per_stage(F), W = kCatThreads / 64;
+    extern __shared__ uint4 stage[];                // [2][ST][F][64]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(stage));
+    const int group = (int)(blockIdx.x % (uint32_t)a.group_blocks) * W + wave, share = (int)(blockIdx.x / (uint32_t)a.group_blocks);
     const int t0 = share * a.tiles_per_share, t1 = min(t0 + a.tiles_per_share, a.item_tiles);
+    const auto issue = [&](int t, int half) {
+#pragma unroll
+        for (int k = 0; k < ST; ++k)
+            if (t + k < t1)
+#pragma unroll
+                for (int i = 0; i < (F + W - 1) / W; ++i)
+                    if (i * W + wave < F)
+                        fragment_to_lds(a.item + ((size_t)(t + k) * F + i * W + wave) * 64, lane, lds + ((half * ST + k) * F + i * W + wave) * 1024);
+    };
+    issue(t0, 0);
 
     Fragment<P> own[OF][KC];
     float m[OF], s[OF], w[OF], hit[OF];
@@ -206,14 +217,14 @@ void catalog_fwd_kernel(FwdArgs a) {
         s[f] = w[f] = 0.f;
         hit[f] = -INFINITY;
     }
-    constexpr bool AHEAD = kAhead<P, KC>;
-    const uint4 *src = a.item + (size_t)t0 * KC * P * 64;
-    Fragment<P> it[AHEAD ? KC : 1];
-    if (AHEAD)
-#pragma unroll
-        for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(src, kc, lane);
     float tops[OF][4];
     for (int t = t0; t < t1; ++t) {
+        const int at = (t - t0) % ST, half = (t - t0) / ST % 2;
+        if (at == 0) {
+            stage_ready();
+            if (t + ST < t1) issue(t + ST, half ^ 1);
+        }
+        const uint4 *src = stage + (half * ST + at) * F * 64;
         f32x16 acc[OF];
 #pragma unroll
         for (int f = 0; f < OF; ++f)
@@ -221,14 +232,10 @@ void catalog_fwd_kernel(FwdArgs a) {
             for (int r = 0; r < 16; ++r) acc[f][r] = 0.f;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
-            if (!AHEAD) it[0] = load_fragment<P>(src, kc, lane);
+            const Fragment<P> it = load_fragment<P>(src, kc, lane);
 #pragma unroll
-            for (int f = 0; f < OF; ++f) multiply<P, P, 2>(acc[f], it[AHEAD ? kc : 0].p, own[f][kc].p);
+            for (int f = 0; f < OF; ++f) multiply<P, P, 2>(acc[f], it.p, own[f][kc].p);
         }
-        src += (size_t)KC * P * 64;
-        if (AHEAD && t + 1 < t1)
-#pragma unroll
-            for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(src, kc, lane);
         float b[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g)
@@ -475,13 +482,14 @@ Cut cut_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
     return c;
 }
 
-constexpr int64_t kWaves = 4096;                    // waves a launch is cut into: four per SIMD
+constexpr int64_t kBlocks = 1024;                   // blocks a launch is cut into: four waves per SIMD
 
-void shares_of(int64_t users, int64_t n_items, int of, int *groups, int *shares, int *per_share) {
+void shares_of(int64_t users, int64_t n_items, int of, int *group_blocks, int *shares, int *per_share) {
+    constexpr int W = gs::kCatThreads / 64;
     const int64_t ut = tiles_of(users), it = tiles_of(n_items);
-    *groups = (int)((ut + of - 1) / of);
-    int64_t sh = kWaves / *groups;
-    if (sh > it / 2) sh = it / 2;
+    *group_blocks = (int)((ut + of * W - 1) / (of * W));
+    int64_t sh = kBlocks / *group_blocks;
+    if (sh > it / 4) sh = it / 4;
     if (sh < 1) sh = 1;
     *per_share = it ? (int)((it + sh - 1) / sh + 3) / 4 * 4 : 4;       // (tile maxima leave by fours)
     *shares = (int)((it + *per_share - 1) / *per_share);
@@ -496,15 +504,15 @@ struct Space {
 Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
     Space s;
     const Cut c = cut_of(n_users, n_items, dim, dtype, top_k);
-    int groups, shares, per;
-    shares_of(c.slice, n_items, c.of, &groups, &shares, &per);
+    int blocks, shares, per;
+    shares_of(c.slice, n_items, c.of, &blocks, &shares, &per);
     size_t off = 0;
     s.user = off; off += align256(layout_bytes(c.slice, dim, dtype));
     s.item = off; off += align256(layout_bytes(n_items, dim, dtype));
     s.bias2 = off; off += align256((size_t)tiles_of(n_items) * 32 * sizeof(float));
     s.part = off;
-    // the last slice may be smaller and have more shares: the product of both is bounded by the waves
-    off += align256((size_t)(c.slice * (int64_t)shares + kWaves * 64) * sizeof(float4));
+    // the last slice may be smaller and have more shares: the product of both is bounded by the blocks' users
+    off += align256((size_t)(c.slice * (int64_t)shares + kBlocks * 256) * sizeof(float4));
     s.lse = off; off += align256((size_t)c.slice * sizeof(float));
     s.tile_abs = off;
     if (top_k > 0) off += align256((size_t)tiles_of(n_items) * sizeof(float));
@@ -514,28 +522,38 @@ Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) 
     return s;
 }
 
+template <int P, int DB, int OF, bool TOP>
+int launch_one(const FwdArgs &a, hipStream_t stream) {
+    constexpr int F = 2 * DB * P, lds = 2 * F * gs::tiles_per_stage(F) * 1024;
+    static_assert(gs::fits_lds(F), "a tile does not fit");
+    const auto kernel = catalog_fwd_kernel<P, DB, OF, TOP>;
+    if (lds > 64 * 1024) {
+        const hipError_t e = gs::raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
+        if (e != hipSuccess) return gs::fail(GS_ELAUNCH, "gs_catalog_fwd: LDS limit: %s", hipGetErrorString(e));
+    }
+    kernel<<<dim3((unsigned)((int64_t)a.group_blocks * a.shares)), kCatThreads, lds, stream>>>(a);
+    return gs::check_launch("gs_catalog_fwd");
+}
+
 template <int P, int DB, int OF>
-void launch_tile(const FwdArgs &a, hipStream_t stream) {
-    const dim3 grid((unsigned)(((int64_t)a.groups * a.shares + kCatThreads / 64 - 1) / (kCatThreads / 64)));
-    if (a.tile_max) catalog_fwd_kernel<P, DB, OF, true><<<grid, kCatThreads, 0, stream>>>(a);
-    else catalog_fwd_kernel<P, DB, OF, false><<<grid, kCatThreads, 0, stream>>>(a);
+int launch_tile(const FwdArgs &a, hipStream_t stream) {
+    return a.tile_max ? launch_one<P, DB, OF, true>(a, stream) : launch_one<P, DB, OF, false>(a, stream);
 }
 
 template <int P>
-void launch_fwd(const FwdArgs &a, int blocks, int of, hipStream_t stream) {
+int launch_fwd(const FwdArgs &a, int blocks, int of, hipStream_t stream) {
     if (of == 2) {
-        if (blocks == 1) launch_tile<P, 1, 2>(a, stream);
-        else if (blocks == 2) launch_tile<P, 2, 2>(a, stream);
-        else if constexpr (P * 4 <= 8) {
-            if (blocks == 4) launch_tile<P, 4, 2>(a, stream);
-            else if constexpr (P == 1) launch_tile<P, 8, 2>(a, stream);
+        if (blocks == 1) return launch_tile<P, 1, 2>(a, stream);
+        if (blocks == 2) return launch_tile<P, 2, 2>(a, stream);
+        if constexpr (P * 4 <= 8) {
+            if (blocks == 4) return launch_tile<P, 4, 2>(a, stream);
         }
-        return;
+        if constexpr (P == 1) return launch_tile<P, 8, 2>(a, stream);
     }
-    if (blocks == 1) launch_tile<P, 1, 1>(a, stream);
-    else if (blocks == 2) launch_tile<P, 2, 1>(a, stream);
-    else if (blocks == 4) launch_tile<P, 4, 1>(a, stream);
-    else launch_tile<P, 8, 1>(a, stream);
+    if (blocks == 1) return launch_tile<P, 1, 1>(a, stream);
+    if (blocks == 2) return launch_tile<P, 2, 1>(a, stream);
+    if (blocks == 4) return launch_tile<P, 4, 1>(a, stream);
+    return launch_tile<P, 8, 1>(a, stream);
 }
 
 }  // namespace
@@ -592,14 +610,13 @@ extern "C" int gs_catalog_fwd(const void *user, int64_t n_users, const void *ite
         a.tile_stride = tile_stride_of(n_items);
         a.n_users = nu; a.n_items = n_items;
         a.user_tiles = (int)gs::tiles_of(nu); a.item_tiles = (int)gs::tiles_of(n_items);
-        shares_of(nu, n_items, cut.of, &a.groups, &a.shares, &a.tiles_per_share);
+        shares_of(nu, n_items, cut.of, &a.group_blocks, &a.shares, &a.tiles_per_share);
         a.scale2 = scale * gs::kLog2e;
         if (n_items == 0) a.shares = 0;
         else {
-            if (pieces == 1) launch_fwd<1>(a, blocks, cut.of, s);
-            else if (pieces == 2) launch_fwd<2>(a, blocks, cut.of, s);
-            else launch_fwd<3>(a, blocks, cut.of, s);
-            if (int rc = gs::check_launch(what)) return rc;
+            if (int rc = pieces == 1 ? launch_fwd<1>(a, blocks, cut.of, s) : pieces == 2 ? launch_fwd<2>(a, blocks, cut.of, s)
+                                                                                        : launch_fwd<3>(a, blocks, cut.of, s))
+                return rc;
         }
         float *lse_out = lse ? lse + u0 : reinterpret_cast<float *>(ws + sp.lse);
         catalog_join_kernel<<<dim3((unsigned)((nu + 3) / 4)), gs::kCatThreads, 0, s>>>(

@@ -25,21 +25,45 @@ struct Side {                                       // one of the two gradients
 struct BwdArgs {
     Side users, items;
     const float *bias2;
-    Stats st;
+    const Stats *stats;                             // of the users' tiles
     float *part_bias, *g_bias;                      // [shares][own tiles * 32]; nullable
-    int user_blocks, dim;
+    int user_blocks, item_blocks, dim;
     float scale, scale2;
 };
 
+// Fragments of a streamed tile: rows, cols and, of users, their statistics.  Where two tiles do not fit into LDS (fp32 of
+// more than 128 elements) every wave reads its own from L2.
+template <int P, int DB, bool USERS> constexpr int kTile = 4 * DB * P + (USERS ? 0 : 1);
+template <int P, int DB> constexpr bool kStaged = fits_lds(kTile<P, DB, false>);
+
 template <class T, int DB, bool USERS>
-__device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uint32_t task) {
-    constexpr int P = Pieces<T>::P, KC = 2 * DB, NZ = P == 3 ? 3 : 2, MOST = P == 3 ? 2 : 1;
-    constexpr bool AHEAD = kAhead<P, KC>;
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    if (task >= (uint32_t)side.own_tiles * (uint32_t)side.shares) return;
-    const int tile = (int)(task % (uint32_t)side.own_tiles), share = (int)(task / (uint32_t)side.own_tiles);
+__device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uint32_t block, uint4 *stage) {
+    constexpr int P = Pieces<T>::P, KC = 2 * DB, NZ = P == 3 ? 3 : 2, MOST = P == 3 ? 2 : 1, W = kCatThreads / 64;
+    constexpr int F = kTile<P, DB, USERS>, ST = kStaged<P, DB> ? tiles_per_stage(F) : 1;
+    constexpr bool STAGED = kStaged<P, DB>;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>(stage));
+    const uint32_t tile_blocks = (side.own_tiles + W - 1) / W;
+    const int tile_mine = (int)(block % tile_blocks) * W + wave, share = (int)(block / tile_blocks);
+    const bool live = tile_mine < side.own_tiles;   // a wave past the last tile repeats it and writes nothing
+    const int tile = live ? tile_mine : side.own_tiles - 1;
     const int t0 = share * side.tiles_per_share, t1 = min(t0 + side.tiles_per_share, side.stream_tiles);
     const int mine = tile * 32 + (lane & 31);
+    const auto issue = [&](int t, int to) {
+#pragma unroll
+        for (int k = 0; k < ST; ++k)
+            if (t + k < t1)
+#pragma unroll
+                for (int i = 0; i < (F + W - 1) / W; ++i) {
+                    const int f = i * W + wave;
+                    if (f >= F) continue;
+                    const uint4 *src = f < KC * P ? side.stream_rows + ((size_t)(t + k) * KC * P + f) * 64
+                                       : f < 2 * KC * P ? side.stream_cols + ((size_t)(t + k) * KC * P + f - KC * P) * 64
+                                                        : reinterpret_cast<const uint4 *>(a.stats + t + k);
+                    fragment_to_lds(src, lane, lds + ((to * ST + k) * F + f) * 1024);
+                }
+    };
+    if (STAGED) issue(t0, 0);
 
     Fragment<P> own[KC];
     {
@@ -49,50 +73,55 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
     }
     float lse2 = 0.f, ca = 0.f, cb = 0.f, cg = 0.f, bias = 0.f, sum = 0.f;
     int target = -1;
-    if (USERS) { lse2 = a.st.lse2[mine]; ca = a.st.a[mine]; cb = a.st.b2[mine]; cg = a.st.g[mine]; target = a.st.target[mine]; }
-    else bias = a.bias2[mine];
+    if (USERS) {
+        const Stats &st = a.stats[tile];
+        const int i = lane & 31;
+        lse2 = st.lse2[i]; ca = st.a[i]; cb = st.b2[i]; cg = st.g[i]; target = st.target[i];
+    } else bias = a.bias2[mine];
     f32x16 out[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) out[d][r] = 0.f;
 
-    const uint4 *rows = side.stream_rows + (size_t)t0 * KC * P * 64, *cols = side.stream_cols + (size_t)t0 * KC * P * 64;
-    Fragment<P> it[AHEAD ? KC : 1], ct[AHEAD ? KC : 1];
-    if (AHEAD)
-#pragma unroll
-        for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(rows, kc, lane);
     for (int t = t0; t < t1; ++t) {
+        const uint4 *rows, *cols;
+        const Stats *st;
+        if constexpr (STAGED) {
+            const int at = (t - t0) % ST, from = (t - t0) / ST % 2;
+            if (at == 0) {
+                stage_ready();
+                if (t + ST < t1) issue(t + ST, from ^ 1);
+            }
+            rows = stage + (from * ST + at) * F * 64;
+            cols = rows + KC * P * 64;
+            st = reinterpret_cast<const Stats *>(cols + KC * P * 64);
+        } else {
+            rows = side.stream_rows + (size_t)t * KC * P * 64;
+            cols = side.stream_cols + (size_t)t * KC * P * 64;
+            st = a.stats + t;
+        }
         // what the scores are turned into dz with: of the streamed rows
         float x[16], y[16], w[16];
         int tg = -1;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int at = t * 32 + 8 * g + 4 * half;
-            if (USERS) *reinterpret_cast<float4 *>(x + 4 * g) = *reinterpret_cast<const float4 *>(a.bias2 + at);
+            const int i = 8 * g + 4 * half;
+            if (USERS) *reinterpret_cast<float4 *>(x + 4 * g) = *reinterpret_cast<const float4 *>(a.bias2 + t * 32 + i);
             else {
-                *reinterpret_cast<float4 *>(x + 4 * g) = *reinterpret_cast<const float4 *>(a.st.lse2 + at);
-                *reinterpret_cast<float4 *>(y + 4 * g) = *reinterpret_cast<const float4 *>(a.st.a + at);
-                *reinterpret_cast<float4 *>(w + 4 * g) = *reinterpret_cast<const float4 *>(a.st.b2 + at);
+                *reinterpret_cast<float4 *>(x + 4 * g) = *reinterpret_cast<const float4 *>(st->lse2 + i);
+                *reinterpret_cast<float4 *>(y + 4 * g) = *reinterpret_cast<const float4 *>(st->a + i);
+                *reinterpret_cast<float4 *>(w + 4 * g) = *reinterpret_cast<const float4 *>(st->b2 + i);
             }
         }
-        if (!USERS) tg = a.st.target[t * 32 + (lane & 31)];
+        if (!USERS) tg = st->target[lane & 31];
         f32x16 acc;
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] = 0.f;
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) {
-            if (!AHEAD) it[0] = load_fragment<P>(rows, kc, lane);
-            multiply<P, P, 2>(acc, it[AHEAD ? kc : 0].p, own[kc].p);
-        }
-        rows += (size_t)KC * P * 64;
-        if (AHEAD) {
-            // this tile's second operand and the next tile's first are on their way while dz is formed
-#pragma unroll
-            for (int kc = 0; kc < KC; ++kc) ct[kc] = load_fragment<P>(cols, kc, lane);
-            if (t + 1 < t1)
-#pragma unroll
-                for (int kc = 0; kc < KC; ++kc) it[kc] = load_fragment<P>(rows, kc, lane);
+            const Fragment<P> it = load_fragment<P>(rows, kc, lane);
+            multiply<P, P, 2>(acc, it.p, own[kc].p);
         }
         float dz[16];
 #pragma unroll
@@ -110,7 +139,7 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
                 for (int r = 0; r < 16; ++r) dz[r] += on && local == row_of_reg(r, lane) ? cg : 0.f;
             }
         } else if (__any(tg >= 0 && (tg >> 5) == tile)) {
-            const float g = a.st.g[t * 32 + (lane & 31)];
+            const float g = st->g[lane & 31];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int src = row_of_reg(r, lane);
@@ -128,12 +157,12 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
             cut_pieces<NZ>(dz + 8 * h, z);
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                if (!AHEAD) ct[0] = load_fragment<P>(cols, h * DB + d, lane);
-                multiply<NZ, P, MOST>(out[d], z, ct[AHEAD ? h * DB + d : 0].p);
+                const Fragment<P> ct = load_fragment<P>(cols, h * DB + d, lane);
+                multiply<NZ, P, MOST>(out[d], z, ct.p);
             }
         }
-        cols += (size_t)KC * P * 64;
     }
+    if (!live) return;
     if (side.out && side.shares == 1) {
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -159,11 +188,11 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
 
 // Both gradients in one launch: the first blocks own users, the others items.
 template <class T, int DB>
-__global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * Pieces<T>::P * (kAhead<Pieces<T>::P, 2 * DB> ? 3 : 1) + 16 * DB + 16))
+__global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * Pieces<T>::P + 16 * DB + 72))
 void catalog_bwd_kernel(BwdArgs a) {
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if ((int)blockIdx.x < a.user_blocks) backward<T, DB, true>(a, a.users, blockIdx.x * (kCatThreads / 64) + wave);
-    else backward<T, DB, false>(a, a.items, (blockIdx.x - a.user_blocks) * (kCatThreads / 64) + wave);
+    extern __shared__ uint4 stage[];
+    if ((int)blockIdx.x < a.user_blocks) backward<T, DB, true>(a, a.users, blockIdx.x, stage);
+    else backward<T, DB, false>(a, a.items, blockIdx.x - a.user_blocks, stage);
 }
 
 // Adds the shares in order: users' elements, then items', then the bias.
@@ -210,10 +239,11 @@ struct Space {
     int user_shares, user_per, item_shares, item_per;
 };
 
-constexpr int64_t kWaves = 4096;
+constexpr int64_t kBlocks = 512;                    // blocks each side is cut into: with the other's, four waves per SIMD
 
 void shares_of(int64_t own, int64_t stream, int *shares, int *per) {
-    int64_t s = own ? kWaves / own : 1;
+    constexpr int W = kCatThreads / 64;
+    int64_t s = own ? kBlocks / ((own + W - 1) / W) : 1;
     if (s > stream / 4) s = stream / 4;
     if (s < 1) s = 1;
     *per = stream ? (int)((stream + s - 1) / s) : 1;
@@ -232,7 +262,7 @@ Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype) {
     s.item_rows = off; off += align256(layout_bytes(n_items, dim, dtype));
     s.item_cols = off; off += align256(layout_bytes(n_items, dim, dtype));
     s.bias2 = off; off += align256((size_t)it * 32 * sizeof(float));
-    s.stats = off; off += 5 * align256((size_t)ut * 32 * sizeof(float));
+    s.stats = off; off += (size_t)ut * sizeof(Stats);
     s.user_part = off; off += s.user_shares > 1 ? align256(ut * s.user_shares * row) : 0;
     s.item_part = off; off += s.item_shares > 1 ? align256(it * s.item_shares * row) : 0;
     s.part_bias = off; off += s.item_shares > 1 ? align256((size_t)it * s.item_shares * 32 * sizeof(float)) : 0;
@@ -240,16 +270,26 @@ Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype) {
     return s;
 }
 
+template <class T, int DB>
+int launch_bwd(const BwdArgs &a, hipStream_t stream) {
+    constexpr int P = Pieces<T>::P, FU = kTile<P, DB, true>, FI = kTile<P, DB, false>;
+    constexpr int users = FU * tiles_per_stage(FU), items = FI * tiles_per_stage(FI);
+    constexpr int lds = kStaged<P, DB> ? 2 * (users > items ? users : items) * 1024 : 0;
+    const auto kernel = catalog_bwd_kernel<T, DB>;
+    if (lds > 64 * 1024) {
+        const hipError_t e = gs::raise_lds_limit(reinterpret_cast<const void *>(kernel), lds);
+        if (e != hipSuccess) return gs::fail(GS_ELAUNCH, "gs_catalog_bwd: LDS limit: %s", hipGetErrorString(e));
+    }
+    kernel<<<dim3((unsigned)(a.user_blocks + a.item_blocks)), kCatThreads, lds, stream>>>(a);
+    return gs::check_launch("gs_catalog_bwd");
+}
+
 template <class T>
 int run_bwd(const BwdArgs &a, const JoinArgs &j, int blocks, hipStream_t stream) {
-    constexpr int W = kCatThreads / 64;
-    const unsigned n = (unsigned)(a.user_blocks + ((int64_t)a.items.own_tiles * a.items.shares + W - 1) / W);
-    if (n) {
-        if (blocks == 1) catalog_bwd_kernel<T, 1><<<dim3(n), kCatThreads, 0, stream>>>(a);
-        else if (blocks == 2) catalog_bwd_kernel<T, 2><<<dim3(n), kCatThreads, 0, stream>>>(a);
-        else if (blocks == 4) catalog_bwd_kernel<T, 4><<<dim3(n), kCatThreads, 0, stream>>>(a);
-        else catalog_bwd_kernel<T, 8><<<dim3(n), kCatThreads, 0, stream>>>(a);
-        if (int rc = gs::check_launch("gs_catalog_bwd")) return rc;
+    if (a.user_blocks + a.item_blocks) {
+        if (int rc = blocks == 1 ? launch_bwd<T, 1>(a, stream) : blocks == 2 ? launch_bwd<T, 2>(a, stream)
+                   : blocks == 4 ? launch_bwd<T, 4>(a, stream) : launch_bwd<T, 8>(a, stream))
+            return rc;
     }
     const int64_t elements = j.user_n + j.item_n + j.bias_n;
     if (elements) {
@@ -286,18 +326,14 @@ extern "C" int gs_catalog_bwd(const void *user, int64_t n_users, const void *ite
     char *ws = static_cast<char *>(workspace);
     hipStream_t s = (hipStream_t)stream;
     const int blocks = gs::blocks_of(dim);
+    constexpr int W = gs::kCatThreads / 64;
     const bool items = g_item || g_bias;
     const int ut = (int)gs::tiles_of(n_users), it = (int)gs::tiles_of(n_items);
-    const size_t each = gs::align256((size_t)ut * 32 * sizeof(float));
     gs::Layout lu{}, li{};
     lu.x = user; lu.n_rows = n_users;
     lu.rows = reinterpret_cast<uint4 *>(ws + sp.user_rows);
     lu.cols = items ? reinterpret_cast<uint4 *>(ws + sp.user_cols) : nullptr;
-    lu.st.lse2 = reinterpret_cast<float *>(ws + sp.stats);
-    lu.st.a = reinterpret_cast<float *>(ws + sp.stats + each);
-    lu.st.b2 = reinterpret_cast<float *>(ws + sp.stats + 2 * each);
-    lu.st.g = reinterpret_cast<float *>(ws + sp.stats + 3 * each);
-    lu.st.target = reinterpret_cast<int32_t *>(ws + sp.stats + 4 * each);
+    lu.stats = reinterpret_cast<gs::Stats *>(ws + sp.stats);
     lu.from = gs::StatsFrom{n_items, targets, lse, entropy, g_log_prob, g_entropy};
     li.x = item; li.n_rows = n_items; li.bias = bias;
     li.rows = reinterpret_cast<uint4 *>(ws + sp.item_rows);
@@ -308,7 +344,7 @@ extern "C" int gs_catalog_bwd(const void *user, int64_t n_users, const void *ite
     // a side without anything to stream has no shares: the join writes its zeros
     BwdArgs a{};
     a.bias2 = li.bias2;
-    a.st = lu.st;
+    a.stats = lu.stats;
     a.dim = dim;
     a.scale = scale;
     a.scale2 = scale * gs::kLog2e;
@@ -321,13 +357,14 @@ extern "C" int gs_catalog_bwd(const void *user, int64_t n_users, const void *ite
     if (g_user) {
         a.users = Side{lu.rows, li.rows, li.cols, reinterpret_cast<float *>(ws + sp.user_part), g_user, n_users, ut, it,
                        n_items ? sp.user_shares : 0, sp.user_per};
-        a.user_blocks = (int)(((int64_t)ut * a.users.shares + gs::kCatThreads / 64 - 1) / (gs::kCatThreads / 64));
+        a.user_blocks = (ut + W - 1) / W * a.users.shares;
         j.user_part = a.users.part; j.user_shares = a.users.shares;
         if (a.users.shares != 1) j.user_n = n_users * dim;
     }
     if (items) {
         a.items = Side{li.rows, lu.rows, lu.cols, reinterpret_cast<float *>(ws + sp.item_part), g_item, n_items, it, ut,
                        n_users ? sp.item_shares : 0, sp.item_per};
+        a.item_blocks = (it + W - 1) / W * a.items.shares;
         j.item_part = a.items.part; j.bias_part = a.part_bias; j.item_shares = a.items.shares;
         if (a.items.shares != 1) { j.item_n = g_item ? n_items * dim : 0; j.bias_n = g_bias ? n_items : 0; }
     }
