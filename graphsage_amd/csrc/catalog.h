@@ -2,9 +2,10 @@
 //
 // The scores z = scale <user, item> + bias are a matrix product whose result is only ever reduced, so it stays in
 // registers.  All table types run on the bf16 matrix instruction (v_mfma_f32_32x32x16_bf16, fp32 accumulators): an element
-// is cut by truncation into pieces of eight significand bits whose sum it is exactly -- one piece for bf16, two for
-// fp16, three for fp32 -- and the piece products (exact in fp32) of weight 2^-16 and more are added, smallest first: what
-// is left out is below 2^-23 of |user| |item|, the size of one fp32 rounding.
+// is cut into pieces, each the bf16 nearest to what the ones before leave, whose sum it is exactly -- one piece for bf16,
+// two for fp16, three for fp32 -- and the products (exact in fp32) of pieces i and k with i + k <= 2 are added, smallest
+// first.  Piece i is at most 2^-8i of the element, so what is left out is below 2^-23 of |user| |item|, the size of
+// one fp32 rounding.
 //
 // Operands are laid out once per call in the order in which lanes use them (one kilobyte per fragment, 16 bytes a
 // lane), rows padded to 32, elements to a multiple of 32, with zeros:
@@ -46,35 +47,24 @@ inline size_t layout_bytes(int64_t rows, int dim, int dtype) { return (size_t)ti
 // Row in a tile of register r of a lane.
 __device__ __forceinline__ int row_of_reg(int r, int lane) { return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
 
-// The next piece of x, as a bf16 in the upper half of the word; x becomes the rest.
-__device__ __forceinline__ uint32_t next_piece(float &x) {
-    const uint32_t hi = __float_as_uint(x) & 0xFFFF0000u;
-    x -= __uint_as_float(hi);
-    return hi;
+using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+
+// The bf16 nearest to lo (lower half) and hi; both become what it leaves of them.
+__device__ __forceinline__ uint32_t next_piece(float &lo, float &hi) {
+    const bf16x2 v = {(__bf16)lo, (__bf16)hi};
+    const uint32_t w = __builtin_bit_cast(uint32_t, v);
+    lo -= __uint_as_float(w << 16);
+    hi -= __uint_as_float(w & 0xFFFF0000u);
+    return w;
 }
 
-// Eight floats cut into NZ pieces: all but the last by truncation, the last rounded to nearest (one that takes what is
-// left whole is not changed by it).
-__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) {
-    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-}
+// Eight floats cut into NZ pieces.
 template <int NZ> __device__ __forceinline__ void cut_pieces(float *v, bf16x8 *z) {
 #pragma unroll
     for (int p = 0; p < NZ; ++p) {
         uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float &lo = v[2 * i], &hi = v[2 * i + 1];
-            if (p + 1 < NZ) {
-                w[i] = upper_halves(lo, hi);
-                next_piece(lo);
-                next_piece(hi);
-            } else {
-                using pair = __attribute__((ext_vector_type(2))) __bf16;
-                const pair x = {(__bf16)lo, (__bf16)hi};
-                w[i] = __builtin_bit_cast(uint32_t, x);
-            }
-        }
+        for (int i = 0; i < 4; ++i) w[i] = next_piece(v[2 * i], v[2 * i + 1]);
         z[p] = __builtin_bit_cast(bf16x8, *reinterpret_cast<uint4 *>(w));
     }
 }

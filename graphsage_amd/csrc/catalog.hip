@@ -102,10 +102,7 @@ void layout_kernel(Layout first, Layout second, int first_tiles, int dim, int bl
             for (int p = 0; p < P; ++p) {
                 uint32_t w[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t lo = next_piece(v[2 * k]), hi = next_piece(v[2 * k + 1]);
-                    w[k] = (lo >> 16) | hi;
-                }
+                for (int k = 0; k < 4; ++k) w[k] = next_piece(v[2 * k], v[2 * k + 1]);
                 out[(size_t)p * 64] = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
@@ -119,10 +116,7 @@ void layout_kernel(Layout first, Layout second, int first_tiles, int dim, int bl
             for (int p = 0; p < P; ++p) {
                 uint32_t w[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t lo = next_piece(v[2 * k]), hi = next_piece(v[2 * k + 1]);
-                    w[k] = (lo >> 16) | hi;
-                }
+                for (int k = 0; k < 4; ++k) w[k] = next_piece(v[2 * k], v[2 * k + 1]);
                 out[(size_t)p * 64] = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }

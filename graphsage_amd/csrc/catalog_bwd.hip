@@ -3,10 +3,12 @@
 //     dz[n][j] = p_j (A_n + B_n log p_j) + [j = target_n] g_n,   A = -(g + g_entropy entropy),  B = -g_entropy
 //     g_user = scale dz item,   g_item = scale dz^T user,   g_bias = column sums of dz
 // Two launches of one kernel.  A wave owns 32 rows of one table and streams tiles of the other: the tile product gives
-// it 32 x 32 scores with its own row in the lane, dz is formed in place, cut into bf16 pieces (two for 16-bit tables,
-// three for fp32: what a piece leaves out is 2^-16 or 2^-24 of an element, well under the rounding of the result) and
-// multiplied with the same streamed rows, cols layout, into the accumulators of the 32 gradients.  Nothing of the scores or dz goes
-// through memory; the scores are computed twice.  The streamed table is cut into shares so that the launch fills
+// it 32 x 32 scores with its own row in the lane, dz is formed in place, cut into as many bf16 pieces as the tables'
+// elements have (which leaves out 2^-8 of an element for bf16 tables, 2^-16 for fp16, nothing for fp32; many elements add up
+// to a result that is itself rounded to the tables' type) and multiplied, pieces i and k with i + k below their number,
+// with the same streamed rows, cols layout, into the accumulators of the 32 gradients.  The one large element of a row, the target's
+// g, stays out of that: its term is added whole, in the join for users, in a rare branch for items.  Nothing of the scores
+// or dz goes through memory; the scores are computed twice.  The streamed table is cut into shares so that the launch fills
 // the chip; the shares' sums are added in share order by a second launch.
 #include "catalog.h"
 
@@ -17,7 +19,7 @@ using namespace gs;
 struct Side {                                       // one of the two gradients
     const uint4 *own, *stream_rows, *stream_cols;
     float *part;                                    // [shares][own tiles * 32][blocks * 32]
-    void *out;                                      // written at once where there is one share
+    void *out;                                      // items': written at once where there is one share
     int64_t own_rows;
     int own_tiles, stream_tiles, shares, tiles_per_share;
 };
@@ -38,7 +40,7 @@ template <int P, int DB> constexpr bool kStaged = fits_lds(kTile<P, DB, false>);
 
 template <class T, int DB, bool USERS>
 __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uint32_t block, uint4 *stage) {
-    constexpr int P = Pieces<T>::P, KC = 2 * DB, NZ = P == 3 ? 3 : 2, MOST = P == 3 ? 2 : 1, W = kCatThreads / 64;
+    constexpr int P = Pieces<T>::P, KC = 2 * DB, NZ = P, MOST = P - 1, W = kCatThreads / 64;
     constexpr int F = kTile<P, DB, USERS>, ST = kStaged<P, DB> ? tiles_per_stage(F) : 1;
     constexpr bool STAGED = kStaged<P, DB>;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -71,12 +73,11 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) own[kc] = load_fragment<P>(src, kc, lane);
     }
-    float lse2 = 0.f, ca = 0.f, cb = 0.f, cg = 0.f, bias = 0.f, sum = 0.f;
-    int target = -1;
+    float lse2 = 0.f, ca = 0.f, cb = 0.f, bias = 0.f, sum = 0.f;
     if (USERS) {
         const Stats &st = a.stats[tile];
         const int i = lane & 31;
-        lse2 = st.lse2[i]; ca = st.a[i]; cb = st.b2[i]; cg = st.g[i]; target = st.target[i];
+        lse2 = st.lse2[i]; ca = st.a[i]; cb = st.b2[i];
     } else bias = a.bias2[mine];
     f32x16 out[DB];
 #pragma unroll
@@ -101,20 +102,6 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
             cols = side.stream_cols + (size_t)t * KC * P * 64;
             st = a.stats + t;
         }
-        // what the scores are turned into dz with: of the streamed rows
-        float x[16], y[16], w[16];
-        int tg = -1;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int i = 8 * g + 4 * half;
-            if (USERS) *reinterpret_cast<float4 *>(x + 4 * g) = *reinterpret_cast<const float4 *>(a.bias2 + t * 32 + i);
-            else {
-                *reinterpret_cast<float4 *>(x + 4 * g) = *reinterpret_cast<const float4 *>(st->lse2 + i);
-                *reinterpret_cast<float4 *>(y + 4 * g) = *reinterpret_cast<const float4 *>(st->a + i);
-                *reinterpret_cast<float4 *>(w + 4 * g) = *reinterpret_cast<const float4 *>(st->b2 + i);
-            }
-        }
-        if (!USERS) tg = st->target[lane & 31];
         f32x16 acc;
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] = 0.f;
@@ -125,27 +112,20 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
         }
         float dz[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float lp = USERS ? __builtin_fmaf(acc[r], a.scale2, x[r]) - lse2 : __builtin_fmaf(acc[r], a.scale2, bias) - x[r];
-            dz[r] = fast_exp2(lp) * (USERS ? __builtin_fmaf(cb, lp, ca) : __builtin_fmaf(w[r], lp, y[r]));
-        }
-        // the targets: rarely in this tile
-        if (USERS) {
-            const int local = target - t * 32;
-            const bool here = target >= 0 && (unsigned)local < 32u;
-            if (__any(here)) {
-                const bool on = here && a.bias2[here ? target : 0] > kFloor;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) dz[r] += on && local == row_of_reg(r, lane) ? cg : 0.f;
+        for (int q = 0; q < 4; ++q) {
+            const int i = 8 * q + 4 * half;
+            float x[4], y[4], w[4];
+            if (USERS) *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(a.bias2 + t * 32 + i);
+            else {
+                *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(st->lse2 + i);
+                *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(st->a + i);
+                *reinterpret_cast<float4 *>(w) = *reinterpret_cast<const float4 *>(st->b2 + i);
             }
-        } else if (__any(tg >= 0 && (tg >> 5) == tile)) {
-            const float g = st->g[lane & 31];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int src = row_of_reg(r, lane);
-                const int tr = __shfl(tg, src, 64);
-                const float gr = __shfl(g, src, 64);
-                dz[r] += tr == mine && bias > kFloor ? gr : 0.f;
+            for (int k = 0; k < 4; ++k) {
+                const int r = 4 * q + k;
+                const float lp = USERS ? __builtin_fmaf(acc[r], a.scale2, x[k]) - lse2 : __builtin_fmaf(acc[r], a.scale2, bias) - x[k];
+                dz[r] = fast_exp2(lp) * (USERS ? __builtin_fmaf(cb, lp, ca) : __builtin_fmaf(w[k], lp, y[k]));
             }
         }
         if (!USERS && a.g_bias)
@@ -161,9 +141,30 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
                 multiply<NZ, P, MOST>(out[d], z, ct.p);
             }
         }
+        if (!USERS) {
+            // the terms of targets, whole: rarely in this tile
+            const int tg = st->target[lane & 31];
+            for (uint32_t todo = (uint32_t)__ballot(tg >= 0 && (tg >> 5) == tile); todo; todo &= todo - 1) {
+                const int i = __builtin_ctz(todo), row = __builtin_amdgcn_readlane(tg, i) & 31;
+                if (__int_as_float(__builtin_amdgcn_readlane(__float_as_int(bias), row)) < kFloor) continue;     // not on offer
+                const float g = st->g[i];
+                if (lane == row) sum += g;
+                // user i's element of this lane's column, from its place in the cols fragments
+                const int h = i >> 4, from = ((i >> 2) & 1) * 32 + (lane & 31), at = ((i >> 3) & 1) * 4 + (i & 3);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    float u = 0.f;
+#pragma unroll
+                    for (int p = P - 1; p >= 0; --p)
+                        u += __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(cols + ((h * DB + d) * P + p) * 64 + from)[at] << 16);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) out[d][r] += row_of_reg(r, lane) == row ? g * u : 0.f;
+                }
+            }
+        }
     }
     if (!live) return;
-    if (side.out && side.shares == 1) {
+    if (!USERS && side.out && side.shares == 1) {
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -201,6 +202,9 @@ struct JoinArgs {
     int user_shares, item_shares, dim, width;
     int64_t user_n, item_n, bias_n, user_padded, item_padded;          // *_n: elements to write, 0 for none
     float scale;
+    const void *item;
+    const Stats *stats;
+    const float *bias2;
     void *g_user, *g_item;
     float *g_bias;
 };
@@ -229,7 +233,14 @@ void catalog_bwd_join_kernel(JoinArgs a) {
     float s = 0.f;
 #pragma unroll 8
     for (int k = 0; k < shares; ++k) s += part[(size_t)k * each];
-    if (user) static_cast<T *>(a.g_user)[i] = (T)(s * a.scale);
+    if (user) {
+        // the target's term, whole
+        const int64_t n = i / a.dim;
+        const Stats &st = a.stats[n >> 5];
+        const int t = st.target[n & 31];
+        if (t >= 0 && a.bias2[t] > kFloor) s += st.g[n & 31] * (float)static_cast<const T *>(a.item)[(int64_t)t * a.dim + (i - n * a.dim)];
+        static_cast<T *>(a.g_user)[i] = (T)(s * a.scale);
+    }
     else if (item) static_cast<T *>(a.g_item)[i] = (T)(s * a.scale);
     else a.g_bias[i] = s;
 }
@@ -263,7 +274,7 @@ Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype) {
     s.item_cols = off; off += align256(layout_bytes(n_items, dim, dtype));
     s.bias2 = off; off += align256((size_t)it * 32 * sizeof(float));
     s.stats = off; off += (size_t)ut * sizeof(Stats);
-    s.user_part = off; off += s.user_shares > 1 ? align256(ut * s.user_shares * row) : 0;
+    s.user_part = off; off += align256(ut * s.user_shares * row);
     s.item_part = off; off += s.item_shares > 1 ? align256(it * s.item_shares * row) : 0;
     s.part_bias = off; off += s.item_shares > 1 ? align256((size_t)it * s.item_shares * 32 * sizeof(float)) : 0;
     s.total = off;
@@ -353,13 +364,14 @@ extern "C" int gs_catalog_bwd(const void *user, int64_t n_users, const void *ite
     JoinArgs j{};
     j.dim = dim; j.width = blocks * 32; j.scale = scale;
     j.g_user = g_user; j.g_item = g_item; j.g_bias = g_bias;
+    j.item = item; j.stats = lu.stats; j.bias2 = li.bias2;
     j.user_padded = (int64_t)ut * 32; j.item_padded = (int64_t)it * 32;
     if (g_user) {
         a.users = Side{lu.rows, li.rows, li.cols, reinterpret_cast<float *>(ws + sp.user_part), g_user, n_users, ut, it,
                        n_items ? sp.user_shares : 0, sp.user_per};
         a.user_blocks = (ut + W - 1) / W * a.users.shares;
         j.user_part = a.users.part; j.user_shares = a.users.shares;
-        if (a.users.shares != 1) j.user_n = n_users * dim;
+        j.user_n = n_users * dim;
     }
     if (items) {
         a.items = Side{li.rows, lu.rows, lu.cols, reinterpret_cast<float *>(ws + sp.item_part), g_item, n_items, it, ut,

@@ -4,8 +4,10 @@ needs a GPU.
 Tolerances bound the rounding.  u = 2^-24.  A score is a sum of at most 6 * 256 exact piece products, each addition off by at
 most 2 u of sum |user| |item|, what the pieces leave out below 4 u of it: ez = scale (6 width + 16) 2 u sum |user| |item| +
 8 u |z|, width the padded width.  A sum of exponentials adds at most 256 terms one after the other in any lane at these
-sizes: T = 256 u.  Gradients of 16-bit tables cut dz into two pieces of 8 bits (2^-15 of it with the products left out),
-of fp32 tables into three (2^-22)."""
+sizes: T = 256 u.  Gradients: an element of dz (the target's own term apart) is cut into bf16 pieces, piece i at most 2^-8i of it, and
+products of pieces i and k of dz and the table's element count for i + k < n.  bf16 tables, n = 1: off by 2^-8 of the
+product.  fp16, n = 2: 2^-16 of dz left, 2^-16 for the product left out, together below 2^-14.  fp32, n = 3: nothing
+left, products 1-2, 2-1 and 2-2 left out, 2^-24 + 2^-24 + 2^-32, below 2^-22."""
 import math
 
 import pytest
@@ -76,8 +78,8 @@ def _reference(user, item, t, b, scale, g_lp, g_e):
     lp0 = lp.nan_to_num(neginf=0)
     dz = g[:, None] * (hit.double() - p) - ge[:, None] * (plp + p * entropy[:, None])
     factor = (g + ge * entropy)[:, None].abs() + (ge[:, None] * lp0).abs()
-    cut = 2.0 ** -22 if user.dtype == torch.float32 else 2.0 ** -15
-    off = p * (r[:, None] * factor + ge.abs()[:, None] * (r + tol['entropy'])[:, None] + 8 * U * factor) + cut * dz.abs()
+    cut = {torch.float32: 2.0 ** -22, torch.float16: 2.0 ** -14, torch.bfloat16: 2.0 ** -8}[user.dtype]
+    off = p * (r[:, None] * factor + ge.abs()[:, None] * (r + tol['entropy'])[:, None] + 8 * U * factor) + cut * (p * factor)
     # the sums run over at most 3000 rows here, products of pieces in fp32
     add = (6 * 3000) * U
     half = torch.finfo(user.dtype).eps / 2
