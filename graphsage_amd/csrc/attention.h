@@ -318,7 +318,7 @@ struct Deal {
     bool pieces, is_short;
 };
 
-inline Deal deal_edges(const int64_t *indptr, int64_t n_child, int64_t n_edges, int lanes) {
+inline Deal deal_edges(const int64_t *indptr, int64_t n_lists, int64_t n_child, int64_t n_edges, int lanes) {
     Deal d;
     d.is_short = !indptr && n_child > 0 && n_child <= kShortList;
     if (d.is_short) {
@@ -330,11 +330,15 @@ inline Deal deal_edges(const int64_t *indptr, int64_t n_child, int64_t n_edges, 
         if (d.waves > 16384) d.waves = d.waves / 8 > 16384 ? (d.waves + 7) / 8 : 16384;
         return d;
     }
-    // two rounds of row loads at least, then as many edges as leave 16384 waves (two rounds of eight per
-    // SIMD: a little more than one round leaves a few waves for the second), at most 512
-    const int64_t round = 2 * kAttnRows * (64 / lanes);
-    int64_t c = (n_edges / 16384 + round - 1) / round * round;
-    c = c < round ? round : c > 512 ? 512 : c;
+    // two rounds of row loads, but no more than two lists of the mean length: a wave takes them one after the other
+    // (1450 edges of 13000 lists, 32 a wave: 112 us); as many edges as leave 16384 waves (two rounds of eight per SIMD: a
+    // little more than one round leaves a few waves for the second), at most 512; and a list of the mean length
+    // leaves at most 256 pieces (three lists of 39000: 4900 pieces each took 270 us to join)
+    const int64_t mean = n_lists ? n_edges / n_lists : 0;
+    int64_t c = 2 * kAttnRows * (64 / lanes);
+    if (c > 2 * mean) c = 2 * mean > 2 ? 2 * mean : 2;
+    if (c < n_edges / 16384) c = n_edges / 16384 < 512 ? n_edges / 16384 : 512;
+    if (c < mean / 256) c = mean / 256;
     // lists of one length that are no longer than that: whole lists
     if (!indptr && n_child > 0 && n_child <= c) c = c / n_child * n_child;
     d.chunk = c;
@@ -345,7 +349,7 @@ inline Deal deal_edges(const int64_t *indptr, int64_t n_child, int64_t n_edges, 
 
 // A table without rows leaves every parent without neighbors.
 inline Deal deal_edges(const gs_neighbors *nb, int lanes) {
-    return nb->n_rows ? deal_edges(nb->indptr, nb->n_child, nb->n_edges, lanes) : deal_edges(nullptr, 0, 0, lanes);
+    return nb->n_rows ? deal_edges(nb->indptr, nb->n_parents, nb->n_child, nb->n_edges, lanes) : deal_edges(nullptr, 0, 0, 0, lanes);
 }
 inline Neighbors device_neighbors(const gs_neighbors *nb) {
     if (!nb->n_rows) return Neighbors{nullptr, nb->ids, nb->n_parents, 0, 0, 0, 0};
@@ -355,6 +359,28 @@ inline Neighbors device_neighbors(const gs_neighbors *nb) {
 
 // Whether the second launch has something to do for a list: it is empty, or was cut.
 __device__ __forceinline__ bool needs_join(uint32_t b, uint32_t e, uint32_t chunk) { return b == e || e - b > 4 * chunk; }
+
+// How the lanes of a joining wave share the pieces of a list: 64 / width pieces at a time, width lanes each, for the
+// elements that blockIdx.z stands for (64 of them, or the row where it is shorter).
+struct JoinLanes {
+    int width, sub, subs, d;
+    bool in;
+    __device__ __forceinline__ JoinLanes(int lane, int dim, int column) {
+        width = 64;
+        while (width / 2 >= dim) width /= 2;
+        sub = lane / width;
+        subs = 64 / width;
+        d = column * 64 + lane % width;
+        in = d < dim;
+        if (!in) d = dim - 1;
+    }
+};
+constexpr int kJoinFlight = 8;                      // pieces of a lane on their way
+// Blocks that share the lists out: 64 lists each where there are many, one where there are few.
+inline unsigned join_blocks(int64_t lists) {
+    const int64_t full = (lists + 63) / 64, few = lists < 512 ? lists : 512;
+    return (unsigned)(full > few ? full : few);
+}
 
 __device__ __forceinline__ uint32_t this_wave() {
     return __builtin_amdgcn_readfirstlane(blockIdx.x * (kAttnThreads / 64) + (threadIdx.x >> 6));

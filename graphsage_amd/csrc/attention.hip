@@ -242,98 +242,93 @@ void attn_fwd_short_kernel(FwdArgs a) {
     }
 }
 
-// Joins the pieces of the lists that were cut and writes the parents without edges.  A block looks at 64 parents, far
-// apart (popular parents tend to be neighbors).  A wave joins a list of a few pieces by itself; of a long one every
-// wave takes every sixteenth piece.
+// Joins the pieces of the lists that were cut and writes the parents without edges.  A block looks at up to 64 parents,
+// far apart (popular parents tend to be neighbors), for one head and 64 elements.  A wave joins a list of a few pieces by
+// itself; of a long one every wave takes its share.
 constexpr uint32_t kFewPieces = 16;
 
 struct Joined {
-    float m, s, acc[4];
+    float m, s, acc;
+    __device__ __forceinline__ void add(float mo, float so, float ao) {
+        const float top = fmaxf(m, mo), ref = top == -INFINITY ? 0.f : top;
+        const float ka = gs::fast_exp2(m - ref), kb = gs::fast_exp2(mo - ref);
+        m = top;
+        s = s * ka + so * kb;
+        acc = acc * ka + ao * kb;
+    }
 };
 
-// Pieces i0, i0 + step, ... of list [b, e), four loads in flight.
-__device__ __forceinline__ void join_pieces(const FwdArgs &a, uint32_t b, uint32_t e, uint32_t i0, uint32_t step, int h, int lane, Joined &j) {
+// Pieces first, first + step, ... of list [b, e); then joined across the pieces a wave holds at a time.
+__device__ __forceinline__ Joined join_pieces(const FwdArgs &a, uint32_t b, uint32_t e, uint32_t first, uint32_t step, int h, const gs::JoinLanes &l) {
     const uint32_t n = (e - 1) / a.chunk - b / a.chunk + 1;
-    for (uint32_t i = i0; i < n; i += 4 * step) {
-        float2 ms[4];
-        float x[4][4];
+    Joined j{-INFINITY, 0.f, 0.f};
+    for (uint32_t i = first; i < n; i += gs::kJoinFlight * step) {
+        float2 ms[gs::kJoinFlight];
+        float x[gs::kJoinFlight];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const bool in = i + k * step < n;
-            const size_t at = gs::piece_place(b, a.chunk, in ? i + k * step : i) * a.heads + h;
+        for (int k = 0; k < gs::kJoinFlight; ++k) {
+            const size_t at = gs::piece_place(b, a.chunk, min(i + k * step, n - 1)) * a.heads + h;
             ms[k] = a.piece_ms[at];
-            if (!in) ms[k] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) x[k][c] = in && lane + 64 * c < a.dim ? a.piece_acc[at * a.dim + lane + 64 * c] : 0.f;
+            x[k] = a.piece_acc[at * a.dim + l.d];
         }
         float top = j.m;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top = fmaxf(top, ms[k].x);
+        for (int k = 0; k < gs::kJoinFlight; ++k) {
+            if (i + k * step >= n) { ms[k] = make_float2(-INFINITY, 0.f); x[k] = 0.f; }
+            top = fmaxf(top, ms[k].x);
+        }
         const float ref = top == -INFINITY ? 0.f : top, ko = gs::fast_exp2(j.m - ref);
         j.m = top;
         j.s *= ko;
+        j.acc *= ko;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) j.acc[c] *= ko;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < gs::kJoinFlight; ++k) {
             const float kn = gs::fast_exp2(ms[k].x - ref);
             j.s += ms[k].y * kn;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) j.acc[c] += x[k][c] * kn;
+            j.acc += x[k] * kn;
         }
     }
+    for (int o = l.width; o < 64; o *= 2) j.add(__shfl_xor(j.m, o, 64), __shfl_xor(j.s, o, 64), __shfl_xor(j.acc, o, 64));
+    return j;
 }
 
 template <class T>
 __global__ __launch_bounds__(gs::kJoinWaves * 64)
 void attn_join_kernel(FwdArgs a) {
     constexpr int N = gs::kJoinWaves;
-    __shared__ float part[N][256 + 2];
+    __shared__ Joined part[N][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.y;
+    const gs::JoinLanes l(lane, a.dim, blockIdx.z);
     const int64_t mine = (int64_t)lane * gridDim.x + blockIdx.x;
     uint32_t b = 0, e = 0;
     if (mine < a.nb.n_parents) a.nb.range(mine, b, e);
     const bool mine_todo = mine < a.nb.n_parents && gs::needs_join(b, e, a.chunk);
     const bool many = mine_todo && e > b && (e - 1) / a.chunk - b / a.chunk >= kFewPieces;
     unsigned long long few = __ballot(mine_todo && !many), long_ones = __ballot(many);
+    const auto write = [&](int src, const Joined &j) {
+        const int64_t at = ((int64_t)src * gridDim.x + blockIdx.x) * a.heads + h;
+        if (l.sub == 0 && l.in) static_cast<T *>(a.out)[at * a.dim + l.d] = (T)(j.acc * inverse_of(j.s));
+        if (lane == 0 && blockIdx.z == 0) a.lse[at] = (j.m + gs::fast_log2(j.s)) * gs::kLn2;
+    };
     for (int turn = 0; few; ++turn, few &= few - 1) {
         if (turn % N != wave) continue;
         const int src = __builtin_ctzll(few);
         const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
-        Joined j{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
-        if (se > sb) join_pieces(a, sb, se, 0, 1, h, lane, j);
-        const int64_t at = ((int64_t)src * gridDim.x + blockIdx.x) * a.heads + h;
-        const float inv = inverse_of(j.s);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (lane + 64 * c < a.dim) static_cast<T *>(a.out)[at * a.dim + lane + 64 * c] = (T)(j.acc[c] * inv);
-        if (lane == 0) a.lse[at] = (j.m + gs::fast_log2(j.s)) * gs::kLn2;
+        Joined j{-INFINITY, 0.f, 0.f};
+        if (se > sb) j = join_pieces(a, sb, se, l.sub, l.subs, h, l);
+        write(src, j);
     }
     for (; long_ones; long_ones &= long_ones - 1) {
         const int src = __builtin_ctzll(long_ones);
         const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
-        Joined j{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
-        join_pieces(a, sb, se, wave, N, h, lane, j);
+        const Joined own = join_pieces(a, sb, se, wave * l.subs + l.sub, N * l.subs, h, l);
         __syncthreads();                            // the last list's parts are read
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = j.acc[i];
-        if (lane == 0) { part[wave][256] = j.m; part[wave][257] = j.s; }
+        part[wave][lane] = own;
         __syncthreads();
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < N; ++i) top = fmaxf(top, part[i][256]);
-        const float ref = top == -INFINITY ? 0.f : top;
-        const int d = threadIdx.x & 255;
-        float sum = 0.f, o = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float f = gs::fast_exp2(part[i][256] - ref);
-            sum += part[i][257] * f;
-            o += part[i][d] * f;
-        }
-        const int64_t at = ((int64_t)src * gridDim.x + blockIdx.x) * a.heads + h;
-        if (threadIdx.x < a.dim) static_cast<T *>(a.out)[at * a.dim + d] = (T)(o * inverse_of(sum));
-        if (threadIdx.x == 0) a.lse[at] = (top + gs::fast_log2(sum)) * gs::kLn2;
+        if (wave) continue;
+        Joined j = part[0][lane];
+        for (int i = 1; i < N; ++i) j.add(part[i][lane].m, part[i][lane].s, part[i][lane].acc);
+        write(src, j);
     }
 }
 
@@ -360,7 +355,7 @@ int run_fwd(const FwdArgs &a, const gs::Deal &d, int lanes, hipStream_t stream) 
         if (int rc = gs::check_launch("gs_neighbor_attention_fwd")) return rc;
     }
     if (d.pieces) {
-        const dim3 grid((unsigned)((a.nb.n_parents + 63) / 64), (unsigned)a.heads);
+        const dim3 grid(gs::join_blocks(a.nb.n_parents), (unsigned)a.heads, (unsigned)((a.dim + 63) / 64));
         attn_join_kernel<T><<<grid, gs::kJoinWaves * 64, 0, stream>>>(a);
         return gs::check_launch("gs_neighbor_attention_fwd (join)");
     }

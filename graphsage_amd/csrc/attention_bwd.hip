@@ -334,74 +334,61 @@ void attn_bwd_rows_kernel(BwdArgs a) {
     }
 }
 
-// Adds the pieces of the lists that were cut, in worker order, and writes zeros for empty ones.  `sets` vectors of dim
-// floats per (list, y): the parents' walk has one (y a head), the rows' two (y a key head).  Few pieces: one wave alone.
+// Adds the pieces of the lists that were cut, and writes zeros for empty ones.  `sets` vectors of dim floats per (list, y):
+// the parents' walk has one (y a head), the rows' two (y a key head).  Few pieces: one wave alone.
 constexpr uint32_t kFewPieces = 16;
 
 template <class T>
 __global__ __launch_bounds__(gs::kJoinWaves * 64)
 void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int sets, int dim, uint32_t chunk, T *out0, T *out1) {
     constexpr int N = gs::kJoinWaves;
-    __shared__ float part[N][256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, y = blockIdx.y;
+    __shared__ float part[N][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, y = blockIdx.y / sets, set = blockIdx.y % sets;
+    T *out = set ? out1 : out0;
+    if (!out) return;
+    const gs::JoinLanes l(lane, dim, blockIdx.z);
     const int64_t mine = (int64_t)lane * gridDim.x + blockIdx.x;
     uint32_t b = 0, e = 0;
     if (mine < seg.n_parents) seg.range(mine, b, e);
     const bool mine_todo = mine < seg.n_parents && gs::needs_join(b, e, chunk);
     const bool many = mine_todo && e > b && (e - 1) / chunk - b / chunk >= kFewPieces;
     unsigned long long few = __ballot(mine_todo && !many), long_ones = __ballot(many);
-    const auto add = [&](uint32_t sb, uint32_t se, uint32_t i0, uint32_t step, int set, float (&acc)[4]) {
+    const auto add = [&](uint32_t sb, uint32_t se, uint32_t first, uint32_t step) {
         const uint32_t n = (se - 1) / chunk - sb / chunk + 1;
-        for (uint32_t i = i0; i < n; i += 4 * step) {
-            float x[4][4];
+        float acc = 0.f;
+        for (uint32_t i = first; i < n; i += gs::kJoinFlight * step) {
+            float x[gs::kJoinFlight];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool in = i + k * step < n;
-                const size_t at = ((gs::piece_place(sb, chunk, in ? i + k * step : i) * per_slot + y) * sets + set) * dim;
+            for (int k = 0; k < gs::kJoinFlight; ++k)
+                x[k] = piece[((gs::piece_place(sb, chunk, min(i + k * step, n - 1)) * per_slot + y) * sets + set) * dim + l.d];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) x[k][c] = in && lane + 64 * c < dim ? piece[at + lane + 64 * c] : 0.f;
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[c] += x[k][c];
+            for (int k = 0; k < gs::kJoinFlight; ++k) acc += i + k * step < n ? x[k] : 0.f;
         }
+        for (int o = l.width; o < 64; o *= 2) acc += __shfl_xor(acc, o, 64);
+        return acc;
+    };
+    const auto write = [&](int src, float v) {
+        const int64_t p = (int64_t)src * gridDim.x + blockIdx.x;
+        if (l.sub == 0 && l.in) out[(p * per_slot + y) * dim + l.d] = (T)v;
     };
     for (int turn = 0; few; ++turn, few &= few - 1) {
         if (turn % N != wave) continue;
         const int src = __builtin_ctzll(few);
         const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
-        const int64_t p = (int64_t)src * gridDim.x + blockIdx.x;
-        for (int set = 0; set < sets; ++set) {
-            T *out = set ? out1 : out0;
-            if (!out) continue;
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            if (se > sb) add(sb, se, 0, 1, set, acc);
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (lane + 64 * c < dim) out[(p * per_slot + y) * dim + lane + 64 * c] = (T)acc[c];
-        }
+        write(src, se > sb ? add(sb, se, l.sub, l.subs) : 0.f);
     }
     for (; long_ones; long_ones &= long_ones - 1) {
         const int src = __builtin_ctzll(long_ones);
         const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
-        const int64_t p = (int64_t)src * gridDim.x + blockIdx.x;
-        for (int set = 0; set < sets; ++set) {
-            T *out = set ? out1 : out0;
-            if (!out) continue;
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            add(sb, se, wave, N, set, acc);
-            __syncthreads();
+        const float own = add(sb, se, wave * l.subs + l.sub, N * l.subs);
+        __syncthreads();                            // the last list's parts are read
+        part[wave][lane] = own;
+        __syncthreads();
+        if (wave) continue;
+        float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[wave][lane + 64 * i] = acc[i];
-            __syncthreads();
-            if (threadIdx.x < dim) {
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < N; ++i) sum += part[i][threadIdx.x];
-                out[(p * per_slot + y) * dim + threadIdx.x] = (T)sum;
-            }
-        }
+        for (int i = 0; i < N; ++i) sum += part[i][lane];
+        write(src, sum);
     }
 }
 
@@ -461,7 +448,7 @@ Plan make_plan(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dty
     p.parts = (share + heads_per_wave(share) - 1) / heads_per_wave(share);
     p.parents = gs::deal_edges(nb, lanes);
     static const int64_t ragged = 0;                // any address: the rows' lists are ragged
-    p.rows = gs::deal_edges(&ragged, 0, nb->ids && nb->n_rows && nb->n_parents ? n_inv : 0, lanes);
+    p.rows = gs::deal_edges(&ragged, nb->n_rows, 0, nb->ids && nb->n_rows && nb->n_parents ? n_inv : 0, lanes);
     size_t off = gs::align256((size_t)nb->n_parents * heads * sizeof(float));        // delta
     p.off_parent = off;
     if (nb->indptr && nb->ids) off += gs::align256((size_t)nb->n_edges * sizeof(int32_t));
@@ -483,7 +470,7 @@ int run_bwd(BwdArgs a, const Plan &p, int lanes, hipStream_t stream) {
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents)")) return rc;
     }
     if (a.g_q && a.nb.n_parents && p.parents.pieces) {
-        attn_bwd_join_kernel<T><<<dim3((unsigned)((a.nb.n_parents + 63) / 64), (unsigned)a.heads), gs::kJoinWaves * 64, 0, stream>>>(
+        attn_bwd_join_kernel<T><<<dim3(gs::join_blocks(a.nb.n_parents), (unsigned)a.heads, (unsigned)((a.dim + 63) / 64)), gs::kJoinWaves * 64, 0, stream>>>(
             a.nb, a.piece, a.heads, 1, a.dim, a.chunk, static_cast<T *>(a.g_q), (T *)nullptr);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents' join)")) return rc;
     }
@@ -504,7 +491,7 @@ int run_bwd(BwdArgs a, const Plan &p, int lanes, hipStream_t stream) {
     rows.n_child = 0;
     rows.n_parents = a.nb.n_rows;
     rows.n_edges = a.n_inv;
-    attn_bwd_join_kernel<T><<<dim3((unsigned)((a.nb.n_rows + 63) / 64), (unsigned)a.kv_heads), gs::kJoinWaves * 64, 0, stream>>>(
+    attn_bwd_join_kernel<T><<<dim3(gs::join_blocks(a.nb.n_rows), (unsigned)a.kv_heads * 2, (unsigned)((a.dim + 63) / 64)), gs::kJoinWaves * 64, 0, stream>>>(
         rows, a.piece, a.kv_heads, 2, a.dim, a.chunk, static_cast<T *>(a.g_k), static_cast<T *>(a.g_v));
     return gs::check_launch("gs_neighbor_attention_bwd (rows' join)");
 }

@@ -6,10 +6,10 @@
 // multiply-add).  The shares' (m, s, w) are joined by a second launch: lse = m + log s, entropy = log s - w / s.
 // The score of the target is picked up as its tile passes, so that log_prob is exactly 0 for a catalog of one item.
 //
-// Best items: the first launch also writes the largest score of every tile.  The k best items lie in tiles whose largest
-// score is among the k largest (each of k better tiles would hold a better item), so only about k tiles of a user are
-// scored again, in 64 bits, from the tables themselves; tiles within the rounding error of the first product count as
-// candidates too.  The list is then a function of the tables alone, whatever the product's order of additions.
+// Best items: the first launch also writes the largest score of every group of 4 or 32 items.  The k best items lie in groups
+// whose largest score is among the k largest (each of k better groups would hold a better item), so only about k groups of a
+// user are scored again, in 64 bits, from the tables themselves; groups within the rounding error of the first product
+// count as candidates too.  The list is then a function of the tables alone, whatever the product's order of additions.
 #include "catalog.h"
 
 namespace gs {
@@ -168,14 +168,14 @@ struct FwdArgs {
     const float *bias2;
     const int32_t *targets;
     float4 *part;                                   // [users][shares]: m, s, w, target's score
-    float *tile_max;                                // [users][tile_stride], with TOP
-    int64_t tile_stride;
+    float *group_max;                               // [users][group_stride], with TOP: of every TOP consecutive items
+    int64_t group_stride;
     int64_t n_users, n_items;
     int user_tiles, item_tiles, group_blocks, shares, tiles_per_share;
     float scale2;
 };
 
-template <int P, int DB, int OF, bool TOP>
+template <int P, int DB, int OF, int TOP>
 __global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * P * OF + 16 * OF + 24))
 void catalog_fwd_kernel(FwdArgs a) {
     constexpr int KC = 2 * DB, F = KC * P, ST = tiles_per_stage(F), W = kCatThreads / 64;
@@ -247,12 +247,19 @@ void catalog_fwd_kernel(FwdArgs a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (target[f] >= 0 && local == row_of_reg(r, lane)) hit[f] = z[r];
-            if (TOP) {
+            const int64_t n = ((int64_t)group * OF + f) * 32 + (lane & 31);
+            if (TOP == 32) {
                 // four tiles' largest scores leave together
                 tops[f][t & 3] = half_max(top);
-                const int64_t n = ((int64_t)group * OF + f) * 32 + lane;
                 if (((t & 3) == 3 || t + 1 == t1) && lane < 32 && n < a.n_users)
-                    *reinterpret_cast<float4 *>(a.tile_max + n * a.tile_stride + (t & ~3)) = make_float4(tops[f][0], tops[f][1], tops[f][2], tops[f][3]);
+                    *reinterpret_cast<float4 *>(a.group_max + n * a.group_stride + (t & ~3)) = make_float4(tops[f][0], tops[f][1], tops[f][2], tops[f][3]);
+            } else if (TOP == 4) {
+                // registers 4 q .. 4 q + 3 are items 8 q + 4 (lane / 32) and on of the tile
+                if (n < a.n_users)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        a.group_max[n * a.group_stride + t * 8 + 2 * q + (lane >> 5)] =
+                            fmaxf(fmaxf(z[4 * q], z[4 * q + 1]), fmaxf(z[4 * q + 2], z[4 * q + 3]));
             }
             if (__any(top > m[f])) {
                 const float m1 = fmaxf(m[f], top), step = m[f] - m1, keep = fast_exp2(step);
@@ -260,12 +267,16 @@ void catalog_fwd_kernel(FwdArgs a) {
                 s[f] *= keep;
                 m[f] = m1;
             }
+            // a tile's terms first, in four chains: hundreds one by one would cost digits
+            float sp[4] = {0.f, 0.f, 0.f, 0.f}, wp[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float d = z[r] - m[f], p = fast_exp2(d);
-                s[f] += p;
-                w[f] = __builtin_fmaf(p, d, w[f]);
+                sp[r & 3] += p;
+                wp[r & 3] = __builtin_fmaf(p, d, wp[r & 3]);
             }
+            s[f] += (sp[0] + sp[1]) + (sp[2] + sp[3]);
+            w[f] += (wp[0] + wp[1]) + (wp[2] + wp[3]);
         }
     }
 #pragma unroll
@@ -321,9 +332,9 @@ void catalog_join_kernel(const float4 *part, int shares, int64_t n_users, int64_
 
 struct TopArgs {
     const void *user, *item;
-    const float *bias, *tile_max, *tile_abs, *lse;
-    int64_t n_users, n_items, tile_stride;
-    int dim, item_tiles, k, vector;
+    const float *bias, *group_max, *tile_abs, *lse;
+    int64_t n_users, n_items, group_stride;
+    int dim, item_tiles, groups, log2_items, k, vector;         // log2_items: of a group
     float scale;
     float *top_log_prob;
     int32_t *top_ids;
@@ -346,20 +357,20 @@ void catalog_top_kernel(TopArgs a) {
     __shared__ float low;
     const int tid = threadIdx.x, quad = tid >> 2, part = tid & 3;
     const int64_t n = blockIdx.x;
-    const float *tm = a.tile_max + n * a.tile_stride;
+    const float *gm = a.group_max + n * a.group_stride;
+    const int items = 1 << a.log2_items, at_once = 64 >> a.log2_items;          // a pass scores 64 items
     const T *U = static_cast<const T *>(a.user) + n * a.dim, *I = static_cast<const T *>(a.item);
     for (int d = tid; d < a.dim; d += 256) user[d] = (double)(float)U[d];
     float top = -INFINITY, most_abs = 0.f;
 #pragma unroll 4
-    for (int t = tid; t < a.item_tiles; t += 256) {
-        top = fmaxf(top, tm[t]);
-        most_abs = fmaxf(most_abs, a.tile_abs[t]);
-    }
+    for (int t = tid; t < a.groups; t += 256) top = fmaxf(top, gm[t]);
+#pragma unroll 4
+    for (int t = tid; t < a.item_tiles; t += 256) most_abs = fmaxf(most_abs, a.tile_abs[t]);
     group_max[tid] = top;
     group_abs[tid] = most_abs;
     if (tid == 0) { n_val = 0; n_cand = 0; low = -INFINITY; }
     __syncthreads();
-    // the k-th largest of 256 groups' maxima: at least k tiles reach it
+    // the k-th largest of the maxima of 256 sets of groups: at least k groups reach it
     int rank = 0;
 #pragma unroll 8
     for (int i = 0; i < 256; i += 4) {
@@ -407,17 +418,17 @@ void catalog_top_kernel(TopArgs a) {
     };
     const float thr_tile = (float)(thr * (1.0 / (double)kLn2));
     const float thr_down = thr == -INFINITY ? -INFINITY : thr_tile - fabsf(thr_tile) * 0x1p-20f;
-    for (int t0 = 0; t0 < a.item_tiles; t0 += kChunk) {
-        const int t1 = min(t0 + kChunk, a.item_tiles);
+    for (int t0 = 0; t0 < a.groups; t0 += kChunk) {
+        const int t1 = min(t0 + kChunk, a.groups);
 #pragma unroll 4
         for (int t = t0 + tid; t < t1; t += 256)
-            if (!(tm[t] < thr_down)) cand[atomicAdd(&n_cand, 1)] = (uint16_t)(t - t0);
+            if (!(gm[t] < thr_down)) cand[atomicAdd(&n_cand, 1)] = (uint16_t)(t - t0);
         __syncthreads();
         const int count = n_cand;
-        // two tiles a pass; the buffer takes sixteen between two looks at it
-        for (int c0 = 0; c0 < count; c0 += 16) {
-            for (int c = c0 + (quad >> 5); c < min(c0 + 16, count); c += 2) {
-                const int64_t j = ((int64_t)t0 + cand[c]) * 32 + (quad & 31);
+        // the buffer takes eight passes between two looks at it
+        for (int c0 = 0; c0 < count; c0 += 8 * at_once) {
+            for (int c = c0 + (quad >> a.log2_items); c < min(c0 + 8 * at_once, count); c += at_once) {
+                const int64_t j = (((int64_t)t0 + cand[c]) << a.log2_items) + (quad & (items - 1));
                 const float b = j < a.n_items && a.bias ? a.bias[j] : 0.f;
                 const bool in = j < a.n_items && !(b < kOffer);
                 const T *row = I + (in ? j : 0) * a.dim;
@@ -458,10 +469,13 @@ void catalog_top_kernel(TopArgs a) {
     }
 }
 
+// Groups of a user, to a multiple of four.
+int64_t group_stride_of(int64_t n_items, int top) { return (tiles_of(n_items) * (32 / top) + 3) / 4 * 4; }
+
 // How a call is cut: users in slices that bound the table of tile maxima, a slice in waves.
 struct Cut {
     int64_t slice;                                  // users per slice
-    int of;
+    int of, top;                                    // top: items per group whose largest score is kept, 0 for none
 };
 
 Cut cut_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
@@ -469,8 +483,14 @@ Cut cut_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
     const int regs = pieces_of(dtype) * blocks_of(dim);                   // registers of a fragment row: 8 each
     c.of = n_users > 32 && regs <= 8 ? 2 : 1;
     c.slice = n_users;
+    c.top = 0;
     if (top_k > 0) {
-        const int64_t most = ((int64_t)1 << 26) / (tiles_of(n_items) ? tiles_of(n_items) : 1) / 256 * 256;
+        // What a user costs beside the product: the groups' maxima, written and read, and about k groups of rows read again
+        // (out of L2: half the price).  Groups of 4 for few items, wide rows or long lists (3196 users, 4036 items of 200, 64
+        // best: 543 us with groups of 32, 166 us so), of 32 else (512 users, 100 000 items of 64, 20 best: 104 us, 125 us with groups of 4).
+        const auto cost = [&](double group) { return 8.0 * n_items / group + 0.5 * top_k * group * dim * dtype_size(dtype); };
+        c.top = cost(4) < cost(32) ? 4 : 32;
+        const int64_t most = ((int64_t)1 << 26) / (group_stride_of(n_items, c.top) + 1) / 256 * 256;
         if (c.slice > most) c.slice = most < 256 ? 256 : most;
     }
     return c;
@@ -489,10 +509,8 @@ void shares_of(int64_t users, int64_t n_items, int of, int *group_blocks, int *s
     *shares = (int)((it + *per_share - 1) / *per_share);
 }
 
-int64_t tile_stride_of(int64_t n_items) { return (tiles_of(n_items) + 3) / 4 * 4; }
-
 struct Space {
-    size_t user, item, bias2, part, lse, tile_abs, tile_max, total;
+    size_t user, item, bias2, part, lse, tile_abs, group_max, total;
 };
 
 Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
@@ -510,13 +528,13 @@ Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) 
     s.lse = off; off += align256((size_t)c.slice * sizeof(float));
     s.tile_abs = off;
     if (top_k > 0) off += align256((size_t)tiles_of(n_items) * sizeof(float));
-    s.tile_max = off;
-    if (top_k > 0) off += (size_t)c.slice * tile_stride_of(n_items) * sizeof(float);
+    s.group_max = off;
+    if (top_k > 0) off += (size_t)c.slice * group_stride_of(n_items, c.top) * sizeof(float);
     s.total = off;
     return s;
 }
 
-template <int P, int DB, int OF, bool TOP>
+template <int P, int DB, int OF, int TOP>
 int launch_one(const FwdArgs &a, hipStream_t stream) {
     constexpr int F = 2 * DB * P, lds = 2 * F * gs::tiles_per_stage(F) * 1024;
     static_assert(gs::fits_lds(F), "a tile does not fit");
@@ -530,24 +548,24 @@ int launch_one(const FwdArgs &a, hipStream_t stream) {
 }
 
 template <int P, int DB, int OF>
-int launch_tile(const FwdArgs &a, hipStream_t stream) {
-    return a.tile_max ? launch_one<P, DB, OF, true>(a, stream) : launch_one<P, DB, OF, false>(a, stream);
+int launch_tile(const FwdArgs &a, int top, hipStream_t stream) {
+    return top == 32 ? launch_one<P, DB, OF, 32>(a, stream) : top == 4 ? launch_one<P, DB, OF, 4>(a, stream) : launch_one<P, DB, OF, 0>(a, stream);
 }
 
 template <int P>
-int launch_fwd(const FwdArgs &a, int blocks, int of, hipStream_t stream) {
+int launch_fwd(const FwdArgs &a, int blocks, int of, int top, hipStream_t stream) {
     if (of == 2) {
-        if (blocks == 1) return launch_tile<P, 1, 2>(a, stream);
-        if (blocks == 2) return launch_tile<P, 2, 2>(a, stream);
+        if (blocks == 1) return launch_tile<P, 1, 2>(a, top, stream);
+        if (blocks == 2) return launch_tile<P, 2, 2>(a, top, stream);
         if constexpr (P * 4 <= 8) {
-            if (blocks == 4) return launch_tile<P, 4, 2>(a, stream);
+            if (blocks == 4) return launch_tile<P, 4, 2>(a, top, stream);
         }
-        if constexpr (P == 1) return launch_tile<P, 8, 2>(a, stream);
+        if constexpr (P == 1) return launch_tile<P, 8, 2>(a, top, stream);
     }
-    if (blocks == 1) return launch_tile<P, 1, 1>(a, stream);
-    if (blocks == 2) return launch_tile<P, 2, 1>(a, stream);
-    if (blocks == 4) return launch_tile<P, 4, 1>(a, stream);
-    return launch_tile<P, 8, 1>(a, stream);
+    if (blocks == 1) return launch_tile<P, 1, 1>(a, top, stream);
+    if (blocks == 2) return launch_tile<P, 2, 1>(a, top, stream);
+    if (blocks == 4) return launch_tile<P, 4, 1>(a, top, stream);
+    return launch_tile<P, 8, 1>(a, top, stream);
 }
 
 }  // namespace
@@ -600,16 +618,16 @@ extern "C" int gs_catalog_fwd(const void *user, int64_t n_users, const void *ite
         a.bias2 = reinterpret_cast<const float *>(ws + sp.bias2);
         a.targets = targets ? targets + u0 : nullptr;
         a.part = reinterpret_cast<float4 *>(ws + sp.part);
-        a.tile_max = top_k ? reinterpret_cast<float *>(ws + sp.tile_max) : nullptr;
-        a.tile_stride = tile_stride_of(n_items);
+        a.group_max = top_k ? reinterpret_cast<float *>(ws + sp.group_max) : nullptr;
+        a.group_stride = top_k ? group_stride_of(n_items, cut.top) : 0;
         a.n_users = nu; a.n_items = n_items;
         a.user_tiles = (int)gs::tiles_of(nu); a.item_tiles = (int)gs::tiles_of(n_items);
         shares_of(nu, n_items, cut.of, &a.group_blocks, &a.shares, &a.tiles_per_share);
         a.scale2 = scale * gs::kLog2e;
         if (n_items == 0) a.shares = 0;
         else {
-            if (int rc = pieces == 1 ? launch_fwd<1>(a, blocks, cut.of, s) : pieces == 2 ? launch_fwd<2>(a, blocks, cut.of, s)
-                                                                                        : launch_fwd<3>(a, blocks, cut.of, s))
+            if (int rc = pieces == 1 ? launch_fwd<1>(a, blocks, cut.of, cut.top, s) : pieces == 2 ? launch_fwd<2>(a, blocks, cut.of, cut.top, s)
+                                                                                        : launch_fwd<3>(a, blocks, cut.of, cut.top, s))
                 return rc;
         }
         float *lse_out = lse ? lse + u0 : reinterpret_cast<float *>(ws + sp.lse);
@@ -619,8 +637,9 @@ extern "C" int gs_catalog_fwd(const void *user, int64_t n_users, const void *ite
         if (!top_k) continue;
         TopArgs t;
         t.user = static_cast<const char *>(user) + (size_t)u0 * dim * size;
-        t.item = item; t.bias = bias; t.tile_max = a.tile_max; t.tile_abs = tile_abs; t.lse = lse_out;
-        t.n_users = nu; t.n_items = n_items; t.tile_stride = a.tile_stride; t.dim = dim; t.item_tiles = a.item_tiles; t.k = top_k;
+        t.item = item; t.bias = bias; t.group_max = a.group_max; t.tile_abs = tile_abs; t.lse = lse_out;
+        t.n_users = nu; t.n_items = n_items; t.group_stride = a.group_stride; t.dim = dim; t.item_tiles = a.item_tiles;
+        t.groups = a.item_tiles * (32 / cut.top); t.log2_items = cut.top == 4 ? 2 : 5; t.k = top_k;
         t.vector = vector;
         t.scale = scale; t.top_log_prob = top_log_prob + u0 * top_k; t.top_ids = top_ids + u0 * top_k;
         if (dtype == GS_F32) catalog_top_kernel<float><<<dim3((unsigned)nu), 256, 0, s>>>(t);

@@ -128,9 +128,12 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
                 dz[r] = fast_exp2(lp) * (USERS ? __builtin_fmaf(cb, lp, ca) : __builtin_fmaf(w[k], lp, y[k]));
             }
         }
-        if (!USERS && a.g_bias)
+        if (!USERS && a.g_bias) {                   // (a tile's elements first: thousands one by one would cost digits)
+            float x[8];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum += dz[r];
+            for (int r = 0; r < 8; ++r) x[r] = dz[2 * r] + dz[2 * r + 1];
+            sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             bf16x8 z[NZ];
@@ -196,7 +199,7 @@ void catalog_bwd_kernel(BwdArgs a) {
     else backward<T, DB, false>(a, a.items, blockIdx.x - a.user_blocks, stage);
 }
 
-// Adds the shares in order: users' elements, then items', then the bias.
+// Adds the shares in a fixed order: users' elements, then items', then the bias.
 struct JoinArgs {
     const float *user_part, *item_part, *bias_part;
     int user_shares, item_shares, dim, width;
@@ -209,30 +212,37 @@ struct JoinArgs {
     float *g_bias;
 };
 
+// A block takes 32 elements, eight threads each (five users against 70 000 items leave 441 shares: 21 us with one).
 template <class T>
 __global__ __launch_bounds__(kCatThreads)
 void catalog_bwd_join_kernel(JoinArgs a) {
-    int64_t i = (int64_t)blockIdx.x * kCatThreads + threadIdx.x;
-    const float *part;
-    int64_t each;
-    int shares;
+    constexpr int N = kCatThreads / 32;
+    __shared__ float sums[N][32];
+    const int part_of = threadIdx.x >> 5;
+    int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    const bool in = i < a.user_n + a.item_n + a.bias_n;
     const bool user = i < a.user_n, item = !user && i < a.user_n + a.item_n;
+    const float *part = a.bias_part;
+    int64_t each = a.item_padded;
+    int shares = in ? (user ? a.user_shares : a.item_shares) : 0;
     if (user || item) {
         if (item) i -= a.user_n;
         const int64_t row = i / a.dim;
         part = (user ? a.user_part : a.item_part) + row * a.width + (i - row * a.dim);
         each = (user ? a.user_padded : a.item_padded) * a.width;
-        shares = user ? a.user_shares : a.item_shares;
     } else {
         i -= a.user_n + a.item_n;
-        if (i >= a.bias_n) return;
-        part = a.bias_part + i;
-        each = a.item_padded;
-        shares = a.item_shares;
+        part += i;
     }
     float s = 0.f;
 #pragma unroll 8
-    for (int k = 0; k < shares; ++k) s += part[(size_t)k * each];
+    for (int k = part_of; k < shares; k += N) s += part[(size_t)k * each];
+    sums[part_of][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (part_of || !in) return;
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) s += sums[k][threadIdx.x];
     if (user) {
         // the target's term, whole
         const int64_t n = i / a.dim;
@@ -240,8 +250,7 @@ void catalog_bwd_join_kernel(JoinArgs a) {
         const int t = st.target[n & 31];
         if (t >= 0 && a.bias2[t] > kFloor) s += st.g[n & 31] * (float)static_cast<const T *>(a.item)[(int64_t)t * a.dim + (i - n * a.dim)];
         static_cast<T *>(a.g_user)[i] = (T)(s * a.scale);
-    }
-    else if (item) static_cast<T *>(a.g_item)[i] = (T)(s * a.scale);
+    } else if (item) static_cast<T *>(a.g_item)[i] = (T)(s * a.scale);
     else a.g_bias[i] = s;
 }
 
@@ -304,7 +313,7 @@ int run_bwd(const BwdArgs &a, const JoinArgs &j, int blocks, hipStream_t stream)
     }
     const int64_t elements = j.user_n + j.item_n + j.bias_n;
     if (elements) {
-        catalog_bwd_join_kernel<T><<<dim3((unsigned)((elements + kCatThreads - 1) / kCatThreads)), kCatThreads, 0, stream>>>(j);
+        catalog_bwd_join_kernel<T><<<dim3((unsigned)((elements + 31) / 32)), kCatThreads, 0, stream>>>(j);
         return gs::check_launch("gs_catalog_bwd (join)");
     }
     return GS_OK;
