@@ -10,15 +10,21 @@ The other operators of ``LinkEmbedding.call`` (``link_utils.py:154-176``: ip/dot
 mul/hadamard, l1, l2, avg), other output widths and activations, and the clipped
 regression head (``link_regression``, ``LeakyClippedLinear``) are plain torch
 modules here; a model with one of them trains through autograd.
+
+``link_ranking`` (not in the reference) gives ``CatalogHead``: links are learned as a choice among the items of the batch
+(softmax loss) and users are answered with the best items of a whole catalog.
 """
 import math
 import warnings
 
 import torch
 
+from . import autograd as _ag
+from . import kernels
 from .train import LinkHead
 
-__all__ = ['LinkEmbedding', 'EdgeHead', 'link_inference', 'link_classification', 'link_regression']
+__all__ = ['LinkEmbedding', 'EdgeHead', 'CatalogHead', 'link_inference', 'link_classification', 'link_regression',
+           'link_ranking']
 
 _ACTIVATIONS = {
     'linear': lambda x: x, None: lambda x: x,
@@ -137,3 +143,61 @@ def link_classification(output_dim=1, output_act="sigmoid", edge_embedding_metho
 def link_regression(output_dim=1, clip_limits=None, edge_embedding_method="ip"):
     return link_inference(output_dim=output_dim, output_act="linear", edge_embedding_method=edge_embedding_method,
                           clip_limits=clip_limits, name="link_regression")
+
+
+class CatalogHead:
+    """Scores ``scale * <user, item>`` as logits over a catalog of items.
+
+    ``loss((user_emb, item_emb), targets)``: every positive link (target > 0.5) is a choice of its item among the items of
+    the batch; minus the mean log probability of these choices, minus ``entropy_weight`` times the mean entropy of all
+    users' choices (``gs_catalog_fwd`` / ``gs_catalog_bwd``: the logits never pass through memory).  ``item_bias`` corrects for
+    how the batch's items are drawn (minus the logarithm of their frequencies).
+    ``recommend(user_emb, item_emb, k)``: the k best of all items for every user.
+    Called like the other heads it scores the batch's own pairs, ``sigmoid(scale * <user, item>)``, (B, 1)."""
+
+    def __init__(self, scale=10.0, entropy_weight=0.0):
+        self.scale = float(scale)
+        if not 0.0 < self.scale < float('inf'):
+            raise ValueError("scale must be positive and finite (got %r)" % (scale,))
+        self.entropy_weight = float(entropy_weight)
+
+    def parameters(self):
+        return []
+
+    def __call__(self, x_out):
+        user_emb, item_emb = x_out
+        return torch.sigmoid(self.scale * (user_emb * item_emb).sum(dim=-1, keepdim=True))
+
+    def loss(self, x_out, targets, item_bias=None):
+        """(loss, the pairs' scores (B, 1))."""
+        user_emb, item_emb = (x.contiguous() for x in x_out)
+        n, dev = user_emb.shape[0], user_emb.device
+        positive = torch.as_tensor(targets, dtype=torch.float32, device=dev).reshape(-1) > 0.5
+        if positive.numel() != n or item_emb.shape[0] != n:
+            raise ValueError("one target and one item per user are needed (%d users, %d items, %d targets)" %
+                             (n, item_emb.shape[0], positive.numel()))
+        own = torch.arange(n, dtype=torch.int32, device=dev)
+        log_prob, entropy = _ag.CatalogLogProbs.apply(user_emb, item_emb, torch.where(positive, own, -1).to(torch.int32), item_bias,
+                                                      self.scale)
+        loss = -log_prob.sum() / positive.sum().clamp(min=1) - self.entropy_weight * entropy.mean()
+        with torch.no_grad():
+            pred = self((user_emb, item_emb))
+        return loss, pred
+
+    @torch.no_grad()
+    def recommend(self, user_emb, item_emb, k, item_bias=None):
+        """(item indices int32 (N, k), their log probabilities (N, k)), best first; an item whose bias is -inf is never
+        among them (``kernels.catalog_log_probs``)."""
+        r = kernels.catalog_log_probs(user_emb.contiguous(), item_emb.contiguous(), bias=item_bias, scale=self.scale, top_k=k)
+        return r.top_ids, r.top_log_prob
+
+
+def link_ranking(scale=10.0, entropy_weight=0.0):
+    """The edge function of ``CatalogHead``, taken like those of ``link_inference``."""
+    head = CatalogHead(scale, entropy_weight)
+
+    def edge_function(x_out, seed=None):
+        x_out.build()
+        return head
+
+    return edge_function

@@ -22,6 +22,10 @@ Two execution paths produce the same numbers:
   deepest slots straight from the feature tables through their sampled ids
   (``gs_gather_mean_fwd``), so the largest tensors of the batch, ``(B, n0*n1, F)``,
   are never written or read back.
+
+Two arguments beyond the reference's: ``agg_option='attention'`` with ``heads`` (``Aggregator``), and ``dropout_seed``.
+Without it dropout draws from torch's generator and torch keeps the masks; with it every mask is a function of the seed
+and of how much has been drawn before (``gs_dropout``), drawn again in the backward pass and never stored.
 """
 import itertools as it
 import operator as op
@@ -34,7 +38,7 @@ __all__ = ['GraphSAGE']
 
 class GraphSAGE:
     def __init__(self, layer_sizes, generator=None, agg_option='mean', bias=True, dropout=0.0,
-                 normalize="l2", seed=None):
+                 normalize="l2", seed=None, heads=1, dropout_seed=None):
         self._aggregator = Aggregator
         self.agg_option = agg_option
         self.normalize = normalize
@@ -48,6 +52,9 @@ class GraphSAGE:
                              (self.n_layers, len(layer_sizes)))
         self.bias = bias
         self.dropout = dropout
+        self.heads = heads
+        self.dropout_seed = dropout_seed
+        self._dropout_drawn = 0                              # blocks of eight elements drawn under the seed so far
         self.training = True
         n_slots = len(self.subtree_schema)
 
@@ -61,7 +68,7 @@ class GraphSAGE:
             {
                 node_type: self._aggregator(
                     output_dim, has_bias=self.bias, activation_function=self.activations[layer],
-                    agg_option=self.agg_option,
+                    agg_option=self.agg_option, heads=self.heads,
                     seed=None if seed is None else seed * 1000 + layer * 10 + ti)
                 for ti, (node_type, output_dim) in enumerate(self.dims[layer + 1].items())
             }
@@ -99,6 +106,8 @@ class GraphSAGE:
                 out['l%d.%s.w_neigh' % (layer, node_type)] = agg.w_neigh
                 if agg.bias is not None:
                     out['l%d.%s.bias' % (layer, node_type)] = agg.bias
+                if agg.w_query is not None:
+                    out['l%d.%s.w_query' % (layer, node_type)] = agg.w_query
         return out
 
     def train(self, mode=True):
@@ -111,6 +120,10 @@ class GraphSAGE:
     # ---- forward ------------------------------------------------------------------
     def _drop(self, x):
         if self.dropout and self.training:
+            if self.dropout_seed is not None:
+                first = self._dropout_drawn
+                self._dropout_drawn += (x.numel() + 7) // 8
+                return _ag.Dropout.apply(x.contiguous(), self.dropout, self.dropout_seed, first)
             import torch
             return torch.nn.functional.dropout(x, p=self.dropout, training=True)
         return x
@@ -144,6 +157,15 @@ class GraphSAGE:
             j = neigh_indices[0]
             m = x_self[i].shape[0]
             n = self.n_samples[self._depths[i]]
+            agg = self._aggs[0][node_type]
+            if self.agg_option == 'attention':
+                if j < len(alive):
+                    x_mean = agg.attend(x_self[i], x_self[j], None, n)
+                else:
+                    feat, off = batch.table(self.subtree_schema[j][0])
+                    x_mean = agg.attend(x_self[i], feat, batch.ids[j].reshape(-1), n, off)
+                out.append(agg.project(x_self[i], x_mean).reshape(b, m // b, agg.output_dim))
+                continue
             group, gather = ((_ag.GroupMax, _ag.GatherMax) if self.agg_option == 'max'
                              else (_ag.GroupMean, _ag.GatherMean))
             if j < len(alive):            # neighbor slot is itself gathered: mean (max) of those rows
@@ -151,7 +173,6 @@ class GraphSAGE:
             else:                          # deepest slot: rows are reduced as they are fetched
                 feat, off = batch.table(self.subtree_schema[j][0])
                 x_mean = gather.apply(feat, batch.ids[j].reshape(-1), m, n, off)
-            agg = self._aggs[0][node_type]
             out.append(agg.project(x_self[i], x_mean).reshape(b, m // b, agg.output_dim))
         return out
 

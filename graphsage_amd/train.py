@@ -248,6 +248,9 @@ class Trainer:
                     off += p.numel()
 
     def loss(self, batch, targets):
+        """Mean squared error of the head's scores, or the head's own loss where it has one (``link_utils.CatalogHead``)."""
+        if hasattr(self.head, 'loss'):
+            return self.head.loss(self.model(batch), targets)
         pred = self.head(self.model(batch))
         y = torch.as_tensor(targets, dtype=torch.float32, device=pred.device).reshape(pred.shape)
         return ((pred - y) ** 2).mean(), pred
@@ -571,7 +574,8 @@ class Trainer:
         """(scores (b, 1), targets) of batch i: through the forward engine when the
         batch is a full one of a keyed sequence, else through the model."""
         if (self._graph_obj is not None and self._batch_size and getattr(seq, '_indexed', False)
-                and seq.batch_size == int(self._batch_size) and not (self.model.dropout and self.model.training)):
+                and seq.batch_size == int(self._batch_size) and not (self.model.dropout and self.model.training)
+                and self.model.agg_option != 'attention'):
             staged = seq.epoch_on_device()
             if i < staged['n_batches']:
                 if self._fwd_engine is None:
@@ -591,7 +595,8 @@ class Trainer:
         before the slot's stream is allowed to write them again (``submit`` makes it wait for this stream)."""
         n = len(seq)
         use_engine = (self._graph_obj is not None and self._batch_size and getattr(seq, '_indexed', False)
-                      and seq.batch_size == int(self._batch_size) and not (self.model.dropout and self.model.training))
+                      and seq.batch_size == int(self._batch_size) and not (self.model.dropout and self.model.training)
+                      and self.model.agg_option != 'attention')
         n_eng = 0
         if use_engine:
             staged = seq.epoch_on_device()

@@ -27,6 +27,12 @@ class SageTrainEngine(SageForwardEngine):
         if not 0.0 <= self.dropout < 1.0:
             raise ValueError("dropout rate must lie in [0, 1)")
         self._padded_model = None
+        if getattr(model, 'agg_option', 'mean') == 'attention':
+            raise kernels._lib.GsageError("the training plan covers the mean aggregator; agg_option='attention' trains "
+                                          "through graphsage_amd.train.Trainer(engine='autograd')")
+        if self.dropout and getattr(model, 'dropout_seed', None) is not None:
+            raise kernels._lib.GsageError("the training plan draws its masks by the links' keys; a model with a dropout_seed "
+                                          "trains through graphsage_amd.train.Trainer(engine='autograd')")
         f = graph.node_feature_sizes
         if any(f[t] % 32 for t in _TYPES):
             from .padding import PaddedGraphView, PaddedModelView, padded_widths

@@ -10,6 +10,11 @@ gives ``act(concat(x_self @ w_self, mean_n(x_neigh) @ w_neigh) + bias)`` of shap
 initialisers of ``build`` (``:64-91``: glorot-uniform ``(F, output_dim/2)``
 matrices, zero bias).  The arithmetic runs in two HIP kernels: the neighbor mean
 (``gs_gather_mean_fwd``) and the MFMA projection (``gs_sage_project_fwd``).
+
+``agg_option='attention'`` (not in the reference) takes, in place of the neighbor mean, attention of the head node over its
+neighbors: ``heads`` queries ``x_self @ w_query`` as wide as a neighbor's features, scores against the features themselves, and the
+weighted features of all heads side by side go into ``w_neigh``, which has ``heads`` times as many rows.  The neighbors'
+rows are read once, by id where they come from a feature table, and serve as keys and values of every head.
 """
 import collections.abc
 import math
@@ -42,7 +47,7 @@ _ACTIVATIONS = ('relu', 'linear')
 
 class Aggregator:
     def __init__(self, output_dim=32, has_bias=True, activation_function="relu", agg_option='mean',
-                 seed=None, **kwargs):
+                 seed=None, heads=1, **kwargs):
         self.output_dim = output_dim
         if output_dim % 2 != 0:
             raise ValueError("The output_dim must be a multiple of two.")
@@ -53,8 +58,12 @@ class Aggregator:
         if activation_function not in _ACTIVATIONS:
             raise ValueError("activation_function must be one of %s (the two the model uses)" % (_ACTIVATIONS,))
         self.activation = activation_function
-        assert agg_option in ['mean', 'max'], "agg_option must be mean or max"
+        assert agg_option in ['mean', 'max', 'attention'], "agg_option must be mean, max or attention"
         self.agg_option = agg_option
+        self.heads = int(heads)
+        if self.heads < 1 or (self.heads != 1 and agg_option != 'attention'):
+            raise ValueError("heads must be positive, and 1 unless agg_option is 'attention' (got %r)" % (heads,))
+        self.w_query = None
         self.w_neigh = None
         self.w_self = None
         self.bias = None
@@ -82,14 +91,24 @@ class Aggregator:
             return w.to(torch.float32).to(device).requires_grad_(True)
 
         # creation order as in build(): w_neigh, then w_self, then bias
-        self.w_neigh = glorot(fn, self.half_output_dim)
+        self.w_neigh = glorot(self.heads * fn, self.half_output_dim)
         self.w_self = glorot(fs, self.half_output_dim)
+        if self.agg_option == 'attention':
+            self.w_query = glorot(fs, self.heads * fn)
         if self.has_bias:
             self.bias = torch.zeros(self.output_dim, dtype=torch.float32, device=device, requires_grad=True)
         self.built = True
 
     def parameters(self):
-        return [p for p in (self.w_self, self.w_neigh, self.bias) if p is not None]
+        return [p for p in (self.w_self, self.w_neigh, self.bias, self.w_query) if p is not None]
+
+    def attend(self, x_self2d, rows, ids, n, id_offset=0):
+        """Attention of the (M, Fs) head rows over their neighbors, n consecutive rows of ``rows`` each, or those that
+        ``ids`` names in the table ``rows``: (M, heads * Fn)."""
+        m, fn = x_self2d.shape[0], rows.shape[1]
+        q = (x_self2d @ self.w_query).reshape(m, self.heads, fn)
+        out, _ = _ag.NeighborAttention.apply(q, rows.reshape(-1, 1, fn), None, ids, n, id_offset, None, None, None)
+        return out.reshape(m, self.heads * fn)
 
     def project(self, x_self2d, x_mean2d):
         """The projection alone, on (M, Fs) and (M, Fn) row matrices."""
@@ -102,7 +121,11 @@ class Aggregator:
         b, heads, fs = x_self.shape
         n, fn = x_neigh.shape[2], x_neigh.shape[3]
         m = b * heads
-        reduce = _ag.GroupMax if self.agg_option == 'max' else _ag.GroupMean
-        mean = reduce.apply(x_neigh.reshape(m, n, fn).contiguous(), m, n)
-        out = self.project(x_self.reshape(m, fs).contiguous(), mean)
+        x_self = x_self.reshape(m, fs).contiguous()
+        if self.agg_option == 'attention':
+            mean = self.attend(x_self, x_neigh.reshape(m * n, fn).contiguous(), None, n)
+        else:
+            reduce = _ag.GroupMax if self.agg_option == 'max' else _ag.GroupMean
+            mean = reduce.apply(x_neigh.reshape(m, n, fn).contiguous(), m, n)
+        out = self.project(x_self, mean)
         return out.reshape(b, heads, self.output_dim)
