@@ -130,6 +130,12 @@ void attn_bwd_parents_kernel(BwdArgs a) {
     const bool dense = !a.nb.ids && (a.g_k || a.g_v);
 
     gs::Walk walk(a.nb, gs::this_wave(), a.chunk);
+    if (a.edge_parent && blockIdx.y == 0) {         // edges before the first list and behind the last have no parent
+        const int64_t first = a.nb.offset(0), last = a.nb.offset(a.nb.n_parents);
+        if (walk.e0 < first || walk.e1 > last)
+            for (uint32_t e = walk.e0 + lane64; e < walk.e1; e += 64)
+                if (e < first || e >= last) a.edge_parent[e] = -1;
+    }
     bool have = walk.next();
     if (!have) return;
     gs::Unit cur = walk.u;
@@ -334,8 +340,143 @@ void attn_bwd_rows_kernel(BwdArgs a) {
     }
 }
 
-// Adds the pieces of the lists that were cut, and writes zeros for empty ones.  `sets` vectors of dim floats per (list, y):
-// the parents' walk has one (y a head), the rows' two (y a key head).  Few pieces: one wave alone.
+// The rows' walk where the lists are short on the mean: every L lanes take `chunk` entries of their own by the same rule
+// (lists that begin there, and parts of longer ones).  Which row an entry belongs to is what child_ids say, so nothing is
+// searched, and every entry's loads (the row's key and value again and again, they are near) are known before its turn.
+template <class T, int L, int G, bool SHARED>
+__global__ __launch_bounds__(gs::kAttnThreads)
+void attn_bwd_rows_short_kernel(BwdArgs a) {
+    constexpr int E = gs::Pack<T>::E, W = 64 / L;
+    constexpr int U = L == 2 ? 1 : G == 1 && E == 4 ? 4 : G <= 2 ? 2 : 1;             // (divides L)
+    const int lane64 = threadIdx.x & 63, lane = lane64 & (L - 1), group0 = lane64 & ~(L - 1);
+    const int share = a.heads / a.kv_heads, j = blockIdx.y;
+    Neighbors lists = a.nb;
+    lists.indptr = a.inv_indptr;
+    lists.n_edges = a.n_inv;
+    const T *Q = static_cast<const T *>(a.q), *GO = static_cast<const T *>(a.g_out);
+    const T *K = static_cast<const T *>(a.k) + (int64_t)j * a.dim, *V = SHARED ? nullptr : static_cast<const T *>(a.v) + (int64_t)j * a.dim;
+    const int64_t stride = (int64_t)a.kv_heads * a.dim;
+    const float scale2 = a.scale * gs::kLog2e;
+    const gs::Place<T, L> at(lane, a.dim);
+    const uint32_t chunk = (uint32_t)a.chunk, most = 4 * chunk, run = gs::this_wave() * W + lane64 / L;
+    const uint32_t e0 = (uint32_t)min((uint64_t)run * chunk, (uint64_t)a.n_inv), e1 = min(e0 + chunk, a.n_inv);
+
+    struct Entry { int32_t row, parent; uint32_t begin, end; };        // what a lane knows of entry e
+    const auto entry_at = [&](uint32_t e) {
+        Entry t;
+        const uint32_t edge = (uint32_t)a.inv_edges[min(e, a.n_inv - 1)];
+        const int32_t id = a.nb.ids[min(edge, a.nb.n_edges - 1)];
+        const int32_t p = a.nb.indptr ? a.edge_parent[min(edge, a.nb.n_edges - 1)] : (int32_t)(edge / a.nb.n_child);
+        t.row = edge < a.nb.n_edges ? a.nb.row_of(id) : -1;
+        t.parent = t.row >= 0 && (uint64_t)(int64_t)p < (uint64_t)a.nb.n_parents ? p : -1;
+        lists.range(max(t.row, 0), t.begin, t.end);
+        if (t.row < 0) { t.begin = e; t.end = e + 1; }
+        return t;
+    };
+    // from the end of a list that another has begun and keeps, to the end of the last one that begins here
+    Entry t = entry_at(e0 + lane);
+    uint32_t start = e0, stop = e0;
+    {
+        const uint32_t f_begin = __shfl(t.begin, group0, 64), f_end = __shfl(t.end, group0, 64);
+        const int back = (int)min(chunk, (uint32_t)L) - 1;
+        Entry l;
+        l.begin = __shfl(t.begin, group0 + back, 64);
+        l.end = __shfl(t.end, group0 + back, 64);
+        if (chunk > L || e1 - e0 < chunk) l = entry_at(e1 - 1);
+        if (e0 < e1) {
+            if (f_begin < e0 && f_end - f_begin <= most) start = f_end;
+            stop = l.end - l.begin > most ? e1 : min(l.end, e1 + most);
+        }
+    }
+    float sum[2 * E];
+#pragma unroll
+    for (int i = 0; i < 2 * E; ++i) sum[i] = 0.f;
+    for (uint32_t at_e = e0; __any(at_e < stop && start < stop); at_e += L) {
+        const uint32_t mine = at_e + lane;
+        if (at_e != e0) t = entry_at(mine);
+        const bool cut = t.end - t.begin > most, in = mine >= start && mine < stop;
+        // 1: the list's last entry here, 2: a piece of it, 4: the piece's place
+        const int flags = in && t.row >= 0 && mine + 1 == (cut ? min(t.end, e1) : t.end) ? 1 | (cut ? 2 : 0) | (t.begin > e0 ? 4 : 0) : 0;
+        const int32_t parent = in ? t.parent : -1;
+        const unsigned long long some = __ballot(parent >= 0 || flags);
+        for (int x = 0; x < L; x += U) {
+            unsigned long long turn = 0;                               // the entries of this turn, in all groups
+#pragma unroll
+            for (int g = 0; g < 64; g += L) turn |= ((1ull << U) - 1) << (g + x);
+            if (!(some & turn)) continue;
+            int32_t row[U], p[U];
+            int fl[U];
+            RowPart<T> key[U], val[U];
+            float c[U][2 * E];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                row[u] = __shfl(t.row, group0 + x + u, 64);
+                p[u] = __shfl(parent, group0 + x + u, 64);
+                fl[u] = __shfl(flags, group0 + x + u, 64);
+                const int64_t to = (int64_t)max(row[u], 0) * stride;
+                key[u].load(K + to, at);
+                if (!SHARED) val[u].load(V + to, at);
+#pragma unroll
+                for (int i = 0; i < 2 * E; ++i) c[u][i] = 0.f;
+            }
+            for (int h0 = j * share; h0 < (j + 1) * share; h0 += G) {
+                RowPart<T> qr[U][G], gr[U][G];
+                float lse2[U][G], delta[U][G];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {   // (what is no neighbor, and heads past the last one, read another and forget it)
+                        const int64_t of = (int64_t)max(p[u], 0) * a.heads + min(h0 + g, (j + 1) * share - 1);
+                        qr[u][g].load(Q + of * a.dim, at);
+                        gr[u][g].load(GO + of * a.dim, at);
+                        lse2[u][g] = a.lse[of] * gs::kLog2e;
+                        delta[u][g] = a.delta[of];
+                    }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    RowPart<T> own_key = key[u], own_val = val[u];
+                    own_key.own(at);
+                    if (!SHARED) own_val.own(at);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const bool none = p[u] < 0 || h0 + g >= (j + 1) * share || lse2[u][g] == -INFINITY;
+                        qr[u][g].zero_if(none);
+                        gr[u][g].zero_if(none);
+                        const float s = gs::lanes_sum<L>(gs::dot(own_key, qr[u][g])) * scale2;
+                        const float dp = gs::lanes_sum<L>(gs::dot(SHARED ? own_key : own_val, gr[u][g]));
+                        const float pr = none ? 0.f : gs::fast_exp2(s - lse2[u][g]);
+                        const float ds = none ? 0.f : pr * (dp - delta[u][g]) * a.scale;
+#pragma unroll
+                        for (int i = 0; i < E; ++i) { c[u][i] += ds * qr[u][g].at(i); c[u][E + i] += pr * gr[u][g].at(i); }
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int i = 0; i < 2 * E; ++i) sum[i] += c[u][i];
+                if (!(fl[u] & 1)) continue;
+                if (SHARED)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) sum[i] += sum[E + i];
+                const int64_t to = (int64_t)row[u] * stride + (int64_t)j * a.dim;
+                if (fl[u] & 2) {
+                    float *piece = a.piece + ((size_t)(run * 2 + (fl[u] >> 2)) * a.kv_heads + j) * 2 * a.dim;
+                    gs::store_part<E>(piece, at, 0, sum);
+                    if (!SHARED) gs::store_part<E>(piece + a.dim, at, 0, sum + E);
+                } else {
+                    if (a.g_k) gs::store_part<E>(static_cast<T *>(a.g_k) + to, at, 0, sum);
+                    if (!SHARED && a.g_v) gs::store_part<E>(static_cast<T *>(a.g_v) + to, at, 0, sum + E);
+                }
+#pragma unroll
+                for (int i = 0; i < 2 * E; ++i) sum[i] = 0.f;
+            }
+        }
+    }
+}
+
+// Adds the pieces of the lists that were cut, and writes zeros for empty ones.  `sets` vectors of dim floats per head: the
+// parents' walk has one per (list, head), the rows' two per (list, key head).  Few pieces: one wave alone.
 constexpr uint32_t kFewPieces = 16;
 
 template <class T>
@@ -343,16 +484,17 @@ __global__ __launch_bounds__(gs::kJoinWaves * 64)
 void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int sets, int dim, uint32_t chunk, T *out0, T *out1) {
     constexpr int N = gs::kJoinWaves;
     __shared__ float part[N][64];
+    __shared__ gs::LongLists longs;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, y = blockIdx.y / sets, set = blockIdx.y % sets;
     T *out = set ? out1 : out0;
     if (!out) return;
     const gs::JoinLanes l(lane, dim, blockIdx.z);
-    const int64_t mine = (int64_t)lane * gridDim.x + blockIdx.x;
+    const int64_t mine = gs::join_list(wave, lane);
     uint32_t b = 0, e = 0;
     if (mine < seg.n_parents) seg.range(mine, b, e);
     const bool mine_todo = mine < seg.n_parents && gs::needs_join(b, e, chunk);
     const bool many = mine_todo && e > b && (e - 1) / chunk - b / chunk >= kFewPieces;
-    unsigned long long few = __ballot(mine_todo && !many), long_ones = __ballot(many);
+    unsigned long long few = __ballot(mine_todo && !many);
     const auto add = [&](uint32_t sb, uint32_t se, uint32_t first, uint32_t step) {
         const uint32_t n = (se - 1) / chunk - sb / chunk + 1;
         float acc = 0.f;
@@ -367,28 +509,32 @@ void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int s
         for (int o = l.width; o < 64; o *= 2) acc += __shfl_xor(acc, o, 64);
         return acc;
     };
-    const auto write = [&](int src, float v) {
-        const int64_t p = (int64_t)src * gridDim.x + blockIdx.x;
+    const auto write = [&](int64_t p, float v) {
         if (l.sub == 0 && l.in) out[(p * per_slot + y) * dim + l.d] = (T)v;
     };
-    for (int turn = 0; few; ++turn, few &= few - 1) {
-        if (turn % N != wave) continue;
+    for (; few; few &= few - 1) {
         const int src = __builtin_ctzll(few);
         const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
-        write(src, se > sb ? add(sb, se, l.sub, l.subs) : 0.f);
+        write(gs::join_list(wave, src), se > sb ? add(sb, se, l.sub, l.subs) : 0.f);
     }
-    for (; long_ones; long_ones &= long_ones - 1) {
-        const int src = __builtin_ctzll(long_ones);
-        const uint32_t sb = __shfl(b, src, 64), se = __shfl(e, src, 64);
-        const float own = add(sb, se, wave * l.subs + l.sub, N * l.subs);
+    if (!__syncthreads_or(many)) return;
+    if (threadIdx.x == 0) longs.n = 0;
+    __syncthreads();
+    if (many) {
+        const int i = atomicAdd(&longs.n, 1);
+        longs.slot[i] = threadIdx.x; longs.b[i] = b; longs.e[i] = e;
+    }
+    __syncthreads();
+    for (int i = 0; i < longs.n; ++i) {
+        const float own = add(longs.b[i], longs.e[i], wave * l.subs + l.sub, N * l.subs);
         __syncthreads();                            // the last list's parts are read
         part[wave][lane] = own;
         __syncthreads();
         if (wave) continue;
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum += part[i][lane];
-        write(src, sum);
+        for (int k = 0; k < N; ++k) sum += part[k][lane];
+        write(gs::join_list(longs.slot[i] >> 6, longs.slot[i] & 63), sum);
     }
 }
 
@@ -396,19 +542,20 @@ void attn_bwd_join_kernel(Neighbors seg, const float *piece, int per_slot, int s
 template <class T>
 __global__ __launch_bounds__(256)
 void attn_bwd_dense_kernel(BwdArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = a.nb.n_rows * a.kv_heads * a.dim;
-    if (i >= n) return;
-    const int64_t row = i / ((int64_t)a.kv_heads * a.dim), vec = i / a.dim;
+    const int64_t n = a.nb.n_rows * a.kv_heads * a.dim;
     const int64_t first = a.nb.indptr ? a.nb.indptr[0] : 0, last = a.nb.indptr ? a.nb.indptr[a.nb.n_parents] : (int64_t)a.nb.n_edges;
-    if (row < first || row >= last) return;         // belongs to no parent: left as it is
-    float k = 0.f, v = 0.f;
-    for (int p = 0; p < a.parts; ++p) {
-        const float *part = a.dense_part + ((int64_t)p * n + vec * a.dim) * 2 + i % a.dim;
-        k += part[0];
-        if (a.v) v += part[a.dim];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / ((int64_t)a.kv_heads * a.dim), vec = i / a.dim;
+        if (row < first || row >= last) continue;   // belongs to no parent: left as it is
+        float k = 0.f, v = 0.f;
+        for (int p = 0; p < a.parts; ++p) {
+            const float *part = a.dense_part + ((int64_t)p * n + vec * a.dim) * 2 + i % a.dim;
+            k += part[0];
+            if (a.v) v += part[a.dim];
+        }
+        if (a.g_k) static_cast<T *>(a.g_k)[i] = (T)k;
+        if (a.g_v) static_cast<T *>(a.g_v)[i] = (T)v;
     }
-    if (a.g_k) static_cast<T *>(a.g_k)[i] = (T)k;
-    if (a.g_v) static_cast<T *>(a.g_v)[i] = (T)v;
 }
 
 int heads_per_wave(int share) { return share >= 3 ? 4 : share; }
@@ -427,10 +574,15 @@ void launch_parents(const BwdArgs &a, const gs::Deal &d, hipStream_t stream) {
 }
 
 template <class T, int L, bool SHARED>
-void launch_rows(const BwdArgs &a, int64_t waves, hipStream_t stream) {
+void launch_rows(const BwdArgs &a, const gs::Deal &d, hipStream_t stream) {
     const int g = heads_per_wave(a.heads / a.kv_heads);
+    const int64_t waves = d.is_short ? (d.waves + 64 / L - 1) / (64 / L) : d.waves;
     const dim3 grid((unsigned)((waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)a.kv_heads);
-    if (g == 1) attn_bwd_rows_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+    if (d.is_short) {
+        if (g == 1) attn_bwd_rows_short_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+        else if (g == 2) attn_bwd_rows_short_kernel<T, L, 2, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+        else attn_bwd_rows_short_kernel<T, L, 4, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
+    } else if (g == 1) attn_bwd_rows_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
     else if (g == 2) attn_bwd_rows_kernel<T, L, 2, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
     else attn_bwd_rows_kernel<T, L, 4, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
 }
@@ -441,14 +593,31 @@ struct Plan {
     size_t off_parent, off_dense, off_piece, total;
 };
 
+// Rows whose lists are this long on the mean, or shorter, are taken by L lanes a run of entries (100 000 rows of 64 fp32, a
+// list per wave against this: 96000 entries, 66 us and 16; 750 000 entries, about 80 us and 135).
+constexpr int64_t kShortMean = 4;
+
+gs::Deal deal_rows(int64_t n_rows, int64_t n_inv, int lanes) {
+    static const int64_t ragged = 0;                // any address: the rows' lists are ragged
+    gs::Deal d = gs::deal_edges(&ragged, n_rows, 0, n_inv, lanes);
+    d.is_short = n_inv && n_inv <= kShortMean * n_rows;
+    if (d.is_short) {
+        // 16 entries a run (96000 entries: 16.4 us, 19.1 with 8; 360 000 of 256 bf16: 87 us, 104), 8 where there are few
+        // (16000: 7.6 us, 14.0 with 16), 131072 runs at most (each may leave two pieces)
+        d.chunk = n_inv > 65536 ? 16 : 8;
+        if (d.chunk < (n_inv + 131071) / 131072) d.chunk = (n_inv + 131071) / 131072;
+        d.waves = (n_inv + d.chunk - 1) / d.chunk;  // runs, here
+    }
+    return d;
+}
+
 // The pieces of both walks share a region: the second walk starts when the first one's pieces are joined.
 Plan make_plan(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype, int64_t n_inv) {
     Plan p;
     const int lanes = gs::lanes_for(dim, gs::dtype_size(dtype)), share = heads / kv_heads;
     p.parts = (share + heads_per_wave(share) - 1) / heads_per_wave(share);
     p.parents = gs::deal_edges(nb, lanes);
-    static const int64_t ragged = 0;                // any address: the rows' lists are ragged
-    p.rows = gs::deal_edges(&ragged, nb->n_rows, 0, nb->ids && nb->n_rows && nb->n_parents ? n_inv : 0, lanes);
+    p.rows = deal_rows(nb->n_rows, nb->ids && nb->n_rows && nb->n_parents ? n_inv : 0, lanes);
     size_t off = gs::align256((size_t)nb->n_parents * heads * sizeof(float));        // delta
     p.off_parent = off;
     if (nb->indptr && nb->ids) off += gs::align256((size_t)nb->n_edges * sizeof(int32_t));
@@ -470,19 +639,20 @@ int run_bwd(BwdArgs a, const Plan &p, int lanes, hipStream_t stream) {
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents)")) return rc;
     }
     if (a.g_q && a.nb.n_parents && p.parents.pieces) {
-        attn_bwd_join_kernel<T><<<dim3(gs::join_blocks(a.nb.n_parents), (unsigned)a.heads, (unsigned)((a.dim + 63) / 64)), gs::kJoinWaves * 64, 0, stream>>>(
+        attn_bwd_join_kernel<T><<<gs::join_grid(a.nb.n_parents, a.heads, a.dim), gs::kJoinWaves * 64, 0, stream>>>(
             a.nb, a.piece, a.heads, 1, a.dim, a.chunk, static_cast<T *>(a.g_q), (T *)nullptr);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (parents' join)")) return rc;
     }
     if (!a.g_k && !a.g_v) return GS_OK;
     if (!a.nb.ids) {
         if (a.parts == 1 || !a.nb.n_rows || !p.parents.waves) return GS_OK;
-        attn_bwd_dense_kernel<T><<<dim3((unsigned)((a.nb.n_rows * a.kv_heads * a.dim + 255) / 256)), 256, 0, stream>>>(a);
+        const int64_t blocks = (a.nb.n_rows * a.kv_heads * a.dim + 255) / 256;
+        attn_bwd_dense_kernel<T><<<dim3((unsigned)(blocks < 1 << 20 ? blocks : 1 << 20)), 256, 0, stream>>>(a);
         return gs::check_launch("gs_neighbor_attention_bwd (dense rows)");
     }
     a.chunk = (int)p.rows.chunk;
     if (p.rows.waves) {
-        GS_BY_LANES(launch_rows, a.v == nullptr, a, p.rows.waves, stream);
+        GS_BY_LANES(launch_rows, a.v == nullptr, a, p.rows, stream);
         if (int rc = gs::check_launch("gs_neighbor_attention_bwd (rows)")) return rc;
     }
     if (!a.nb.n_rows) return GS_OK;
@@ -491,7 +661,7 @@ int run_bwd(BwdArgs a, const Plan &p, int lanes, hipStream_t stream) {
     rows.n_child = 0;
     rows.n_parents = a.nb.n_rows;
     rows.n_edges = a.n_inv;
-    attn_bwd_join_kernel<T><<<dim3(gs::join_blocks(a.nb.n_rows), (unsigned)a.kv_heads * 2, (unsigned)((a.dim + 63) / 64)), gs::kJoinWaves * 64, 0, stream>>>(
+    attn_bwd_join_kernel<T><<<gs::join_grid(a.nb.n_rows, a.kv_heads * 2, a.dim), gs::kJoinWaves * 64, 0, stream>>>(
         rows, a.piece, a.kv_heads, 2, a.dim, a.chunk, static_cast<T *>(a.g_k), static_cast<T *>(a.g_v));
     return gs::check_launch("gs_neighbor_attention_bwd (rows' join)");
 }

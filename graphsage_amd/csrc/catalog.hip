@@ -175,6 +175,19 @@ struct FwdArgs {
     float scale2;
 };
 
+// (m, s, w, target's score) of two sets of items.
+__device__ __forceinline__ float4 join_sums(float4 a, float4 b) {
+    const float m = fmaxf(a.x, b.x), da = a.x - m, db = b.x - m, fa = fast_exp2(da), fb = fast_exp2(db);
+    return make_float4(m, a.y * fa + b.y * fb, fa * (a.z + a.y * da) + fb * (b.z + b.y * db), fmaxf(a.w, b.w));
+}
+
+template <int N> __device__ __forceinline__ float4 join_lanes(float4 q) {
+#pragma unroll
+    for (int o = N / 2; o; o >>= 1)
+        q = join_sums(q, make_float4(__shfl_xor(q.x, o, 64), __shfl_xor(q.y, o, 64), __shfl_xor(q.z, o, 64), __shfl_xor(q.w, o, 64)));
+    return q;
+}
+
 template <int P, int DB, int OF, int TOP>
 __global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * P * OF + 16 * OF + 24))
 void catalog_fwd_kernel(FwdArgs a) {
@@ -292,93 +305,251 @@ void catalog_fwd_kernel(FwdArgs a) {
     }
 }
 
-// One wave per user joins the shares.
-__global__ __launch_bounds__(kCatThreads)
-void catalog_join_kernel(const float4 *part, int shares, int64_t n_users, int64_t n_items, const int32_t *targets,
-                         float *log_prob, float *entropy, float *lse) {
-    const int lane = threadIdx.x & 63;
-    const int64_t n = (int64_t)blockIdx.x * (kCatThreads / 64) + (threadIdx.x >> 6);
-    if (n >= n_users) return;
-    float m = kFloor, s = 0.f, w = 0.f, hit = -INFINITY;
-    for (int i = lane; i < shares; i += 64) {
-        const float4 q = part[(size_t)n * shares + i];
-        const float m1 = fmaxf(m, q.x), da = m - m1, db = q.x - m1, fa = fast_exp2(da), fb = fast_exp2(db);
-        w = fa * (w + s * da) + fb * (q.z + q.y * db);
-        s = s * fa + q.y * fb;
+// A few users: one wave has them all, so every item row is used once and laying the table out would cost more than the
+// product.  The waves read the rows as they are, eight elements a lane, and cut them into pieces in registers.
+struct FewArgs {
+    const void *user, *item;
+    const float *bias;
+    const int32_t *targets;
+    float4 *part;                                   // [users][blocks]
+    float *group_max, *tile_abs;                    // tile_abs: [blocks], the largest |element| of their tiles
+    int64_t group_stride, n_items;
+    int n_users, dim, item_tiles;
+    float scale2;
+};
+
+// Elements e0 .. e0 + 7 of a row, zeros for those past its end: the last eight lie elsewhere in v, but in the same places
+// for every row.
+template <class T> __device__ __forceinline__ void load8(const T *row, int e0, int dim, float *v) {
+    if (dim >= 8) {
+        const int off = min(e0, dim - 8), skip = e0 - off;
+        T x[8];
+        __builtin_memcpy(x, row + off, sizeof(x));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < skip ? 0.f : (float)x[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = (float)row[min(e0 + i, dim - 1)];
+            v[i] = e0 + i < dim ? x : 0.f;
+        }
+    }
+}
+
+template <class T, int DB, int TOP>
+__global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * Pieces<T>::P + 16 * DB + 80))
+void catalog_few_kernel(FewArgs a) {
+    constexpr int P = Pieces<T>::P, KC = 2 * DB, W = kCatThreads / 64;
+    __shared__ float4 sums[W][32];
+    __shared__ float tops[W];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, half = lane >> 5;
+    Fragment<P> own[KC];
+    const T *U = static_cast<const T *>(a.user) + (int64_t)min(r, a.n_users - 1) * a.dim;
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) {
+        float v[8];
+        load8(U, 16 * kc + 8 * half, a.dim, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = r < a.n_users ? v[i] : 0.f;
+        cut_pieces<P>(v, own[kc].p);
+    }
+    int target = a.targets && r < a.n_users ? a.targets[r] : -1;
+    if (target >= a.n_items) target = -1;
+    float m = kFloor, s = 0.f, w = 0.f, hit = -INFINITY, most_abs = 0.f;
+    for (int t = blockIdx.x * W + wave; t < a.item_tiles; t += gridDim.x * W) {
+        const int64_t row = min((int64_t)t * 32 + r, a.n_items - 1);
+        const T *src = static_cast<const T *>(a.item) + row * a.dim;
+        const bool on = !(a.bias && a.bias[row] < kOffer);
+        float b[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t j = (int64_t)t * 32 + 8 * g + 4 * half + i;
+                const float x = a.bias ? a.bias[min(j, a.n_items - 1)] : 0.f;
+                b[4 * g + i] = j >= a.n_items || x < kOffer ? kMasked : x * kLog2e;
+            }
+        f32x16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+        float v[KC][8];
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) load8(src, 16 * kc + 8 * half, a.dim, v[kc]);
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[kc][i] = on ? v[kc][i] : 0.f;
+                if (TOP) most_abs = fmaxf(most_abs, fabsf(v[kc][i]));
+            }
+            Fragment<P> it;
+            cut_pieces<P>(v[kc], it.p);
+            multiply<P, P, 2>(acc, it.p, own[kc].p);
+        }
+        float z[16], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            z[i] = __builtin_fmaf(acc[i], a.scale2, b[i]);
+            top = fmaxf(top, z[i]);
+        }
+        const int local = target - t * 32;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (target >= 0 && local == row_of_reg(i, lane)) hit = z[i];
+        if (TOP == 32) {
+            const float most = half_max(top);
+            if (lane < 32 && r < a.n_users) a.group_max[r * a.group_stride + t] = most;
+        } else if (TOP == 4) {
+            if (r < a.n_users)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    a.group_max[r * a.group_stride + (int64_t)t * 8 + 2 * q + half] =
+                        fmaxf(fmaxf(z[4 * q], z[4 * q + 1]), fmaxf(z[4 * q + 2], z[4 * q + 3]));
+        }
+        const float m1 = fmaxf(m, top), step = m - m1, keep = fast_exp2(step);
+        w = keep * (w + s * step);
+        s *= keep;
         m = m1;
-        hit = fmaxf(hit, q.w);
-    }
-    float top = m;
+        float sp[4] = {0.f, 0.f, 0.f, 0.f}, wp[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const float d = m - top, f = fast_exp2(d);
-    w = f * (w + s * d);
-    s *= f;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        s += __shfl_xor(s, o, 64);
-        w += __shfl_xor(w, o, 64);
-        hit = fmaxf(hit, __shfl_xor(hit, o, 64));
+        for (int i = 0; i < 16; ++i) {
+            const float d = z[i] - m, p = fast_exp2(d);
+            sp[i & 3] += p;
+            wp[i & 3] = __builtin_fmaf(p, d, wp[i & 3]);
+        }
+        s += (sp[0] + sp[1]) + (sp[2] + sp[3]);
+        w += (wp[0] + wp[1]) + (wp[2] + wp[3]);
     }
-    if (lane) return;
+    // the two lanes of a user, then the four waves
+    const float m1 = half_max(m), step = m - m1, keep = fast_exp2(step);
+    const float s1 = s * keep, w1 = keep * (w + s * step);
+    const float s2 = s1 + __shfl_xor(s1, 32, 64), w2 = w1 + __shfl_xor(w1, 32, 64);
+    const float hit1 = half_max(hit);
+    if (lane < 32) sums[wave][r] = make_float4(m1, s2, w2, hit1);
+    if (TOP) {
+#pragma unroll
+        for (int o = 32; o; o >>= 1) most_abs = fmaxf(most_abs, __shfl_xor(most_abs, o, 64));
+        if (lane == 0) tops[wave] = most_abs;
+    }
+    __syncthreads();
+    if (threadIdx.x >= a.n_users) return;
+    float4 q = sums[0][r];
+#pragma unroll
+    for (int k = 1; k < W; ++k) q = join_sums(q, sums[k][r]);
+    a.part[(size_t)r * gridDim.x + blockIdx.x] = q;
+    if (TOP && r == 0) a.tile_abs[blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+}
+
+// What the shares of a user leave, and where it goes (nullable, one entry a user).
+struct JoinArgs {
+    const float4 *part;
+    int shares;
+    int64_t n_items;
+    const int32_t *targets;
+    float *log_prob, *entropy, *lse;
+};
+
+// N threads join the shares of user n, thread t of them the ones t, t + N, ...; a wave's part of it, in every lane.
+template <int N> __device__ __forceinline__ float4 join_shares(const JoinArgs &a, int64_t n, int t) {
+    const float4 none = make_float4(kFloor, 0.f, 0.f, -INFINITY);
+    float4 q = none;
+    for (int i = t; i < a.shares; i += 4 * N) {
+        float4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = a.part[(size_t)n * a.shares + min(i + N * k, a.shares - 1)];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q = join_sums(q, i + N * k < a.shares ? x[k] : none);
+    }
+    return join_lanes<64>(q);
+}
+
+// The results of user n; log sum exp.
+__device__ __forceinline__ float finish_user(const JoinArgs &a, int64_t n, float4 q, bool writes) {
+    const float top = q.x, s = q.y, w = q.z, hit = q.w;
     const float l2 = fast_log2(s);                  // s 0: nothing on offer
-    if (lse) lse[n] = s == 0.f ? -INFINITY : (top + l2) * kLn2;
-    if (entropy) entropy[n] = s == 0.f ? 0.f : (l2 - w / s) * kLn2;
-    if (log_prob) {
-        const bool there = targets && targets[n] >= 0 && targets[n] < n_items;
-        log_prob[n] = !there ? 0.f : s != s ? s : hit < kFloor ? -INFINITY : (hit - (top + l2)) * kLn2;
+    const float lse = s == 0.f ? -INFINITY : (top + l2) * kLn2;
+    if (writes) {
+        if (a.lse) a.lse[n] = lse;
+        if (a.entropy) a.entropy[n] = s == 0.f ? 0.f : (l2 - w / s) * kLn2;
+        if (a.log_prob) {
+            const bool there = a.targets && a.targets[n] >= 0 && a.targets[n] < a.n_items;
+            a.log_prob[n] = !there ? 0.f : s != s ? s : hit < kFloor ? -INFINITY : (hit - (top + l2)) * kLn2;
+        }
     }
+    return lse;
+}
+
+// A wave per user.
+__global__ __launch_bounds__(kCatThreads)
+void catalog_join_kernel(JoinArgs a, int64_t n_users) {
+    const int64_t n = (int64_t)blockIdx.x * (kCatThreads / 64) + (threadIdx.x >> 6);
+    if (n < n_users) finish_user(a, n, join_shares<64>(a, n, threadIdx.x & 63), (threadIdx.x & 63) == 0);
 }
 
 struct TopArgs {
     const void *user, *item;
-    const float *bias, *group_max, *tile_abs, *lse;
+    const float *bias, *group_max, *tile_abs;
     int64_t n_users, n_items, group_stride;
-    int dim, item_tiles, groups, log2_items, k, vector;         // log2_items: of a group
+    int dim, n_abs, groups, log2_items, k, vector;  // log2_items: of a group
     float scale;
     float *top_log_prob;
     int32_t *top_ids;
 };
 
-// One block per user.  Thresholds and candidates: see the head of the file.  Four lanes score an item.
-template <class T>
-__global__ __launch_bounds__(256)
-void catalog_top_kernel(TopArgs a) {
-    constexpr int kBuf = 1024, kChunk = 4096, E = 16 / sizeof(T);
+// One block of N threads per user, which first joins the user's shares.  Thresholds and candidates: see the head of the file.
+// Four lanes score an item.
+template <class T, int N>
+__global__ __launch_bounds__(N)
+void catalog_top_kernel(TopArgs a, JoinArgs join) {
+    constexpr int kBuf = 1024, kChunk = 4096, E = 16 / sizeof(T), kSets = 256, kPasses = 2048 / N;
     __shared__ double user[256];
     __shared__ double val[kBuf];
     __shared__ int32_t id[kBuf];
     __shared__ double best_val[kMaxTop];
     __shared__ int32_t best_id[kMaxTop];
-    __shared__ __align__(16) float group_max[256];
-    __shared__ float group_abs[256];
+    __shared__ __align__(16) float group_max[kSets];
+    __shared__ float group_abs[kSets];
     __shared__ uint16_t cand[kChunk];
     __shared__ int n_val, n_cand;
-    __shared__ float low;
+    __shared__ float low, lse;
+    __shared__ float4 joined[N / 64];
     const int tid = threadIdx.x, quad = tid >> 2, part = tid & 3;
     const int64_t n = blockIdx.x;
     const float *gm = a.group_max + n * a.group_stride;
-    const int items = 1 << a.log2_items, at_once = 64 >> a.log2_items;          // a pass scores 64 items
+    const int items = 1 << a.log2_items, at_once = (N / 4) >> a.log2_items;     // a pass scores N / 4 items
     const T *U = static_cast<const T *>(a.user) + n * a.dim, *I = static_cast<const T *>(a.item);
-    for (int d = tid; d < a.dim; d += 256) user[d] = (double)(float)U[d];
+    for (int d = tid; d < a.dim; d += N) user[d] = (double)(float)U[d];
     float top = -INFINITY, most_abs = 0.f;
 #pragma unroll 4
-    for (int t = tid; t < a.groups; t += 256) top = fmaxf(top, gm[t]);
+    for (int t = tid; t < a.groups; t += N) top = fmaxf(top, gm[t]);
 #pragma unroll 4
-    for (int t = tid; t < a.item_tiles; t += 256) most_abs = fmaxf(most_abs, a.tile_abs[t]);
-    group_max[tid] = top;
-    group_abs[tid] = most_abs;
-    if (tid == 0) { n_val = 0; n_cand = 0; low = -INFINITY; }
-    __syncthreads();
-    // the k-th largest of the maxima of 256 sets of groups: at least k groups reach it
-    int rank = 0;
-#pragma unroll 8
-    for (int i = 0; i < 256; i += 4) {
-        const float4 o = *reinterpret_cast<const float4 *>(group_max + i);
-        rank += (o.x > top || (o.x == top && i < tid)) + (o.y > top || (o.y == top && i + 1 < tid)) +
-                (o.z > top || (o.z == top && i + 2 < tid)) + (o.w > top || (o.w == top && i + 3 < tid));
+    for (int t = tid; t < a.n_abs; t += N) most_abs = fmaxf(most_abs, a.tile_abs[t]);
+#pragma unroll
+    for (int o = 1; o < N / kSets; o *= 2) {
+        top = fmaxf(top, __shfl_xor(top, o, 64));
+        most_abs = fmaxf(most_abs, __shfl_xor(most_abs, o, 64));
     }
-    if (rank == a.k - 1) low = top;
+    if (tid % (N / kSets) == 0) { group_max[tid / (N / kSets)] = top; group_abs[tid / (N / kSets)] = most_abs; }
+    if (tid == 0) { n_val = 0; n_cand = 0; low = -INFINITY; }
+    const float4 share = join_shares<N>(join, n, tid);
+    if (tid % 64 == 0) joined[tid / 64] = share;
+    __syncthreads();
+    if (tid >= N - 64) {
+        const float l = finish_user(join, n, join_lanes<N / 64>(joined[tid % (N / 64)]), tid == N - 1);
+        if (tid == N - 1) lse = l;
+    }
+    // the k-th largest of the maxima of 256 sets of groups: at least k groups reach it
+    if (tid < kSets) {
+        int rank = 0;
+        top = group_max[tid];
+#pragma unroll 8
+        for (int i = 0; i < kSets; i += 4) {
+            const float4 o = *reinterpret_cast<const float4 *>(group_max + i);
+            rank += (o.x > top || (o.x == top && i < tid)) + (o.y > top || (o.y == top && i + 1 < tid)) +
+                    (o.z > top || (o.z == top && i + 2 < tid)) + (o.w > top || (o.w == top && i + 3 < tid));
+        }
+        if (rank == a.k - 1) low = top;
+    }
     // |user|, and the largest |element| of an item, by every wave for itself
     double norm = 0.0;
     for (int d = tid & 63; d < a.dim; d += 64) norm += user[d] * user[d];
@@ -401,7 +572,7 @@ void catalog_top_kernel(TopArgs a) {
     const auto compress = [&]() {
         __syncthreads();
         const int c = n_val;
-        for (int i = tid; i < c; i += 256) {
+        for (int i = tid; i < c; i += N) {
             const double v = val[i];
             const int32_t at = id[i];
             int r = 0;
@@ -421,13 +592,13 @@ void catalog_top_kernel(TopArgs a) {
     for (int t0 = 0; t0 < a.groups; t0 += kChunk) {
         const int t1 = min(t0 + kChunk, a.groups);
 #pragma unroll 4
-        for (int t = t0 + tid; t < t1; t += 256)
+        for (int t = t0 + tid; t < t1; t += N)
             if (!(gm[t] < thr_down)) cand[atomicAdd(&n_cand, 1)] = (uint16_t)(t - t0);
         __syncthreads();
         const int count = n_cand;
-        // the buffer takes eight passes between two looks at it
-        for (int c0 = 0; c0 < count; c0 += 8 * at_once) {
-            for (int c = c0 + (quad >> a.log2_items); c < min(c0 + 8 * at_once, count); c += at_once) {
+        // the buffer takes 512 items between two looks at it
+        for (int c0 = 0; c0 < count; c0 += kPasses * at_once) {
+            for (int c = c0 + (quad >> a.log2_items); c < min(c0 + kPasses * at_once, count); c += at_once) {
                 const int64_t j = (((int64_t)t0 + cand[c]) << a.log2_items) + (quad & (items - 1));
                 const float b = j < a.n_items && a.bias ? a.bias[j] : 0.f;
                 const bool in = j < a.n_items && !(b < kOffer);
@@ -464,13 +635,18 @@ void catalog_top_kernel(TopArgs a) {
     compress();
     if (tid < a.k) {
         const bool has = tid < n_val;
-        a.top_log_prob[n * a.k + tid] = has ? (float)(val[tid] - (double)a.lse[n]) : -INFINITY;
+        a.top_log_prob[n * a.k + tid] = has ? (float)(val[tid] - (double)lse) : -INFINITY;
         a.top_ids[n * a.k + tid] = has ? id[tid] : -1;
     }
 }
 
 // Groups of a user, to a multiple of four.
 int64_t group_stride_of(int64_t n_items, int top) { return (tiles_of(n_items) * (32 / top) + 3) / 4 * 4; }
+
+constexpr int64_t kBlocks = 1024;                   // blocks a launch is cut into: four waves per SIMD
+
+// Users of one wave.
+constexpr int64_t kFewUsers = 32;
 
 // How a call is cut: users in slices that bound the table of tile maxima, a slice in waves.
 struct Cut {
@@ -481,13 +657,17 @@ struct Cut {
 Cut cut_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
     Cut c;
     const int regs = pieces_of(dtype) * blocks_of(dim);                   // registers of a fragment row: 8 each
-    c.of = n_users > 32 && regs <= 8 ? 2 : 1;
+    // two tiles of users a wave halve the reads of the items where the pairs still fill the chip (4096 users, 100 000 items of
+    // 64 bf16: 126 us, 133 with one; 512 users of fp32: 64 us, 68) and leave it idle where they do not (1024 users and items: 17 us,
+    // 14 with one; 64 users: 30 us, 26)
+    constexpr int W = gs::kCatThreads / 64;
+    c.of = regs <= 8 && tiles_of(n_users) / (2 * W) * (tiles_of(n_items) / 4) >= kBlocks ? 2 : 1;
     c.slice = n_users;
     c.top = 0;
     if (top_k > 0) {
         // What a user costs beside the product: the groups' maxima, written and read, and about k groups of rows read again
-        // (out of L2: half the price).  Groups of 4 for few items, wide rows or long lists (3196 users, 4036 items of 200, 64
-        // best: 543 us with groups of 32, 166 us so), of 32 else (512 users, 100 000 items of 64, 20 best: 104 us, 125 us with groups of 4).
+        // (out of L2: half the price).  Groups of 4 for few items, wide rows or long lists (3196 users, 4036 items of 200 fp32, 64
+        // best: 185 us, 540 with groups of 32), of 32 else (512 users, 100 000 items of 64 fp32, 20 best: 100 us, 142 with groups of 4).
         const auto cost = [&](double group) { return 8.0 * n_items / group + 0.5 * top_k * group * dim * dtype_size(dtype); };
         c.top = cost(4) < cost(32) ? 4 : 32;
         const int64_t most = ((int64_t)1 << 26) / (group_stride_of(n_items, c.top) + 1) / 256 * 256;
@@ -495,8 +675,6 @@ Cut cut_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
     }
     return c;
 }
-
-constexpr int64_t kBlocks = 1024;                   // blocks a launch is cut into: four waves per SIMD
 
 void shares_of(int64_t users, int64_t n_items, int of, int *group_blocks, int *shares, int *per_share) {
     constexpr int W = gs::kCatThreads / 64;
@@ -510,7 +688,7 @@ void shares_of(int64_t users, int64_t n_items, int of, int *group_blocks, int *s
 }
 
 struct Space {
-    size_t user, item, bias2, part, lse, tile_abs, group_max, total;
+    size_t user, item, bias2, part, tile_abs, group_max, total;
 };
 
 Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
@@ -519,13 +697,13 @@ Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) 
     int blocks, shares, per;
     shares_of(c.slice, n_items, c.of, &blocks, &shares, &per);
     size_t off = 0;
-    s.user = off; off += align256(layout_bytes(c.slice, dim, dtype));
-    s.item = off; off += align256(layout_bytes(n_items, dim, dtype));
-    s.bias2 = off; off += align256((size_t)tiles_of(n_items) * 32 * sizeof(float));
+    const bool few = n_users <= kFewUsers;          // lays nothing out
+    s.user = off; off += few ? 0 : align256(layout_bytes(c.slice, dim, dtype));
+    s.item = off; off += few ? 0 : align256(layout_bytes(n_items, dim, dtype));
+    s.bias2 = off; off += few ? 0 : align256((size_t)tiles_of(n_items) * 32 * sizeof(float));
     s.part = off;
     // the last slice may be smaller and have more shares: the product of both is bounded by the blocks' users
-    off += align256((size_t)(c.slice * (int64_t)shares + kBlocks * 256) * sizeof(float4));
-    s.lse = off; off += align256((size_t)c.slice * sizeof(float));
+    off += align256((few ? (size_t)(n_users * kBlocks) : (size_t)(c.slice * (int64_t)shares + kBlocks * 256)) * sizeof(float4));
     s.tile_abs = off;
     if (top_k > 0) off += align256((size_t)tiles_of(n_items) * sizeof(float));
     s.group_max = off;
@@ -568,6 +746,29 @@ int launch_fwd(const FwdArgs &a, int blocks, int of, int top, hipStream_t stream
     return launch_tile<P, 8, 1>(a, top, stream);
 }
 
+template <class T, int TOP>
+int launch_few(const FewArgs &a, int shares, hipStream_t stream) {
+    switch (gs::blocks_of(a.dim)) {
+    case 1: catalog_few_kernel<T, 1, TOP><<<dim3((unsigned)shares), kCatThreads, 0, stream>>>(a); break;
+    case 2: catalog_few_kernel<T, 2, TOP><<<dim3((unsigned)shares), kCatThreads, 0, stream>>>(a); break;
+    case 4: catalog_few_kernel<T, 4, TOP><<<dim3((unsigned)shares), kCatThreads, 0, stream>>>(a); break;
+    default: catalog_few_kernel<T, 8, TOP><<<dim3((unsigned)shares), kCatThreads, 0, stream>>>(a);
+    }
+    return gs::check_launch("gs_catalog_fwd");
+}
+
+template <class T>
+int run_few(const FewArgs &a, int shares, int top, hipStream_t stream) {
+    return top == 32 ? launch_few<T, 32>(a, shares, stream) : top == 4 ? launch_few<T, 4>(a, shares, stream) : launch_few<T, 0>(a, shares, stream);
+}
+
+template <class T>
+int run_top(const TopArgs &t, const JoinArgs &j, hipStream_t stream) {
+    if (t.n_users <= 2 * kFewUsers) catalog_top_kernel<T, 1024><<<dim3((unsigned)t.n_users), 1024, 0, stream>>>(t, j);
+    else catalog_top_kernel<T, 256><<<dim3((unsigned)t.n_users), 256, 0, stream>>>(t, j);
+    return gs::check_launch("gs_catalog_fwd (best items)");
+}
+
 }  // namespace
 
 extern "C" size_t gs_catalog_workspace(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
@@ -601,51 +802,67 @@ extern "C" int gs_catalog_fwd(const void *user, int64_t n_users, const void *ite
     const int vector = ((uintptr_t)item & 15) == 0 && (dim * size) % 16 == 0;
     for (int64_t u0 = 0; u0 < n_users; u0 += cut.slice) {
         const int64_t nu = n_users - u0 < cut.slice ? n_users - u0 : cut.slice;
-        gs::Layout lu{}, li{};
-        lu.x = static_cast<const char *>(user) + (size_t)u0 * dim * size;
-        lu.n_rows = nu;
-        lu.rows = reinterpret_cast<uint4 *>(ws + sp.user);
-        if (u0 == 0) {
-            li.x = item; li.n_rows = n_items; li.bias = bias;
-            li.rows = reinterpret_cast<uint4 *>(ws + sp.item);
-            li.bias2 = reinterpret_cast<float *>(ws + sp.bias2);
-            li.tile_abs = tile_abs;
+        const void *users = static_cast<const char *>(user) + (size_t)u0 * dim * size;
+        const int32_t *aims = targets ? targets + u0 : nullptr;
+        float4 *part = reinterpret_cast<float4 *>(ws + sp.part);
+        float *group_max = top_k ? reinterpret_cast<float *>(ws + sp.group_max) : nullptr;
+        const int64_t group_stride = top_k ? group_stride_of(n_items, cut.top) : 0;
+        const int item_tiles = (int)gs::tiles_of(n_items);
+        int shares = 0, n_abs = item_tiles;
+        if (n_users <= kFewUsers) {
+            constexpr int W = gs::kCatThreads / 64;
+            shares = (int)((item_tiles + W - 1) / W < kBlocks ? (item_tiles + W - 1) / W : kBlocks);
+            n_abs = shares;
+            const FewArgs f{users, item, bias, aims, part, group_max, tile_abs, group_stride, n_items, (int)nu, dim, item_tiles, scale * gs::kLog2e};
+            if (shares)
+                if (int rc = dtype == GS_F32 ? run_few<float>(f, shares, cut.top, s) : dtype == GS_BF16 ? run_few<__bf16>(f, shares, cut.top, s)
+                                                                                     : run_few<_Float16>(f, shares, cut.top, s))
+                    return rc;
+        } else {
+            gs::Layout lu{}, li{};
+            lu.x = users;
+            lu.n_rows = nu;
+            lu.rows = reinterpret_cast<uint4 *>(ws + sp.user);
+            if (u0 == 0) {
+                li.x = item; li.n_rows = n_items; li.bias = bias;
+                li.rows = reinterpret_cast<uint4 *>(ws + sp.item);
+                li.bias2 = reinterpret_cast<float *>(ws + sp.bias2);
+                li.tile_abs = tile_abs;
+            }
+            if (int rc = gs::launch_layouts(lu, li, dim, dtype, s)) return rc;
+            FwdArgs a;
+            a.user = lu.rows;
+            a.item = reinterpret_cast<const uint4 *>(ws + sp.item);
+            a.bias2 = reinterpret_cast<const float *>(ws + sp.bias2);
+            a.targets = aims;
+            a.part = part;
+            a.group_max = group_max;
+            a.group_stride = group_stride;
+            a.n_users = nu; a.n_items = n_items;
+            a.user_tiles = (int)gs::tiles_of(nu); a.item_tiles = item_tiles;
+            shares_of(nu, n_items, cut.of, &a.group_blocks, &a.shares, &a.tiles_per_share);
+            a.scale2 = scale * gs::kLog2e;
+            if (n_items) {
+                shares = a.shares;
+                if (int rc = pieces == 1 ? launch_fwd<1>(a, blocks, cut.of, cut.top, s) : pieces == 2 ? launch_fwd<2>(a, blocks, cut.of, cut.top, s)
+                                                                                            : launch_fwd<3>(a, blocks, cut.of, cut.top, s))
+                    return rc;
+            }
         }
-        if (int rc = gs::launch_layouts(lu, li, dim, dtype, s)) return rc;
-        FwdArgs a;
-        a.user = reinterpret_cast<const uint4 *>(ws + sp.user);
-        a.item = reinterpret_cast<const uint4 *>(ws + sp.item);
-        a.bias2 = reinterpret_cast<const float *>(ws + sp.bias2);
-        a.targets = targets ? targets + u0 : nullptr;
-        a.part = reinterpret_cast<float4 *>(ws + sp.part);
-        a.group_max = top_k ? reinterpret_cast<float *>(ws + sp.group_max) : nullptr;
-        a.group_stride = top_k ? group_stride_of(n_items, cut.top) : 0;
-        a.n_users = nu; a.n_items = n_items;
-        a.user_tiles = (int)gs::tiles_of(nu); a.item_tiles = (int)gs::tiles_of(n_items);
-        shares_of(nu, n_items, cut.of, &a.group_blocks, &a.shares, &a.tiles_per_share);
-        a.scale2 = scale * gs::kLog2e;
-        if (n_items == 0) a.shares = 0;
-        else {
-            if (int rc = pieces == 1 ? launch_fwd<1>(a, blocks, cut.of, cut.top, s) : pieces == 2 ? launch_fwd<2>(a, blocks, cut.of, cut.top, s)
-                                                                                        : launch_fwd<3>(a, blocks, cut.of, cut.top, s))
-                return rc;
+        const JoinArgs j{part, shares, n_items, aims, log_prob ? log_prob + u0 : nullptr, entropy ? entropy + u0 : nullptr, lse ? lse + u0 : nullptr};
+        if (!top_k) {
+            catalog_join_kernel<<<dim3((unsigned)((nu + 3) / 4)), gs::kCatThreads, 0, s>>>(j, nu);
+            if (int rc = gs::check_launch("gs_catalog_fwd (join)")) return rc;
+            continue;
         }
-        float *lse_out = lse ? lse + u0 : reinterpret_cast<float *>(ws + sp.lse);
-        catalog_join_kernel<<<dim3((unsigned)((nu + 3) / 4)), gs::kCatThreads, 0, s>>>(
-            a.part, a.shares, nu, n_items, a.targets, log_prob ? log_prob + u0 : nullptr, entropy ? entropy + u0 : nullptr, lse_out);
-        if (int rc = gs::check_launch("gs_catalog_fwd (join)")) return rc;
-        if (!top_k) continue;
         TopArgs t;
-        t.user = static_cast<const char *>(user) + (size_t)u0 * dim * size;
-        t.item = item; t.bias = bias; t.group_max = a.group_max; t.tile_abs = tile_abs; t.lse = lse_out;
-        t.n_users = nu; t.n_items = n_items; t.group_stride = a.group_stride; t.dim = dim; t.item_tiles = a.item_tiles;
-        t.groups = a.item_tiles * (32 / cut.top); t.log2_items = cut.top == 4 ? 2 : 5; t.k = top_k;
+        t.user = users; t.item = item; t.bias = bias; t.group_max = group_max; t.tile_abs = tile_abs;
+        t.n_users = nu; t.n_items = n_items; t.group_stride = group_stride; t.dim = dim; t.n_abs = n_abs;
+        t.groups = item_tiles * (32 / cut.top); t.log2_items = cut.top == 4 ? 2 : 5; t.k = top_k;
         t.vector = vector;
         t.scale = scale; t.top_log_prob = top_log_prob + u0 * top_k; t.top_ids = top_ids + u0 * top_k;
-        if (dtype == GS_F32) catalog_top_kernel<float><<<dim3((unsigned)nu), 256, 0, s>>>(t);
-        else if (dtype == GS_BF16) catalog_top_kernel<__bf16><<<dim3((unsigned)nu), 256, 0, s>>>(t);
-        else catalog_top_kernel<_Float16><<<dim3((unsigned)nu), 256, 0, s>>>(t);
-        if (int rc = gs::check_launch("gs_catalog_fwd (best items)")) return rc;
+        if (int rc = dtype == GS_F32 ? run_top<float>(t, j, s) : dtype == GS_BF16 ? run_top<__bf16>(t, j, s) : run_top<_Float16>(t, j, s))
+            return rc;
     }
     return GS_OK;
 }

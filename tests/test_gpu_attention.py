@@ -362,3 +362,48 @@ def test_refusals(cuda):
                                                     inverse=(z(11, t=torch.int64), z(13, t=torch.int32))), ValueError)]:
         with pytest.raises(err):
             bad()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('heads,kv,dim,shared', [(1, 1, 64, True), (2, 1, 33, False), (5, 1, 100, True), (6, 3, 8, False), (4, 4, 256, True),
+                                                 (3, 1, 3, False), (1, 1, 1, True)])
+def test_gradients_of_many_rows_that_few_read(cuda, dtype, heads, kv, dim, shared):
+    """Lists of rows that are short on the mean: empty, of one entry, and a few read by so many that they are cut."""
+    c = _case(21, dtype, 600, heads, kv, dim, 3000, child=11, masked=0.05, shared=shared, offset=7)
+    ids = c['child_ids']
+    ids[::3] = torch.where(ids[::3] >= 0, 7 + 1234, ids[::3])         # row 1234: 2000 entries
+    ids[1::30] = 7 + 2999                                             # the last row: 220
+    _check(c)
+    lengths = torch.randint(0, 12, (500,), generator=torch.Generator().manual_seed(5)).tolist()
+    _check(_case(22, dtype, 500, heads, kv, dim, 9000, lengths=lengths, shared=shared))
+
+
+def test_edges_outside_the_lists_count_nowhere(cuda):
+    """child_ids may hold more than the lists of indptr name, on either side."""
+    for rows in (60, 4000):                                           # long and short lists of the rows
+        c = _case(23, torch.float32, 40, 2, 1, 64, rows, lengths=[30, 0, 700] + [5] * 37)
+        whole = _check(c)
+        more = lambda n, s: torch.randint(0, rows, (n,), generator=torch.Generator(device='cuda').manual_seed(s), device='cuda').to(torch.int32)
+        ids = torch.cat([more(333, 1), c['child_ids'], more(3000, 2)])
+        indptr = c['indptr'] + 333
+        out, lse = kernels.neighbor_attention(c['q'], c['k'], c['v'], ids, None, 0, None, indptr)
+        junk = torch.zeros(64 << 20, dtype=torch.uint8, device='cuda')        # what a workspace may find: parent 0 everywhere
+        del junk
+        g_q, g_k, g_v = kernels.neighbor_attention_bwd(c['q'], c['k'], c['v'], ids, None, out, lse, c['go'], 0, None, indptr)
+        want = _reference(c, 64 ** -0.5)
+        for name, got in zip(('out', 'lse', 'g_q', 'g_k', 'g_v'), (out, lse, g_q, g_k, g_v)):
+            _near(name, got, want[name])
+        assert len(whole) == 5
+
+
+@pytest.mark.parametrize('n', [1, 511, 513, 2000, 40000])
+def test_every_row_of_a_table_gets_its_gradient(cuda, n):
+    """Counts around the borders of how lists are shared out to be joined: all rows empty but the first and the last."""
+    k = torch.randn(n, 1, 16, device='cuda')
+    q = torch.randn(3, 1, 16, device='cuda')
+    ids = torch.tensor([0, n - 1, 0, n - 1, -1, 0], dtype=torch.int32, device='cuda')
+    out, lse = kernels.neighbor_attention(q, k, None, ids, 2)
+    g_k = torch.full_like(k, 7.0)
+    kernels.neighbor_attention_bwd(q, k, None, ids, 2, out, lse, torch.ones_like(q), g_k=g_k)
+    c = dict(q=q, k=k, v=None, go=torch.ones_like(q), child_ids=ids, child=2, indptr=None, offset=0, edges=6)
+    _near('g_k', g_k, _reference(c, 0.25)['g_k'])
