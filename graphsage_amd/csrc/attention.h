@@ -14,7 +14,7 @@
 // one load ahead: the next list's ids are on their way while this list's rows are used.
 //
 // Short lists of one length (a sampled batch) are the exception: there every L lanes take a list of their own, one row
-// after the other, and nothing has to be joined (102400 lists of 10 rows of 64 fp32: 52 us a list per wave, 37 us so).
+// after the other, and nothing has to be joined (short_lists below).
 //
 // Lists are dealt by edges: wave w takes the lists that begin in edges [w C, (w + 1) C) and, of a list longer than 4 C, the
 // part that lies in there, so that a popular parent's list is spread over the chip.  Every wave leaves a piece (maximum,
@@ -309,10 +309,16 @@ inline int lanes_for(int dim, int size) {
     return l;
 }
 
-// Lists of one length up to this many entries are taken by L lanes each (rows of 64 fp32: 102400 lists of 10, 42 us against
-// 59 a list per wave; 40000 of 24, 36 against 38, but 512 of 25, 6.5 against 5.4; 30000 of 32, 35 both ways, 500 of 32, 6.5
-// against 4.6).
-constexpr int64_t kShortList = 16;
+// Heads of one key head that a wave takes at once (a share of three fills four: 20000 lists of 10, gradients 139 us, 192 by twos).
+inline int heads_per_wave(int share) { return share >= 3 ? 4 : share; }
+
+// Lists of one length that L lanes take each.  Up to 12 entries always (500 lists of 10 rows of 64 fp32: 4.5 us against 5.4 a list
+// per wave; 102400: 42 against 59); with lists enough for every SIMD also longer ones, since a wave's end of a list costs more the more
+// heads it has (40000 lists, forward and backward, this against a list per wave: 20 of 64 fp32 125 us and 127, 32: 206 and
+// 199; two heads, 32 of 64 bf16: 126 and 143; four: 203 and 328).  500 lists of 25 leave most SIMDs idle: 18 us and 12.
+inline bool short_lists(int64_t n_lists, int64_t n_child, int heads_at_once) {
+    return n_child <= 12 || (n_lists >= 8192 && n_child <= (heads_at_once == 1 ? 20 : 32));
+}
 
 // Edges per wave, and whether any list may be cut.  Short: lists of one length, a list per `lanes` lanes.
 struct Deal {
@@ -320,9 +326,9 @@ struct Deal {
     bool pieces, is_short;
 };
 
-inline Deal deal_edges(const int64_t *indptr, int64_t n_lists, int64_t n_child, int64_t n_edges, int lanes) {
+inline Deal deal_edges(const int64_t *indptr, int64_t n_lists, int64_t n_child, int64_t n_edges, int lanes, int heads_at_once) {
     Deal d;
-    d.is_short = !indptr && n_child > 0 && n_child <= kShortList;
+    d.is_short = !indptr && n_child > 0 && short_lists(n_lists, n_child, heads_at_once);
     if (d.is_short) {
         // eight lists a group, if that leaves enough waves
         const int64_t lists = n_edges / n_child, groups = 64 / lanes;
@@ -350,8 +356,9 @@ inline Deal deal_edges(const int64_t *indptr, int64_t n_lists, int64_t n_child, 
 }
 
 // A table without rows leaves every parent without neighbors.
-inline Deal deal_edges(const gs_neighbors *nb, int lanes) {
-    return nb->n_rows ? deal_edges(nb->indptr, nb->n_parents, nb->n_child, nb->n_edges, lanes) : deal_edges(nullptr, 0, 0, 0, lanes);
+inline Deal deal_edges(const gs_neighbors *nb, int lanes, int share) {
+    const int g = heads_per_wave(share);
+    return nb->n_rows ? deal_edges(nb->indptr, nb->n_parents, nb->n_child, nb->n_edges, lanes, g) : deal_edges(nullptr, 0, 0, 0, lanes, g);
 }
 inline Neighbors device_neighbors(const gs_neighbors *nb) {
     if (!nb->n_rows) return Neighbors{nullptr, nb->ids, nb->n_parents, 0, 0, 0, 0};

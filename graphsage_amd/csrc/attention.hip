@@ -106,10 +106,12 @@ template <class T, int L, int G, bool SHARED> struct FwdState {
 // 1 / s; nothing to divide by: zeros; a NaN stays one
 __device__ __forceinline__ float inverse_of(float s) { return s > 0.f ? __builtin_amdgcn_rcpf(s) : s == 0.f ? 0.f : s; }
 
+// Two rows at a time for four heads, which have enough to do (2M edges of eight heads of 64 bf16, two a key head: 313 us, 342 with four
+// rows, of which a list's end leaves more unused).
 template <class T, int L, int G, bool SHARED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_fwd_kernel(FwdArgs a) {
-    constexpr int E = gs::Pack<T>::E, W = 64 / L, U = L == 2 ? 2 : gs::kAttnRows;
+    constexpr int E = gs::Pack<T>::E, W = 64 / L, U = L == 2 || G == 4 ? 2 : gs::kAttnRows;
     const int lane64 = threadIdx.x & 63, lane = lane64 & (L - 1), group = lane64 / L;
     const int share = a.heads / a.kv_heads;
     const int j = blockIdx.y / a.parts, h0 = j * share + (blockIdx.y % a.parts) * G;
@@ -342,7 +344,7 @@ template <class T, int L, bool SHARED>
 void launch_fwd(const FwdArgs &a, const gs::Deal &d, hipStream_t stream) {
     const int share = a.heads / a.kv_heads;
     FwdArgs b = a;
-    const int g = share >= 3 ? 4 : share;
+    const int g = gs::heads_per_wave(share);
     b.parts = (share + g - 1) / g;
     const dim3 grid((unsigned)((d.waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)(a.kv_heads * b.parts));
     if (d.is_short) {
@@ -378,7 +380,7 @@ size_t pieces_bytes(const gs::Deal &d, int heads, int dim, size_t *off_acc) {
 
 extern "C" size_t gs_neighbor_attention_workspace(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype) {
     if (gs::check_neighbors("gs_neighbor_attention_workspace", nb, heads, kv_heads, dim, dtype)) return 0;
-    const gs::Deal d = gs::deal_edges(nb, gs::lanes_for(dim, gs::dtype_size(dtype)));
+    const gs::Deal d = gs::deal_edges(nb, gs::lanes_for(dim, gs::dtype_size(dtype)), heads / kv_heads);
     return pieces_bytes(d, heads, dim, nullptr);
 }
 
@@ -391,7 +393,7 @@ extern "C" int gs_neighbor_attention_fwd(const void *q, const void *k, const voi
     const int size = gs::dtype_size(dtype), lanes = gs::lanes_for(dim, size);
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & (size - 1))
         return gs::fail(GS_EINVAL, "gs_neighbor_attention_fwd: pointer not aligned to its element");
-    const gs::Deal d = gs::deal_edges(nb, lanes);
+    const gs::Deal d = gs::deal_edges(nb, lanes, heads / kv_heads);
     size_t off_acc = 0;
     const size_t need = pieces_bytes(d, heads, dim, &off_acc);
     if (workspace_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 15))))

@@ -116,10 +116,12 @@ template <class T, int L, int G, bool SHARED> struct ParentState {
     }
 };
 
+// The parents' walk.  Two rows at a time for four heads, as in the forward pass (300 lists of 2000, four heads of 128 bf16, the whole
+// backward pass: 251 us, 326 with four rows).
 template <class T, int L, int G, bool SHARED>
 __global__ __launch_bounds__(gs::kAttnThreads)
 void attn_bwd_parents_kernel(BwdArgs a) {
-    constexpr int E = gs::Pack<T>::E, W = 64 / L, U = L == 2 ? 2 : gs::kAttnRows;
+    constexpr int E = gs::Pack<T>::E, W = 64 / L, U = L == 2 || G == 4 ? 2 : gs::kAttnRows;
     const int lane64 = threadIdx.x & 63, lane = lane64 & (L - 1), group = lane64 / L;
     const int share = a.heads / a.kv_heads;
     const int j = blockIdx.y / a.parts, h0 = j * share + (blockIdx.y % a.parts) * G;
@@ -558,11 +560,9 @@ void attn_bwd_dense_kernel(BwdArgs a) {
     }
 }
 
-int heads_per_wave(int share) { return share >= 3 ? 4 : share; }
-
 template <class T, int L, bool SHARED>
 void launch_parents(const BwdArgs &a, const gs::Deal &d, hipStream_t stream) {
-    const int g = heads_per_wave(a.heads / a.kv_heads);
+    const int g = gs::heads_per_wave(a.heads / a.kv_heads);
     const dim3 grid((unsigned)((d.waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)(a.kv_heads * a.parts));
     if (d.is_short) {
         if (g == 1) attn_bwd_short_kernel<T, L, 1, SHARED><<<grid, gs::kAttnThreads, 0, stream>>>(a);
@@ -575,7 +575,7 @@ void launch_parents(const BwdArgs &a, const gs::Deal &d, hipStream_t stream) {
 
 template <class T, int L, bool SHARED>
 void launch_rows(const BwdArgs &a, const gs::Deal &d, hipStream_t stream) {
-    const int g = heads_per_wave(a.heads / a.kv_heads);
+    const int g = gs::heads_per_wave(a.heads / a.kv_heads);
     const int64_t waves = d.is_short ? (d.waves + 64 / L - 1) / (64 / L) : d.waves;
     const dim3 grid((unsigned)((waves + gs::kAttnThreads / 64 - 1) / (gs::kAttnThreads / 64)), (unsigned)a.kv_heads);
     if (d.is_short) {
@@ -599,7 +599,7 @@ constexpr int64_t kShortMean = 4;
 
 gs::Deal deal_rows(int64_t n_rows, int64_t n_inv, int lanes) {
     static const int64_t ragged = 0;                // any address: the rows' lists are ragged
-    gs::Deal d = gs::deal_edges(&ragged, n_rows, 0, n_inv, lanes);
+    gs::Deal d = gs::deal_edges(&ragged, n_rows, 0, n_inv, lanes, 1);
     d.is_short = n_inv && n_inv <= kShortMean * n_rows;
     if (d.is_short) {
         // 16 entries a run (96000 entries: 16.4 us, 19.1 with 8; 360 000 of 256 bf16: 87 us, 104), 8 where there are few
@@ -615,8 +615,8 @@ gs::Deal deal_rows(int64_t n_rows, int64_t n_inv, int lanes) {
 Plan make_plan(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype, int64_t n_inv) {
     Plan p;
     const int lanes = gs::lanes_for(dim, gs::dtype_size(dtype)), share = heads / kv_heads;
-    p.parts = (share + heads_per_wave(share) - 1) / heads_per_wave(share);
-    p.parents = gs::deal_edges(nb, lanes);
+    p.parts = (share + gs::heads_per_wave(share) - 1) / gs::heads_per_wave(share);
+    p.parents = gs::deal_edges(nb, lanes, share);
     p.rows = deal_rows(nb->n_rows, nb->ids && nb->n_rows && nb->n_parents ? n_inv : 0, lanes);
     size_t off = gs::align256((size_t)nb->n_parents * heads * sizeof(float));        // delta
     p.off_parent = off;
