@@ -602,9 +602,10 @@ gs::Deal deal_rows(int64_t n_rows, int64_t n_inv, int lanes) {
     gs::Deal d = gs::deal_edges(&ragged, n_rows, 0, n_inv, lanes, 1);
     d.is_short = n_inv && n_inv <= kShortMean * n_rows;
     if (d.is_short) {
-        // 16 entries a run (96000 entries: 16.4 us, 19.1 with 8; 360 000 of 256 bf16: 87 us, 104), 8 where there are few
-        // (16000: 7.6 us, 14.0 with 16), 131072 runs at most (each may leave two pieces)
-        d.chunk = n_inv > 65536 ? 16 : 8;
+        // runs for two waves per SIMD, of 2 to 16 entries (7600 entries of 16 fp32: 22 us with 8, 9 with 2; 96000 of 64: 19 us with 8,
+        // 16 with 16; 360 000 of 256 bf16: 104 and 87), 131072 runs at most (each may leave two pieces)
+        d.chunk = n_inv / (2048 * (64 / lanes));
+        d.chunk = d.chunk < 2 ? 2 : d.chunk > 16 ? 16 : d.chunk;
         if (d.chunk < (n_inv + 131071) / 131072) d.chunk = (n_inv + 131071) / 131072;
         d.waves = (n_inv + d.chunk - 1) / d.chunk;  // runs, here
     }
