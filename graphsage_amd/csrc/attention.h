@@ -386,11 +386,16 @@ struct JoinLanes {
 };
 constexpr int kJoinFlight = 8;                      // pieces of a lane on their way
 // A joining launch: y a vector, z 64 elements of it.  List x of block b is x * blocks + b (popular lists tend to be neighbors),
-// and wave x % kJoinWaves looks after it: one list a block while there are few, 512 blocks until a lane has one each (100 000
-// lists, most of them empty: 8 us, 32 us in blocks of 64 lists).
+// and wave x % kJoinWaves looks after it: one list a block while there are few, then about 2048 blocks in all, 512 for a vector at
+// most, until a lane has one each (100 000 lists, most of them empty: 8 us, 32 us in blocks of 64 lists; 1053 lists for twelve
+// heads of 200: 67 us with 512 for each of the 48).
 inline dim3 join_grid(int64_t lists, int vectors, int dim) {
-    const int64_t full = (lists + 64 * kJoinWaves - 1) / (64 * kJoinWaves), few = lists < 512 ? lists : 512;
-    return dim3((unsigned)(full > few ? full : few), (unsigned)vectors, (unsigned)((dim + 63) / 64));
+    const int columns = (dim + 63) / 64;
+    const int64_t full = (lists + 64 * kJoinWaves - 1) / (64 * kJoinWaves);
+    int64_t few = 2048 / ((int64_t)vectors * columns);
+    few = few < 16 ? 16 : few > 512 ? 512 : few;
+    if (few > lists) few = lists;
+    return dim3((unsigned)(full > few ? full : few), (unsigned)vectors, (unsigned)columns);
 }
 __device__ __forceinline__ int64_t join_list(int wave, int lane) { return (int64_t)(lane * kJoinWaves + wave) * gridDim.x + blockIdx.x; }
 // The lists of a block that take all its waves, in any order.

@@ -568,17 +568,36 @@ void catalog_top_kernel(TopArgs a, JoinArgs join) {
     if (thr != thr) thr = -INFINITY;
 
     const auto better = [](double v, int32_t i, double w, int32_t j) { return v > w || (v == w && i < j); };
-    // keeps the k best of the buffer, in order
+    // keeps the k best of the buffer, in order: by rank where there are few, by a bitonic sort else (6 users, the 64 best of 1082
+    // items of 64 bf16: 114 us by rank)
     const auto compress = [&]() {
         __syncthreads();
         const int c = n_val;
-        for (int i = tid; i < c; i += N) {
-            const double v = val[i];
-            const int32_t at = id[i];
-            int r = 0;
+        if (c <= 128) {
+            for (int i = tid; i < c; i += N) {
+                const double v = val[i];
+                const int32_t at = id[i];
+                int r = 0;
 #pragma unroll 4
-            for (int j = 0; j < c; ++j) r += better(val[j], id[j], v, at);
-            if (r < a.k) { best_val[r] = v; best_id[r] = at; }
+                for (int j = 0; j < c; ++j) r += better(val[j], id[j], v, at);
+                if (r < a.k) { best_val[r] = v; best_id[r] = at; }
+            }
+        } else {
+            int p = 256;
+            while (p < c) p *= 2;                   // at most kBuf
+            for (int i = c + tid; i < p; i += N) { val[i] = -INFINITY; id[i] = 0x7fffffff; }
+            __syncthreads();
+            for (int size = 2; size <= p; size *= 2)
+                for (int step = size / 2; step; step /= 2) {
+                    for (int t = tid; t < p / 2; t += N) {
+                        const int i = 2 * t - (t & (step - 1)), j = i + step;
+                        const double v = val[i], w = val[j];
+                        const int32_t vi = id[i], wi = id[j];
+                        if ((i & size) ? better(v, vi, w, wi) : better(w, wi, v, vi)) { val[i] = w; id[i] = wi; val[j] = v; id[j] = vi; }
+                    }
+                    __syncthreads();
+                }
+            if (tid < a.k) { best_val[tid] = val[tid]; best_id[tid] = id[tid]; }       // (k <= 64 < c)
         }
         __syncthreads();
         const int kept = min(c, a.k);
