@@ -8,8 +8,8 @@
 // the elements it shares with its neighbor count there alone.
 //
 // A wave works on one list (the neighbors of one parent) at a time: control flow and list bounds are scalar, lists of any
-// length leave no lane waiting for another lane's list (measured against a list per L lanes: the ragged whole graph, 2M
-// edges, 768 -> 303 us), and the running softmax of each of the 64 / L row groups is joined at the end of the list by
+// length leave no lane waiting for another lane's list (2M ragged edges of eight heads: 840 us with a list per L lanes, 528 us
+// with the first form of this), and the running softmax of each of the 64 / L row groups is joined at the end of the list by
 // half-wave and quarter-wave swaps that leave every lane the results it stores.  Entries come 64 at a time, one a lane,
 // one load ahead: the next list's ids are on their way while this list's rows are used.
 //

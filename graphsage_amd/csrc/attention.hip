@@ -1,8 +1,9 @@
 // Attention of every parent over its neighbors, forward (the dealing of edges: attention.h).
 //
-// Bound by the row gathers: an edge costs one row of dim elements (two with separate values) and, per head, dim
-// multiply-adds for the score and as many for the sum, about a fifth of what the vector ALU does in the time the row
-// takes to arrive.  Scores are kept in units of log 2 (scale * log2 e goes into the query), so an exponential is one
+// An edge costs one row of dim elements (two with separate values) and, per head, dim multiply-adds for the score and as
+// many for the sum.  One head is bound by the row gathers: 1 024 000 rows of 64 fp32 in lists of 10 take 37 us, 7.0 TB/s out of
+// the caches (their mean, which gathers the same rows, 34 us).  Four heads a key head keep the vector ALU busy two thirds of the
+// time, the rest is the ends of lists: 2M ragged edges of eight heads of 64 bf16, 4M row pairs, take 308 us.  Scores are kept in units of log 2 (scale * log2 e goes into the query), so an exponential is one
 // instruction.
 #include "attention.h"
 

@@ -8,6 +8,10 @@
 // as they pass.  For rows read by id the rows' walk is the same with the roles exchanged: the row's keys and values
 // stay in registers and the queries and g_out of the edges that read it arrive, so a row's gradient is summed in registers
 // in the order of its list, and no atomics are needed.
+//
+// 8192 dense lists of 25 rows of 32 fp32, four heads: 24 us (the forward 12 us, most of it launch and latency).  226 000 ragged edges
+// into 3700 rows of 2 x 33 fp16: parents 38 us, rows 30 us, each with a join of 7 to 9 us; the tables lie in the caches and
+// what bounds both walks is the work per list (3700 to 6040 lists of 40 to 60 edges) and its latency.
 #include "attention.h"
 
 namespace {

@@ -2,7 +2,7 @@
 //
 //     dz[n][j] = p_j (A_n + B_n log p_j) + [j = target_n] g_n,   A = -(g + g_entropy entropy),  B = -g_entropy
 //     g_user = scale dz item,   g_item = scale dz^T user,   g_bias = column sums of dz
-// Two launches of one kernel.  A wave owns 32 rows of one table and streams tiles of the other: the tile product gives
+// One launch for both tables.  A wave owns 32 rows of one table and streams tiles of the other: the tile product gives
 // it 32 x 32 scores with its own row in the lane, dz is formed in place, cut into as many bf16 pieces as the tables'
 // elements have (which leaves out 2^-8 of an element for bf16 tables, 2^-16 for fp16, nothing for fp32; many elements add up
 // to a result that is itself rounded to the tables' type) and multiplied, pieces i and k with i + k below their number,
@@ -10,6 +10,9 @@
 // g, stays out of that: its term is added whole, in the join for users, in a rare branch for items.  Nothing of the scores
 // or dz goes through memory; the scores are computed twice.  The streamed table is cut into shares so that the launch fills
 // the chip; the shares' sums are added in share order by a second launch.
+//
+// 4096 users, 100 000 items of 64 bf16: 300 to 385 us for 105 + 52 GFLOP (scores twice, two gradients), bound by the vector ALU, which
+// forms 2 x 410M dz at an exponential and about ten more instructions each while the matrix cores wait.
 #include "catalog.h"
 
 namespace {
