@@ -6,6 +6,10 @@ of the reference model (they are inputs, not variables, ``models.py:241``), so
 the indexed gather-mean only propagates a gradient into the table when the
 table itself requires one (trainable embeddings); then it is the float-atomic
 scatter-add kernel.
+
+A backward pass may be captured into a HIP graph.  Results of eager calls on the
+same leaves have to be gone by then: torch's engine would wait for the stream
+they ran on, which a capture does not survive.
 """
 import torch
 

@@ -376,7 +376,7 @@ void attn_bwd_rows_short_kernel(BwdArgs a) {
         t.row = edge < a.nb.n_edges ? a.nb.row_of(id) : -1;
         t.parent = t.row >= 0 && (uint64_t)(int64_t)p < (uint64_t)a.nb.n_parents ? p : -1;
         lists.range(max(t.row, 0), t.begin, t.end);
-        if (t.row < 0) { t.begin = e; t.end = e + 1; }
+        if (t.row < 0 || e < t.begin || e >= t.end) { t.row = t.parent = -1; t.begin = e; t.end = e + 1; }    // (in no row's list)
         return t;
     };
     // from the end of a list that another has begun and keeps, to the end of the last one that begins here

@@ -26,6 +26,7 @@ Two execution paths produce the same numbers:
 Two arguments beyond the reference's: ``agg_option='attention'`` with ``heads`` (``Aggregator``), and ``dropout_seed``.
 Without it dropout draws from torch's generator and torch keeps the masks; with it every mask is a function of the seed
 and of how much has been drawn before (``gs_dropout``), drawn again in the backward pass and never stored.
+(What has been drawn is counted on the host: a step that is captured into a graph replays its masks.)
 """
 import itertools as it
 import operator as op

@@ -15,6 +15,7 @@ matrices, zero bias).  The arithmetic runs in two HIP kernels: the neighbor mean
 neighbors: ``heads`` queries ``x_self @ w_query`` as wide as a neighbor's features, scores against the features themselves, and the
 weighted features of all heads side by side go into ``w_neigh``, which has ``heads`` times as many rows.  The neighbors'
 rows are read once, by id where they come from a feature table, and serve as keys and values of every head.
+Rows of at most 256 columns; wider ones are refused when the model runs.
 """
 import collections.abc
 import math

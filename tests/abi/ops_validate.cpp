@@ -35,7 +35,7 @@ int main() {
     void *p = arena, *odd = arena + 1;
     int32_t *i32 = reinterpret_cast<int32_t *>(arena + 1024);
     int64_t *i64 = reinterpret_cast<int64_t *>(arena + 2048);
-    uint64_t *u64 = reinterpret_cast<uint64_t *>(arena + 3072);
+    uint64_t *u64 = reinterpret_cast<uint64_t *>(arena + 4096);
 
     // ---- dropout ----
     ACCEPTED(gs_dropout(nullptr, 0, GS_F32, 0.5, 1, nullptr, 0, nullptr, nullptr));
@@ -47,7 +47,7 @@ int main() {
     REFUSED(GS_EINVAL, gs_dropout(nullptr, 8, GS_F32, 0.5, 1, nullptr, 0, p, nullptr));
     REFUSED(GS_EINVAL, gs_dropout(p, 8, GS_F32, 0.5, 1, nullptr, 0, nullptr, nullptr));
     REFUSED(GS_EINVAL, gs_dropout(odd, 8, GS_BF16, 0.5, 1, nullptr, 0, p, nullptr));
-    REFUSED(GS_EINVAL, gs_dropout(p, 8, GS_F16, 0.5, 1, reinterpret_cast<uint64_t *>(arena + 3076), 0, p, nullptr));
+    REFUSED(GS_EINVAL, gs_dropout(p, 8, GS_F16, 0.5, 1, reinterpret_cast<uint64_t *>(arena + 4100), 0, p, nullptr));
     REFUSED(GS_EINVAL, gs_dropout(p, 64, GS_F32, 0.5, 1, u64, 0, arena + 64, nullptr));          // in part the same memory
     REFUSED(GS_ELIMIT, gs_dropout(p, INT64_MAX / 4, GS_BF16, 0.5, 1, nullptr, 0, p, nullptr));
 

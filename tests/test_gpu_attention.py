@@ -407,3 +407,18 @@ def test_every_row_of_a_table_gets_its_gradient(cuda, n):
     kernels.neighbor_attention_bwd(q, k, None, ids, 2, out, lse, torch.ones_like(q), g_k=g_k)
     c = dict(q=q, k=k, v=None, go=torch.ones_like(q), child_ids=ids, child=2, indptr=None, offset=0, edges=6)
     _near('g_k', g_k, _reference(c, 0.25)['g_k'])
+
+
+@pytest.mark.parametrize('rows', [40, 4000])
+def test_inverse_lists_that_are_part_of_larger_ones(cuda, rows):
+    """Entries before the first row's list and behind the last one's are no row's, whatever they name."""
+    c = _case(24, torch.float32, 300, 2, 1, 32, rows, child=6)
+    out, lse = kernels.neighbor_attention(c['q'], c['k'], c['v'], c['child_ids'], 6)
+    indptr, edges = kernels.neighbor_inverse(c['child_ids'], rows)
+    n = int(indptr[-1])
+    moved = torch.cat([edges[50:150], edges[:n], edges[:30]])
+    args = (c['q'], c['k'], c['v'], c['child_ids'], 6, out, lse, c['go'])
+    g_q, g_k, g_v = kernels.neighbor_attention_bwd(*args, inverse=(indptr + 100, moved))
+    want = _reference(c, 32 ** -0.5)
+    for name, got in (('g_q', g_q), ('g_k', g_k), ('g_v', g_v)):
+        _near(name, got, want[name])
