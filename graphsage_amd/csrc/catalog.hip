@@ -309,9 +309,10 @@ void catalog_fwd_kernel(FwdArgs a) {
     }
 }
 
-// A few users: one wave has them all, so every item row is used once and laying the table out would cost more than the
-// product.  The waves read the rows as they are, eight elements a lane, and cut them into pieces in registers (one user, 100 000
-// items of 32 fp32: 10.5 us; 12 us to lay the items out and 11 us for their product else).
+// A few users: a block has them all, 32 a wave, so an item row is used by few waves and laying the table out would cost more than
+// that saves.  The waves read the rows as they are, eight elements a lane, and cut them into pieces in registers (one user, 100 000
+// items of 32 fp32: 10.5 us; 12 us to lay the items out and 11 us for their product else).  With less than 33 users the four
+// waves take a tile of items each, with less than 65 two, else all the same one.
 struct FewArgs {
     const void *user, *item;
     const float *bias;
@@ -325,7 +326,7 @@ struct FewArgs {
 
 // Elements 16 kc + 8 half + 0 .. 7 of a row for all kc, zeros for those past its end: the last eight lie elsewhere among the eight,
 // but in the same places for every row.  All loads leave before the first is used: four of them share a line that other waves
-// would drive out of the first cache (5 users, 73 000 items of 256 bf16: 46 us, 61 one after the other).
+// would drive out of the first cache (5 users, 73 000 items of 256 bf16, if taken so: 46 us, 61 one after the other).
 template <class T, int KC> struct RawRow {
     T x[KC][8];
     __device__ __forceinline__ void load(const T *row, int half, int dim) {
@@ -354,21 +355,24 @@ void catalog_few_kernel(FewArgs a) {
     __shared__ float4 sums[W][32];
     __shared__ float tops[W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 31, half = lane >> 5;
+    const int user_tiles = (a.n_users + 31) / 32, at_once = max(W / user_tiles, 1);        // tiles of items a block has at once
+    const int n = wave % user_tiles * 32 + r;       // the user of this lane
     Fragment<P> own[KC];
-    const T *U = static_cast<const T *>(a.user) + (int64_t)min(r, a.n_users - 1) * a.dim;
+    const T *U = static_cast<const T *>(a.user) + (int64_t)min(n, a.n_users - 1) * a.dim;
     RawRow<T, KC> raw;
     raw.load(U, half, a.dim);
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = r < a.n_users ? raw.at(kc, i, half, a.dim) : 0.f;
+        for (int i = 0; i < 8; ++i) v[i] = n < a.n_users ? raw.at(kc, i, half, a.dim) : 0.f;
         cut_pieces<P>(v, own[kc].p);
     }
-    int target = a.targets && r < a.n_users ? a.targets[r] : -1;
+    int target = a.targets && n < a.n_users ? a.targets[n] : -1;
     if (target >= a.n_items) target = -1;
     float m = kFloor, s = 0.f, w = 0.f, hit = -INFINITY, most_abs = 0.f;
-    for (int t = blockIdx.x * W + wave; t < a.item_tiles; t += gridDim.x * W) {
+    const int first = wave < at_once * user_tiles ? blockIdx.x * at_once + wave / user_tiles : a.item_tiles;
+    for (int t = first; t < a.item_tiles; t += gridDim.x * at_once) {
         const int64_t row = min((int64_t)t * 32 + r, a.n_items - 1);
         raw.load(static_cast<const T *>(a.item) + row * a.dim, half, a.dim);
         const bool on = !(a.bias && a.bias[row] < kOffer);
@@ -408,12 +412,12 @@ void catalog_few_kernel(FewArgs a) {
             if (target >= 0 && local == row_of_reg(i, lane)) hit = z[i];
         if (TOP == 32) {
             const float most = half_max(top);
-            if (lane < 32 && r < a.n_users) a.group_max[r * a.group_stride + t] = most;
+            if (lane < 32 && n < a.n_users) a.group_max[n * a.group_stride + t] = most;
         } else if (TOP == 4) {
-            if (r < a.n_users)
+            if (n < a.n_users)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    a.group_max[r * a.group_stride + (int64_t)t * 8 + 2 * q + half] =
+                    a.group_max[n * a.group_stride + (int64_t)t * 8 + 2 * q + half] =
                         fmaxf(fmaxf(z[4 * q], z[4 * q + 1]), fmaxf(z[4 * q + 2], z[4 * q + 3]));
         }
         const float m1 = fmaxf(m, top), step = m - m1, keep = fast_exp2(step);
@@ -430,7 +434,7 @@ void catalog_few_kernel(FewArgs a) {
         s += (sp[0] + sp[1]) + (sp[2] + sp[3]);
         w += (wp[0] + wp[1]) + (wp[2] + wp[3]);
     }
-    // the two lanes of a user, then the four waves
+    // the two lanes of a user, then the waves that have it
     const float m1 = half_max(m), step = m - m1, keep = fast_exp2(step);
     const float s1 = s * keep, w1 = keep * (w + s * step);
     const float s2 = s1 + __shfl_xor(s1, 32, 64), w2 = w1 + __shfl_xor(w1, 32, 64);
@@ -443,11 +447,11 @@ void catalog_few_kernel(FewArgs a) {
     }
     __syncthreads();
     if (threadIdx.x >= a.n_users) return;
-    float4 q = sums[0][r];
-#pragma unroll
-    for (int k = 1; k < W; ++k) q = join_sums(q, sums[k][r]);
-    a.part[(size_t)r * gridDim.x + blockIdx.x] = q;
-    if (TOP && r == 0) a.tile_abs[blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const int mine = threadIdx.x;
+    float4 q = sums[mine >> 5][mine & 31];
+    for (int k = 1; k < at_once; ++k) q = join_sums(q, sums[k * user_tiles + (mine >> 5)][mine & 31]);
+    a.part[(size_t)mine * gridDim.x + blockIdx.x] = q;
+    if (TOP && mine == 0) a.tile_abs[blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 }
 
 // What the shares of a user leave, and where it goes (nullable, one entry a user).
@@ -682,8 +686,14 @@ int64_t group_stride_of(int64_t n_items, int top) { return (tiles_of(n_items) * 
 
 constexpr int64_t kBlocks = 1024;                   // blocks a launch is cut into: four waves per SIMD
 
-// Users of one wave.
-constexpr int64_t kFewUsers = 32;
+// Whether a block has all users at once and the tables stay as they are (this against laid-out tables): 100 users, 3700 items of 32
+// fp32 9.1 us and 11.8; 64 users, 100 000 items of 64 bf16 22 and 26, but 128 users 32 and 26.  Wide rows are fetched in
+// pieces of lines and pay only where fp32 would be laid out as three pieces (5 users, 73 000 items of 200 fp32: 60 us and 75;
+// of 256 bf16: 46 and 37; 100 users, 50 000 items of 128 fp32: 61 and 32).
+inline bool few_users(int64_t n_users, int64_t n_items, int dim, int dtype) {
+    if (dim > 64) return n_users <= 32 && dtype == GS_F32;
+    return n_users <= 64 || (n_users <= 128 && n_items <= 16384);
+}
 
 // How a call is cut: users in slices that bound the table of tile maxima, a slice in waves.
 struct Cut {
@@ -734,7 +744,7 @@ Space space_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) 
     int blocks, shares, per;
     shares_of(c.slice, n_items, c.of, &blocks, &shares, &per);
     size_t off = 0;
-    const bool few = n_users <= kFewUsers;          // lays nothing out
+    const bool few = few_users(n_users, n_items, dim, dtype);        // lays nothing out
     s.user = off; off += few ? 0 : align256(layout_bytes(c.slice, dim, dtype));
     s.item = off; off += few ? 0 : align256(layout_bytes(n_items, dim, dtype));
     s.bias2 = off; off += few ? 0 : align256((size_t)tiles_of(n_items) * 32 * sizeof(float));
@@ -785,11 +795,13 @@ int launch_fwd(const FwdArgs &a, int blocks, int of, int top, hipStream_t stream
 
 template <class T, int TOP>
 int launch_few(const FewArgs &a, int shares, hipStream_t stream) {
-    switch (gs::blocks_of(a.dim)) {
-    case 1: catalog_few_kernel<T, 1, TOP><<<dim3((unsigned)shares), kCatThreads, 0, stream>>>(a); break;
-    case 2: catalog_few_kernel<T, 2, TOP><<<dim3((unsigned)shares), kCatThreads, 0, stream>>>(a); break;
-    case 4: catalog_few_kernel<T, 4, TOP><<<dim3((unsigned)shares), kCatThreads, 0, stream>>>(a); break;
-    default: catalog_few_kernel<T, 8, TOP><<<dim3((unsigned)shares), kCatThreads, 0, stream>>>(a);
+    const int blocks = gs::blocks_of(a.dim);
+    const dim3 grid((unsigned)shares);
+    if (blocks == 1) catalog_few_kernel<T, 1, TOP><<<grid, kCatThreads, 0, stream>>>(a);
+    else if (blocks == 2) catalog_few_kernel<T, 2, TOP><<<grid, kCatThreads, 0, stream>>>(a);
+    if constexpr (Pieces<T>::P == 3) {              // (wider rows: few_users)
+        if (blocks == 4) catalog_few_kernel<T, 4, TOP><<<grid, kCatThreads, 0, stream>>>(a);
+        else if (blocks == 8) catalog_few_kernel<T, 8, TOP><<<grid, kCatThreads, 0, stream>>>(a);
     }
     return gs::check_launch("gs_catalog_fwd");
 }
@@ -848,9 +860,10 @@ extern "C" int gs_catalog_fwd(const void *user, int64_t n_users, const void *ite
         const int64_t group_stride = top_k ? group_stride_of(n_items, cut.top) : 0;
         const int item_tiles = (int)gs::tiles_of(n_items);
         int shares = 0, n_abs = item_tiles;
-        if (n_users <= kFewUsers) {
-            constexpr int W = gs::kCatThreads / 64;
-            shares = (int)((item_tiles + W - 1) / W < kBlocks ? (item_tiles + W - 1) / W : kBlocks);
+        if (few_users(n_users, n_items, dim, dtype)) {
+            const int user_tiles = (int)gs::tiles_of(nu), at_once = user_tiles == 1 ? 4 : user_tiles == 2 ? 2 : 1;
+            const int all = (item_tiles + at_once - 1) / at_once;
+            shares = all < kBlocks ? all : (int)kBlocks;
             n_abs = shares;
             const FewArgs f{users, item, bias, aims, part, group_max, tile_abs, group_stride, n_items, (int)nu, dim, item_tiles, scale * gs::kLog2e};
             if (shares)

@@ -343,3 +343,10 @@ def test_refusals(cuda):
                      (lambda: kernels.catalog_log_probs_bwd(u, e, t, b, 1.0, z(5), z(4)), ValueError)]:
         with pytest.raises(err):
             bad()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('users', [1, 31, 32, 33, 63, 64, 65, 96, 97, 128, 129])
+def test_counts_of_users_around_the_tiles_of_a_block(cuda, dtype, users):
+    for items, dim, k in ((1, 5, 1), (130, 64, 20), (2100, 33, 5)):
+        _check(*_case(users + items, dtype, users, items, dim), top=k)
