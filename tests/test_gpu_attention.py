@@ -422,3 +422,12 @@ def test_inverse_lists_that_are_part_of_larger_ones(cuda, rows):
     want = _reference(c, 32 ** -0.5)
     for name, got in (('g_q', g_q), ('g_k', g_k), ('g_v', g_v)):
         _near(name, got, want[name])
+
+
+@pytest.mark.parametrize('heads,kv', [(1, 1), (2, 1), (4, 1), (6, 2)])
+@pytest.mark.parametrize('child,dim,dtype', [(13, 64, torch.float32), (20, 3, torch.float32), (32, 16, torch.bfloat16), (25, 33, torch.float16),
+                                             (21, 32, torch.float32)])
+def test_many_lists_of_one_length(cuda, heads, kv, child, dim, dtype):
+    """Enough lists that several share a wave, of lengths around where that begins and ends."""
+    for ids in (True, False):
+        _check(_case(25, dtype, 8195, heads, kv, dim, 900 if ids else 8195 * child, child=child, ids=ids, shared=dim != 33))
