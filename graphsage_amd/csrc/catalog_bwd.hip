@@ -5,11 +5,16 @@
 // One launch for both tables.  A wave owns 32 rows of one table and streams tiles of the other: the tile product gives
 // it 32 x 32 scores with its own row in the lane, dz is formed in place, cut into as many bf16 pieces as the tables'
 // elements have (which leaves out 2^-8 of an element for bf16 tables, 2^-16 for fp16, nothing for fp32; many elements add up
-// to a result that is itself rounded to the tables' type) and multiplied, pieces i and k with i + k below their number,
-// with the same streamed rows, cols layout, into the accumulators of the 32 gradients.  The one large element of a row, the target's
-// g, stays out of that: its term is added whole, in the join for users, in a rare branch for items.  Nothing of the scores
+// to a result that is itself rounded to the tables' type) and multiplied, pieces i and k with i + k <= 2,
+// with the same streamed rows, cols layout, into the accumulators of the 32 gradients.  Nothing of the scores
 // or dz goes through memory; the scores are computed twice.  The streamed table is cut into shares so that the launch fills
 // the chip; the shares' sums are added in share order by a second launch.
+//
+// Targets: where one is predicted well, g and -g p cancel, and what a cut leaves out of -g p would stand where g (1 - p) should
+// (bf16: 2^-9 of g against the 1e-4 of it that p = 0.9999 leaves).  So a tile that holds targets is followed by a second product
+// of matrices that are zero elsewhere: g and what the cut left of -g p, in three pieces.  The sum then lacks nothing but fp32
+// roundings of g.  All targets of a tile cost one such product (4096 users and items of 32 fp32, every user's target an item of its
+// own: 47 us with the call, 75 us with a loop over the targets; all the same item: 49 and 106 us).
 //
 // 4096 users, 100 000 items of 64 bf16: 300 to 385 us for 105 + 52 GFLOP (scores twice, two gradients), bound by the vector ALU, which
 // forms 2 x 410M dz at an exponential and about ten more instructions each while the matrix cores wait.
@@ -43,7 +48,7 @@ template <int P, int DB> constexpr bool kStaged = fits_lds(kTile<P, DB, false>);
 
 template <class T, int DB, bool USERS>
 __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uint32_t block, uint4 *stage) {
-    constexpr int P = Pieces<T>::P, KC = 2 * DB, NZ = P, MOST = P - 1, W = kCatThreads / 64;
+    constexpr int P = Pieces<T>::P, KC = 2 * DB, W = kCatThreads / 64;
     constexpr int F = kTile<P, DB, USERS>, ST = kStaged<P, DB> ? tiles_per_stage(F) : 1;
     constexpr bool STAGED = kStaged<P, DB>;
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -76,11 +81,13 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
 #pragma unroll
         for (int kc = 0; kc < KC; ++kc) own[kc] = load_fragment<P>(src, kc, lane);
     }
-    float lse2 = 0.f, ca = 0.f, cb = 0.f, bias = 0.f, sum = 0.f;
+    float lse2 = 0.f, ca = 0.f, cb = 0.f, bias = 0.f, sum = 0.f, g = 0.f;
+    int target = -1;
     if (USERS) {
         const Stats &st = a.stats[tile];
         const int i = lane & 31;
         lse2 = st.lse2[i]; ca = st.a[i]; cb = st.b2[i];
+        g = st.g[i]; target = st.target[i];
     } else bias = a.bias2[mine];
     f32x16 out[DB];
 #pragma unroll
@@ -139,33 +146,42 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            bf16x8 z[NZ];
-            cut_pieces<NZ>(dz + 8 * h, z);
+            bf16x8 z[P];
+            cut_pieces<P>(dz + 8 * h, z);           // (dz keeps what is left of it: nothing of fp32)
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 const Fragment<P> ct = load_fragment<P>(cols, h * DB + d, lane);
-                multiply<NZ, P, MOST>(out[d], z, ct.p);
+                multiply<P, P, 2>(out[d], z, ct.p);
             }
         }
-        if (!USERS) {
-            // the terms of targets, whole: rarely in this tile
-            const int tg = st->target[lane & 31];
-            for (uint32_t todo = (uint32_t)__ballot(tg >= 0 && (tg >> 5) == tile); todo; todo &= todo - 1) {
-                const int i = __builtin_ctz(todo), row = __builtin_amdgcn_readlane(tg, i) & 31;
-                if (__int_as_float(__builtin_amdgcn_readlane(__float_as_int(bias), row)) < kFloor) continue;     // not on offer
-                const float g = st->g[i];
-                if (lane == row) sum += g;
-                // user i's element of this lane's column, from its place in the cols fragments
-                const int h = i >> 4, from = ((i >> 2) & 1) * 32 + (lane & 31), at = ((i >> 3) & 1) * 4 + (i & 3);
+        // targets: rarely in this tile
+        const int tg = USERS ? target - t * 32 : st->target[lane & 31] - tile * 32;
+        if (!__any((unsigned)tg < 32u)) continue;
 #pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    float u = 0.f;
+        for (int h = 0; h < 2; ++h) {
+            float w[8];
 #pragma unroll
-                    for (int p = P - 1; p >= 0; --p)
-                        u += __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(cols + ((h * DB + d) * P + p) * 64 + from)[at] << 16);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) out[d][r] += row_of_reg(r, lane) == row ? g * u : 0.f;
+            for (int q = 0; q < 2; ++q) {
+                const int i = 16 * h + 8 * q + 4 * half;
+                int32_t to[4];
+                float gr[4];
+                if (!USERS) {
+                    *reinterpret_cast<int4 *>(to) = *reinterpret_cast<const int4 *>(st->target + i);
+                    *reinterpret_cast<float4 *>(gr) = *reinterpret_cast<const float4 *>(st->g + i);
                 }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const bool hit = USERS ? tg == i + k : to[k] == mine && !(bias < kFloor);       // (not on offer: nothing)
+                    w[4 * q + k] = hit ? (USERS ? g : gr[k]) + (P < 3 ? dz[8 * h + 4 * q + k] : 0.f) : 0.f;
+                    if (!USERS) sum += hit ? gr[k] : 0.f;
+                }
+            }
+            bf16x8 z[3];
+            cut_pieces<3>(w, z);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const Fragment<P> ct = load_fragment<P>(cols, h * DB + d, lane);
+                multiply<3, P, 2>(out[d], z, ct.p);
             }
         }
     }
@@ -195,7 +211,7 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
 
 // Both gradients in one launch: the first blocks own users, the others items.
 template <class T, int DB>
-__global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * Pieces<T>::P + 16 * DB + 72))
+__global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * Pieces<T>::P + 16 * DB + 32))
 void catalog_bwd_kernel(BwdArgs a) {
     extern __shared__ uint4 stage[];
     if ((int)blockIdx.x < a.user_blocks) backward<T, DB, true>(a, a.users, blockIdx.x, stage);
@@ -208,9 +224,6 @@ struct JoinArgs {
     int user_shares, item_shares, dim, width;
     int64_t user_n, item_n, bias_n, user_padded, item_padded;          // *_n: elements to write, 0 for none
     float scale;
-    const void *item;
-    const Stats *stats;
-    const float *bias2;
     void *g_user, *g_item;
     float *g_bias;
 };
@@ -245,14 +258,8 @@ void catalog_bwd_join_kernel(JoinArgs a) {
     s = 0.f;
 #pragma unroll
     for (int k = 0; k < N; ++k) s += sums[k][threadIdx.x];
-    if (user) {
-        // the target's term, whole
-        const int64_t n = i / a.dim;
-        const Stats &st = a.stats[n >> 5];
-        const int t = st.target[n & 31];
-        if (t >= 0 && a.bias2[t] > kFloor) s += st.g[n & 31] * (float)static_cast<const T *>(a.item)[(int64_t)t * a.dim + (i - n * a.dim)];
-        static_cast<T *>(a.g_user)[i] = (T)(s * a.scale);
-    } else if (item) static_cast<T *>(a.g_item)[i] = (T)(s * a.scale);
+    if (user) static_cast<T *>(a.g_user)[i] = (T)(s * a.scale);
+    else if (item) static_cast<T *>(a.g_item)[i] = (T)(s * a.scale);
     else a.g_bias[i] = s;
 }
 
@@ -378,7 +385,6 @@ extern "C" int gs_catalog_bwd(const void *user, int64_t n_users, const void *ite
     JoinArgs j{};
     j.dim = dim; j.width = blocks * 32; j.scale = scale;
     j.g_user = g_user; j.g_item = g_item; j.g_bias = g_bias;
-    j.item = item; j.stats = lu.stats; j.bias2 = li.bias2;
     j.user_padded = (int64_t)ut * 32; j.item_padded = (int64_t)it * 32;
     if (g_user) {
         a.users = Side{lu.rows, li.rows, li.cols, reinterpret_cast<float *>(ws + sp.user_part), g_user, n_users, ut, it,
