@@ -16,6 +16,8 @@
 // tables out, 52 us, 39 us for the best items.
 #include "catalog.h"
 
+#include <algorithm>
+
 namespace gs {
 
 int check_catalog(const char *what, int64_t n_users, int64_t n_items, int dim, int dtype, float scale) {
@@ -718,7 +720,7 @@ Cut cut_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
         const auto cost = [&](double group) { return 8.0 * n_items / group + 0.5 * top_k * group * dim * dtype_size(dtype); };
         c.top = cost(4) < cost(32) ? 4 : 32;
         const int64_t most = ((int64_t)1 << 26) / (group_stride_of(n_items, c.top) + 1) / 256 * 256;
-        if (c.slice > most) c.slice = most < 256 ? 256 : most;
+        c.slice = std::min(n_users, std::max<int64_t>(most, 256));
     }
     return c;
 }
