@@ -29,6 +29,8 @@ constexpr float kOffer = -1e10f;
 constexpr float kFloor = -1e12f;                    // in units of log 2, as all scores in the kernels
 constexpr float kMasked = -1e14f;
 constexpr int kCatThreads = 256;
+// A dispatch has fewer than 2^32 threads along x: kernels of a block per few rows or elements are started in parts.
+constexpr int64_t kMostThreads = (int64_t)1 << 31;
 
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f32x16 = __attribute__((ext_vector_type(16))) float;

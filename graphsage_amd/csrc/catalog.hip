@@ -38,14 +38,15 @@ constexpr int kLdsPad = 4;
 
 template <class T>
 __global__ __launch_bounds__(kCatThreads)
-void layout_kernel(Layout first, Layout second, int first_tiles, int dim, int blocks, uint32_t magic, int vector) {
+void layout_kernel(Layout first, Layout second, int first_tiles, int block0, int dim, int blocks, uint32_t magic, int vector) {
     constexpr int P = Pieces<T>::P, E = 16 / sizeof(T);
     extern __shared__ float buf[];                  // [32][blocks * 32 + kLdsPad]
     __shared__ int on[32];
     __shared__ float tops[kCatThreads / 64];
-    const bool is_first = (int)blockIdx.x < first_tiles;
+    const int block = block0 + (int)blockIdx.x;
+    const bool is_first = block < first_tiles;
     const Layout &l = is_first ? first : second;
-    const int64_t tile = is_first ? blockIdx.x : blockIdx.x - first_tiles, row0 = tile * 32;
+    const int64_t tile = is_first ? block : block - first_tiles, row0 = tile * 32;
     const int rows = (int)min((int64_t)32, l.n_rows - row0), width = blocks * 32, ld = width + kLdsPad, tid = threadIdx.x;
     if (tid < 32) {
         const bool offered = tid < rows && !(l.bias && l.bias[row0 + tid] < kOffer);
@@ -149,8 +150,12 @@ int launch_layouts_of(const Layout &first, const Layout &second, int dim, hipStr
     // i / dim for i < 2^13: exact with the rounded-up reciprocal
     const uint32_t magic = dim == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + dim - 1) / dim);
     const int vector = (((uintptr_t)first.x | (uintptr_t)second.x) & 15) == 0;
-    layout_kernel<T><<<dim3((unsigned)(t0 + t1)), kCatThreads, lds, stream>>>(first, second, (int)t0, dim, blocks, magic, vector);
-    return check_launch("gs_catalog (layout)");
+    constexpr int64_t most = kMostThreads / kCatThreads;
+    for (int64_t b = 0; b < t0 + t1; b += most) {
+        layout_kernel<T><<<dim3((unsigned)std::min(most, t0 + t1 - b)), kCatThreads, lds, stream>>>(first, second, (int)t0, (int)b, dim, blocks, magic, vector);
+        if (int rc = check_launch("gs_catalog (layout)")) return rc;
+    }
+    return GS_OK;
 }
 
 }  // namespace
@@ -497,8 +502,8 @@ __device__ __forceinline__ float finish_user(const JoinArgs &a, int64_t n, float
 
 // A wave per user.
 __global__ __launch_bounds__(kCatThreads)
-void catalog_join_kernel(JoinArgs a, int64_t n_users) {
-    const int64_t n = (int64_t)blockIdx.x * (kCatThreads / 64) + (threadIdx.x >> 6);
+void catalog_join_kernel(JoinArgs a, int64_t first_user, int64_t n_users) {
+    const int64_t n = first_user + (int64_t)blockIdx.x * (kCatThreads / 64) + (threadIdx.x >> 6);
     if (n < n_users) finish_user(a, n, join_shares<64>(a, n, threadIdx.x & 63), (threadIdx.x & 63) == 0);
 }
 
@@ -720,7 +725,8 @@ Cut cut_of(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k) {
         const auto cost = [&](double group) { return 8.0 * n_items / group + 0.5 * top_k * group * dim * dtype_size(dtype); };
         c.top = cost(4) < cost(32) ? 4 : 32;
         const int64_t most = ((int64_t)1 << 26) / (group_stride_of(n_items, c.top) + 1) / 256 * 256;
-        c.slice = std::min(n_users, std::max<int64_t>(most, 256));
+        // (256 threads a user in the launch of the best items)
+        c.slice = std::min({n_users, std::max<int64_t>(most, 256), gs::kMostThreads / 256});
     }
     return c;
 }
@@ -905,8 +911,12 @@ extern "C" int gs_catalog_fwd(const void *user, int64_t n_users, const void *ite
         }
         const JoinArgs j{part, shares, n_items, aims, log_prob ? log_prob + u0 : nullptr, entropy ? entropy + u0 : nullptr, lse ? lse + u0 : nullptr};
         if (!top_k) {
-            catalog_join_kernel<<<dim3((unsigned)((nu + 3) / 4)), gs::kCatThreads, 0, s>>>(j, nu);
-            if (int rc = gs::check_launch("gs_catalog_fwd (join)")) return rc;
+            constexpr int64_t most = gs::kMostThreads / 64;
+            for (int64_t n = 0; n < nu; n += most) {
+                const int64_t users_now = std::min(most, nu - n);
+                catalog_join_kernel<<<dim3((unsigned)((users_now + 3) / 4)), gs::kCatThreads, 0, s>>>(j, n, nu);
+                if (int rc = gs::check_launch("gs_catalog_fwd (join)")) return rc;
+            }
             continue;
         }
         TopArgs t;

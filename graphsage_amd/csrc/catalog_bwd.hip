@@ -20,6 +20,8 @@
 // forms 2 x 410M dz at an exponential and about ten more instructions each while the matrix cores wait.
 #include "catalog.h"
 
+#include <algorithm>
+
 namespace {
 
 using namespace gs;
@@ -220,6 +222,7 @@ void catalog_bwd_kernel(BwdArgs a) {
 
 // Adds the shares in a fixed order: users' elements, then items', then the bias.
 struct JoinArgs {
+    int64_t first;                                  // the element that the launch begins with
     const float *user_part, *item_part, *bias_part;
     int user_shares, item_shares, dim, width;
     int64_t user_n, item_n, bias_n, user_padded, item_padded;          // *_n: elements to write, 0 for none
@@ -234,7 +237,7 @@ __global__ __launch_bounds__(32 * N)
 void catalog_bwd_join_kernel(JoinArgs a) {
     __shared__ float sums[N][32];
     const int part_of = threadIdx.x >> 5;
-    int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    int64_t i = a.first + (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
     const bool in = i < a.user_n + a.item_n + a.bias_n;
     const bool user = i < a.user_n, item = !user && i < a.user_n + a.item_n;
     const float *part = a.bias_part;
@@ -314,19 +317,20 @@ int launch_bwd(const BwdArgs &a, hipStream_t stream) {
 }
 
 template <class T>
-int run_bwd(const BwdArgs &a, const JoinArgs &j, int blocks, hipStream_t stream) {
+int run_bwd(const BwdArgs &a, JoinArgs j, int blocks, hipStream_t stream) {
     if (a.user_blocks + a.item_blocks) {
         if (int rc = blocks == 1 ? launch_bwd<T, 1>(a, stream) : blocks == 2 ? launch_bwd<T, 2>(a, stream)
                    : blocks == 4 ? launch_bwd<T, 4>(a, stream) : launch_bwd<T, 8>(a, stream))
             return rc;
     }
     const int64_t elements = j.user_n + j.item_n + j.bias_n;
-    if (elements) {
-        // 32 threads an element where a side has many shares (five users against 70 000 items leave 441: 19 us with eight)
-        const dim3 grid((unsigned)((elements + 31) / 32));
-        if ((j.user_n && j.user_shares > 64) || (j.item_n + j.bias_n && j.item_shares > 64)) catalog_bwd_join_kernel<T, 32><<<grid, 1024, 0, stream>>>(j);
+    // 32 threads an element where a side has many shares (five users against 70 000 items leave 441: 19 us with eight)
+    const int each = (j.user_n && j.user_shares > 64) || (j.item_n + j.bias_n && j.item_shares > 64) ? 32 : 8;
+    for (j.first = 0; j.first < elements; j.first += gs::kMostThreads / each) {
+        const dim3 grid((unsigned)((std::min(gs::kMostThreads / each, elements - j.first) + 31) / 32));
+        if (each == 32) catalog_bwd_join_kernel<T, 32><<<grid, 1024, 0, stream>>>(j);
         else catalog_bwd_join_kernel<T, 8><<<grid, 256, 0, stream>>>(j);
-        return gs::check_launch("gs_catalog_bwd (join)");
+        if (int rc = gs::check_launch("gs_catalog_bwd (join)")) return rc;
     }
     return GS_OK;
 }
@@ -352,6 +356,8 @@ extern "C" int gs_catalog_bwd(const void *user, int64_t n_users, const void *ite
     const int size = gs::dtype_size(dtype);
     if (((uintptr_t)user | (uintptr_t)item | (uintptr_t)g_user | (uintptr_t)g_item) & (size - 1))
         return gs::fail(GS_EINVAL, "%s: pointer not aligned to its element", what);
+    if (n_users + n_items >= (int64_t)1 << 31)      // (a wave for 32 rows of either table, in one launch)
+        return gs::fail(GS_ELIMIT, "%s: %lld users and %lld items (less than 2^31 together)", what, (long long)n_users, (long long)n_items);
     const Space sp = space_of(n_users, n_items, dim, dtype);
     if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < sp.total)
         return gs::fail(GS_EINVAL, "%s: 256-byte aligned workspace of %zu bytes needed, %zu given", what, sp.total, workspace_bytes);

@@ -110,7 +110,7 @@ int gs_neighbor_attention_bwd(const void *q, const void *k, const void *v, const
  *   top_log_prob / top_ids  device float / int32 [n_users][top_k], with top_k > 0;
  *            places beyond the items on offer hold -inf / -1
  *   workspace of gs_catalog_workspace(...) bytes, 256-byte aligned
- * scale > 0 and finite; 1 <= dim <= 256, top_k <= 64, n_items < 2^31 - 512, else GS_ELIMIT.
+ * scale > 0 and finite; 1 <= dim <= 256, top_k <= 64, n_users and n_items < 2^31 - 512, else GS_ELIMIT.
  */
 size_t gs_catalog_workspace(int64_t n_users, int64_t n_items, int dim, int dtype, int top_k);
 int gs_catalog_fwd(const void *user, int64_t n_users, const void *item, int64_t n_items, int dim, int dtype,
@@ -124,6 +124,7 @@ int gs_catalog_fwd(const void *user, int64_t n_users, const void *item, int64_t 
  *     dz_j = g_log_prob ([j = target] - p_j) - g_entropy p_j (log p_j + entropy)
  * into g_user [n_users][dim], g_item [n_items][dim] (of `dtype`) and g_bias float[n_items],
  * each nullable.  An item that is not on offer gets zeros.  The order of every sum is fixed.
+ * n_users + n_items < 2^31, else GS_ELIMIT.
  * For the tables' gradients dz_j is cut to the bits of the tables' type (bf16 2^-8, fp16 2^-16 of it left out), except
  * the target's, of which nothing is left out: g (1 - p) of a well predicted target is as exact as p is in fp32.
  */

@@ -25,3 +25,11 @@ def test_one_user_of_a_large_catalog():
     lib = _lib.load()
     assert lib.gs_catalog_workspace(1, 9_000_000, 32, 1, 10) < 12 << 20
     assert lib.gs_catalog_workspace(1, 50_000_000, 32, 1, 10) < 60 << 20
+
+
+def test_gradients_of_more_rows_than_a_launch_holds_are_refused():
+    """Before anything is launched or read: the addresses are those of tables that are not there."""
+    lib = _lib.load()
+    at = 1 << 20
+    rc = lib.gs_catalog_bwd(at, 1 << 30, at, 1 << 30, 1, 1, None, 1.0, None, at, None, None, None, at, None, None, at, 1 << 62, None)
+    assert rc == -3 and b'together' in lib.gs_last_error()
