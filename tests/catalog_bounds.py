@@ -131,3 +131,36 @@ def case(dtype, users, items, dim, gap, shift, seed, device, user_zero, same=Fal
     g_log_prob = -0.5 - torch.rand(users, generator=gen)
     g_entropy = 0.01 * torch.randn(users, generator=gen)
     return [x.to(device) for x in (user, item, target, bias)] + [2.5] + [x.to(device) for x in (g_log_prob, g_entropy)]
+
+
+# ---- scores of fp32 tables: two elements a row, the others zeros ---------------------------------------------------------
+
+def thin_tables(users, items, dim, seed, device):
+    """fp32 rows whose first and last elements, in [1/2, 1), are all they have: a score is a sum of 12 products of pieces."""
+    gen = torch.Generator().manual_seed(seed)
+    tables = []
+    for n in (users, items):
+        x = torch.zeros(n, dim)
+        x[:, 0] = 0.5 + 0.5 * torch.rand(n, generator=gen)
+        x[:, -1] = 0.5 + 0.5 * torch.rand(n, generator=gen)
+        tables.append(x.to(device))
+    return tables
+
+
+def thin_scores(user, item, scale):
+    """(scores in 64 bits, their bound): 12 additions of products, the three products left out (2 u), the fused
+    multiply-add with its constant and the conversion to units of log 2 (4 u) and back (2 u)."""
+    z = scale * torch.matmul(user.double(), item.double().T.contiguous())
+    return z, 20 * U * z.abs()                       # (all terms are positive: the sum of their sizes is the score)
+
+
+def cut_scores(user, item, scale, pieces):
+    """The scores of tables cut into fewer pieces than fp32 has."""
+    cut = []
+    for x in (user, item):
+        left, total = x.clone(), torch.zeros_like(x)
+        for _ in range(pieces):
+            p = left.bfloat16().float()
+            total, left = total + p, left - p
+        cut.append(total.double())
+    return scale * cut[0] @ cut[1].T

@@ -31,3 +31,18 @@ def test_a_target_whose_two_halves_are_rounded_apart_is_outside(dtype, gap):
     assert _ratios(dtype, 2, gap, True, whole_target=False)[0] > 1.5
     if dtype == torch.bfloat16:
         assert _ratios(dtype, 2, gap, False, same=True, whole_target=False)[1] > 1.5
+
+
+@pytest.mark.parametrize('dim', [32, 64, 128, 256])
+def test_gradients_of_fp32_in_two_pieces_are_outside(dim):
+    """Two rows to sum: the bound is a few roundings, what a third piece holds is more."""
+    for user_zero, which, users in ((True, 0, 200), (False, 1, 2)):
+        ratio = _ratios(torch.float32, 2, 1.0, user_zero, dim=dim, users=users, pieces=2)[which]
+        assert ratio > 1.2, (user_zero, ratio)
+
+
+def test_scores_of_fp32_in_two_pieces_are_outside():
+    user, item = cb.thin_tables(200, 3, 32, 1, 'cpu')
+    z, tol = cb.thin_scores(user, item, 1.5)
+    assert cb.worst(cb.cut_scores(user, item, 1.5, 3), z, tol) <= 0.1
+    assert cb.worst(cb.cut_scores(user, item, 1.5, 2), z, tol) > 1.5
