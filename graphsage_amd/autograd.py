@@ -136,6 +136,31 @@ class L2Normalize(torch.autograd.Function):
         return kernels.l2_normalize_bwd(x, g.contiguous())
 
 
+class _Refuse(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, *grads):
+        ctx.what = what
+        return tuple(None if g is None else g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the gradients of %s cannot be differentiated again" % ctx.what)
+
+
+def _once(backward):
+    """A backward pass whose results depend on the saved inputs but have no derivatives of their own: where a graph of it is
+    asked for, whoever differentiates them gets an error (torch's own mark for this lets them pass as constants when the gradient
+    that came in is one)."""
+    def once(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        return _Refuse.apply(type(ctx).__name__.replace('Backward', ''),
+                             *(None if g is None else g.detach().requires_grad_() for g in out))
+    return once
+
+
 class Dropout(torch.autograd.Function):
     """``kernels.dropout``; the backward pass draws the mask again.  A seed that lives in GPU memory is copied, so that
     the gradient goes by the mask that was drawn even if the caller has changed the seed since."""
@@ -149,12 +174,15 @@ class Dropout(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        return kernels.dropout(g.contiguous(), *ctx.mask), None, None, None
+        # (the map is linear: where the gradient is to be differentiated again, it is this function once more)
+        again = Dropout.apply if torch.is_grad_enabled() and g.requires_grad else kernels.dropout
+        return again(g.contiguous(), *ctx.mask), None, None, None
 
 
 class NeighborAttention(torch.autograd.Function):
     """``kernels.neighbor_attention``: (out, lse); gradients through ``out`` only.  With child_ids, the gradient of
-    the tables takes ``inverse`` (``kernels.neighbor_inverse``; built in the backward pass when it is None)."""
+    the tables takes ``inverse`` (``kernels.neighbor_inverse``; built in the backward pass when it is None).  The gradients
+    cannot be differentiated again (an error says so)."""
 
     @staticmethod
     def forward(ctx, q, k, v, child_ids, n_child, id_offset, scale, indptr, inverse):
@@ -165,6 +193,7 @@ class NeighborAttention(torch.autograd.Function):
         return out, lse
 
     @staticmethod
+    @_once
     def backward(ctx, g, _):
         q, k, v, child_ids, out, lse, indptr = ctx.saved_tensors
         n_child, id_offset, scale, inverse = ctx.meta
@@ -177,7 +206,7 @@ class NeighborAttention(torch.autograd.Function):
 
 class CatalogLogProbs(torch.autograd.Function):
     """``kernels.catalog_log_probs``: (log_prob, entropy) of users over a catalog, with gradients to users, items and
-    bias."""
+    bias, which cannot be differentiated again (an error says so)."""
 
     @staticmethod
     def forward(ctx, user, item, targets, bias, scale):
@@ -187,6 +216,7 @@ class CatalogLogProbs(torch.autograd.Function):
         return r.log_prob, r.entropy
 
     @staticmethod
+    @_once
     def backward(ctx, g_log_prob, g_entropy):
         user, item, targets, bias, lse, entropy = ctx.saved_tensors
         need = ctx.needs_input_grad
