@@ -26,15 +26,23 @@ Two execution paths produce the same numbers:
 Two arguments beyond the reference's: ``agg_option='attention'`` with ``heads`` (``Aggregator``), and ``dropout_seed``.
 Without it dropout draws from torch's generator and torch keeps the masks; with it every mask is a function of the seed
 and of how much has been drawn before (``gs_dropout``), drawn again in the backward pass and never stored.
-(What has been drawn is counted on the host: a step that is captured into a graph replays its masks.)
+What has been drawn is counted on the host, call by call: a step that is captured into a graph replays its masks unless the
+seed is an int64 tensor in GPU memory that the caller changes in between, and a forward pass that the backward pass runs again (``torch.utils.checkpoint``) would draw others, which is refused.  There, and
+wherever a call has to be repeatable, ``model(batch, dropout_offset=n)`` says where its masks begin: the n-th block of eight
+elements under the seed, whatever was drawn before (``step << 24`` keeps steps of up to 2^27 elements apart).
 """
 import itertools as it
 import operator as op
+import threading
 
 from . import autograd as _ag
+from ._lib import GsageError
 from .utils import Aggregator
 
 __all__ = ['GraphSAGE']
+
+
+_drawing = threading.Lock()                                  # threads that share a model draw one after the other
 
 
 class GraphSAGE:
@@ -119,15 +127,33 @@ class GraphSAGE:
         return self.train(False)
 
     # ---- forward ------------------------------------------------------------------
-    def _drop(self, x):
-        if self.dropout and self.training:
-            if self.dropout_seed is not None:
-                first = self._dropout_drawn
-                self._dropout_drawn += (x.numel() + 7) // 8
-                return _ag.Dropout.apply(x.contiguous(), self.dropout, self.dropout_seed, first)
-            import torch
-            return torch.nn.functional.dropout(x, p=self.dropout, training=True)
-        return x
+    def _dropper(self, offset=None):
+        """Dropout as one call of the model applies it; ``offset``: the block its first mask begins with."""
+        if offset is not None and self.dropout_seed is None:
+            raise ValueError("dropout_offset needs a model with a dropout_seed")
+        if not (self.dropout and self.training):
+            return lambda x: x
+        import torch
+        if self.dropout_seed is None:
+            return lambda x: torch.nn.functional.dropout(x, p=self.dropout, training=True)
+        drawn = None if offset is None else int(offset)
+        if drawn is not None and drawn < 0:
+            raise ValueError("dropout_offset must not be negative")
+
+        def drop(x):
+            nonlocal drawn
+            blocks = (x.numel() + 7) // 8
+            if drawn is not None:
+                first, drawn = drawn, drawn + blocks
+            else:
+                if torch._C._current_graph_task_id() != -1:
+                    raise GsageError("a forward pass run again by the backward pass would draw other masks than the first one: "
+                                     "call the model with dropout_offset")
+                with _drawing:
+                    first = self._dropout_drawn
+                    self._dropout_drawn += blocks
+            return _ag.Dropout.apply(x.contiguous(), self.dropout, self.dropout_seed, first)
+        return drop
 
     def _finish(self, h):
         out = [x.reshape(x.shape[0], x.shape[2]) for x in h if x.shape[1] == 1]
@@ -135,15 +161,15 @@ class GraphSAGE:
             out = [_ag.L2Normalize.apply(x.contiguous()) for x in out]
         return out[0] if len(out) == 1 else out
 
-    def _dense_layer(self, h, layer):
+    def _dense_layer(self, h, layer, drop):
         out = []
         for i, (node_type, neigh_indices) in enumerate(self.neigh_trees[layer]):
             j = neigh_indices[0]
             heads = h[i].shape[1]
             n = self.n_samples[self._depths[i]]
             f_neigh = self.dims[layer][self.subtree_schema[j][0]]
-            x_neigh = self._drop(h[j].reshape(h[j].shape[0], heads, n, f_neigh))
-            out.append(self._aggs[layer][node_type]([self._drop(h[i]), x_neigh]))
+            x_neigh = drop(h[j].reshape(h[j].shape[0], heads, n, f_neigh))
+            out.append(self._aggs[layer][node_type]([drop(h[i]), x_neigh]))
         return out
 
     def _fused_first_layer(self, batch):
@@ -177,8 +203,9 @@ class GraphSAGE:
             out.append(agg.project(x_self[i], x_mean).reshape(b, m // b, agg.output_dim))
         return out
 
-    def __call__(self, xin):
+    def __call__(self, xin, dropout_offset=None):
         self.build()
+        drop = self._dropper(dropout_offset)
         self.layer_tensors = []
         from .generator import BatchFeatures
         if isinstance(xin, BatchFeatures) and not (self.dropout and self.training):
@@ -189,7 +216,7 @@ class GraphSAGE:
             h = [xin[i] for i in range(len(self.subtree_schema))]
             first = 0
         for layer in range(first, self.n_layers):
-            h = self._dense_layer(h, layer)
+            h = self._dense_layer(h, layer, drop)
             self.layer_tensors.append(h)
         return self._finish(h)
 
