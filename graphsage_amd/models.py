@@ -27,9 +27,12 @@ Two arguments beyond the reference's: ``agg_option='attention'`` with ``heads`` 
 Without it dropout draws from torch's generator and torch keeps the masks; with it every mask is a function of the seed
 and of how much has been drawn before (``gs_dropout``), drawn again in the backward pass and never stored.
 What has been drawn is counted on the host, call by call: a step that is captured into a graph replays its masks unless the
-seed is an int64 tensor in GPU memory that the caller changes in between, and a forward pass that the backward pass runs again (``torch.utils.checkpoint``) would draw others, which is refused.  There, and
-wherever a call has to be repeatable, ``model(batch, dropout_offset=n)`` says where its masks begin: the n-th block of eight
-elements under the seed, whatever was drawn before (``step << 24`` keeps steps of up to 2^27 elements apart).
+seed is an int64 tensor in GPU memory that the caller changes in between, and a forward pass that the backward pass runs
+again (``torch.utils.checkpoint``) would draw others, which is refused.  There, and wherever a call has to be repeatable,
+``model(batch, dropout_offset=n)`` says where its masks begin: the n-th block of eight elements under the seed, whatever was
+drawn before (``step << 24`` keeps steps of up to 2^27 elements apart).
+A seed is one sequence of masks for every process that has it.  The ranks of a ``Trainer`` begin 2^48 blocks apart
+(``dropout_base``), so that they drop other positions; processes that train otherwise take seeds of their own.
 """
 import itertools as it
 import operator as op
@@ -64,6 +67,7 @@ class GraphSAGE:
         self.heads = heads
         self.dropout_seed = dropout_seed
         self._dropout_drawn = 0                              # blocks of eight elements drawn under the seed so far
+        self.dropout_base = 0                                # the block this process begins with
         self.training = True
         n_slots = len(self.subtree_schema)
 
@@ -152,7 +156,7 @@ class GraphSAGE:
                 with _drawing:
                     first = self._dropout_drawn
                     self._dropout_drawn += blocks
-            return _ag.Dropout.apply(x.contiguous(), self.dropout, self.dropout_seed, first)
+            return _ag.Dropout.apply(x.contiguous(), self.dropout, self.dropout_seed, self.dropout_base + first)
         return drop
 
     def _finish(self, h):

@@ -229,6 +229,11 @@ class Trainer:
         elif engine == 'plan':
             raise ValueError("engine='plan' needs graph and batch_size")
         self.broadcast_parameters()
+        if getattr(self.model, 'dropout_seed', None) is not None:
+            # the masks of one sequence: ranks take stretches of it that do not meet
+            import torch.distributed as dist
+            if dist.is_available() and dist.is_initialized():
+                self.model.dropout_base = dist.get_rank(self.group) << 48
 
     def broadcast_parameters(self):
         """Rank 0's initial weights everywhere (ranks seed their own generators)."""
