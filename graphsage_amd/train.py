@@ -252,9 +252,12 @@ class Trainer:
                     p.copy_(flat[off:off + p.numel()].view_as(p))
                     off += p.numel()
 
+    def _own_loss(self):
+        return callable(getattr(self.head, 'loss', None))
+
     def loss(self, batch, targets):
         """Mean squared error of the head's scores, or the head's own loss where it has one (``link_utils.CatalogHead``)."""
-        if hasattr(self.head, 'loss'):
+        if self._own_loss():
             return self.head.loss(self.model(batch), targets)
         pred = self.head(self.model(batch))
         y = torch.as_tensor(targets, dtype=torch.float32, device=pred.device).reshape(pred.shape)
@@ -574,9 +577,16 @@ class Trainer:
             if eng is not None:
                 BreadthFirstWalker.raise_on_error(eng.err_flag)
 
+    def _result(self, emb, y, with_loss):
+        """(scores (b, 1), targets) of a batch's embeddings and, ``with_loss``, the head's own loss of them."""
+        if not with_loss:
+            return self.head(emb), y
+        loss, pred = self.head.loss(emb, y)
+        return pred, y, loss
+
     @torch.no_grad()
-    def _scores(self, seq, i):
-        """(scores (b, 1), targets) of batch i: through the forward engine when the
+    def _scores(self, seq, i, with_loss=False):
+        """``_result`` of batch i: through the forward engine when the
         batch is a full one of a keyed sequence, else through the model."""
         if (self._graph_obj is not None and self._batch_size and getattr(seq, '_indexed', False)
                 and seq.batch_size == int(self._batch_size) and not (self.model.dropout and self.model.training)
@@ -588,13 +598,13 @@ class Trainer:
                     self._fwd_engine = SageForwardEngine(self._graph_obj, self.model, self._batch_size)
                 emb = self._fwd_engine.forward(staged['roots'][i], staged['walk_ids'][i], rng_seed=staged['key'])
                 y = None if staged['targets'] is None else staged['targets'][i]
-                return self.head(emb), y
+                return self._result(emb, y, with_loss)
         batch, y = seq[i]
-        return self.head(self.model(batch)), y
+        return self._result(self.model(batch), y, with_loss)
 
     @torch.no_grad()
-    def _score_stream(self, seq):
-        """(scores, targets) of every batch of ``seq`` in order.  Full batches of a keyed sequence go through the
+    def _score_stream(self, seq, with_loss=False):
+        """``_result`` of every batch of ``seq`` in order.  Full batches of a keyed sequence go through the
         forward engine with two batches in flight where its route allows (``SageForwardEngine.pipeline``): batch
         i + 1 is launched before batch i's embeddings are scored, and a slot's rows are scored on this stream
         before the slot's stream is allowed to write them again (``submit`` makes it wait for this stream)."""
@@ -618,7 +628,7 @@ class Trainer:
             def score(i, out):
                 cur.wait_event(out[2])
                 y = None if staged['targets'] is None else staged['targets'][i]
-                return self.head((out[0], out[1])), y
+                return self._result((out[0], out[1]), y, with_loss)
             pending = None
             for i in range(n_eng):
                 out = pipe.submit(staged['roots'][i], staged['walk_ids'][i], rng_seed=staged['key'])
@@ -629,9 +639,9 @@ class Trainer:
             pipe.drain()
         else:
             for i in range(n_eng):
-                yield self._scores(seq, i)
+                yield self._scores(seq, i, with_loss)
         for i in range(n_eng, n):
-            yield self._scores(seq, i)
+            yield self._scores(seq, i, with_loss)
 
     def _inference(self):
         """Context in which the model runs with dropout off, as Keras runs ``evaluate``, ``predict`` and the
@@ -650,16 +660,20 @@ class Trainer:
 
     @torch.no_grad()
     def evaluate(self, seq):
-        """Loss and metrics of the current weights over a sequence (no update, no dropout)."""
+        """Loss and metrics of the current weights over a sequence (no update, no dropout).  The loss is what ``fit`` reports:
+        the head's own, batch by batch, where it has one."""
         dev = self.bucket.flat.device
         ys, preds = [], []
+        losses = [] if self._own_loss() else None
         self.flush()
         with self._inference():
-            for pred, y in self._score_stream(seq):
+            for pred, y, *loss in self._score_stream(seq, losses is not None):
+                if loss:
+                    losses.append(loss[0].reshape(1))
                 ys.append((y if isinstance(y, torch.Tensor)
                            else torch.as_tensor(np.asarray(y, dtype=np.float32), device=dev)).reshape(-1))
                 preds.append(pred.reshape(-1))
-        out = self._epoch_logs(self._metrics(), ys, preds, None)
+        out = self._epoch_logs(self._metrics(), ys, preds, losses)
         self._raise_sampling_errors()
         return out
 

@@ -1,0 +1,59 @@
+"""What ``fit`` and ``evaluate`` report as the loss of a head that has one of its own -- needs a GPU."""
+import numpy as np
+import pytest
+import torch
+
+import graphsage_amd as ga
+from graphsage_amd.link_utils import CatalogHead
+from graphsage_amd.train import LinkHead, Trainer
+
+pytestmark = pytest.mark.gpu
+
+
+def _toy(seed=0, nu=120, ni=35):
+    rng = np.random.default_rng(seed)
+    u = np.concatenate([rng.integers(0, nu, 3000), np.arange(nu)])
+    it = np.concatenate([rng.integers(0, ni, 3000), np.arange(nu) % ni]) + nu
+    e = np.stack([u, it])
+    feats = {'user': rng.standard_normal((nu, 24)).astype(np.float32), 'item': rng.standard_normal((ni, 19)).astype(np.float32)}
+    g = ga.Graph(feats, {'user': list(range(nu)), 'item': list(range(nu, nu + ni))}, np.concatenate([e, e[::-1]], axis=1))
+    links = [(int(a), int(b) + nu) for a, b in zip(rng.integers(0, nu, 230), rng.integers(0, ni, 230))]
+    return g, links, (rng.random(230) < 0.6).astype(np.float32)
+
+
+def _own(tr, seq):
+    """The head's loss of every batch, in 64 bits, weighted by the batches' sizes."""
+    total = count = 0.0
+    for i in range(len(seq)):
+        batch, y = seq[i]
+        user, item = (x.detach().double() for x in tr.model(batch))
+        logp = torch.log_softmax(tr.head.scale * user @ item.T, 1)
+        pos = torch.from_numpy(np.asarray(y) > 0.5)
+        loss = -logp.diagonal()[pos].sum() / max(int(pos.sum()), 1) + tr.head.entropy_weight * (logp.exp() * logp).sum(1).mean()
+        total, count = total + float(loss) * len(y), count + len(y)
+    return total / count
+
+
+@pytest.mark.parametrize('agg_option,sizes', [('attention', [16, 8]), ('mean', [32, 32])])
+@pytest.mark.parametrize('entropy_weight', [0.0, 0.1])
+def test_evaluate_reports_the_loss_that_is_trained(cuda, agg_option, sizes, entropy_weight):
+    g, links, targets = _toy()
+    gen = ga.GraphSAGEGenerator(g, 50, [5, 3], head_node_types=['user', 'item'], seed=4)
+    model = ga.GraphSAGE(sizes, gen, agg_option=agg_option, seed=6)
+    tr = Trainer(model, head=CatalogHead(8.0, entropy_weight), lr=1e-2, graph=g, batch_size=50)
+    seq = gen.flow(links, targets=targets, shuffle=False)        # four full batches and one of 30
+    got, want = tr.evaluate(seq)['loss'], _own(tr, seq)
+    assert abs(got - want) <= 1e-5 * abs(want)                   # fp32 embeddings and scores of at most 8
+    history = tr.fit(gen.flow(links, targets=targets, seed=1), validation_data=seq, epochs=1, verbose=0)
+    assert abs(history['val_loss'][0] - _own(tr, seq)) <= 1e-5 * abs(want)
+    assert tr.predict(seq).shape == (230, 1)
+
+
+def test_heads_without_a_loss_report_the_squared_error(cuda):
+    g, links, targets = _toy()
+    gen = ga.GraphSAGEGenerator(g, 50, [5, 3], head_node_types=['user', 'item'], seed=4)
+    model = ga.GraphSAGE([32, 32], gen, seed=6).build()
+    tr = Trainer(model, head=LinkHead(32, cuda, seed=1), lr=1e-2, graph=g, batch_size=50)
+    seq = gen.flow(links, targets=targets, shuffle=False)
+    want = float(((tr.predict(seq).double().cpu().reshape(-1) - torch.from_numpy(targets).double()) ** 2).mean())
+    assert abs(tr.evaluate(seq)['loss'] - want) <= 1e-6
