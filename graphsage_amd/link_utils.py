@@ -151,15 +151,23 @@ class CatalogHead:
     ``loss((user_emb, item_emb), targets)``: every positive link (target > 0.5) is a choice of its item among the items of
     the batch; minus the mean log probability of these choices, minus ``entropy_weight`` times the mean entropy of all
     users' choices (``gs_catalog_fwd`` / ``gs_catalog_bwd``: the logits never pass through memory).  ``item_bias`` corrects for
-    how the batch's items are drawn (minus the logarithm of their frequencies).
+    how the batch's items are drawn (minus the logarithm of their frequencies): one value per item of the batch in the call, or
+    one per item of the catalog (its row in the graph's item table) in the constructor; the call is then told which the
+    batch's are (``items``, as ``Trainer`` does).
     ``recommend(user_emb, item_emb, k)``: the k best of all items for every user.
     Called like the other heads it scores the batch's own pairs, ``sigmoid(scale * <user, item>)``, (B, 1)."""
 
-    def __init__(self, scale=10.0, entropy_weight=0.0):
+    def __init__(self, scale=10.0, entropy_weight=0.0, item_bias=None):
         self.scale = float(scale)
         if not 0.0 < self.scale < float('inf'):
             raise ValueError("scale must be positive and finite (got %r)" % (scale,))
         self.entropy_weight = float(entropy_weight)
+        self.item_bias = None if item_bias is None else torch.as_tensor(item_bias, dtype=torch.float32).reshape(-1)
+
+    @property
+    def needs_items(self):
+        """Whether ``loss`` has to be told the items' rows in the catalog."""
+        return self.item_bias is not None
 
     def parameters(self):
         return []
@@ -168,14 +176,21 @@ class CatalogHead:
         user_emb, item_emb = x_out
         return torch.sigmoid(self.scale * (user_emb * item_emb).sum(dim=-1, keepdim=True))
 
-    def loss(self, x_out, targets, item_bias=None):
-        """(loss, the pairs' scores (B, 1))."""
+    def loss(self, x_out, targets, item_bias=None, items=None):
+        """(loss, the pairs' scores (B, 1)).  ``items``: the rows of the batch's items in the catalog, whole numbers on the
+        embeddings' device."""
         user_emb, item_emb = (x.contiguous() for x in x_out)
         n, dev = user_emb.shape[0], user_emb.device
         positive = torch.as_tensor(targets, dtype=torch.float32, device=dev).reshape(-1) > 0.5
         if positive.numel() != n or item_emb.shape[0] != n:
             raise ValueError("one target and one item per user are needed (%d users, %d items, %d targets)" %
                              (n, item_emb.shape[0], positive.numel()))
+        if self.needs_items and items is None:
+            raise ValueError("the head's item_bias needs the batch's items")
+        if items is not None and items.numel() != n:
+            raise ValueError("%d items for %d links" % (items.numel(), n))
+        if item_bias is None and self.item_bias is not None:
+            item_bias = self._bias_of(items.reshape(-1))
         own = torch.arange(n, dtype=torch.int32, device=dev)
         log_prob, entropy = _ag.CatalogLogProbs.apply(user_emb, item_emb, torch.where(positive, own, -1).to(torch.int32), item_bias,
                                                       self.scale)
@@ -183,6 +198,16 @@ class CatalogHead:
         with torch.no_grad():
             pred = self((user_emb, item_emb))
         return loss, pred
+
+    def _bias_of(self, items):
+        if self.item_bias.device != items.device:
+            self.item_bias = self.item_bias.to(items.device)
+        n = self.item_bias.numel()
+        if n == 0:
+            raise ValueError("the head's item_bias is empty")
+        inside = (items >= 0) & (items < n)                   # (an item that the catalog does not have: NaN, not another's)
+        bias = self.item_bias[torch.where(inside, items, torch.zeros_like(items)).long()]
+        return torch.where(inside, bias, torch.full_like(bias, math.nan))
 
     @torch.no_grad()
     def recommend(self, user_emb, item_emb, k, item_bias=None):
@@ -192,9 +217,9 @@ class CatalogHead:
         return r.top_ids, r.top_log_prob
 
 
-def link_ranking(scale=10.0, entropy_weight=0.0):
+def link_ranking(scale=10.0, entropy_weight=0.0, item_bias=None):
     """The edge function of ``CatalogHead``, taken like those of ``link_inference``."""
-    head = CatalogHead(scale, entropy_weight)
+    head = CatalogHead(scale, entropy_weight, item_bias)
 
     def edge_function(x_out, seed=None):
         x_out.build()

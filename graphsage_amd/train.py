@@ -255,10 +255,27 @@ class Trainer:
     def _own_loss(self):
         return callable(getattr(self.head, 'loss', None))
 
+    def _head_loss(self, emb, targets, batch=None, roots=None):
+        """(loss, scores) by the head's own loss, which is told the rows of the batch's items in the graph's item table where it
+        wants them (``needs_items``): from the batch, or from its roots (sources, then destinations)."""
+        if not getattr(self.head, 'needs_items', False):
+            return self.head.loss(emb, targets)
+        graph = self._graph_obj
+        if batch is not None:
+            if not hasattr(batch, 'ids'):
+                raise TypeError("this head needs the ids of the batch's items: batches of GraphSAGEGenerator.flow have them")
+            graph, items = batch.graph, batch.ids[1].reshape(-1)
+        else:
+            items = roots[roots.numel() // 2:]
+        bias = getattr(self.head, 'item_bias', None)
+        if bias is not None and bias.numel() != graph.num_items:
+            raise ValueError("the head's item_bias has %d entries, the graph %d items" % (bias.numel(), graph.num_items))
+        return self.head.loss(emb, targets, items=items - graph.correction_constant)
+
     def loss(self, batch, targets):
         """Mean squared error of the head's scores, or the head's own loss where it has one (``link_utils.CatalogHead``)."""
         if self._own_loss():
-            return self.head.loss(self.model(batch), targets)
+            return self._head_loss(self.model(batch), targets, batch)
         pred = self.head(self.model(batch))
         y = torch.as_tensor(targets, dtype=torch.float32, device=pred.device).reshape(pred.shape)
         return ((pred - y) ** 2).mean(), pred
@@ -577,11 +594,11 @@ class Trainer:
             if eng is not None:
                 BreadthFirstWalker.raise_on_error(eng.err_flag)
 
-    def _result(self, emb, y, with_loss):
+    def _result(self, emb, y, with_loss, **of):
         """(scores (b, 1), targets) of a batch's embeddings and, ``with_loss``, the head's own loss of them."""
         if not with_loss:
             return self.head(emb), y
-        loss, pred = self.head.loss(emb, y)
+        loss, pred = self._head_loss(emb, y, **of)
         return pred, y, loss
 
     @torch.no_grad()
@@ -598,9 +615,9 @@ class Trainer:
                     self._fwd_engine = SageForwardEngine(self._graph_obj, self.model, self._batch_size)
                 emb = self._fwd_engine.forward(staged['roots'][i], staged['walk_ids'][i], rng_seed=staged['key'])
                 y = None if staged['targets'] is None else staged['targets'][i]
-                return self._result(emb, y, with_loss)
+                return self._result(emb, y, with_loss, roots=staged['roots'][i])
         batch, y = seq[i]
-        return self._result(self.model(batch), y, with_loss)
+        return self._result(self.model(batch), y, with_loss, batch=batch)
 
     @torch.no_grad()
     def _score_stream(self, seq, with_loss=False):
@@ -628,7 +645,7 @@ class Trainer:
             def score(i, out):
                 cur.wait_event(out[2])
                 y = None if staged['targets'] is None else staged['targets'][i]
-                return self._result((out[0], out[1]), y, with_loss)
+                return self._result((out[0], out[1]), y, with_loss, roots=staged['roots'][i])
             pending = None
             for i in range(n_eng):
                 out = pipe.submit(staged['roots'][i], staged['walk_ids'][i], rng_seed=staged['key'])

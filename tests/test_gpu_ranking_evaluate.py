@@ -57,3 +57,46 @@ def test_heads_without_a_loss_report_the_squared_error(cuda):
     seq = gen.flow(links, targets=targets, shuffle=False)
     want = float(((tr.predict(seq).double().cpu().reshape(-1) - torch.from_numpy(targets).double()) ** 2).mean())
     assert abs(tr.evaluate(seq)['loss'] - want) <= 1e-6
+
+
+@pytest.mark.parametrize('agg_option,sizes', [('attention', [16, 8]), ('mean', [32, 32])])
+def test_a_bias_of_the_catalog_reaches_every_batch(cuda, agg_option, sizes):
+    g, links, targets = _toy()
+    gen = ga.GraphSAGEGenerator(g, 50, [5, 3], head_node_types=['user', 'item'], seed=4)
+    model = ga.GraphSAGE(sizes, gen, agg_option=agg_option, seed=6)
+    count = np.bincount([b - 120 for _, b in links], minlength=35) + 1.0
+    bias = -np.log(count)
+    tr = Trainer(model, head=CatalogHead(8.0, item_bias=bias), lr=1e-2, graph=g, batch_size=50)
+    seq = gen.flow(links, targets=targets, shuffle=False)
+    total = 0.0
+    for i in range(len(seq)):
+        batch, y = seq[i]
+        rows = torch.tensor([b - 120 for _, b in links[50 * i:50 * i + 50]])
+        leaves = [x.detach().double().requires_grad_() for x in model(batch)]
+        logp = torch.log_softmax(8.0 * leaves[0] @ leaves[1].T + torch.from_numpy(bias).cuda()[rows.cuda()], 1)
+        pos = torch.from_numpy(y > 0.5)
+        loss = -logp.diagonal()[pos].sum() / int(pos.sum())
+        got, _ = tr.loss(batch, y)
+        assert abs(float(got.detach()) - float(loss.detach())) <= 1e-5 * abs(float(loss.detach()))
+        total += float(loss.detach()) * len(y)
+    assert abs(tr.evaluate(seq)['loss'] - total / 230) <= 1e-5 * abs(total / 230)
+    assert np.isfinite(tr.fit(gen.flow(links, targets=targets, seed=1), epochs=1, verbose=0)['loss'][0])
+
+
+def test_refusals_of_a_catalog_bias(cuda):
+    g, links, targets = _toy()
+    gen = ga.GraphSAGEGenerator(g, 50, [5, 3], head_node_types=['user', 'item'], seed=4)
+    model = ga.GraphSAGE([16, 8], gen, agg_option='attention', seed=6)
+    batch, y = gen.flow(links, targets=targets, shuffle=False)[0]
+    with pytest.raises(ValueError, match='35 items'):
+        Trainer(model, head=CatalogHead(8.0, item_bias=np.zeros(34)), graph=g, batch_size=50).loss(batch, y)
+    tr = Trainer(model, head=CatalogHead(8.0, item_bias=np.zeros(35)), graph=g, batch_size=50)
+    with pytest.raises(TypeError, match='ids'):
+        tr.loss([batch[i] for i in range(len(batch))], y)
+    emb = model(batch)
+    with pytest.raises(ValueError, match='items'):
+        tr.head.loss(emb, y)
+    with pytest.raises(ValueError, match='links'):
+        tr.head.loss(emb, y, items=torch.zeros(49, dtype=torch.int64, device='cuda'))
+    far = torch.full((50,), 35, dtype=torch.int64, device='cuda')
+    assert bool(tr.head.loss(emb, y, items=far)[0].isnan())
