@@ -145,6 +145,17 @@ def link_regression(output_dim=1, clip_limits=None, edge_embedding_method="ip"):
                           clip_limits=clip_limits, name="link_regression")
 
 
+def _first_places(ids):
+    """For every entry the first place in which its value stands (nothing waits for the device)."""
+    n = ids.numel()
+    value, at = torch.sort(ids, stable=True)
+    place = torch.arange(n, device=ids.device)
+    new = torch.ones(n, dtype=torch.bool, device=ids.device)
+    new[1:] = value[1:] != value[:-1]
+    run = torch.cummax(torch.where(new, place, torch.zeros_like(place)), 0)[0] if n else place
+    return torch.empty_like(place).scatter_(0, at, at[run])
+
+
 class CatalogHead:
     """Scores ``scale * <user, item>`` as logits over a catalog of items.
 
@@ -154,20 +165,23 @@ class CatalogHead:
     how the batch's items are drawn (minus the logarithm of their frequencies): one value per item of the batch in the call, or
     one per item of the catalog (its row in the graph's item table) in the constructor; the call is then told which the
     batch's are (``items``, as ``Trainer`` does).
+    An item that occurs several times in the batch is as many choices, so that a user's own item is a wrong one, too, in every
+    other place; with ``distinct_items`` (and ``items``) it is one choice, for which its first place in the batch stands.
     ``recommend(user_emb, item_emb, k)``: the k best of all items for every user.
     Called like the other heads it scores the batch's own pairs, ``sigmoid(scale * <user, item>)``, (B, 1)."""
 
-    def __init__(self, scale=10.0, entropy_weight=0.0, item_bias=None):
+    def __init__(self, scale=10.0, entropy_weight=0.0, item_bias=None, distinct_items=False):
         self.scale = float(scale)
         if not 0.0 < self.scale < float('inf'):
             raise ValueError("scale must be positive and finite (got %r)" % (scale,))
         self.entropy_weight = float(entropy_weight)
         self.item_bias = None if item_bias is None else torch.as_tensor(item_bias, dtype=torch.float32).reshape(-1)
+        self.distinct_items = bool(distinct_items)
 
     @property
     def needs_items(self):
         """Whether ``loss`` has to be told the items' rows in the catalog."""
-        return self.item_bias is not None
+        return self.item_bias is not None or self.distinct_items
 
     def parameters(self):
         return []
@@ -186,12 +200,18 @@ class CatalogHead:
             raise ValueError("one target and one item per user are needed (%d users, %d items, %d targets)" %
                              (n, item_emb.shape[0], positive.numel()))
         if self.needs_items and items is None:
-            raise ValueError("the head's item_bias needs the batch's items")
+            raise ValueError("item_bias and distinct_items of the head need the batch's items")
         if items is not None and items.numel() != n:
             raise ValueError("%d items for %d links" % (items.numel(), n))
         if item_bias is None and self.item_bias is not None:
             item_bias = self._bias_of(items.reshape(-1))
         own = torch.arange(n, dtype=torch.int32, device=dev)
+        if self.distinct_items:
+            first = _first_places(items.reshape(-1))
+            repeated = first != own
+            own = first.to(torch.int32)
+            item_bias = torch.zeros(n, device=dev) if item_bias is None else item_bias
+            item_bias = torch.where(repeated, torch.full_like(item_bias, -math.inf), item_bias)
         log_prob, entropy = _ag.CatalogLogProbs.apply(user_emb, item_emb, torch.where(positive, own, -1).to(torch.int32), item_bias,
                                                       self.scale)
         loss = -log_prob.sum() / positive.sum().clamp(min=1) - self.entropy_weight * entropy.mean()
@@ -217,9 +237,9 @@ class CatalogHead:
         return r.top_ids, r.top_log_prob
 
 
-def link_ranking(scale=10.0, entropy_weight=0.0, item_bias=None):
+def link_ranking(scale=10.0, entropy_weight=0.0, item_bias=None, distinct_items=False):
     """The edge function of ``CatalogHead``, taken like those of ``link_inference``."""
-    head = CatalogHead(scale, entropy_weight, item_bias)
+    head = CatalogHead(scale, entropy_weight, item_bias, distinct_items)
 
     def edge_function(x_out, seed=None):
         x_out.build()

@@ -100,3 +100,39 @@ def test_refusals_of_a_catalog_bias(cuda):
         tr.head.loss(emb, y, items=torch.zeros(49, dtype=torch.int64, device='cuda'))
     far = torch.full((50,), 35, dtype=torch.int64, device='cuda')
     assert bool(tr.head.loss(emb, y, items=far)[0].isnan())
+
+
+@pytest.mark.parametrize('with_bias', [False, True])
+def test_distinct_items_are_one_choice_each(cuda, with_bias):
+    g, links, targets = _toy()
+    gen = ga.GraphSAGEGenerator(g, 50, [5, 3], head_node_types=['user', 'item'], seed=4)
+    model = ga.GraphSAGE([16, 8], gen, agg_option='attention', seed=6)
+    bias = np.linspace(-1, 1, 35) if with_bias else None
+    tr = Trainer(model, head=CatalogHead(8.0, 0.1, bias, distinct_items=True), lr=1e-2, graph=g, batch_size=50)
+    seq = gen.flow(links, targets=targets, shuffle=False)
+    batch, y = seq[0]
+    rows = [b - 120 for _, b in links[:50]]
+    distinct = sorted(set(rows), key=rows.index)
+    assert len(distinct) < 40                                    # 50 links, 35 items
+    places = torch.tensor([rows.index(r) for r in distinct], device='cuda')
+    own = torch.tensor([distinct.index(r) for r in rows], device='cuda')
+    emb = [x.detach().requires_grad_() for x in model(batch)]
+    loss, pred = tr.head.loss(emb, y, items=torch.tensor(rows, device='cuda'))
+    loss.backward()
+    leaves = [x.detach().double().requires_grad_() for x in emb]
+    z = 8.0 * torch.matmul(leaves[0], leaves[1][places].T.contiguous())
+    if with_bias:
+        z = z + torch.from_numpy(bias).cuda()[torch.tensor(distinct).cuda()]
+    logp = torch.log_softmax(z, 1)
+    pos = torch.from_numpy(y > 0.5).cuda()
+    want = -logp.gather(1, own[:, None])[pos].sum() / int(pos.sum()) + 0.1 * (logp.exp() * logp).sum(1).mean()
+    want.backward()
+    # fp32 scores of at most 9: 1e-5 of the loss, 1e-4 of the largest gradient
+    assert abs(float(loss.detach()) - float(want.detach())) <= 1e-5 * abs(float(want.detach())) and pred.shape == (50, 1)
+    for a, b in zip(emb, leaves):
+        assert float((a.grad.double() - b.grad).abs().max()) <= 1e-4 * float(b.grad.abs().max())
+    repeated = [i for i in range(50) if rows.index(rows[i]) != i]
+    assert not emb[1].grad[repeated].any()
+    assert abs(float(tr.loss(batch, y)[0].detach()) - float(want.detach())) <= 1e-5 * abs(float(want.detach()))
+    assert np.isfinite(tr.evaluate(seq)['loss'])
+    assert np.isfinite(tr.fit(gen.flow(links, targets=targets, seed=1), epochs=1, verbose=0)['loss'][0])
