@@ -484,7 +484,8 @@ template <int N> __device__ __forceinline__ float4 join_shares(const JoinArgs &a
     return join_lanes<64>(q);
 }
 
-// The results of user n; log sum exp.
+// The results of user n; log sum exp.  The target's distance to the largest score first: where it is the largest, what is left of
+// 1 - p is log s alone, however far from zero the scores lie.
 __device__ __forceinline__ float finish_user(const JoinArgs &a, int64_t n, float4 q, bool writes) {
     const float top = q.x, s = q.y, w = q.z, hit = q.w;
     const float l2 = fast_log2(s);                  // s 0: nothing on offer
@@ -494,7 +495,7 @@ __device__ __forceinline__ float finish_user(const JoinArgs &a, int64_t n, float
         if (a.entropy) a.entropy[n] = s == 0.f ? 0.f : (l2 - w / s) * kLn2;
         if (a.log_prob) {
             const bool there = a.targets && a.targets[n] >= 0 && a.targets[n] < a.n_items;
-            a.log_prob[n] = !there ? 0.f : s != s ? s : hit < kFloor ? -INFINITY : (hit - (top + l2)) * kLn2;
+            a.log_prob[n] = !there ? 0.f : s != s ? s : hit < kFloor ? -INFINITY : ((hit - top) - l2) * kLn2;
         }
     }
     return lse;

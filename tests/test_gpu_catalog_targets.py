@@ -48,3 +48,18 @@ def test_one_item_leaves_next_to_nothing(cuda, dtype):
     tiny = 2.0 ** -24 if dtype == torch.float16 else 0.0
     assert bool((g_user.double().abs() <= 3.0 * left[:, None] * item.double().abs() * 1.01 + tiny).all())
     assert bool((g_item.double().abs() <= 3.0 * (left[:, None] * user.double().abs()).sum(0) * 1.01 + tiny).all())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('users', [5, 66, 300])
+@pytest.mark.parametrize('shift', [0.0, 40.0, -300.0])
+def test_log_probs_of_well_predicted_targets_far_from_zero(cuda, dtype, users, shift):
+    """log p of -1e-2 to -1e-5: as exact as the sum beside the largest score, not as the scores themselves."""
+    for items in (1, 2, 8, 40):
+        for gap in (4.6, 9.2, 11.5):
+            case = cb.case(dtype, users, items, 64, gap, shift, items, 'cuda', True)
+            want, tol = cb.reference(*case)
+            user, item, target, bias, scale = case[:5]
+            got = kernels.catalog_log_probs(user, item, target, bias, scale).log_prob
+            off = cb.worst(got, want['log_prob'], tol['log_prob'])
+            assert off <= 1.0, "%d items, gap %g: %.3g times the bound" % (items, gap, off)
