@@ -312,12 +312,15 @@ inline int lanes_for(int dim, int size) {
 // Heads of one key head that a wave takes at once (a share of three fills four: 20000 lists of 10, gradients 139 us, 192 by twos).
 inline int heads_per_wave(int share) { return share >= 3 ? 4 : share; }
 
-// Lists of one length that L lanes take each.  Up to 12 entries always (500 lists of 10 rows of 64 fp32: 4.5 us against 5.4 a list
-// per wave; 102400: 42 against 59); with lists enough for every SIMD also longer ones, since a wave's end of a list costs more the more
-// heads it has (40000 lists, forward and backward, this against a list per wave: 20 of 64 fp32 125 us and 127, 32: 206 and
-// 199; two heads, 32 of 64 bf16: 126 and 143; four: 203 and 328).  500 lists of 25 leave most SIMDs idle: 18 us and 12.
-inline bool short_lists(int64_t n_lists, int64_t n_child, int heads_at_once) {
-    return n_child <= 12 || (n_lists >= 8192 && n_child <= (heads_at_once == 1 ? 20 : 32));
+// Lists of one length that L lanes take each.  Up to 12 entries always (lists of 12 rows of 64 fp32, four heads, forward and backward,
+// this against a list per wave: 64 lists 16 us and 19, 4096 lists 20 and 27; one head, 64 lists 11 and 12); up to 32 where
+// the lists fill a wave for each of the chip's 1024 SIMDs, at which the crossing lies for any number of lanes:
+//   8 lanes, four heads, 25 rows   4096 lists 32 us and 27, 8192 lists 36 and 43, 16384 lists 50 and 69
+//   16 lanes, one head, 20 rows    2048 lists 16 us and 13, 4096 lists 18 and 18, 8192 lists 27 and 31
+//   64 lanes, four heads, 25 rows  1024 lists 44 us and 56, 4096 lists 110 and 157
+// (4 lanes cross earlier, one head, 20 rows: 8192 lists 17 us and 20).
+inline bool short_lists(int64_t n_lists, int64_t n_child, int lanes) {
+    return n_child <= 12 || (n_lists * lanes >= 1024 * 64 && n_child <= 32);
 }
 
 // Edges per wave, and whether any list may be cut.  Short: lists of one length, a list per `lanes` lanes.
@@ -326,9 +329,9 @@ struct Deal {
     bool pieces, is_short;
 };
 
-inline Deal deal_edges(const int64_t *indptr, int64_t n_lists, int64_t n_child, int64_t n_edges, int lanes, int heads_at_once) {
+inline Deal deal_edges(const int64_t *indptr, int64_t n_lists, int64_t n_child, int64_t n_edges, int lanes) {
     Deal d;
-    d.is_short = !indptr && n_child > 0 && short_lists(n_lists, n_child, heads_at_once);
+    d.is_short = !indptr && n_child > 0 && short_lists(n_lists, n_child, lanes);
     if (d.is_short) {
         // eight lists a group, if that leaves enough waves
         const int64_t lists = n_edges / n_child, groups = 64 / lanes;
@@ -356,9 +359,8 @@ inline Deal deal_edges(const int64_t *indptr, int64_t n_lists, int64_t n_child, 
 }
 
 // A table without rows leaves every parent without neighbors.
-inline Deal deal_edges(const gs_neighbors *nb, int lanes, int share) {
-    const int g = heads_per_wave(share);
-    return nb->n_rows ? deal_edges(nb->indptr, nb->n_parents, nb->n_child, nb->n_edges, lanes, g) : deal_edges(nullptr, 0, 0, 0, lanes, g);
+inline Deal deal_edges(const gs_neighbors *nb, int lanes) {
+    return nb->n_rows ? deal_edges(nb->indptr, nb->n_parents, nb->n_child, nb->n_edges, lanes) : deal_edges(nullptr, 0, 0, 0, lanes);
 }
 inline Neighbors device_neighbors(const gs_neighbors *nb) {
     if (!nb->n_rows) return Neighbors{nullptr, nb->ids, nb->n_parents, 0, 0, 0, 0};

@@ -381,7 +381,7 @@ size_t pieces_bytes(const gs::Deal &d, int heads, int dim, size_t *off_acc) {
 
 extern "C" size_t gs_neighbor_attention_workspace(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dtype) {
     if (gs::check_neighbors("gs_neighbor_attention_workspace", nb, heads, kv_heads, dim, dtype)) return 0;
-    const gs::Deal d = gs::deal_edges(nb, gs::lanes_for(dim, gs::dtype_size(dtype)), heads / kv_heads);
+    const gs::Deal d = gs::deal_edges(nb, gs::lanes_for(dim, gs::dtype_size(dtype)));
     return pieces_bytes(d, heads, dim, nullptr);
 }
 
@@ -394,7 +394,7 @@ extern "C" int gs_neighbor_attention_fwd(const void *q, const void *k, const voi
     const int size = gs::dtype_size(dtype), lanes = gs::lanes_for(dim, size);
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & (size - 1))
         return gs::fail(GS_EINVAL, "gs_neighbor_attention_fwd: pointer not aligned to its element");
-    const gs::Deal d = gs::deal_edges(nb, lanes, heads / kv_heads);
+    const gs::Deal d = gs::deal_edges(nb, lanes);
     size_t off_acc = 0;
     const size_t need = pieces_bytes(d, heads, dim, &off_acc);
     if (workspace_bytes < need || (need && (!workspace || ((uintptr_t)workspace & 15))))

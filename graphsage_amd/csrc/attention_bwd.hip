@@ -603,7 +603,7 @@ constexpr int64_t kShortMean = 4;
 
 gs::Deal deal_rows(int64_t n_rows, int64_t n_inv, int lanes) {
     static const int64_t ragged = 0;                // any address: the rows' lists are ragged
-    gs::Deal d = gs::deal_edges(&ragged, n_rows, 0, n_inv, lanes, 1);
+    gs::Deal d = gs::deal_edges(&ragged, n_rows, 0, n_inv, lanes);
     d.is_short = n_inv && n_inv <= kShortMean * n_rows;
     if (d.is_short) {
         // runs for two waves per SIMD, of 2 to 16 entries (7600 entries of 16 fp32: 22 us with 8, 9 with 2; 96000 of 64: 19 us with 8,
@@ -621,7 +621,7 @@ Plan make_plan(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dty
     Plan p;
     const int lanes = gs::lanes_for(dim, gs::dtype_size(dtype)), share = heads / kv_heads;
     p.parts = (share + gs::heads_per_wave(share) - 1) / gs::heads_per_wave(share);
-    p.parents = gs::deal_edges(nb, lanes, share);
+    p.parents = gs::deal_edges(nb, lanes);
     p.rows = deal_rows(nb->n_rows, nb->ids && nb->n_rows && nb->n_parents ? n_inv : 0, lanes);
     size_t off = gs::align256((size_t)nb->n_parents * heads * sizeof(float));        // delta
     p.off_parent = off;
