@@ -597,14 +597,16 @@ struct Plan {
     size_t off_parent, off_dense, off_piece, total;
 };
 
-// Rows whose lists are this long on the mean, or shorter, are taken by L lanes a run of entries (100 000 rows of 64 fp32, a
-// list per wave against this: 96000 entries, 66 us and 16; 750 000 entries, about 80 us and 135).
-constexpr int64_t kShortMean = 4;
+// Rows whose lists are this long on the mean, or shorter, are taken by L lanes a run of entries, which pays the longer the fewer
+// heads a wave has at once (the backward pass without g_q, rows of 64, a list per wave against this: 10 000 fp32 rows, one head,
+// mean 4 26 us and 22, 8 28 and 32; 100 000 bf16 rows, one head, mean 8 159 us and 109, 12 176 and 160; two heads, 4 142 us and 93,
+// 8 165 and 165; four heads, 4 160 us and 153; 10 000 bf16 rows, four heads, 4 35 us and 37, 6 37 and 45).
+constexpr int64_t short_mean(int heads_at_once) { return heads_at_once == 1 ? 8 : heads_at_once == 2 ? 6 : 4; }
 
-gs::Deal deal_rows(int64_t n_rows, int64_t n_inv, int lanes) {
+gs::Deal deal_rows(int64_t n_rows, int64_t n_inv, int lanes, int heads_at_once) {
     static const int64_t ragged = 0;                // any address: the rows' lists are ragged
     gs::Deal d = gs::deal_edges(&ragged, n_rows, 0, n_inv, lanes);
-    d.is_short = n_inv && n_inv <= kShortMean * n_rows;
+    d.is_short = n_inv && n_inv <= short_mean(heads_at_once) * n_rows;
     if (d.is_short) {
         // runs for two waves per SIMD, of 2 to 16 entries (7600 entries of 16 fp32: 22 us with 8, 9 with 2; 96000 of 64: 19 us with 8,
         // 16 with 16; 360 000 of 256 bf16: 104 and 87), 131072 runs at most (each may leave two pieces)
@@ -622,7 +624,7 @@ Plan make_plan(const gs_neighbors *nb, int heads, int kv_heads, int dim, int dty
     const int lanes = gs::lanes_for(dim, gs::dtype_size(dtype)), share = heads / kv_heads;
     p.parts = (share + gs::heads_per_wave(share) - 1) / gs::heads_per_wave(share);
     p.parents = gs::deal_edges(nb, lanes);
-    p.rows = deal_rows(nb->n_rows, nb->ids && nb->n_rows && nb->n_parents ? n_inv : 0, lanes);
+    p.rows = deal_rows(nb->n_rows, nb->ids && nb->n_rows && nb->n_parents ? n_inv : 0, lanes, gs::heads_per_wave(share));
     size_t off = gs::align256((size_t)nb->n_parents * heads * sizeof(float));        // delta
     p.off_parent = off;
     if (nb->indptr && nb->ids) off += gs::align256((size_t)nb->n_edges * sizeof(int32_t));
