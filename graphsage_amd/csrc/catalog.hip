@@ -694,10 +694,12 @@ int64_t group_stride_of(int64_t n_items, int top) { return (tiles_of(n_items) * 
 
 constexpr int64_t kBlocks = 1024;                   // blocks a launch is cut into: four waves per SIMD
 
-// Whether a block has all users at once and the tables stay as they are (this against laid-out tables): 100 users, 3700 items of 32
-// fp32 9.1 us and 11.8; 64 users, 100 000 items of 64 bf16 22 and 26, but 128 users 32 and 26.  Wide rows are fetched in
-// pieces of lines and pay only where fp32 would be laid out as three pieces (5 users, 73 000 items of 200 fp32: 60 us and 75;
-// of 256 bf16: 46 and 37; 100 users, 50 000 items of 128 fp32: 61 and 32).
+// Whether a block has all users at once and the tables stay as they are (this against laid-out tables; the border of users lies at
+// two tiles of them, for up to 16384 items at the four that a block's waves hold): rows of 32 fp32, 64 users 9.3 us and 12.7 for 16 000
+// items, 11.5 and 14.6 for 32 000, 128 users 11.8 and 12.8, 17.8 and 14.7; rows of 64 bf16, 64 users 9.8 and 11.9, 12.2 and 13.4, 128 users
+// 12.6 and 12.1, 19.5 and 13.6.  Wide rows are fetched in pieces of lines and pay only for few users where fp32 would be laid out as
+// three pieces (32 000 items of 128 fp32: 32 users 16.4 us and 25.9, 64 users 28.0 and 26.6; 73 000 of 200: 5 users 60 and 75; of 256
+// bf16: 46 and 37).
 inline bool few_users(int64_t n_users, int64_t n_items, int dim, int dtype) {
     if (dim > 64) return n_users <= 32 && dtype == GS_F32;
     return n_users <= 64 || (n_users <= 128 && n_items <= 16384);
