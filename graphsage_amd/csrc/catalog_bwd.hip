@@ -5,14 +5,14 @@
 // One launch for both tables.  A wave owns 32 rows of one table and streams tiles of the other: the tile product gives
 // it 32 x 32 scores with its own row in the lane, dz is formed in place, cut into as many bf16 pieces as the tables'
 // elements have (which leaves out 2^-8 of an element for bf16 tables, 2^-16 for fp16, nothing for fp32; many elements add up
-// to a result that is itself rounded to the tables' type) and multiplied, pieces i and k with i + k <= 2,
+// to a result that is itself rounded to the tables' type) and multiplied, pieces i and k with i + k below their number,
 // with the same streamed rows, cols layout, into the accumulators of the 32 gradients.  Nothing of the scores
 // or dz goes through memory; the scores are computed twice.  The streamed table is cut into shares so that the launch fills
 // the chip; the shares' sums are added in share order by a second launch.
 //
 // Targets: where one is predicted well, g and -g p cancel, and what a cut leaves out of -g p would stand where g (1 - p) should
 // (bf16: 2^-9 of g against the 1e-4 of it that p = 0.9999 leaves).  So a tile that holds targets is followed by a second product
-// of matrices that are zero elsewhere: g and what the cut left of -g p, in three pieces.  The sum then lacks nothing but fp32
+// of matrices that are zero elsewhere: g and what the cut left of -g p, in three pieces, and the product of fp16's second pieces.  The sum then lacks nothing but fp32
 // roundings of g.  All targets of a tile cost one such product (4096 users and items of 32 fp32, every user's target an item of its
 // own: 47 us with the call, 75 us with a loop over the targets; all the same item: 49 and 106 us).
 //
@@ -146,6 +146,7 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
             for (int r = 0; r < 8; ++r) x[r] = dz[2 * r] + dz[2 * r + 1];
             sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
         }
+        bf16x8 last[2];                             // fp16: the piece whose product with the elements' second one is left out
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             bf16x8 z[P];
@@ -153,8 +154,9 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 const Fragment<P> ct = load_fragment<P>(cols, h * DB + d, lane);
-                multiply<P, P, 2>(out[d], z, ct.p);
+                multiply<P, P, P - 1>(out[d], z, ct.p);
             }
+            last[h] = z[P - 1];
         }
         // targets: rarely in this tile
         const int tg = USERS ? target - t * 32 : st->target[lane & 31] - tile * 32;
@@ -176,6 +178,7 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
                     const bool hit = USERS ? tg == i + k : to[k] == mine && !(bias < kFloor);       // (not on offer: nothing)
                     w[4 * q + k] = hit ? (USERS ? g : gr[k]) + (P < 3 ? dz[8 * h + 4 * q + k] : 0.f) : 0.f;
                     if (!USERS) sum += hit ? gr[k] : 0.f;
+                    if (P == 2 && !hit) last[h][4 * q + k] = (__bf16)0.f;
                 }
             }
             bf16x8 z[3];
@@ -184,6 +187,7 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
             for (int d = 0; d < DB; ++d) {
                 const Fragment<P> ct = load_fragment<P>(cols, h * DB + d, lane);
                 multiply<3, P, 2>(out[d], z, ct.p);
+                if constexpr (P == 2) multiply<1, 1, 0>(out[d], last + h, ct.p + 1);
             }
         }
     }
@@ -211,9 +215,12 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
     }
 }
 
+// Three waves per SIMD where 168 registers do (4096 users, 100 000 items of 64 fp32: 1174 us, 1210 with 170 and two).
+constexpr int waves_of(int registers) { return registers <= 112 ? 3 : waves_for(registers); }
+
 // Both gradients in one launch: the first blocks own users, the others items.
 template <class T, int DB>
-__global__ __launch_bounds__(kCatThreads, waves_for(8 * DB * Pieces<T>::P + 16 * DB + 32))
+__global__ __launch_bounds__(kCatThreads, waves_of(8 * DB * Pieces<T>::P + 16 * DB + 32))
 void catalog_bwd_kernel(BwdArgs a) {
     extern __shared__ uint4 stage[];
     if ((int)blockIdx.x < a.user_blocks) backward<T, DB, true>(a, a.users, blockIdx.x, stage);
