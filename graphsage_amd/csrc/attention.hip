@@ -2,9 +2,10 @@
 //
 // An edge costs one row of dim elements (two with separate values) and, per head, dim multiply-adds for the score and as
 // many for the sum.  One head is bound by the row gathers: 1 024 000 rows of 64 fp32 in lists of 10 take 37 us, 7.0 TB/s out of
-// the caches (their mean, which gathers the same rows, 34 us).  Four heads a key head keep the vector ALU busy two thirds of the
-// time, the rest is the ends of lists: 2M ragged edges of eight heads of 64 bf16, 4M row pairs, take 308 us.  Scores are kept in units of log 2 (scale * log2 e goes into the query), so an exponential is one
-// instruction.
+// the caches (their mean, which gathers the same rows, 34 us).  Four heads a key head are bound by the vector ALU: 2M ragged edges of
+// eight heads of 64 bf16, 4M row pairs, take 308 us, 94% of them busy with 140M instructions, a part of which repeats in the lanes of a
+// row group (the softmax step of a score) or ends a list.  Scores are kept in units of log 2 (scale * log2 e goes into the query), so
+// an exponential is one instruction.
 #include "attention.h"
 
 namespace gs {
@@ -246,8 +247,8 @@ void attn_fwd_short_kernel(FwdArgs a) {
 }
 
 // Joins the pieces of the lists that were cut and writes the parents without edges, for one head and 64 elements.  A wave
-// joins a list of a few pieces by itself; of a long one every wave takes its share (one list of 20000 rows of 64: 12.4 us forward,
-// 31.7 with one wave; 2000 lists of 2000, 9 pieces each: 57 us, 70 with every wave).
+// joins a list of a few pieces by itself; of a long one every wave takes its share (one list of 20000 rows of 64, four heads: 17 us
+// with the walk, 38 with one wave; 2000 lists of 2000, 9 pieces each: 133 us, 143 with every wave).
 constexpr uint32_t kFewPieces = 16;
 
 struct Joined {

@@ -9,9 +9,10 @@
 // stay in registers and the queries and g_out of the edges that read it arrive, so a row's gradient is summed in registers
 // in the order of its list, and no atomics are needed.
 //
-// 8192 dense lists of 25 rows of 32 fp32, four heads: 24 us (the forward 12 us, most of it launch and latency).  226 000 ragged edges
-// into 3700 rows of 2 x 33 fp16: parents 38 us, rows 30 us, each with a join of 7 to 9 us; the tables lie in the caches and
-// what bounds both walks is the work per list (3700 to 6040 lists of 40 to 60 edges) and its latency.
+// 8192 dense lists of 25 rows of 32 fp32, four heads: 25 us (the forward 13 us), one wave per SIMD, whose vector ALU is busy 43% of the
+// time (48%) and which waits for loads 41% of it (43%).  226 000 ragged edges into 3700 rows of 2 x 33 fp16: parents 40 us, rows 31 us,
+// each with a join of 7 to 9 us; nine in ten requests hit L2, the vector ALU is busy 55 to 60% of the time and waves wait 44 to
+// 52% of theirs: the work per list (3700 to 6040 lists of 40 to 60 edges) and its latency bound both walks.
 #include "attention.h"
 
 namespace {

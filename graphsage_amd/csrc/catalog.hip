@@ -11,9 +11,10 @@
 // user are scored again, in 64 bits, from the tables themselves; groups within the rounding error of the first product
 // count as candidates too.  The list is then a function of the tables alone, whatever the product's order of additions.
 //
-// 4096 users, 100 000 items of 64 bf16: 126 to 140 us for 52 GFLOP, bound by the vector ALU (the exponential and about ten more
-// instructions a score; the product alone would take 47 us at a large product's rate).  512 users of fp32, 20 best: 14 us to lay the
-// tables out, 52 us, 39 us for the best items.
+// 4096 users, 100 000 items of 64 bf16: 126 to 146 us for 52 GFLOP, bound by the vector ALU, which is busy 87% of the time (the
+// exponential and about ten more instructions a score; the product alone would take 47 us at a large product's rate).  512 users of
+// fp32, 20 best: 14 us to lay the tables out, 52 us (matrix cores busy 43%, vector ALU 41% of the time), 38 us for the best items,
+// whose waves wait two thirds of theirs: phases with barriers between them.
 #include "catalog.h"
 
 #include <algorithm>

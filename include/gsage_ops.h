@@ -126,8 +126,9 @@ int gs_catalog_fwd(const void *user, int64_t n_users, const void *item, int64_t 
  * into g_user [n_users][dim], g_item [n_items][dim] (of `dtype`) and g_bias float[n_items],
  * each nullable.  An item that is not on offer gets zeros.  The order of every sum is fixed.
  * n_users + n_items < 2^31, else GS_ELIMIT.
- * For the tables' gradients dz_j is cut to the bits of the tables' type (bf16 2^-8, fp16 2^-16 of it left out), except
- * the target's, of which nothing is left out: g (1 - p) of a well predicted target is as exact as p is in fp32.
+ * For the tables' gradients dz_j is cut to the bits of the tables' type (bf16: below 2^-8, fp16: below 2^-14 of a term left
+ * out), except the target's, of which nothing is left out: g (1 - p) of a well predicted target is as exact as p is in
+ * fp32.  g_bias takes every dz_j whole.
  */
 size_t gs_catalog_bwd_workspace(int64_t n_users, int64_t n_items, int dim, int dtype);
 int gs_catalog_bwd(const void *user, int64_t n_users, const void *item, int64_t n_items, int dim, int dtype,
