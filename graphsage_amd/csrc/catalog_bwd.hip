@@ -164,6 +164,8 @@ __device__ __forceinline__ void backward(const BwdArgs &a, const Side &side, uin
         if (!__any((unsigned)tg < 32u)) continue;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            // (a half of the streamed rows at a time: the lane's target there, or the lane is the target's user)
+            if (!__any((unsigned)tg < 32u && (USERS ? tg : lane & 31) >> 4 == h)) continue;
             float w[8];
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
