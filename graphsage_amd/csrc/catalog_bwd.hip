@@ -16,7 +16,7 @@
 // roundings of g.  All targets of a tile cost one such product (4096 users and items of 32 fp32, every user's target an item of its
 // own: 47 us with the call, 75 us with a loop over the targets; all the same item: 49 and 106 us).
 //
-// 4096 users, 100 000 items of 64 bf16: 343 to 394 us for 105 + 52 GFLOP (scores twice, two gradients), bound by issue: the vector ALU
+// 4096 users, 100 000 items of 64 bf16: 335 to 390 us for 105 + 52 GFLOP (scores twice, two gradients), bound by issue: the vector ALU
 // is busy 68% of the time (2 x 410M dz at an exponential and about ten more instructions each), the matrix cores 33%, one after the
 // other.
 #include "catalog.h"

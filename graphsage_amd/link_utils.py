@@ -167,6 +167,7 @@ class CatalogHead:
     batch's are (``items``, as ``Trainer`` does).
     An item that occurs several times in the batch is as many choices, so that a user's own item is a wrong one, too, in every
     other place; with ``distinct_items`` (and ``items``) it is one choice, for which its first place in the batch stands.
+    Under several ranks each rank's batch is a choice of its own, and their gradients are averaged.
     ``recommend(user_emb, item_emb, k)``: the k best of all items for every user.
     Called like the other heads it scores the batch's own pairs, ``sigmoid(scale * <user, item>)``, (B, 1)."""
 
