@@ -106,7 +106,7 @@ int gs_neighbor_attention_bwd(const void *q, const void *k, const void *v, const
  *            not on offer, and its row is never looked at.  A user for whom nothing is on offer: lse -inf, entropy 0
  *   targets  nullable device int32[n_users]; outside [0, n_items): no target, log_prob 0;
  *            a target that is not on offer: log_prob -inf
- *   scores   are held in fp32; one below -5e11 counts as not on offer
+ *   scores   are held in fp32; one below -6.9e11 (-1e12 in units of log 2) counts as not on offer
  *   log_prob, entropy, lse  device float[n_users], each nullable
  *   top_log_prob / top_ids  device float / int32 [n_users][top_k], with top_k > 0;
  *            places beyond the items on offer hold -inf / -1
